@@ -352,6 +352,65 @@ int strata_attn_decode(strata_ctx* ctx, uint64_t q, uint64_t kc, uint64_t vc, ui
 int strata_attn_decode_gq(strata_ctx* ctx, uint64_t q, uint64_t kc, uint64_t vc, uint64_t qg, uint64_t out, uint64_t part,
                           uint64_t step, uint64_t nh, uint64_t nkv, uint64_t hd, float scale, int gq_min, uint64_t nt,
                           uint64_t sink, uint64_t win);
+
+/* ---- serving a batch of sequences over a paged f16 KV cache (no counterpart in the reference, which serves one sequence
+ *      with a contiguous cache) ----
+ * The caches kc and vc are pools of n_pages pages of `page` positions (a power of two, 16 to 65536): page p's position i is
+ * cache row (slot) p page + i, n_kv_head * head_dim f16 values a row. Sequence s's own position j lies on page tables[s
+ * max_pages + j / page]; all tables, lengths and positions are device int32 arrays. A batch's new tokens are packed by
+ * sequence: sequence s's are rows q_start[s] .. q_start[s + 1] - 1. At most 4096 sequences a call. All sequences may share a
+ * prefix of P positions that lies on pages of its own: own position j is then position P + j. */
+
+/* One step of the page tables, all on the device: sequence s (nseq of them, len[s] positions cached) brings add[s] new tokens.
+ * add[s] < 0: it ends; its pages go back on the stack of free pages (free_pages: n_pages entries, *n_free of them in use, the
+ * top last) in order of sequence and page, before any page is taken. Then, in order of sequence, new pages come from the
+ * top of the stack into the tables. Writes q_start[nseq + 1], for each row t < q_start[nseq] its position pos[t] (*prefix_len
+ * more than its own one; prefix_len may be 0) and its slot slots[t], -1 in both for the rows up to t_max behind them, and len_out
+ * and *n_free_out (which may be len and n_free). A sequence is refused where its positions exceed max_pages pages, its rows
+ * exceed t_max, the stack holds too few pages for it and the sequences before it, or len[s] is below 0: its length, table and
+ * the stack stay as they are, its rows keep their places (q_start is cut at t_max, positions at 2^31 - 1) and have slot -1, and *err (device int32,
+ * may be 0) goes up by one for each of them. Page ids are not checked against each other: a page listed twice is handed out
+ * twice; the slot of a page id outside 0 .. n_pages - 1 is -1. Pages given back that the stack has no room for are lost, and
+ * *err goes up by one. */
+int strata_kv_pages_step(strata_ctx* ctx, uint64_t nseq, uint64_t add, uint64_t len, uint64_t tables, uint64_t max_pages,
+                         uint64_t page, uint64_t free_pages, uint64_t n_pages, uint64_t n_free, uint64_t prefix_len,
+                         uint64_t t_max, uint64_t q_start, uint64_t pos, uint64_t slots, uint64_t len_out,
+                         uint64_t n_free_out, uint64_t err);
+/* strata_rms_norm_rope_qk_t for a batch: token i of t (qper query heads, kper key and value heads of n values) at position
+ * pos[i] instead of step[0] + i, its normed, roped keys and its values stored as f16 at cache row slots[i] kper + head. The
+ * same bits for the same position. A row with pos[i] < 0 is left out (its qo row stays as it was), one whose slot is outside
+ * 0 .. n_slots - 1 is not stored. No two tokens of a call may have the same slot. Token i's query head h at q + i q_tstride
+ * + h q_stride, key head g at k + i k_tstride + g n, value row at v + i v_tstride + g n (floats); qo rows of qper * n. */
+int strata_rms_norm_rope_qk_paged(strata_ctx* ctx, uint64_t q, uint64_t q_tstride, uint64_t q_stride, uint64_t qw, uint64_t qo,
+                                  uint64_t qper, uint64_t k, uint64_t k_tstride, uint64_t kw, uint64_t kper, uint64_t n,
+                                  float eps, uint64_t n_rot, uint64_t pos, float base, uint64_t v, uint64_t v_tstride,
+                                  uint64_t kc, uint64_t vc, uint64_t slots, uint64_t n_slots, uint64_t t);
+/* Attention of a ragged batch: t query rows (q and out rows of nh * hd floats, after norm and rope) of nseq sequences, at most
+ * max_q rows of one sequence (a host bound: longer ones may be left uncomputed). Row r of sequence s sees the keys at
+ * positions up to pos[r] (of them the last `win` when win > 0): the prefix's *prefix_len (at most max_prefix) on the pages
+ * prefix[0 ..], computed once for all rows, and the sequence's own len[s] (new ones included), as strata_attn_decode_gq and
+ * strata_attn_prefill_m compute it: sigmoid gates qg, per-head sink logits, head_dim 64 or 128, nh / nkv 1, 2, 4 or 8. No
+ * prefix: max_prefix 0. A row that sees no key is 0; the keys of a page id outside 0 .. n_pages - 1 are not seen; values of
+ * keys that a row does not see do not reach it, not even infinities and NaN. Rows from q_start[nseq] on stay as they were. */
+int strata_attn_paged(strata_ctx* ctx, uint64_t q, uint64_t kc, uint64_t vc, uint64_t qg, uint64_t out, uint64_t t,
+                      uint64_t max_q, uint64_t pos, uint64_t q_start, uint64_t len, uint64_t nseq, uint64_t tables,
+                      uint64_t max_pages, uint64_t page, uint64_t n_pages, uint64_t prefix, uint64_t prefix_len,
+                      uint64_t max_prefix, uint64_t nh, uint64_t nkv, uint64_t hd, float scale, uint64_t sink, uint64_t win);
+/* Rows of n logits (x_stride floats apart) into out (out_stride apart; may be x) ahead of a choice. With pen (device f32, 3 a
+ * row: repetition, frequency, presence) the row's history (device int32, rows hist_stride apart, hist_len[r] tokens; the last
+ * `last` of them when last > 0) counts: for a token that it holds y = y > 0 ? y / repetition : y * repetition, then, c times at
+ * index hist_from[r] or later (0: any; the index of the first generated token, say), y -= frequency c and, if c > 0, y -=
+ * presence. With bias_start (device int32, rows + 1) y += bias_vals[e] for the token bias_ids[e], bias_start[r] <= e <
+ * bias_start[r + 1], all e < n_bias; of a token listed twice the last entry counts. With mask (device uint32 words, rows
+ * mask_stride apart) y = -inf, whatever it was, where bit v % 32 of word v / 32 is 0. Each step rounds to f32 once, in this
+ * order. Ids outside 0 .. n - 1 are ignored. ids (not 0): the greatest allowed token of each row, the first on ties, as
+ * strata_argmax_rows orders them; -1 if none is allowed. append: it also goes to the end of the row's history (when that has
+ * room: hist_len < hist_stride), so that a recorded step sees it when it is replayed. */
+int strata_logits_process(strata_ctx* ctx, uint64_t x, uint64_t x_stride, uint64_t out, uint64_t out_stride, uint64_t n,
+                          uint64_t rows, uint64_t hist, uint64_t hist_stride, uint64_t hist_len, uint64_t hist_from,
+                          uint64_t last, uint64_t pen, uint64_t bias_start, uint64_t bias_ids, uint64_t bias_vals,
+                          uint64_t n_bias, uint64_t mask, uint64_t mask_stride, uint64_t ids, int append);
+
 /* Backend::add (src/backend.rs:282): x += y over n floats. */
 int strata_add(strata_ctx* ctx, uint64_t x, uint64_t y, uint64_t n);
 /* Backend::swiglu (src/backend.rs:284): g = silu(g) * u over n floats. */

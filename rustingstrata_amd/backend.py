@@ -113,6 +113,10 @@ SIGNATURES = {
     "strata_attn_part_floats": [U64, U64],
     "strata_attn_decode": [CTX, U64, U64, U64, U64, U64, U64, U64, U64, U64, U64, F32, U64],
     "strata_attn_decode_gq": [CTX, U64, U64, U64, U64, U64, U64, U64, U64, U64, U64, F32, I32, U64, U64, U64],
+    "strata_kv_pages_step": [CTX] + [U64] * 17,
+    "strata_rms_norm_rope_qk_paged": [CTX] + [U64] * 11 + [F32, U64, U64, F32] + [U64] * 7,
+    "strata_attn_paged": [CTX] + [U64] * 21 + [F32, U64, U64],
+    "strata_logits_process": [CTX] + [U64] * 19 + [I32],
     "strata_add": [CTX, U64, U64, U64],
     "strata_swiglu": [CTX, U64, U64, U64],
     "strata_get_rows": [CTX, TP, U64, U64, U64],
@@ -523,6 +527,37 @@ class HipBackend:
     def attn_decode(self, q, kc, vc, qg, out, part, step, nh, nkv, hd, scale, nt, sink=0, win=0):
         _check(lib().strata_attn_decode_gq(self._ctx, int(q), int(kc), int(vc), int(qg), int(out), int(part), int(step),
                                            nh, nkv, hd, scale, 0, nt, int(sink), win))
+
+    # ---- serving a batch of sequences over a paged cache ----
+    def kv_pages_step(self, nseq, add, length, tables, max_pages, page, free, n_pages, n_free, t_max, q_start, pos, slots,
+                      len_out, n_free_out, prefix_len=0, err=0):
+        """One step of the page tables: add[s] new tokens of sequence s (< 0: it ends and gives its pages back) get
+        positions and cache slots, new pages come from the stack `free`; a sequence that finds no room is refused."""
+        _check(lib().strata_kv_pages_step(self._ctx, nseq, int(add), int(length), int(tables), max_pages, page, int(free),
+                                          n_pages, int(n_free), int(prefix_len), t_max, int(q_start), int(pos),
+                                          int(slots), int(len_out), int(n_free_out), int(err)))
+
+    def rms_norm_rope_qk_paged(self, q, q_tstride, q_stride, qw, qo, qper, k, k_tstride, kw, kper, n, eps, n_rot, pos, base,
+                               v, v_tstride, kc, vc, slots, n_slots, t):
+        """rms_norm_rope_qk_t with each token at its own position, keys and values into the cache rows of its slot."""
+        _check(lib().strata_rms_norm_rope_qk_paged(self._ctx, int(q), q_tstride, q_stride, int(qw), int(qo), qper, int(k),
+                                                   k_tstride, int(kw), kper, n, eps, n_rot, int(pos), base, int(v),
+                                                   v_tstride, int(kc), int(vc), int(slots), n_slots, t))
+
+    def attn_paged(self, q, kc, vc, qg, out, t, max_q, pos, q_start, length, nseq, tables, max_pages, page, n_pages, nh,
+                   nkv, hd, scale, prefix=0, prefix_len=0, max_prefix=0, sink=0, win=0):
+        """Attention of a ragged batch over paged caches, the prefix that all sequences share computed once for all."""
+        _check(lib().strata_attn_paged(self._ctx, int(q), int(kc), int(vc), int(qg), int(out), t, max_q, int(pos),
+                                       int(q_start), int(length), nseq, int(tables), max_pages, page, n_pages,
+                                       int(prefix), int(prefix_len), max_prefix, nh, nkv, hd, scale, int(sink), win))
+
+    def logits_process(self, x, x_stride, out, out_stride, n, rows, hist=0, hist_stride=0, hist_len=0, hist_from=0, last=0,
+                       pen=0, bias_start=0, bias_ids=0, bias_vals=0, n_bias=0, mask=0, mask_stride=0, ids=0, append=False):
+        """Penalties for repeated tokens, biases and a mask on rows of logits (out may be x), and the greedy choice."""
+        _check(lib().strata_logits_process(self._ctx, int(x), x_stride, int(out), out_stride, n, rows, int(hist),
+                                           hist_stride, int(hist_len), int(hist_from), last, int(pen), int(bias_start),
+                                           int(bias_ids), int(bias_vals), n_bias, int(mask), mask_stride, int(ids),
+                                           int(append)))
 
     def add(self, x, y, n):
         _check(lib().strata_add(self._ctx, int(x), int(y), n))

@@ -11,6 +11,7 @@
 #include "moe.h"
 #include "gemm.h"
 #include "decoder.h"
+#include "serve.h"
 #include "../../include/strata_hip.h"
 
 using namespace strata;
@@ -115,6 +116,7 @@ struct strata_ctx {
     uint64_t gx_key[4] = {0, 0, 0, 0};   // x, x_stride, n_x, cols of gx's contents (all 0: none)
     Scratch misc;
     Scratch am;                          // argmax partials
+    Scratch sv;                          // page steps, choices of processed logits, paged attention's split sums
     void* noalloc = nullptr;             // this device's address of the file-scope `scratch`
     bool recording = false;              // between strata_graph_begin and strata_graph_end
     int graphs = 0;                      // executable graphs made by this context and not yet destroyed
@@ -218,6 +220,7 @@ void strata_close(strata_ctx* c) {
     c->gx.release();
     c->misc.release();
     c->am.release();
+    c->sv.release();
     hipStreamDestroy(c->stream);
     delete c;
 }
@@ -367,6 +370,7 @@ int strata_graph_destroy(strata_ctx* c, void* graph) {
         c->gx.free_retired();
         c->misc.free_retired();
         c->am.free_retired();
+        c->sv.free_retired();
     }
     return 0;
 }
@@ -1026,6 +1030,124 @@ int strata_attn_prefill_m(strata_ctx* c, uint64_t q, uint64_t kc, uint64_t vc, u
 int strata_attn_prefill(strata_ctx* c, uint64_t q, uint64_t kc, uint64_t vc, uint64_t qg, uint64_t out, uint64_t step,
                         uint64_t t, uint64_t nh, uint64_t nkv, uint64_t hd, float scale) {
     return strata_attn_prefill_m(c, q, kc, vc, qg, out, step, t, nh, nkv, hd, scale, 0, 0, 0, 0);
+}
+
+// ---- serving a batch of sequences over a paged cache ----
+
+static int check_pages(uint64_t nseq, uint64_t max_pages, uint64_t page, uint64_t n_pages, const char* what) {
+    if (nseq > (uint64_t)SERVE_MAX_SEQ)
+        return set_error(std::string(what) + ": " + std::to_string(nseq) + " sequences (at most " + std::to_string(SERVE_MAX_SEQ) + ")");
+    if (page < 16 || page > 65536 || (page & (page - 1)))
+        return set_error(std::string(what) + ": pages of " + std::to_string(page) + " (a power of two, 16 to 65536)");
+    if (!n_pages || n_pages >= (1ull << 30) || n_pages * page >= (1ull << 31))
+        return set_error(std::string(what) + ": " + std::to_string(n_pages) + " pages of " + std::to_string(page) + " (1 to 2^31 - 1 cached positions)");
+    if (!max_pages || max_pages >= (1ull << 30) || max_pages * page > (1ull << 30))
+        return set_error(std::string(what) + ": " + std::to_string(max_pages) + " pages a sequence (1 to 2^30 positions)");
+    return 0;
+}
+static int log2_of(uint64_t v) {
+    int s = 0;
+    while ((1ull << s) < v) s++;
+    return s;
+}
+
+int strata_kv_pages_step(strata_ctx* c, uint64_t nseq, uint64_t add, uint64_t len, uint64_t tables, uint64_t max_pages,
+                         uint64_t page, uint64_t free_pages, uint64_t n_pages, uint64_t n_free, uint64_t prefix_len,
+                         uint64_t t_max, uint64_t q_start, uint64_t pos, uint64_t slots, uint64_t len_out,
+                         uint64_t n_free_out, uint64_t err) {
+    if (check_ctx(c) || check_pages(nseq, max_pages, page, n_pages, "kv_pages_step")) return -1;
+    if ((nseq && (!add || !len || !tables || !len_out)) || !free_pages || !n_free || !q_start || !n_free_out || (t_max && (!pos || !slots)))
+        return set_error("kv_pages_step: null argument");
+    if (t_max > (1ull << 24)) return set_error("kv_pages_step: " + std::to_string(t_max) + " tokens (at most 2^24)");
+    PagesStep a;
+    a.nseq = (int)nseq; a.add = (const int*)add; a.len = (const int*)len;
+    a.tables = (int*)tables; a.max_pages = (int)max_pages; a.page_shift = log2_of(page);
+    a.free_pages = (int*)free_pages; a.n_pages = (int)n_pages; a.n_free = (const int*)n_free; a.prefix_len = (const int*)prefix_len;
+    a.t_max = (int)t_max; a.q_start = (int*)q_start; a.pos = (int*)pos; a.slots = (int*)slots;
+    a.len_out = (int*)len_out; a.n_free_out = (int*)n_free_out; a.err = (int*)err;
+    STRATA_HIP(c->need(c->sv, pages_scratch_bytes((int)nseq)));
+    a.scratch = (int*)c->sv.p;
+    STRATA_HIP(launch_pages_step(a, c->stream));
+    return 0;
+}
+
+int strata_rms_norm_rope_qk_paged(strata_ctx* c, uint64_t q, uint64_t q_tstride, uint64_t q_stride, uint64_t qw, uint64_t qo,
+                                  uint64_t qper, uint64_t k, uint64_t k_tstride, uint64_t kw, uint64_t kper, uint64_t n,
+                                  float eps, uint64_t n_rot, uint64_t pos, float base, uint64_t v, uint64_t v_tstride,
+                                  uint64_t kc, uint64_t vc, uint64_t slots, uint64_t n_slots, uint64_t t) {
+    if (check_ctx(c) || check_rope(n, n_rot)) return -1;
+    if (!qper || !kper) return set_error("rms_norm_rope_qk_paged: no heads a token");
+    if (!q || !qw || !qo || !k || !kw || !pos || !v || !kc || !vc || !slots) return set_error("rms_norm_rope_qk_paged: null argument");
+    if (t >= (1u << 31) || qper >= (1u << 31) || kper >= (1u << 31) || t * (qper + kper) >= (1ull << 31))
+        return set_error("rms_norm_rope: too many rows");
+    if (q_stride < n || q_tstride < (qper - 1) * q_stride + n || k_tstride < kper * n || v_tstride < kper * n)
+        return set_error("rms_norm_rope: a token stride shorter than its heads");
+    if (!t) return 0;
+    NormRope a;
+    a.x = (const float*)k; a.x_stride = n; a.x_tstride = k_tstride; a.w = (const float*)kw;
+    a.n = (int)n; a.rows = (int)(t * kper); a.per = (int)kper;
+    a.v = (const float*)v; a.v_tstride = v_tstride; a.kc = (uint16_t*)kc; a.vc = (uint16_t*)vc;
+    a.qrows = (int)(t * qper); a.qx = (const float*)q; a.q_stride = q_stride; a.q_tstride = q_tstride; a.qw = (const float*)qw;
+    a.qo = (float*)qo; a.qper = (int)qper;
+    a.eps = eps; a.base = base; a.n_rot = (int)n_rot;
+    a.pos = (const int*)pos; a.slots = (const int*)slots; a.n_slots = n_slots;
+    STRATA_HIP(launch_norm_rope(a, c->stream));
+    return 0;
+}
+
+int strata_attn_paged(strata_ctx* c, uint64_t q, uint64_t kc, uint64_t vc, uint64_t qg, uint64_t out, uint64_t t,
+                      uint64_t max_q, uint64_t pos, uint64_t q_start, uint64_t len, uint64_t nseq, uint64_t tables,
+                      uint64_t max_pages, uint64_t page, uint64_t n_pages, uint64_t prefix, uint64_t prefix_len,
+                      uint64_t max_prefix, uint64_t nh, uint64_t nkv, uint64_t hd, float scale, uint64_t sink, uint64_t win) {
+    if (check_ctx(c) || check_attn(nh, nkv, hd, "paged attention") || check_pages(nseq, max_pages, page, n_pages, "paged attention")) return -1;
+    if (!t || !nseq) return 0;
+    if (!q || !kc || !vc || !out || !pos || !q_start || !len || !tables) return set_error("paged attention: null argument");
+    if (max_prefix && (!prefix || !prefix_len)) return set_error("paged attention: null prefix or its length");
+    if (t > (1ull << 20) || !max_q || max_q > t) return set_error("paged attention: " + std::to_string(t) + " rows (at most 2^20), at most " + std::to_string(max_q) + " a sequence");
+    if (max_prefix > (1ull << 30) || win >= (1ull << 31) || nkv > 65535 || nh > 65535) return set_error("paged attention: too large");
+    if (nseq * nkv * (max_pages * page / 64 + 1) >= (1ull << 31)) return set_error("paged attention: more than 2^31 chunks of keys (sequences x KV heads x positions / 64)");
+    if (q % 16 || out % 16 || kc % 16 || vc % 16) return set_error("paged attention: q, out and the caches must be 16-byte aligned");
+    PagedAttn a;
+    a.q = (const float*)q; a.kc = (const uint16_t*)kc; a.vc = (const uint16_t*)vc; a.qg = (const float*)qg; a.out = (float*)out;
+    a.t = (int)t; a.max_q = (int)max_q; a.pos = (const int*)pos; a.q_start = (const int*)q_start; a.len = (const int*)len;
+    a.nseq = (int)nseq; a.tables = (const int*)tables; a.max_pages = (int)max_pages; a.page_shift = log2_of(page);
+    a.n_pages = (int)n_pages;
+    if (max_prefix) { a.prefix = (const int*)prefix; a.prefix_len = (const int*)prefix_len; a.max_prefix = (int)max_prefix; }
+    a.nh = (int)nh; a.nkv = (int)nkv; a.hd = (int)hd; a.scale = scale; a.sink = (const float*)sink; a.win = (int)win;
+    STRATA_HIP(c->need(c->sv, paged_attn_ws_bytes(a)));
+    a.ws = c->sv.p;
+    STRATA_HIP(launch_attn_paged(a, c->stream));
+    return 0;
+}
+
+int strata_logits_process(strata_ctx* c, uint64_t x, uint64_t x_stride, uint64_t out, uint64_t out_stride, uint64_t n,
+                          uint64_t rows, uint64_t hist, uint64_t hist_stride, uint64_t hist_len, uint64_t hist_from,
+                          uint64_t last, uint64_t pen, uint64_t bias_start, uint64_t bias_ids, uint64_t bias_vals,
+                          uint64_t n_bias, uint64_t mask, uint64_t mask_stride, uint64_t ids, int append) {
+    if (check_ctx(c)) return -1;
+    if (!rows) return 0;
+    if (n == 0 || n >= (1ull << 31) || rows > 65535) return set_error("logits_process: " + std::to_string(rows) + " rows of " + std::to_string(n));
+    if (!x || !out) return set_error("logits_process: null x or out");
+    if (rows > 1 && (x_stride < n || out_stride < n)) return set_error("logits_process: a row stride shorter than " + std::to_string(n));
+    if (x == out && x_stride != out_stride && rows > 1) return set_error("logits_process: in place with two row strides");
+    if ((pen || append) && (!hist || !hist_len)) return set_error("logits_process: penalties or append without a history");
+    if (hist_stride >= (1ull << 31) || last >= (1ull << 31) || n_bias >= (1ull << 31)) return set_error("logits_process: too large");
+    if (bias_start && n_bias && (!bias_ids || !bias_vals)) return set_error("logits_process: null bias_ids or bias_vals");
+    if (mask && rows > 1 && mask_stride < (n + 31) / 32) return set_error("logits_process: a mask row shorter than " + std::to_string((n + 31) / 32) + " words");
+    if (append && !ids) return set_error("logits_process: append without ids");
+    LogitsProcess a;
+    a.x = (const float*)x; a.x_stride = x_stride; a.out = (float*)out; a.out_stride = out_stride; a.n = (int)n; a.rows = (int)rows;
+    a.hist = (int*)hist; a.hist_stride = hist_stride; a.hist_len = (int*)hist_len; a.hist_from = (const int*)hist_from;
+    a.last = (int)last; a.pen = (const float*)pen;
+    a.bias_start = n_bias ? (const int*)bias_start : nullptr; a.bias_ids = (const int*)bias_ids;
+    a.bias_vals = (const float*)bias_vals; a.n_bias = (int)n_bias;
+    a.mask = (const uint32_t*)mask; a.mask_stride = mask_stride; a.ids = (int*)ids; a.append = append;
+    if (ids) {
+        STRATA_HIP(c->need(c->sv, logits_key_bytes((int)n, (int)rows)));
+        a.keys = (uint64_t*)c->sv.p;
+    }
+    STRATA_HIP(launch_logits_process(a, c->stream));
+    return 0;
 }
 
 int strata_add(strata_ctx* c, uint64_t x, uint64_t y, uint64_t n) {

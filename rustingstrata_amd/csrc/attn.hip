@@ -14,51 +14,11 @@
 // query heads of one KV head) and merges the partial softmax sums in a second launch.
 #include <climits>
 
+#include "attn_dev.h"
 #include "decoder.h"
 #include "quant8.h"
-#include "xlane.h"
 
 namespace strata {
-
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef float f4 __attribute__((ext_vector_type(4)));
-
-__device__ __forceinline__ float h2f(uint16_t b) {
-    _Float16 h;
-    __builtin_memcpy(&h, &b, 2);
-    return (float)h;
-}
-__device__ __forceinline__ float sigmoid_f(float x) { return 1.0f / (1.0f + expf(-x)); }
-
-// Maximum and sum over the 64 lanes of a wave, returned to every lane: DPP and swizzle steps within each half, then
-// the two halves' results through scalar lane reads (no LDS round trip per step).
-__device__ __forceinline__ float wave_max64(float v) {
-    v = fmaxf(v, xl32f<0>(v));
-    v = fmaxf(v, xl32f<1>(v));
-    v = fmaxf(v, xl32f<2>(v));
-    v = fmaxf(v, xl32f<3>(v));
-    v = fmaxf(v, xl32f<4>(v));
-    return fmaxf(__int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 0)),
-                 __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 32)));
-}
-__device__ __forceinline__ float wave_sum64(float v) {
-    v += xl32f<0>(v);
-    v += xl32f<1>(v);
-    v += xl32f<2>(v);
-    v += xl32f<3>(v);
-    v += xl32f<4>(v);
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 0)) +
-           __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 32));
-}
-
-// 2^x by the hardware's v_exp_f32 (within 1 ulp; 2^-inf = 0). The softmaxes work in log2 units: scores times log2(e)
-// (one rounding, relative 2^-24 of the exponent, so about |s| 2^-24 ln 2 of each weight: ~1e-7 for the scores that
-// carry the weight), then exp2 of the difference from the running maximum.
-constexpr float LOG2E = 1.44269504088896341f;
-__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// Word i (0..3, a constant) of v.
-__device__ __forceinline__ uint32_t u4c(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 // Positions of token t: base .. end (inclusive); a sliding window keeps the last `win`.
 __device__ __forceinline__ void att_range(const int* step, int t, int win, int& base, int& n_pos) {
@@ -70,12 +30,6 @@ __device__ __forceinline__ void att_range(const int* step, int t, int win, int& 
 // ---------------- decode ----------------
 // Positions a split of a token with n_pos positions: at least one chunk of 64, so short contexts use few waves.
 __device__ __forceinline__ int split_len(int n_pos, int ns) { return max((n_pos + ns - 1) / ns, 64); }
-
-// Layout of the K tile ([key][dim]) and the V tile transposed ([dim][key]) in LDS, 64 keys.
-template <int HD> struct PfLayout {
-    static constexpr int KP = HD + 8;          // halves per K row in LDS (16-byte pad: rows start in spread banks)
-    static constexpr int VP = 64 + 4;          // halves per V^T row (8-byte pad)
-};
 
 // grid (ATT_SPLITS, nkv, nt), 4 waves a block. Block (s, g, t) serves the G = nh / nkv query heads of KV head g over
 // the s-th share of token t's positions, 64 keys a chunk, and wave w takes keys 16 w .. 16 w + 15 of each chunk with
@@ -92,15 +46,6 @@ template <int HD> struct PfLayout {
 // arithmetic: the same bits), and the block whose split holds the token's own position also norms and ropes its key
 // head, stores the new key and value into the f16 caches and uses them for that position (no block reads it from the
 // cache): one launch in place of rms_norm_rope_qk + kv store + attention.
-constexpr int DEC_WAVES = 4;
-template <int HD>
-struct DecLayout {
-    static constexpr int KP = HD + 8;    // halves per K row (16-byte pad: rows start in spread banks)
-    static constexpr int VP = 16 + 4;    // halves per V^T row of a wave's 16 keys (8-byte pad)
-    static constexpr int WAVE = 16 * KP * 2 + HD * VP * 2;  // bytes of one wave's K and V^T tiles
-    static constexpr int MERGE = DEC_WAVES * (HD * 16 + 32) * 4;  // the waves' o, m and l for the block merge
-    static constexpr int BYTES = DEC_WAVES * WAVE > MERGE ? DEC_WAVES * WAVE : MERGE;
-};
 template <int HD, int G, bool NR>
 __global__ __launch_bounds__(64 * DEC_WAVES) void attn_decode_kernel(const float* __restrict__ q,
                                                                      const uint16_t* __restrict__ kc,
@@ -571,29 +516,6 @@ hipError_t launch_attn_decode(const float* q, const uint16_t* kc, const uint16_t
 // tile instead of two from opposite ends keep a sliding window's key range short (window 1024: 545 -> 147 us).
 constexpr int PF_BK = 64;  // keys a tile (PfLayout's 64)
 constexpr int PF_Q = 32, PF_W = 4;  // query rows a wave; waves a block
-typedef float f16v __attribute__((ext_vector_type(16)));
-
-// Eight softmax weights p (at most 2) times PF_SCALE as f16 hi and lo parts for the P V MFMA: hi = f16(p c), lo the exact
-// remainder p c - hi rounded likewise, both to nearest, so hi + lo carries each weight to 2^-22 of its value and the lo
-// parts stay normal f16 numbers for weights down to 2^-17. (2^14 is the largest scale that p = 2 leaves in f16, hence the
-// lag of 1: with a lag of 3 and 2^11, rows of weights around 2^-18 beside one of 1 were 1.4e-6 off, 7e-6 around 2^-20; the
-// time is the same.) Written so that the compiler selects the mixed-precision multiply-adds, which scale, round and read
-// the f16 halves in place (and keeps the wait states between them, the exps before and the MFMAs after, as it could not
-// for inline assembly).
-constexpr float PF_SCALE = 16384.0f;
-__device__ __forceinline__ void split_w8(const float* p, h8& hi, h8& lo) {
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        hi[e] = (_Float16)__builtin_fmaf(p[e], PF_SCALE, 0.0f);
-        lo[e] = (_Float16)__builtin_fmaf(p[e], PF_SCALE, -(float)hi[e]);
-    }
-}
-// The larger of this lane's value and that of the lane 32 away.
-__device__ __forceinline__ float max_half(float v) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-
 // One query row of head h again, by a wave in float32 over the keys it sees alone (lo .. qp): scores and weights a lane a key,
 // then a lane a dim. (For rows near a value that is not finite only, so built for few registers, not for speed; the check
 // costs nothing that can be measured: 269.8 -> 269.6 us at 4096 tokens, 32 heads of 128 over 4.)

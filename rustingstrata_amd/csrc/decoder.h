@@ -20,6 +20,9 @@ struct NormRope {
     // floats between consecutive tokens' first heads of q, x (keys) and v; 0: the heads of all tokens back to back
     // (qper q_stride, per x_stride, per n)
     uint64_t q_tstride = 0, x_tstride = 0, v_tstride = 0;
+    // a paged cache (pos not null): token i at position pos[i] (below 0: skipped), its key and value rows at cache row
+    // slots[i] per + head (a slot outside 0 .. n_slots - 1: not stored); step and out are not used
+    const int* pos = nullptr; const int* slots = nullptr; uint64_t n_slots = 0;
     // base^(-2 i / n_rot) for the first nfreq pairs (filled by launch_norm_rope on the host)
     static constexpr int NFREQ = 128;
     int nfreq = 0; double freq[NFREQ] = {};

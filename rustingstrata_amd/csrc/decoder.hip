@@ -5,6 +5,7 @@
 // synthetic GGUF blocks.
 #include <cmath>
 
+#include "argmax_key.h"
 #include "decoder.h"
 #include "formats.h"
 #include "xlane.h"
@@ -62,10 +63,21 @@ __device__ __forceinline__ NrHead nr_head(const NormRope& a, int gb) {
 
 // One head by one wave: out = x * (1 / sqrt(ss / n + eps)) * w, rope, and (key heads of a storing launch) the f16
 // KV store. s: the wave's 512-float LDS stage. HAVE_SS: ss is given (else lane 0 sums the head from the stage).
-template <bool HAVE_SS>
+// PAGED: token b / per at position pos[b / per] (below 0: nothing is read or written), stored at cache row slots[b / per] per
+// + b % per (a slot outside 0 .. n_slots - 1: not stored), the key heads not written elsewhere.
+template <bool HAVE_SS, bool PAGED>
 __device__ __forceinline__ void nr_run(const NormRope& a, const NrHead& h, float* s, int lane, float ss) {
     const int n = a.n, half = a.n_rot / 2;
-    const bool store = h.vr != nullptr;
+    bool store = h.vr != nullptr;
+    int slot = 0;
+    if constexpr (PAGED) {
+        if (a.pos[h.b / h.per] < 0) return;
+        if (store) {
+            slot = a.slots[h.b / h.per];
+            store = slot >= 0 && (uint64_t)slot < a.n_slots;
+            if (!store) return;
+        }
+    }
     // every load of the wave first (the head, its norm weights, the value row), then the rope angles while they land
     constexpr int NV = 512 / 64;
     float xv[NV], wv[NV], vv[NV];
@@ -78,7 +90,7 @@ __device__ __forceinline__ void nr_run(const NormRope& a, const NrHead& h, float
             if (store) vv[j] = h.vr[i];
         }
     }
-    const int pos = a.step[0] + h.b / h.per;
+    const int pos = PAGED ? a.pos[h.b / h.per] : a.step[0] + h.b / h.per;
     float sn[NV / 2], cs[NV / 2];
 #pragma unroll
     for (int j = 0; j < NV / 2; j++) {
@@ -119,13 +131,13 @@ __device__ __forceinline__ void nr_run(const NormRope& a, const NrHead& h, float
         }
     }
     __builtin_amdgcn_wave_barrier();
-    const uint64_t e = ((uint64_t)pos * h.per + h.b % h.per) * n;
+    const uint64_t e = ((uint64_t)(PAGED ? slot : pos) * h.per + h.b % h.per) * n;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int i = lane + 64 * j;
         if (i < n) {
             const float r = s[i];
-            h.o[i] = r;
+            if (!PAGED || !store) h.o[i] = r;
             if (store) {
                 a.kc[e + i] = f32_to_f16_bits(r);
                 a.vc[e + i] = f32_to_f16_bits(vv[j]);
@@ -136,12 +148,13 @@ __device__ __forceinline__ void nr_run(const NormRope& a, const NrHead& h, float
 }
 
 // A wave per head (decode: few heads, each wave's latency is the launch's).
+template <bool PAGED>
 __global__ __launch_bounds__(64 * NR_WAVES) void norm_rope_kernel(NormRope a) {
     __shared__ __align__(16) float sh[NR_WAVES][512];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int gb = (int)blockIdx.x * NR_WAVES + wave;
     if (gb >= a.qrows + a.rows) return;
-    nr_run<false>(a, nr_head(a, gb), sh[wave], lane, 0.0f);
+    nr_run<false, PAGED>(a, nr_head(a, gb), sh[wave], lane, 0.0f);
 }
 
 // Many heads of 128 values, all rotated (a prefill chunk): a block takes NR_MANY heads. Its threads stage the heads
@@ -151,7 +164,7 @@ __global__ __launch_bounds__(64 * NR_WAVES) void norm_rope_kernel(NormRope a) {
 // norm_rope_kernel's, so both kernels give the same bits. STAGED: the value rows of stored key heads are requested with
 // the heads and wait in LDS (66 KB a block, two a CU), else they are read where they are stored (33 KB, four a CU).
 constexpr int NR_MANY = 64, NR_P = 129;  // heads a block; LDS pitch of a staged head (bank spread for the sums)
-template <bool STAGED>
+template <bool STAGED, bool PAGED>
 __global__ __launch_bounds__(64 * NR_WAVES) void norm_rope_many_kernel(NormRope a) {
     __shared__ float xs[NR_MANY][NR_P], vs[STAGED ? NR_MANY : 1][NR_P];
     __shared__ float ssq[NR_MANY];
@@ -201,7 +214,15 @@ __global__ __launch_bounds__(64 * NR_WAVES) void norm_rope_many_kernel(NormRope 
         const int j = (NR_MANY / NR_WAVES) * wave + jj, g = g0 + j;
         if (g >= total) break;
         const NrHead h = nr_head(a, g);
-        const int pos = a.step[0] + h.b / h.per;
+        const int pos = PAGED ? a.pos[h.b / h.per] : a.step[0] + h.b / h.per;
+        int row = pos;  // the token's cache row
+        if constexpr (PAGED) {
+            if (pos < 0) continue;
+            if (h.vr) {
+                row = a.slots[h.b / h.per];
+                if (row < 0 || (uint64_t)row >= a.n_slots) continue;
+            }
+        }
         if (pos != cur) {
             cur = pos;
             const double f = lane < a.nfreq ? a.freq[lane] : pow((double)a.base, -2.0 * (double)lane / 128.0);
@@ -214,10 +235,12 @@ __global__ __launch_bounds__(64 * NR_WAVES) void norm_rope_many_kernel(NormRope 
         const float sc = 1.0f / sqrtf(ssq[j] / 128.0f + a.eps);
         const float p = xs[j][lane] * sc * (q ? qw0 : kw0), r = xs[j][lane + 64] * sc * (q ? qw1 : kw1);
         const float o0 = p * cs - r * sn, o1 = p * sn + r * cs;
-        h.o[lane] = o0;
-        h.o[lane + 64] = o1;
+        if (!PAGED || !h.vr) {
+            h.o[lane] = o0;
+            h.o[lane + 64] = o1;
+        }
         if (h.vr) {
-            const uint64_t e = ((uint64_t)pos * h.per + h.b % h.per) * 128;
+            const uint64_t e = ((uint64_t)row * h.per + h.b % h.per) * 128;
             a.kc[e + lane] = f32_to_f16_bits(o0);
             a.kc[e + lane + 64] = f32_to_f16_bits(o1);
             const float* vr = STAGED ? vs[j] : h.vr;
@@ -251,6 +274,16 @@ __global__ __launch_bounds__(64 * NR_WAVES) void rope_pairs_kernel(float* x, uin
 // four a CU are faster (1501 x 36 29.0 staged, 26.5 not, 4096 x 36 59.2, 44.4; 1501 x 32 28.0, 23.9).
 bool nr_staged(int heads, int ncu) { return (heads + NR_MANY - 1) / NR_MANY <= 2 * ncu; }
 
+template <bool PAGED>
+static void norm_rope_t(const NormRope& a, int total, bool vec, hipStream_t s) {
+    const unsigned many = (unsigned)((total + NR_MANY - 1) / NR_MANY);
+    if (total >= 4 * NR_MANY && vec && a.n == 128 && a.n_rot == 128) {  // the many-heads form: 16-byte chunks, heads of 128
+        if (!nr_staged(total, cu_count())) norm_rope_many_kernel<false, PAGED><<<dim3(many), dim3(64 * NR_WAVES), 0, s>>>(a);
+        else norm_rope_many_kernel<true, PAGED><<<dim3(many), dim3(64 * NR_WAVES), 0, s>>>(a);
+    } else
+        norm_rope_kernel<PAGED><<<dim3((unsigned)((total + NR_WAVES - 1) / NR_WAVES)), dim3(64 * NR_WAVES), 0, s>>>(a);
+}
+
 hipError_t launch_norm_rope(const NormRope& a0, hipStream_t s) {
     const int total = a0.qrows + a0.rows;
     if (total <= 0) return hipSuccess;
@@ -264,12 +297,8 @@ hipError_t launch_norm_rope(const NormRope& a0, hipStream_t s) {
     for (int i = 0; i < a.nfreq; i++) a.freq[i] = std::pow((double)a.base, -2.0 * (double)i / (double)a.n_rot);
     const bool vec = ((uintptr_t)a.qx | (uintptr_t)a.x | (uintptr_t)a.v) % 16 == 0 && a.q_stride % 4 == 0 &&
                      a.x_stride % 4 == 0 && a.q_tstride % 4 == 0 && a.x_tstride % 4 == 0 && a.v_tstride % 4 == 0;
-    const unsigned many = (unsigned)((total + NR_MANY - 1) / NR_MANY);
-    if (total >= 4 * NR_MANY && vec && a.n == 128 && a.n_rot == 128) {  // the many-heads form: 16-byte chunks, heads of 128
-        if (!nr_staged(total, cu_count())) norm_rope_many_kernel<false><<<dim3(many), dim3(64 * NR_WAVES), 0, s>>>(a);
-        else norm_rope_many_kernel<true><<<dim3(many), dim3(64 * NR_WAVES), 0, s>>>(a);
-    } else
-        norm_rope_kernel<<<dim3((unsigned)((total + NR_WAVES - 1) / NR_WAVES)), dim3(64 * NR_WAVES), 0, s>>>(a);
+    if (a.pos) norm_rope_t<true>(a, total, vec, s);
+    else norm_rope_t<false>(a, total, vec, s);
     return hipGetLastError();
 }
 
@@ -301,25 +330,7 @@ hipError_t launch_kv_store(const float* k, const float* v, uint16_t* kc, uint16_
 }
 
 // ---- argmax ----
-// ops::argmax's order (src/ops.rs:110-112): the largest value under f32::total_cmp, the first index on ties. A value
-// and its index pack into one 64-bit key whose unsigned maximum is that choice: the total-order image of the bits
-// above, ~index below.
 constexpr int AMAX_PARTS = 64;
-
-__device__ __forceinline__ uint64_t amax_key(float v, int i) {
-    const int32_t b = __float_as_int(v);
-    const uint32_t u = (uint32_t)(b ^ (int32_t)((uint32_t)(b >> 31) >> 1)) ^ 0x80000000u;
-    return ((uint64_t)u << 32) | (uint32_t)(0xFFFFFFFFu - (uint32_t)i);
-}
-__device__ __forceinline__ uint64_t wave_max_u64(uint64_t k) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-        const uint32_t lo = __shfl_xor((uint32_t)k, o, 64), hi = __shfl_xor((uint32_t)(k >> 32), o, 64);
-        const uint64_t other = ((uint64_t)hi << 32) | lo;
-        k = other > k ? other : k;
-    }
-    return k;
-}
 
 __global__ __launch_bounds__(256) void argmax_part_kernel(const float* x, int n, uint64_t* part) {
     __shared__ uint64_t sk[4];

@@ -1,0 +1,335 @@
+// Serving a batch of sequences: the step of the page tables (strata_kv_pages_step) and the processing of logits before the
+// choice of a token (strata_logits_process). Neither has a counterpart in the reference's Backend trait, which serves one
+// sequence with a contiguous cache and samples on the host.
+#include "serve.h"
+
+#include <algorithm>
+
+#include "argmax_key.h"
+#include "xlane.h"
+
+namespace strata {
+
+// ---------------- page tables and slot maps ----------------
+// From the sequences' cached lengths and new tokens, all integers:
+//   have[s] = ceil(len / page) pages held, need[s] = ceil((len + add) / page) - have[s] pages wanted;
+//   sequences that end (add < 0) push their pages on the stack of free pages in (sequence, page) order;
+//   off = exclusive prefix sum of need: page j of sequence s's new ones is the (off + j)-th from the stack's top;
+//   q_start = prefix sum of the new tokens, token t at own index i = len + t - q_start[s]: slot = page(i) * page + i % page.
+// Sums saturate at SAT (2^30), beyond every limit they are compared with, so no count overflows. One block of 1024 threads:
+// a thread sums 4 consecutive sequences, the waves' totals meet in LDS, and the tokens find their sequence by a binary search
+// of q_start in LDS. Bound by latency (two rounds of loads and three barriers of scans): 8 sequences, one token each 6.6 us, 512
+// with 8192 new tokens 11.6.
+// More than PAGES_ONE tokens take a second launch over many blocks that searches q_start in memory.
+constexpr int PAGES_ONE = 4096;
+constexpr unsigned SAT = 1u << 30;
+__device__ __forceinline__ unsigned sat_add(unsigned a, unsigned b) { return min(a + b, SAT); }  // a, b <= SAT
+
+// Exclusive saturating prefix sum of 4 values a thread over a block of 1024 threads; the total to every thread. ws: 17 words.
+__device__ __forceinline__ unsigned scan4(const unsigned (&v)[4], unsigned (&ex)[4], unsigned* ws) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const unsigned mine = sat_add(sat_add(v[0], v[1]), sat_add(v[2], v[3]));
+    unsigned inc = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const unsigned u = __shfl_up(inc, o, 64);
+        if (lane >= o) inc = sat_add(inc, u);
+    }
+    unsigned before = __shfl_up(inc, 1, 64);
+    if (lane == 0) before = 0;
+    __syncthreads();  // (ws is free: its readers of the scan before are done)
+    if (lane == 63) ws[wave] = inc;
+    __syncthreads();
+    unsigned base = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < 16; w++) {
+        const unsigned u = ws[w];
+        if (w < wave) base = sat_add(base, u);
+        total = sat_add(total, u);
+    }
+    base = sat_add(base, before);
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        ex[k] = base;
+        base = sat_add(base, v[k]);
+    }
+    return total;
+}
+
+// The last i in 0 .. n - 1 with a[i] <= v (a[0] <= v, a not decreasing).
+template <typename P>
+__device__ __forceinline__ int last_le(P a, int n, int v) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a[mid] <= v) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Token t of sequence s: its position and slot, and the table entry of a page that it opens. len: the cached tokens before
+// this step; refused: the sequence gets nothing.
+__device__ __forceinline__ void place_token(const PagesStep& a, int t, int s, int start, int len, bool refused, int off, int top, int P) {
+    const long long i = (long long)len + (t - start);
+    a.pos[t] = (int)min(P + i, (long long)INT32_MAX);
+    int slot = -1;
+    if (!refused) {
+        const int page = 1 << a.page_shift, have = (int)(((long long)len + page - 1) >> a.page_shift), pi = (int)(i >> a.page_shift);
+        int* cell = a.tables + (uint64_t)s * a.max_pages + pi;
+        int pg;
+        if (pi >= have) {
+            pg = a.free_pages[top - 1 - (off + pi - have)];
+            if ((i & (page - 1)) == 0) *cell = pg;
+        } else {
+            pg = *cell;
+        }
+        if (pg >= 0 && pg < a.n_pages) slot = (pg << a.page_shift) + (int)(i & (page - 1));
+    }
+    a.slots[t] = slot;
+}
+
+// st[s]: the cached length before the step, or ~length of a refused sequence.
+template <bool ONE>
+__global__ __launch_bounds__(1024) void pages_plan_kernel(PagesStep a) {
+    __shared__ int qs[SERVE_MAX_SEQ], po[SERVE_MAX_SEQ], st[SERVE_MAX_SEQ];
+    __shared__ unsigned ws[17];
+    const int tid = threadIdx.x, page = 1 << a.page_shift;
+    const int limit = (int)min((long long)a.max_pages << a.page_shift, (long long)INT32_MAX);
+    int add[4], len[4];
+    unsigned v[4], ex[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const int s = 4 * tid + k;
+        add[k] = s < a.nseq ? a.add[s] : 0;
+        len[k] = s < a.nseq ? a.len[s] : 0;
+        v[k] = add[k] < 0 && len[k] > 0 ? (unsigned)((min(len[k], limit) + (long long)page - 1) >> a.page_shift) : 0u;
+    }
+    const int held = min(max(*a.n_free, 0), a.n_pages), P = a.prefix_len ? *a.prefix_len : 0;
+    // sequences that end: their pages on the stack, entry i by thread i
+    const unsigned back = scan4(v, ex, ws);
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+        if (4 * tid + k < a.nseq) po[4 * tid + k] = (int)ex[k];
+    __syncthreads();
+    const int top = min(held + (int)back, a.n_pages);
+    for (int i = tid; i < top - held; i += 1024) {
+        const int s = last_le(po, a.nseq, i);
+        a.free_pages[held + i] = a.tables[(uint64_t)s * a.max_pages + (i - po[s])];
+    }
+    // new tokens, then the pages that they need
+    unsigned start[4];
+    bool bad[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) v[k] = add[k] > 0 ? min((unsigned)add[k], SAT) : 0u;
+    const unsigned total = scan4(v, start, ws);
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const long long end = (long long)len[k] + add[k];
+        bad[k] = add[k] > 0 && (len[k] < 0 || end > limit || sat_add(start[k], v[k]) > (unsigned)a.t_max);
+        v[k] = add[k] > 0 && !bad[k] ? (unsigned)(((end + page - 1) >> a.page_shift) - (((long long)len[k] + page - 1) >> a.page_shift)) : 0u;
+    }
+    scan4(v, ex, ws);  // (its barriers: the pushed pages are written, po has been read)
+    int refused = back > (unsigned)(a.n_pages - held) ? 1 : 0;
+    refused = tid ? 0 : refused;  // (a stack that overflows counts once)
+    unsigned used = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const int s = 4 * tid + k;
+        if (v[k] && sat_add(ex[k], v[k]) > (unsigned)top) bad[k] = true;
+        if (!bad[k] && v[k]) used = ex[k] + v[k];  // (the sequences that get pages come before all that do not)
+        refused += bad[k];
+        if (s < a.nseq) {
+            qs[s] = (int)min(start[k], (unsigned)a.t_max);
+            po[s] = (int)ex[k];
+            st[s] = bad[k] ? ~max(len[k], 0) : max(len[k], 0);
+            a.q_start[s] = qs[s];
+            a.len_out[s] = add[k] < 0 ? 0 : bad[k] || add[k] == 0 ? len[k] : len[k] + add[k];
+            if constexpr (!ONE) {
+                a.scratch[4 + s] = po[s];
+                a.scratch[4 + SERVE_MAX_SEQ + s] = st[s];
+            }
+        }
+    }
+    // the pages taken (the largest `used`) and the sequences refused, over the block
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        used = max(used, (unsigned)__shfl_xor((int)used, o, 64));
+        refused += __shfl_xor(refused, o, 64);
+    }
+    __shared__ unsigned us[16];
+    __shared__ int rs[16];
+    if ((tid & 63) == 0) {
+        us[tid >> 6] = used;
+        rs[tid >> 6] = refused;
+    }
+    __syncthreads();
+    const int rows = (int)min(total, (unsigned)a.t_max);
+    if (tid == 0) {
+        for (int w = 1; w < 16; w++) {
+            used = max(used, us[w]);
+            refused += rs[w];
+        }
+        a.q_start[a.nseq] = rows;
+        *a.n_free_out = top - (int)used;
+        if (a.err && refused) *a.err += refused;
+        if constexpr (!ONE) {
+            a.scratch[0] = rows;
+            a.scratch[1] = top;
+            a.scratch[2] = P;
+        }
+    }
+    if constexpr (ONE) {
+        for (int t = tid; t < a.t_max; t += 1024) {
+            if (t < rows) {
+                const int s = last_le(qs, a.nseq, t), f = st[s];
+                place_token(a, t, s, qs[s], f < 0 ? ~f : f, f < 0, po[s], top, P);
+            } else {
+                a.pos[t] = a.slots[t] = -1;
+            }
+        }
+    }
+}
+
+__global__ __launch_bounds__(256) void pages_place_kernel(PagesStep a) {
+    const int t = blockIdx.x * 256 + threadIdx.x;
+    if (t >= a.t_max) return;
+    if (t < a.scratch[0]) {
+        const int s = last_le(a.q_start, a.nseq, t), f = a.scratch[4 + SERVE_MAX_SEQ + s];
+        place_token(a, t, s, a.q_start[s], f < 0 ? ~f : f, f < 0, a.scratch[4 + s], a.scratch[1], a.scratch[2]);
+    } else {
+        a.pos[t] = a.slots[t] = -1;
+    }
+}
+
+size_t pages_scratch_bytes(int) { return (4 + 2 * SERVE_MAX_SEQ) * sizeof(int); }
+
+hipError_t launch_pages_step(const PagesStep& a, hipStream_t s) {
+    if (a.t_max <= PAGES_ONE) {
+        pages_plan_kernel<true><<<dim3(1), dim3(1024), 0, s>>>(a);
+    } else {
+        pages_plan_kernel<false><<<dim3(1), dim3(1024), 0, s>>>(a);
+        pages_place_kernel<<<dim3((unsigned)((a.t_max + 255) / 256)), dim3(256), 0, s>>>(a);
+    }
+    return hipGetLastError();
+}
+
+// ---------------- penalties, biases and masks on logits ----------------
+// For token v of a row, with c its count among the history's tokens at index >= from and seen whether the history (its last
+// `last` tokens) holds it:
+//   y = x; seen: y = y > 0 ? y / rep : y * rep; y = y - freq * c; c > 0: y = y - pres; y = y + bias; not allowed: -inf
+// one rounding a step, in this order. A block takes LP_CHUNK tokens of a row: it counts the history's tokens of its chunk and
+// marks the biases in LDS (integer atomics, so the order does not matter; of a token's biases the largest index counts), then
+// passes once over its logits. Bound by the logits' bytes for many rows (64 rows of 151936 from x into out 60 us, 1.3 TB/s), by
+// latency for one (10 us). Every block of a row reads the row's history again, from L2.
+constexpr int LP_CHUNK = 4096, LP_T = 256;
+constexpr uint32_t LP_SEEN = 0x80000000u;
+
+__global__ __launch_bounds__(LP_T) void logits_process_kernel(LogitsProcess a) {
+    __shared__ uint32_t cnt[LP_CHUNK], bix[LP_CHUNK];
+    __shared__ uint64_t sk[LP_T / 64];
+    const int r = blockIdx.y, base = blockIdx.x * LP_CHUNK, tid = threadIdx.x, m = min(LP_CHUNK, a.n - base);
+    const float* x = a.x + (uint64_t)r * a.x_stride + base;
+    float* out = a.out + (uint64_t)r * a.out_stride + base;
+    int h0 = 0, h1 = 0, from = 0, b0 = 0, b1 = 0;
+    float rep = 1.0f, freq = 0.0f, pres = 0.0f;
+    if (a.pen) {
+        h1 = (int)min((uint64_t)max(a.hist_len[r], 0), a.hist_stride);
+        h0 = a.last > 0 ? max(h1 - a.last, 0) : 0;
+        from = a.hist_from ? a.hist_from[r] : 0;
+        rep = a.pen[3 * r];
+        freq = a.pen[3 * r + 1];
+        pres = a.pen[3 * r + 2];
+    }
+    if (a.bias_start) {
+        b0 = min(max(a.bias_start[r], 0), a.n_bias);
+        b1 = min(max(a.bias_start[r + 1], b0), a.n_bias);
+    }
+    const bool pen = h1 > h0, bias = b1 > b0;
+    if (pen)
+        for (int i = tid; i < m; i += LP_T) cnt[i] = 0;
+    if (bias)
+        for (int i = tid; i < m; i += LP_T) bix[i] = 0;
+    if (pen || bias) __syncthreads();
+    if (pen) {
+        const int* hr = a.hist + (uint64_t)r * a.hist_stride;
+        for (int i = h0 + tid; i < h1; i += LP_T) {
+            const unsigned v = (unsigned)hr[i] - (unsigned)base;
+            if (v < (unsigned)m) {
+                if (i >= from) atomicAdd(&cnt[v], 1u);
+                else atomicOr(&cnt[v], LP_SEEN);
+            }
+        }
+    }
+    if (bias)
+        for (int e = b0 + tid; e < b1; e += LP_T) {
+            const unsigned v = (unsigned)a.bias_ids[e] - (unsigned)base;
+            if (v < (unsigned)m) atomicMax(&bix[v], (uint32_t)(e + 1));
+        }
+    if (pen || bias) __syncthreads();
+    const uint32_t* mask = a.mask ? a.mask + (uint64_t)r * a.mask_stride : nullptr;
+    const bool place = x == out;
+    uint64_t best = 0;
+    for (int i = tid; i < m; i += LP_T) {
+        const float x0 = x[i];
+        float y = x0;
+        if (pen) {
+            const uint32_t c = cnt[i], k = c & ~LP_SEEN;
+            if (c) y = y > 0.0f ? y / rep : y * rep;
+            if (k) {
+                y = y - freq * (float)k;
+                y = y - pres;
+            }
+        }
+        if (bias && bix[i]) y = y + a.bias_vals[bix[i] - 1];
+        const bool ok = !mask || ((mask[(base + i) >> 5] >> ((base + i) & 31)) & 1u);
+        if (!ok) y = -INFINITY;
+        if (!place || __float_as_uint(y) != __float_as_uint(x0)) out[i] = y;
+        if (ok) {
+            const uint64_t k = amax_key(y, base + i);
+            best = k > best ? k : best;
+        }
+    }
+    if (!a.ids) return;
+    best = wave_max_u64(best);
+    if ((tid & 63) == 0) sk[tid >> 6] = best;
+    __syncthreads();
+    if (tid == 0) {
+        for (int w = 1; w < LP_T / 64; w++) best = sk[w] > best ? sk[w] : best;
+        a.keys[(uint64_t)r * gridDim.x + blockIdx.x] = best;
+    }
+}
+
+// A row's choice from its chunks' keys (a key is 0 only where no token of the chunk is allowed), and the history's next token.
+__global__ __launch_bounds__(64) void logits_choose_kernel(LogitsProcess a, int parts) {
+    const int r = blockIdx.x, lane = threadIdx.x;
+    uint64_t best = 0;
+    for (int i = lane; i < parts; i += 64) {
+        const uint64_t k = a.keys[(uint64_t)r * parts + i];
+        best = k > best ? k : best;
+    }
+    best = wave_max_u64(best);
+    if (lane == 0) {
+        const int id = best ? (int)(0xFFFFFFFFu - (uint32_t)best) : -1;
+        a.ids[r] = id;
+        if (a.append && id >= 0) {
+            const int k = a.hist_len[r];
+            if (k >= 0 && (uint64_t)k < a.hist_stride) {
+                a.hist[(uint64_t)r * a.hist_stride + k] = id;
+                a.hist_len[r] = k + 1;
+            }
+        }
+    }
+}
+
+static int logits_parts(int n) { return (n + LP_CHUNK - 1) / LP_CHUNK; }
+size_t logits_key_bytes(int n, int rows) { return (size_t)rows * logits_parts(n) * sizeof(uint64_t); }
+
+hipError_t launch_logits_process(const LogitsProcess& a, hipStream_t s) {
+    const int parts = logits_parts(a.n);
+    logits_process_kernel<<<dim3((unsigned)parts, (unsigned)a.rows), dim3(LP_T), 0, s>>>(a);
+    if (a.ids) logits_choose_kernel<<<dim3((unsigned)a.rows), dim3(64), 0, s>>>(a, parts);
+    return hipGetLastError();
+}
+
+}  // namespace strata
