@@ -164,7 +164,7 @@ __global__ __launch_bounds__(64 * NR_WAVES) void norm_rope_kernel(NormRope a) {
 // norm_rope_kernel's, so both kernels give the same bits. STAGED: the value rows of stored key heads are requested with
 // the heads and wait in LDS (66 KB a block, two a CU), else they are read where they are stored (33 KB, four a CU).
 constexpr int NR_MANY = 64, NR_P = 129;  // heads a block; LDS pitch of a staged head (bank spread for the sums)
-template <bool STAGED, bool PAGED>
+template <bool STAGED>
 __global__ __launch_bounds__(64 * NR_WAVES) void norm_rope_many_kernel(NormRope a) {
     __shared__ float xs[NR_MANY][NR_P], vs[STAGED ? NR_MANY : 1][NR_P];
     __shared__ float ssq[NR_MANY];
@@ -214,15 +214,7 @@ __global__ __launch_bounds__(64 * NR_WAVES) void norm_rope_many_kernel(NormRope 
         const int j = (NR_MANY / NR_WAVES) * wave + jj, g = g0 + j;
         if (g >= total) break;
         const NrHead h = nr_head(a, g);
-        const int pos = PAGED ? a.pos[h.b / h.per] : a.step[0] + h.b / h.per;
-        int row = pos;  // the token's cache row
-        if constexpr (PAGED) {
-            if (pos < 0) continue;
-            if (h.vr) {
-                row = a.slots[h.b / h.per];
-                if (row < 0 || (uint64_t)row >= a.n_slots) continue;
-            }
-        }
+        const int pos = a.step[0] + h.b / h.per;
         if (pos != cur) {
             cur = pos;
             const double f = lane < a.nfreq ? a.freq[lane] : pow((double)a.base, -2.0 * (double)lane / 128.0);
@@ -235,17 +227,97 @@ __global__ __launch_bounds__(64 * NR_WAVES) void norm_rope_many_kernel(NormRope 
         const float sc = 1.0f / sqrtf(ssq[j] / 128.0f + a.eps);
         const float p = xs[j][lane] * sc * (q ? qw0 : kw0), r = xs[j][lane + 64] * sc * (q ? qw1 : kw1);
         const float o0 = p * cs - r * sn, o1 = p * sn + r * cs;
-        if (!PAGED || !h.vr) {
-            h.o[lane] = o0;
-            h.o[lane + 64] = o1;
-        }
+        h.o[lane] = o0;
+        h.o[lane + 64] = o1;
         if (h.vr) {
-            const uint64_t e = ((uint64_t)row * h.per + h.b % h.per) * 128;
+            const uint64_t e = ((uint64_t)pos * h.per + h.b % h.per) * 128;
             a.kc[e + lane] = f32_to_f16_bits(o0);
             a.kc[e + lane + 64] = f32_to_f16_bits(o1);
             const float* vr = STAGED ? vs[j] : h.vr;
             a.vc[e + lane] = f32_to_f16_bits(vr[lane]);
             a.vc[e + lane + 64] = f32_to_f16_bits(vr[lane + 64]);
+        }
+    }
+}
+
+// A token's heads over a paged cache (rms_norm_rope_qk_paged), N = 64 or 128 values: block (token, group of hb heads) stages
+// the heads in LDS; wave 0 sums their squares a lane a head (norm_rope_kernel's order: the same bits) while wave 1 computes the
+// token's angles, once for all heads; then each wave (N = 64: each half of one) takes a head at a time, two values a lane: a
+// rope pair (i, i + n_rot / 2), or two values behind n_rot. Values go from memory to the cache without a stop. Bound by its
+// bytes for many tokens (4096 of 36 heads: X us, X TB/s), by one block's chain for few (X us).
+constexpr int NR_HB = 40;  // heads a block at most (21 KB, seven blocks a CU)
+template <int N>
+__global__ __launch_bounds__(64 * NR_WAVES) void norm_rope_paged_kernel(NormRope a, int hb) {
+    constexpr int PT = N + 4, T = 64 * NR_WAVES, LPH = N / 2, HPW = 64 / LPH;  // pitch (spreads the sums' 16-byte reads); lanes a head
+    constexpr int NX = (NR_HB * N / 4 + T - 1) / T;  // 16-byte chunks a thread
+    __shared__ __align__(16) float xs[NR_HB * PT];
+    __shared__ float ssc[NR_HB], rsn[N / 2], rcs[N / 2];
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, tok = blockIdx.x, h0 = blockIdx.y * hb;
+    const int H = a.qper + a.per, nb = min(hb, H - h0), half = a.n_rot / 2;
+    const int pos = sload(a.pos + tok), slot = sload(a.slots + tok);
+    if (pos < 0) return;
+    const bool store = slot >= 0 && (uint64_t)slot < a.n_slots;
+    const float* xq = a.qx + (uint64_t)tok * a.q_tstride;
+    const float* xk = a.x + (uint64_t)tok * a.x_tstride;
+    // every load first: the heads' chunks (past the last the last again), and the value rows of this group's key heads
+    typedef float f4v __attribute__((ext_vector_type(4)));
+    f4v x[NX], v[NX];
+#pragma unroll
+    for (int u = 0; u < NX; u++) {
+        const int c = min(tid + T * u, nb * (N / 4) - 1), h = h0 + c / (N / 4), i = 4 * (c % (N / 4));
+        x[u] = *(const f4v*)((h < a.qper ? xq + (uint64_t)h * a.q_stride : xk + (uint64_t)(h - a.qper) * N) + i);
+    }
+    const int k0 = max(h0 - a.qper, 0), nv = store ? (max(h0 + nb - a.qper, 0) - k0) * (N / 4) : 0;  // chunks of value rows
+    const uint64_t row = (uint64_t)(store ? slot : 0) * a.per * N;
+    const float* xv = a.v + (uint64_t)tok * a.v_tstride + (uint64_t)k0 * N;
+#pragma unroll
+    for (int u = 0; u < NX; u++)
+        if (T * u < nv) v[u] = *(const f4v*)(xv + 4 * min(tid + T * u, nv - 1));
+    // this lane's two values of a head: a rope pair, or two values behind n_rot
+    const int l = lane % LPH, ea = l < half ? l : 2 * l, eb = l < half ? l + half : 2 * l + 1;
+    const float qw0 = a.qw[ea], qw1 = a.qw[eb], kw0 = a.w[ea], kw1 = a.w[eb];
+#pragma unroll
+    for (int u = 0; u < NX; u++) {
+        const int c = tid + T * u;
+        if (c < nb * (N / 4)) *(f4v*)&xs[c / (N / 4) * PT + 4 * (c % (N / 4))] = x[u];
+    }
+#pragma unroll
+    for (int u = 0; u < NX; u++)
+        if (tid + T * u < nv) {
+            const uint32_t lo = f32_to_f16_bits(v[u][0]) | ((uint32_t)f32_to_f16_bits(v[u][1]) << 16);
+            const uint32_t hi = f32_to_f16_bits(v[u][2]) | ((uint32_t)f32_to_f16_bits(v[u][3]) << 16);
+            *(uint2*)(a.vc + row + (uint64_t)k0 * N + 4 * (tid + T * u)) = make_uint2(lo, hi);
+        }
+    __syncthreads();
+    if (wave == 0 && lane < nb) {
+        const float ss = nr_sumsq(N, [&](int i0, float4 (&r)[8]) {
+#pragma unroll
+            for (int c = 0; c < 8; c++) r[c] = *(const float4*)&xs[lane * PT + i0 + 4 * c];
+        });
+        ssc[lane] = 1.0f / sqrtf(ss / (float)N + a.eps);
+    }
+    if (wave == 1 && lane < half) {
+        const double f = lane < a.nfreq ? a.freq[lane] : pow((double)a.base, -2.0 * (double)lane / (double)a.n_rot);
+        double sd, cd;
+        sincos((double)pos * f, &sd, &cd);
+        rsn[lane] = (float)sd;
+        rcs[lane] = (float)cd;
+    }
+    __syncthreads();
+    const float sn = l < half ? rsn[l] : 0.0f, cs = l < half ? rcs[l] : 1.0f;
+    for (int j = wave * HPW + lane / LPH; j < nb; j += NR_WAVES * HPW) {
+        const int h = h0 + j;
+        const bool q = h < a.qper;
+        const float sc = ssc[j], p = xs[j * PT + ea] * sc * (q ? qw0 : kw0), r = xs[j * PT + eb] * sc * (q ? qw1 : kw1);
+        const float o0 = l < half ? p * cs - r * sn : p, o1 = l < half ? p * sn + r * cs : r;
+        if (q) {
+            float* o = a.qo + ((uint64_t)tok * a.qper + h) * N;
+            o[ea] = o0;
+            o[eb] = o1;
+        } else if (store) {
+            uint16_t* o = a.kc + row + (uint64_t)(h - a.qper) * N;
+            o[ea] = f32_to_f16_bits(o0);
+            o[eb] = f32_to_f16_bits(o1);
         }
     }
 }
@@ -274,16 +346,6 @@ __global__ __launch_bounds__(64 * NR_WAVES) void rope_pairs_kernel(float* x, uin
 // four a CU are faster (1501 x 36 29.0 staged, 26.5 not, 4096 x 36 59.2, 44.4; 1501 x 32 28.0, 23.9).
 bool nr_staged(int heads, int ncu) { return (heads + NR_MANY - 1) / NR_MANY <= 2 * ncu; }
 
-template <bool PAGED>
-static void norm_rope_t(const NormRope& a, int total, bool vec, hipStream_t s) {
-    const unsigned many = (unsigned)((total + NR_MANY - 1) / NR_MANY);
-    if (total >= 4 * NR_MANY && vec && a.n == 128 && a.n_rot == 128) {  // the many-heads form: 16-byte chunks, heads of 128
-        if (!nr_staged(total, cu_count())) norm_rope_many_kernel<false, PAGED><<<dim3(many), dim3(64 * NR_WAVES), 0, s>>>(a);
-        else norm_rope_many_kernel<true, PAGED><<<dim3(many), dim3(64 * NR_WAVES), 0, s>>>(a);
-    } else
-        norm_rope_kernel<PAGED><<<dim3((unsigned)((total + NR_WAVES - 1) / NR_WAVES)), dim3(64 * NR_WAVES), 0, s>>>(a);
-}
-
 hipError_t launch_norm_rope(const NormRope& a0, hipStream_t s) {
     const int total = a0.qrows + a0.rows;
     if (total <= 0) return hipSuccess;
@@ -297,8 +359,20 @@ hipError_t launch_norm_rope(const NormRope& a0, hipStream_t s) {
     for (int i = 0; i < a.nfreq; i++) a.freq[i] = std::pow((double)a.base, -2.0 * (double)i / (double)a.n_rot);
     const bool vec = ((uintptr_t)a.qx | (uintptr_t)a.x | (uintptr_t)a.v) % 16 == 0 && a.q_stride % 4 == 0 &&
                      a.x_stride % 4 == 0 && a.q_tstride % 4 == 0 && a.x_tstride % 4 == 0 && a.v_tstride % 4 == 0;
-    if (a.pos) norm_rope_t<true>(a, total, vec, s);
-    else norm_rope_t<false>(a, total, vec, s);
+    const unsigned many = (unsigned)((total + NR_MANY - 1) / NR_MANY), few = (unsigned)((total + NR_WAVES - 1) / NR_WAVES);
+    if (a.pos) {
+        if (vec && (uintptr_t)a.vc % 8 == 0 && (a.n == 64 || a.n == 128)) {
+            const int H = a.qper + a.per, groups = (H + NR_HB - 1) / NR_HB, hb = (H + groups - 1) / groups;
+            const dim3 grid((unsigned)(a.rows / a.per), (unsigned)groups);
+            if (a.n == 128) norm_rope_paged_kernel<128><<<grid, dim3(64 * NR_WAVES), 0, s>>>(a, hb);
+            else norm_rope_paged_kernel<64><<<grid, dim3(64 * NR_WAVES), 0, s>>>(a, hb);
+        } else
+            norm_rope_kernel<true><<<dim3(few), dim3(64 * NR_WAVES), 0, s>>>(a);
+    } else if (total >= 4 * NR_MANY && vec && a.n == 128 && a.n_rot == 128) {  // the many-heads form: 16-byte chunks, heads of 128
+        if (!nr_staged(total, cu_count())) norm_rope_many_kernel<false><<<dim3(many), dim3(64 * NR_WAVES), 0, s>>>(a);
+        else norm_rope_many_kernel<true><<<dim3(many), dim3(64 * NR_WAVES), 0, s>>>(a);
+    } else
+        norm_rope_kernel<false><<<dim3(few), dim3(64 * NR_WAVES), 0, s>>>(a);
     return hipGetLastError();
 }
 

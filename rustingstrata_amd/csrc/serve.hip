@@ -222,15 +222,44 @@ hipError_t launch_pages_step(const PagesStep& a, hipStream_t s) {
 // marks the biases in LDS (integer atomics, so the order does not matter; of a token's biases the largest index counts), then
 // passes once over its logits. Bound by the logits' bytes for many rows (64 rows of 151936 from x into out 60 us, 1.3 TB/s), by
 // latency for one (10 us). Every block of a row reads the row's history again, from L2.
-constexpr int LP_CHUNK = 4096, LP_T = 256;
+constexpr int LP_T = 256;
 constexpr uint32_t LP_SEEN = 0x80000000u;
 
+// NU: tokens a thread / 4. VEC: rows that are 16-byte aligned in x and out, 4 consecutive tokens a load; else a token a load.
+template <int NU, bool VEC>
 __global__ __launch_bounds__(LP_T) void logits_process_kernel(LogitsProcess a) {
-    __shared__ uint32_t cnt[LP_CHUNK], bix[LP_CHUNK];
+    constexpr int CHUNK = 4 * NU * LP_T;
+    __shared__ __align__(16) uint32_t cnt[CHUNK], bix[CHUNK];
     __shared__ uint64_t sk[LP_T / 64];
-    const int r = blockIdx.y, base = blockIdx.x * LP_CHUNK, tid = threadIdx.x, m = min(LP_CHUNK, a.n - base);
+    const int r = blockIdx.y, base = blockIdx.x * CHUNK, tid = threadIdx.x, m = min(CHUNK, a.n - base);
     const float* x = a.x + (uint64_t)r * a.x_stride + base;
     float* out = a.out + (uint64_t)r * a.out_stride + base;
+    // this thread's tokens: at(u, e) of the chunk
+    auto at = [&](int u, int e) { return VEC ? 4 * (u * LP_T + tid) + e : (4 * u + e) * LP_T + tid; };
+    float y[NU][4];
+    uint32_t mw[NU][VEC ? 1 : 4];
+    const uint32_t* mask = a.mask ? a.mask + (uint64_t)r * a.mask_stride : nullptr;
+#pragma unroll
+    for (int u = 0; u < NU; u++) {
+        if constexpr (VEC) {
+            const int i = at(u, 0);
+            if (i + 4 <= m) {
+                const float4 v = *(const float4*)(x + i);
+                y[u][0] = v.x; y[u][1] = v.y; y[u][2] = v.z; y[u][3] = v.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[u][e] = i + e < m ? x[i + e] : 0.0f;
+            }
+            mw[u][0] = mask && i < m ? mask[(base + i) >> 5] >> ((base + i) & 31) : 0xFu;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int i = at(u, e);
+                y[u][e] = i < m ? x[i] : 0.0f;
+                mw[u][e] = mask && i < m ? mask[(base + i) >> 5] >> ((base + i) & 31) : 1u;
+            }
+        }
+    }
     int h0 = 0, h1 = 0, from = 0, b0 = 0, b1 = 0;
     float rep = 1.0f, freq = 0.0f, pres = 0.0f;
     if (a.pen) {
@@ -245,19 +274,30 @@ __global__ __launch_bounds__(LP_T) void logits_process_kernel(LogitsProcess a) {
         b0 = min(max(a.bias_start[r], 0), a.n_bias);
         b1 = min(max(a.bias_start[r + 1], b0), a.n_bias);
     }
+    if (a.pen) {
+#pragma unroll
+        for (int u = 0; u < NU; u++) *(uint4*)&cnt[4 * (u * LP_T + tid)] = make_uint4(0, 0, 0, 0);
+    }
+    if (a.bias_start) {
+#pragma unroll
+        for (int u = 0; u < NU; u++) *(uint4*)&bix[4 * (u * LP_T + tid)] = make_uint4(0, 0, 0, 0);
+    }
     const bool pen = h1 > h0, bias = b1 > b0;
-    if (pen)
-        for (int i = tid; i < m; i += LP_T) cnt[i] = 0;
-    if (bias)
-        for (int i = tid; i < m; i += LP_T) bix[i] = 0;
     if (pen || bias) __syncthreads();
     if (pen) {
         const int* hr = a.hist + (uint64_t)r * a.hist_stride;
-        for (int i = h0 + tid; i < h1; i += LP_T) {
-            const unsigned v = (unsigned)hr[i] - (unsigned)base;
-            if (v < (unsigned)m) {
-                if (i >= from) atomicAdd(&cnt[v], 1u);
-                else atomicOr(&cnt[v], LP_SEEN);
+        constexpr int HU = 8;  // history loads in flight
+        for (int i0 = h0 + tid; i0 < h1; i0 += HU * LP_T) {
+            int tok[HU];
+#pragma unroll
+            for (int k = 0; k < HU; k++) tok[k] = i0 + k * LP_T < h1 ? hr[i0 + k * LP_T] : -1;
+#pragma unroll
+            for (int k = 0; k < HU; k++) {
+                const unsigned v = (unsigned)tok[k] - (unsigned)base;
+                if (v < (unsigned)m) {  // (no id below 0: base + m is at most 2^31 - 1)
+                    if (i0 + k * LP_T >= from) atomicAdd(&cnt[v], 1u);
+                    else atomicOr(&cnt[v], LP_SEEN);
+                }
             }
         }
     }
@@ -267,27 +307,48 @@ __global__ __launch_bounds__(LP_T) void logits_process_kernel(LogitsProcess a) {
             if (v < (unsigned)m) atomicMax(&bix[v], (uint32_t)(e + 1));
         }
     if (pen || bias) __syncthreads();
-    const uint32_t* mask = a.mask ? a.mask + (uint64_t)r * a.mask_stride : nullptr;
     const bool place = x == out;
     uint64_t best = 0;
-    for (int i = tid; i < m; i += LP_T) {
-        const float x0 = x[i];
-        float y = x0;
-        if (pen) {
-            const uint32_t c = cnt[i], k = c & ~LP_SEEN;
-            if (c) y = y > 0.0f ? y / rep : y * rep;
-            if (k) {
-                y = y - freq * (float)k;
-                y = y - pres;
+#pragma unroll
+    for (int u = 0; u < NU; u++) {
+        uint32_t cv[4] = {}, bv[4] = {};
+        if constexpr (VEC) {
+            if (pen) *(uint4*)cv = *(const uint4*)&cnt[at(u, 0)];
+            if (bias) *(uint4*)bv = *(const uint4*)&bix[at(u, 0)];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (pen) cv[e] = cnt[at(u, e)];
+                if (bias) bv[e] = bix[at(u, e)];
             }
         }
-        if (bias && bix[i]) y = y + a.bias_vals[bix[i] - 1];
-        const bool ok = !mask || ((mask[(base + i) >> 5] >> ((base + i) & 31)) & 1u);
-        if (!ok) y = -INFINITY;
-        if (!place || __float_as_uint(y) != __float_as_uint(x0)) out[i] = y;
-        if (ok) {
-            const uint64_t k = amax_key(y, base + i);
-            best = k > best ? k : best;
+        bool changed = !place;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float x0 = y[u][e];
+            float v = x0;
+            if (cv[e]) v = v > 0.0f ? v / rep : v * rep;
+            const uint32_t k = cv[e] & ~LP_SEEN;
+            if (k) {
+                v = v - freq * (float)k;
+                v = v - pres;
+            }
+            if (bv[e]) v = v + a.bias_vals[bv[e] - 1];
+            const bool ok = VEC ? (mw[u][0] >> e) & 1u : mw[u][VEC ? 0 : e] & 1u;
+            if (!ok) v = -INFINITY;
+            changed |= __float_as_uint(v) != __float_as_uint(x0);
+            y[u][e] = v;
+            if (ok && at(u, e) < m) {
+                const uint64_t key = amax_key(v, base + at(u, e));
+                best = key > best ? key : best;
+            }
+        }
+        if (VEC && at(u, 0) + 4 <= m) {
+            if (changed) *(float4*)(out + at(u, 0)) = make_float4(y[u][0], y[u][1], y[u][2], y[u][3]);
+        } else if (changed) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (at(u, e) < m) out[at(u, e)] = y[u][e];
         }
     }
     if (!a.ids) return;
@@ -322,12 +383,19 @@ __global__ __launch_bounds__(64) void logits_choose_kernel(LogitsProcess a, int 
     }
 }
 
-static int logits_parts(int n) { return (n + LP_CHUNK - 1) / LP_CHUNK; }
-size_t logits_key_bytes(int n, int rows) { return (size_t)rows * logits_parts(n) * sizeof(uint64_t); }
+// Tokens a block: 4096, or 1024 where the larger blocks leave CUs idle.
+static int logits_nu(int n, int rows) { return (long long)rows * ((n + 16 * LP_T - 1) / (16 * LP_T)) >= 512 ? 4 : 1; }
+static int logits_parts(int n, int nu) { return (n + 4 * nu * LP_T - 1) / (4 * nu * LP_T); }
+size_t logits_key_bytes(int n, int rows) { return (size_t)rows * logits_parts(n, logits_nu(n, rows)) * sizeof(uint64_t); }
 
 hipError_t launch_logits_process(const LogitsProcess& a, hipStream_t s) {
-    const int parts = logits_parts(a.n);
-    logits_process_kernel<<<dim3((unsigned)parts, (unsigned)a.rows), dim3(LP_T), 0, s>>>(a);
+    const int nu = logits_nu(a.n, a.rows), parts = logits_parts(a.n, nu);
+    const dim3 grid((unsigned)parts, (unsigned)a.rows);
+    const bool vec = ((uintptr_t)a.x | (uintptr_t)a.out) % 16 == 0 && (a.rows == 1 || (a.x_stride | a.out_stride) % 4 == 0);
+    if (nu == 4 && vec) logits_process_kernel<4, true><<<grid, dim3(LP_T), 0, s>>>(a);
+    else if (nu == 4) logits_process_kernel<4, false><<<grid, dim3(LP_T), 0, s>>>(a);
+    else if (vec) logits_process_kernel<1, true><<<grid, dim3(LP_T), 0, s>>>(a);
+    else logits_process_kernel<1, false><<<grid, dim3(LP_T), 0, s>>>(a);
     if (a.ids) logits_choose_kernel<<<dim3((unsigned)a.rows), dim3(64), 0, s>>>(a, parts);
     return hipGetLastError();
 }

@@ -269,7 +269,8 @@ def test_logits_refused_arguments(hip):
 
 
 # ---------------- q/k norms and rope into pages ----------------
-@pytest.mark.parametrize("t,nh,nkv,hd,n_rot", [(1, 32, 4, 128, 128), (5, 8, 8, 64, 64), (7, 4, 1, 96, 32), (16, 16, 2, 128, 128), (333, 32, 4, 128, 128), (700, 4, 4, 64, 32)])
+@pytest.mark.parametrize("t,nh,nkv,hd,n_rot", [(1, 32, 4, 128, 128), (5, 8, 8, 64, 64), (7, 4, 1, 96, 32), (16, 16, 2, 128, 128), (333, 32, 4, 128, 128), (700, 4, 4, 64, 32),
+                                                 (3, 64, 8, 128, 128), (2, 40, 40, 64, 0), (9, 3, 2, 64, 64)])
 def test_norm_rope_paged(hip, t, nh, nkv, hd, n_rot):
     """The bits of rms_norm_rope_qk_t where tokens sit at consecutive positions; at positions of their own within 2e-6 of
     float64 (an angle's sine is rounded once to float32, the norm sums in float32: at most hd + 6 roundings of 2^-24, on
