@@ -35,25 +35,29 @@ struct PagedWs {
 };
 
 // ---------------- sequences ----------------
+constexpr int DEC_CHUNK = 128;  // 32 keys a wave
 struct SeqInfo {
     int q0, qn;   // query rows
     int len;      // own keys
-    int c0, nc;   // the first chunk of 64 own keys that a row sees, and how many (decode sequences)
+    int c0, nc;   // the first chunk of DEC_CHUNK own keys that a row sees, and how many (decode sequences)
 };
-__device__ __forceinline__ int prefix_len(const PagedAttn& a) { return a.prefix_len ? min(max(*a.prefix_len, 0), a.max_prefix) : 0; }
+__device__ __forceinline__ int prefix_len(const PagedAttn& a) { return a.prefix_len ? min(max(sload(a.prefix_len), 0), a.max_prefix) : 0; }
+// UNI: s is the same in the whole wave (scalar loads, so that what follows from them stays in scalar registers).
+template <bool UNI>
 __device__ __forceinline__ SeqInfo seq_info(const PagedAttn& a, int s, int G, int dr, int P) {
+    auto ld = [](const int* p) { return UNI ? sload(p) : *p; };
     SeqInfo r;
-    r.q0 = min(max(a.q_start[s], 0), a.t);
-    r.qn = min(max(a.q_start[s + 1], r.q0), a.t) - r.q0;
-    r.len = (int)min((long long)max(a.len[s], 0), (long long)a.max_pages << a.page_shift);
+    r.q0 = min(max(ld(a.q_start + s), 0), a.t);
+    r.qn = min(max(ld(a.q_start + s + 1), r.q0), a.t) - r.q0;
+    r.len = (int)min((long long)max(ld(a.len + s), 0), (long long)a.max_pages << a.page_shift);
     r.c0 = r.nc = 0;
     if (r.qn > 0 && r.qn * G <= dr) {
         if (a.win > 0) {
             int first = INT_MAX;  // (a window hides keys before the first row's)
-            for (int i = 0; i < r.qn; i++) first = min(first, a.pos[r.q0 + i]);
-            r.c0 = (int)(max((long long)first + 1 - a.win - P, 0ll) >> 6);
+            for (int i = 0; i < r.qn; i++) first = min(first, ld(a.pos + r.q0 + i));
+            r.c0 = (int)(max((long long)first + 1 - a.win - P, 0ll) / DEC_CHUNK);
         }
-        r.nc = max((int)(((long long)r.len + 63) >> 6) - r.c0, 0);
+        r.nc = max((int)(((long long)r.len + DEC_CHUNK - 1) / DEC_CHUNK) - r.c0, 0);
     }
     return r;
 }
@@ -172,54 +176,165 @@ __device__ __forceinline__ void split_q8(const f4& x0, const f4& x1, float up, h
     }
 }
 
+// The A fragment of V^T for 16 dims a 16-lane group from V rows as they are in memory: each group of 16 lanes reads 4 rows x
+// 16 columns (lane i: row i / 4, columns 4 (i % 4) ..) and lane i gets column i of the 4 rows.
+__device__ __forceinline__ h4 read_tr(const uint16_t* p) {
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p));
+}
+
 // ---------------- few rows a sequence ----------------
-// The work is the list of all (sequence, KV head, chunk of 64 own keys), chunk fastest; a block takes an equal run of it, so
-// contexts of any lengths load the CUs evenly. A run covers pieces of one or more (sequence, KV head) pairs; block b's piece
-// of pair i leaves its softmax sums at slot b + i (along the list either b or i goes up by one, so slots are distinct). The
-// block that holds a pair's first chunk notes which blocks follow.
-// Inside a piece, wave w takes keys 16 w .. 16 w + 15 of each chunk with its own online softmax for all rows (R = 16 NT columns:
-// token c / G, head c % G), as attn_decode_kernel of attn.hip does; the four waves meet in LDS at the piece's end.
+// The work is the list of all (sequence, KV head, chunk of DEC_CHUNK own keys), chunk fastest; a block takes an equal run of
+// it, so contexts of any lengths load the CUs evenly. A run covers pieces of one or more (sequence, KV head) pairs; block b's
+// piece of pair i leaves its softmax sums at slot b + i (along the list either b or i goes up by one, so slots are distinct).
+// The block that holds a pair's first chunk notes which blocks follow.
+// Inside a piece, wave w takes keys 32 w .. 32 w + 31 of each chunk with its own online softmax for all rows (16 NT columns:
+// token c / G, head c % G), on f16 MFMA with f32 accuracy:
+//   S^T (2 tiles of 16 keys x 16 columns) = K Q^T (v_mfma_f32_16x16x32_f16; A: the key rows, read straight from memory in the
+//   fragments' layout, 16 rows x 64 bytes a load; B: q's hi and lo parts);
+//   O^T (16 dims x 16 columns, DT tiles) += V^T P^T (K = 32; B: the lane's own 8 weights, hi and lo; A: V's rows through the
+//   wave's LDS, read transposed).
+// The next chunk's V is requested when this one's has gone to LDS, its K when the scores are done: both fly during the softmax
+// and the V products without more registers. The four waves meet in LDS at the piece's end.
+template <int HD>
+struct PagedDec {
+    static constexpr int VP = HD + 16;             // halves a V row in LDS (32 bytes on: the transposed reads' 16 rows spread)
+    static constexpr int WAVE = 32 * VP * 2;
+    static constexpr int MERGE = DEC_WAVES * (HD * 16 + 32) * 4;
+    static constexpr int BYTES = DEC_WAVES * WAVE > MERGE ? DEC_WAVES * WAVE : MERGE;
+};
 template <int HD, int NT>
-__global__ __launch_bounds__(256) void attn_paged_dec_kernel(PagedAttn a, PagedWs w) {
-    using L = DecLayout<HD>;
-    constexpr int KS = HD / 32, DT = HD / 16, NDG = HD / 8;
-    static_assert(L::BYTES >= SERVE_MAX_SEQ * 4, "the prefix sums use the tiles' LDS");
+__global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attn_paged_dec_kernel(PagedAttn a, PagedWs w) {
+    using L = PagedDec<HD>;
+    typedef unsigned v4u __attribute__((ext_vector_type(4)));
+    constexpr int KS = HD / 32, DT = HD / 16, LPR = HD / 8, RPI = 64 / LPR, NV = 32 / RPI;  // lanes a V row, rows a load, loads
     __shared__ __align__(16) uint8_t lds[L::BYTES];
     __shared__ int ws[8];
+    __shared__ SeqInfo sq;
+    __shared__ int sb[2];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
     const int G = a.nh / a.nkv, P = prefix_len(a), b = blockIdx.x;
-    // this block's run of the list, and where it starts
-    int s, base, W0, W1, share;
+    // this block's run of the list: the thread that holds the sequence of its start says which it is
+    int W0, W1, share;
     {
-        int* cum = (int*)lds;
-        int largest;
-        const int total = scan_seqs(a.nseq, [&](int i) { return seq_info(a, i, G, w.dr, P).nc; }, cum, ws, largest) * a.nkv;
+        const int per = (a.nseq + 255) / 256;
+        SeqInfo mine{};
+        int sum = 0, big = 0;
+        for (int i = 0; i < per; i++)
+            if (tid * per + i < a.nseq) {
+                mine = seq_info<false>(a, tid * per + i, G, w.dr, P);
+                sum += mine.nc;
+                big = max(big, mine.nc);
+            }
+        int at = sum;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(at, o, 64);
+            if (lane >= o) at += u;
+            big = max(big, __shfl_xor(big, o, 64));
+        }
+        if (lane == 63) {
+            ws[wave] = at;
+            ws[4 + wave] = big;
+        }
+        __syncthreads();
+        int total = 0;
+        at -= sum;
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            if (v < wave) at += ws[v];
+            total += ws[v];
+            big = max(big, ws[4 + v]);
+        }
+        total *= a.nkv;
         // (at most 128 pieces a pair: the merge's work)
-        share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, (largest + 127) / 128);
+        share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, (big + 127) / 128);
         W0 = (int)min((long long)b * share, (long long)total);
         W1 = (int)min((long long)W0 + share, (long long)total);
         if (W0 >= W1) return;
-        s = seq_of(cum, a.nseq, W0 / a.nkv);
-        base = cum[s] * a.nkv;
-        __syncthreads();  // cum has been read
+        if (W0 >= at * a.nkv && W0 < (at + sum) * a.nkv)
+            for (int i = 0; i < per && tid * per + i < a.nseq; i++) {
+                const SeqInfo q = per == 1 ? mine : seq_info<false>(a, tid * per + i, G, w.dr, P);
+                if (W0 >= at * a.nkv && W0 < (at + q.nc) * a.nkv) {
+                    sq = q;
+                    sb[0] = tid * per + i;
+                    sb[1] = at * a.nkv;
+                }
+                at += q.nc;
+            }
+        __syncthreads();
     }
-    uint16_t* ks = (uint16_t*)(lds + wave * L::WAVE);
-    uint16_t* vs = ks + 16 * L::KP;
-    const uint64_t kvd = (uint64_t)a.nkv * HD;
-    const int kq = lane & 3, dg = lane >> 2;
-    const bool loader = dg < NDG;
-    SeqInfo q = seq_info(a, s, G, w.dr, P);
+    auto uni = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
+    SeqInfo q{uni(sq.q0), uni(sq.qn), uni(sq.len), uni(sq.c0), uni(sq.nc)};
+    int s = uni(sb[0]), base = uni(sb[1]);
+    W0 = uni(W0), W1 = uni(W1), share = uni(share);
+    uint16_t* vs = (uint16_t*)(lds + wave * L::WAVE);
+    const uint32_t kvd2 = 2 * a.nkv * HD;
+    const int vr = lane / LPR, vcol = 8 * (lane % LPR);
+    const uint32_t vcol2 = 2 * vcol;
     for (int at = W0; at < W1;) {
         while (at - base >= q.nc * a.nkv) {  // the next sequence that has work
             base += q.nc * a.nkv;
             if (++s >= a.nseq) return;
-            q = seq_info(a, s, G, w.dr, P);
+            q = seq_info<true>(a, s, G, w.dr, P);
         }
         const int g = (at - base) / q.nc, f = (at - base) % q.nc, n = min(q.nc - f, W1 - at);
         const int pair = s * a.nkv + g;
         if (f == 0 && tid == 0) w.map[pair] = make_int2(b, (at + q.nc - 1) / share - b + 1);
         at += n;
         const int* table = a.tables + (uint64_t)s * a.max_pages;
+        const uint64_t kg = (uint64_t)(a.kc + g * HD), vg = (uint64_t)(a.vc + g * HD);
+        // The wave's two groups of 16 keys of chunk c (each in one page): their cache rows; ok: bit t where group t has keys. A
+        // group without keys reads the other's rows.
+        struct Rows {
+            uint64_t at[2];  // bytes into either cache
+            int last[2], ok;
+        };
+        auto pages = [&](int c, int (&pg)[2]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int t = 0; t < 2; t++) pg[t] = sload(table + (min(DEC_CHUNK * c + 32 * wave + 16 * t, q.len - 1) >> a.page_shift));
+        };
+        auto rows = [&](int c, const int (&pg)[2]) __attribute__((always_inline)) {
+            Rows r;
+            r.ok = 0;
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const int k0 = DEC_CHUNK * c + 32 * wave + 16 * t;
+                r.at[t] = (((uint64_t)(uint32_t)pg[t] << a.page_shift) + (k0 & ((1 << a.page_shift) - 1))) * kvd2;
+                r.last[t] = min(q.len - 1 - k0, 15);
+                r.ok |= (r.last[t] >= 0 && (uint32_t)pg[t] < (uint32_t)a.n_pages) << t;
+            }
+            if (r.ok == 1) r.at[1] = r.at[0], r.last[1] = r.last[0];
+            if (r.ok == 2) r.at[0] = r.at[1], r.last[0] = r.last[1];
+            return r;
+        };
+        // (a group's rows: a scalar base and a lane's 32-bit offset)
+        v4u kf[2][KS], vb[NV];
+        auto load_v = [&](const Rows& r) __attribute__((always_inline)) {
+#pragma unroll
+            for (int u = 0; u < NV; u++) {
+                const int t = u * RPI / 16, k = (u * RPI) % 16 + vr;  // key k of group t
+                const uint32_t off = __umul24(min(k, r.last[t]), kvd2) + vcol2;
+                vb[u] = *gptr<v4u>(vg + r.at[t] + off);
+            }
+        };
+        auto load_k = [&](const Rows& r) __attribute__((always_inline)) {
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const uint32_t off = __umul24(min(l16, r.last[t]), kvd2) + 16 * lg;
+#pragma unroll
+                for (int k = 0; k < KS; k++) kf[t][k] = *gptr<v4u>(kg + r.at[t] + off + 64 * k);
+            }
+        };
+        const int c0 = q.c0 + f, c1 = c0 + n;
+        int pg[2];
+        pages(c0, pg);
+        Rows cur = rows(c0, pg);
+        if (cur.ok) {
+            load_v(cur);
+            load_k(cur);
+        }
+        if (n > 1) pages(c0 + 1, pg);
         // the rows' queries and the keys they see
         h8 qh[NT][KS], ql[NT][KS];
         float usc[NT], m[NT], l[NT];
@@ -232,17 +347,21 @@ __global__ __launch_bounds__(256) void attn_paged_dec_kernel(PagedAttn a, PagedW
             f4 qv[2 * KS];
             float mx = 0.0f;
             const float* qr = a.q + ((uint64_t)(q.q0 + (live ? tok : 0)) * a.nh + h) * HD;
+            const int pos = a.pos[q.q0 + (live ? tok : 0)];
 #pragma unroll
             for (int k = 0; k < KS; k++)
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    qv[2 * k + e] = live ? *(const f4*)(qr + 32 * k + 8 * lg + 4 * e) : (f4){0.0f, 0.0f, 0.0f, 0.0f};
+                    qv[2 * k + e] = *(const f4*)(qr + 32 * k + 8 * lg + 4 * e);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) mx = fmaxf(mx, fabsf(qv[2 * k + e][i]));
+                    for (int i = 0; i < 4; i++) {
+                        qv[2 * k + e][i] = live ? qv[2 * k + e][i] : 0.0f;
+                        mx = fmaxf(mx, fabsf(qv[2 * k + e][i]));
+                    }
                 }
             lo[u] = 1;
             hi[u] = 0;
-            if (live) own_range(a, a.pos[q.q0 + tok], q.len, P, lo[u], hi[u]);
+            if (live) own_range(a, pos, q.len, P, lo[u], hi[u]);
             mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
             int ex = 0;
@@ -256,86 +375,91 @@ __global__ __launch_bounds__(256) void attn_paged_dec_kernel(PagedAttn a, PagedW
 #pragma unroll
             for (int d = 0; d < DT; d++) o[u][d] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
         }
-        for (int c = q.c0 + f; c < q.c0 + f + n; c++) {
-            const int k0 = 64 * c + 16 * wave, nk = min(16, q.len - k0);
-            if (nk <= 0) continue;
-            const int pg = sload(table + (k0 >> a.page_shift));
-            if (pg < 0 || pg >= a.n_pages) continue;
-            const uint64_t row0 = ((uint64_t)pg << a.page_shift) + (k0 & ((1 << a.page_shift) - 1));
-            uint4 kb[4], vb[4];
+        for (int c = c0; c < c1; c++) {
+            const Rows r = cur;
+            if (r.ok) {
 #pragma unroll
-            for (int kk = 0; kk < 4; kk++) {
-                const uint64_t off = (row0 + min(4 * kq + kk, nk - 1)) * kvd + g * HD + 8 * min(dg, NDG - 1);
-                kb[kk] = *(const uint4*)(a.kc + off);
-                vb[kk] = *(const uint4*)(a.vc + off);
-            }
-            if (loader) {
-#pragma unroll
-                for (int kk = 0; kk < 4; kk++) *(uint4*)&ks[(4 * kq + kk) * L::KP + 8 * dg] = kb[kk];
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int sh = 16 * (e & 1);
-                    const uint32_t a0 = (u4c(vb[0], e >> 1) >> sh) & 0xFFFFu, a1 = (u4c(vb[1], e >> 1) >> sh) & 0xFFFFu;
-                    const uint32_t a2 = (u4c(vb[2], e >> 1) >> sh) & 0xFFFFu, a3 = (u4c(vb[3], e >> 1) >> sh) & 0xFFFFu;
-                    *(uint2*)&vs[(8 * dg + e) * L::VP + 4 * kq] = make_uint2(a0 | (a1 << 16), a2 | (a3 << 16));
-                }
+                for (int u = 0; u < NV; u++) *(v4u*)&vs[(u * RPI + vr) * L::VP + vcol] = vb[u];
             }
             __builtin_amdgcn_wave_barrier();
-            f4 sv[NT];
-#pragma unroll
-            for (int u = 0; u < NT; u++) sv[u] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int k = 0; k < KS; k++) {
-                const h8 kf = *(const h8*)&ks[l16 * L::KP + 32 * k + 8 * lg];
-#pragma unroll
-                for (int u = 0; u < NT; u++) {
-                    sv[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[u][k], sv[u], 0, 0, 0);
-                    sv[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[u][k], sv[u], 0, 0, 0);
-                }
+            const bool more = c + 1 < c1;
+            if (more) {
+                cur = rows(c + 1, pg);
+                if (cur.ok) load_v(cur);
             }
-            h4 ph[NT], pl[NT];
+            f4 sv[NT][2];
+            if (r.ok) {
+#pragma unroll
+                for (int u = 0; u < NT; u++)
+#pragma unroll
+                    for (int t = 0; t < 2; t++) sv[u][t] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int k = 0; k < KS; k++)
+#pragma unroll
+                    for (int u = 0; u < NT; u++)
+#pragma unroll
+                        for (int t = 0; t < 2; t++) {
+                            const h8 kv = __builtin_bit_cast(h8, kf[t][k]);
+                            sv[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, qh[u][k], sv[u][t], 0, 0, 0);
+                            sv[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, ql[u][k], sv[u][t], 0, 0, 0);
+                        }
+            }
+            if (more) {
+                if (cur.ok) load_k(cur);
+                if (c + 2 < c1) pages(c + 2, pg);
+            }
+            if (!r.ok) continue;
+            const int k0 = DEC_CHUNK * c + 32 * wave;
+            h8 ph[NT], pl[NT];
 #pragma unroll
             for (int u = 0; u < NT; u++) {
                 float mx = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int j = k0 + 4 * lg + i;
-                    if (j < lo[u] || j > hi[u]) sv[u][i] = -INFINITY;
-                    mx = fmaxf(mx, sv[u][i]);
-                }
+                for (int t = 0; t < 2; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int j = k0 + 16 * t + 4 * lg + i;
+                        if (j < lo[u] || j > hi[u] || !((r.ok >> t) & 1)) sv[u][t][i] = -INFINITY;
+                        mx = fmaxf(mx, sv[u][t][i]);
+                    }
                 mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
                 mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                const float mnew = fmaxf(m[u], mx * usc[u]);
-                const float alpha = m[u] == -INFINITY ? 0.0f : exp2_hw(m[u] - mnew);
-                const float mref = mnew == -INFINITY ? 0.0f : mnew;
-                float p[4], sum = 0.0f;
+                const float mxs = mx * usc[u];  // (a positive factor keeps the order)
+                if (__ballot(mxs > m[u] + 1.0f)) {  // (m follows the maximum when a weight would pass 2, column by column)
+                    const float mnew = mxs > m[u] + 1.0f ? mxs : m[u], alpha = m[u] == -INFINITY ? 0.0f : exp2_hw(m[u] - mnew);
+                    l[u] *= alpha;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    p[i] = exp2_hw(__builtin_fmaf(sv[u][i], usc[u], -mref));
-                    sum += p[i];
+                    for (int d = 0; d < DT; d++) o[u][d] *= alpha;
+                    m[u] = mnew;
                 }
-                sum += __shfl_xor(sum, 16, 64);
-                sum += __shfl_xor(sum, 32, 64);
-                l[u] = l[u] * alpha + sum;
-                m[u] = mnew;
+                const float mref = m[u] == -INFINITY ? 0.0f : m[u];
+                float p[8];
 #pragma unroll
-                for (int d = 0; d < DT; d++) o[u][d] *= alpha;
+                for (int t = 0; t < 2; t++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    ph[u][i] = (_Float16)__builtin_fmaf(p[i], PF_SCALE, 0.0f);
-                    pl[u][i] = (_Float16)__builtin_fmaf(p[i], PF_SCALE, -(float)ph[u][i]);
-                }
+                    for (int i = 0; i < 4; i++) {
+                        p[4 * t + i] = exp2_hw(__builtin_fmaf(sv[u][t][i], usc[u], -mref));
+                        l[u] += p[4 * t + i];
+                    }
+                split_w8(p, ph[u], pl[u]);
             }
 #pragma unroll
             for (int d = 0; d < DT; d++) {
-                const h4 vf = __builtin_bit_cast(h4, *(const uint2*)&vs[(16 * d + l16) * L::VP + 4 * lg]);
+                const uint16_t* vp = &vs[(4 * lg + (l16 >> 2)) * L::VP + 16 * d + 4 * (l16 & 3)];
+                const h4 v0 = read_tr(vp), v1 = read_tr(vp + 16 * L::VP);
+                const h8 vf = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
                 for (int u = 0; u < NT; u++) {
-                    o[u][d] = __builtin_amdgcn_mfma_f32_16x16x16f16(vf, ph[u], o[u][d], 0, 0, 0);
-                    o[u][d] = __builtin_amdgcn_mfma_f32_16x16x16f16(vf, pl[u], o[u][d], 0, 0, 0);
+                    o[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, ph[u], o[u][d], 0, 0, 0);
+                    o[u][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pl[u], o[u][d], 0, 0, 0);
                 }
             }
             __builtin_amdgcn_wave_barrier();
+        }
+#pragma unroll
+        for (int u = 0; u < NT; u++) {
+            l[u] += __shfl_xor(l[u], 16, 64);
+            l[u] += __shfl_xor(l[u], 32, 64);
         }
         // the waves' sums meet in LDS, 16 rows at a time
         float* ow = (float*)lds;
@@ -385,8 +509,8 @@ __global__ __launch_bounds__(256) void attn_paged_dec_kernel(PagedAttn a, PagedW
                 int klo, khi;
                 own_range(a, a.pos[q.q0 + tok], q.len, P, klo, khi);
                 float ac[HD / 64], mm, ll;
-                paged_row_again<HD>(a, a.q + ((uint64_t)(q.q0 + tok) * a.nh + g * G + cb % G) * HD, g, table, max(klo, 64 * (q.c0 + f)),
-                                    min(khi, 64 * (q.c0 + f + n) - 1), ac, mm, ll);
+                paged_row_again<HD>(a, a.q + ((uint64_t)(q.q0 + tok) * a.nh + g * G + cb % G) * HD, g, table, max(klo, DEC_CHUNK * c0),
+                                    min(khi, DEC_CHUNK * c1 - 1), ac, mm, ll);
                 const uint64_t r = (uint64_t)(b + pair) * w.dr + cb;
 #pragma unroll
                 for (int d = 0; d < HD / 64; d++) w.dacc[r * HD + lane + 64 * d] = ac[d];
@@ -434,7 +558,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedAttn a, Pa
         int* cum = (int*)lds;
         int largest;
         const int total = scan_seqs(a.nseq, [&](int i) {
-            const SeqInfo q = seq_info(a, i, G, w.dr, P);
+            const SeqInfo q = seq_info<false>(a, i, G, w.dr, P);
             return q.qn * G > w.dr ? (q.qn + TT - 1) / TT : 0;
         }, cum, ws, largest);
         tt = total - 1 - tt;  // (a sequence's last, longest tiles first)
@@ -442,7 +566,7 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedAttn a, Pa
         const int s = seq_of(cum, a.nseq, tt);
         const int j = tt - cum[s];
         __syncthreads();
-        const SeqInfo q = seq_info(a, s, G, w.dr, P);
+        const SeqInfo q = seq_info<true>(a, __builtin_amdgcn_readfirstlane(s), G, w.dr, P);
         t0 = q.q0 + j * TT;
         nt = min(TT, q.qn - j * TT);
         len = q.len;
@@ -485,9 +609,12 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedAttn a, Pa
         for (int k = 0; k < KS; k++)
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                v[2 * k + e] = live ? *(const f4*)(qr + 16 * k + 8 * hf + 4 * e) : (f4){0.0f, 0.0f, 0.0f, 0.0f};
+                v[2 * k + e] = *(const f4*)(qr + 16 * k + 8 * hf + 4 * e);
 #pragma unroll
-                for (int i = 0; i < 4; i++) mx = fmaxf(mx, fabsf(v[2 * k + e][i]));
+                for (int i = 0; i < 4; i++) {
+                    v[2 * k + e][i] = live ? v[2 * k + e][i] : 0.0f;
+                    mx = fmaxf(mx, fabsf(v[2 * k + e][i]));
+                }
             }
         mx = max_half(mx);
         int ex = 0;
@@ -705,18 +832,27 @@ __device__ __forceinline__ int row_seq(const PagedAttn& a, int r) {
 }
 
 // Row r, query head h from its partial sums: out = sum_i acc_i 2^(m_i - M) / (sum_i l_i 2^(m_i - M) + 2^(sink - M)). Block
-// (row x, heads y) of MW waves a head: wave v of a head takes partials v, v + MW, .. (the prefix's splits, then the own keys'
-// pieces or splits), their maxima a lane each, then the weighted rows with the loads of 8 in flight.
-template <int HD, int MW>
-__global__ __launch_bounds__(256) void attn_paged_merge_kernel(PagedAttn a, PagedWs w) {
+// (x, heads y) of MW waves a head: wave v of a head takes partials v, v + MW, .. (the prefix's splits, then the own keys'
+// pieces or splits), their maxima a lane each, then the weighted rows with the loads of 8 in flight. DEC: x is row x % per of
+// sequence x / per, the sequences of the decode kernel; else x is a row, those of the tile kernel.
+template <int HD, int MW, bool DEC>
+__global__ __launch_bounds__(256) void attn_paged_merge_kernel(PagedAttn a, PagedWs w, int per) {
     constexpr int DL = HD / 64, HPB = 4 / MW;
     __shared__ float sm[HPB][MW], sl[HPB][MW], so[HPB][MW][HD];
-    const int r = blockIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (r >= a.q_start[a.nseq]) return;
-    const int G = a.nh / a.nkv, P = prefix_len(a), s = __builtin_amdgcn_readfirstlane(row_seq(a, r));
-    const SeqInfo q = seq_info(a, s, G, w.dr, P);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int G = a.nh / a.nkv, P = prefix_len(a);
+    int s, r;
+    if constexpr (DEC) {
+        s = blockIdx.x / per;
+    } else {
+        r = blockIdx.x;
+        if (r >= a.q_start[a.nseq]) return;
+        s = __builtin_amdgcn_readfirstlane(row_seq(a, r));
+    }
+    const SeqInfo q = seq_info<true>(a, s, G, w.dr, P);
+    if constexpr (DEC) r = q.q0 + blockIdx.x % per;
     const bool dec = q.qn * G <= w.dr;
-    if (r < q.q0 || r >= q.q0 + q.qn || (!dec && (w.final_tiles || !w.tml))) return;
+    if (r < q.q0 || r >= q.q0 + q.qn || dec != DEC) return;
     const int hi = wave / MW, v = wave % MW;
     for (int h = blockIdx.y * HPB + hi; h < a.nh; h += gridDim.y * HPB) {
         const int g = h / G;
@@ -724,9 +860,9 @@ __global__ __launch_bounds__(256) void attn_paged_merge_kernel(PagedAttn a, Page
         const int np = P > 0 ? w.nsp : 0;
         int no = 0;
         uint64_t first = 0, step = 1;  // partial i >= np: row first + (i - np) step of (ml, acc)
-        const float2* oml = dec ? w.dml : w.tml;
-        const float* oacc = dec ? w.dacc : w.tacc;
-        if (dec) {
+        const float2* oml = DEC ? w.dml : w.tml;
+        const float* oacc = DEC ? w.dacc : w.tacc;
+        if constexpr (DEC) {
             if (q.nc > 0) {
                 const int2 mp = w.map[s * a.nkv + g];
                 no = mp.y;
@@ -821,8 +957,8 @@ static PagedWs plan(const PagedAttn& a, uint8_t* at, size_t* end) {
     const long long most_rows = (long long)a.max_q * G;
     w.nct = most_rows > 16 && most_rows <= 32 ? 2 : 1;
     w.dr = (int)std::min<long long>(16 * w.nct, most_rows);
-    const long long most = (long long)a.nseq * a.nkv * (((long long)a.max_pages << a.page_shift) / 64 + 1);
-    w.dblocks = (int)std::min<long long>(most, 1024);
+    const long long most = (long long)a.nseq * a.nkv * (((long long)a.max_pages << a.page_shift) / DEC_CHUNK + 1);
+    w.dblocks = (int)std::min<long long>(most, w.nct == 1 ? 512 : 256);  // the blocks that run at once
     // splits of the tile kernels: enough blocks for two a CU
     auto splits = [&](long long tiles, long long keys) {
         const long long blocks = tiles * a.nkv, want = div_up(512, std::max(blocks, 1ll));
@@ -877,11 +1013,9 @@ static void launch_t(const PagedAttn& a, const PagedWs& w, hipStream_t s) {
         attn_paged_dec_kernel<HD, 2><<<dim3((unsigned)w.dblocks), dim3(256), 0, s>>>(a, w);
     else
         attn_paged_dec_kernel<HD, 1><<<dim3((unsigned)w.dblocks), dim3(256), 0, s>>>(a, w);
-    // a wave a head where there are many rows, else four
-    if ((long long)a.t * a.nh >= 8192)
-        attn_paged_merge_kernel<HD, 1><<<dim3((unsigned)a.t), dim3(256), 0, s>>>(a, w);
-    else
-        attn_paged_merge_kernel<HD, 4><<<dim3((unsigned)a.t, (unsigned)a.nh), dim3(256), 0, s>>>(a, w);
+    const int per = w.dr / G;
+    attn_paged_merge_kernel<HD, 4, true><<<dim3((unsigned)(a.nseq * per), (unsigned)a.nh), dim3(256), 0, s>>>(a, w, per);
+    if (w.tml) attn_paged_merge_kernel<HD, 1, false><<<dim3((unsigned)a.t, (unsigned)((a.nh + 3) / 4)), dim3(256), 0, s>>>(a, w, 0);
 }
 
 hipError_t launch_attn_paged(const PagedAttn& a, hipStream_t s) {
