@@ -26,12 +26,13 @@ struct PagedWs {
     int2* map;     // [nseq nkv] first block and pieces of a decode sequence's KV head
     float2* dml;   // [slots][dr] max and sum of a piece's rows
     float* dacc;   // [slots][dr][hd]
-    float2* pml;   // [t nh][nsp]: the prefix's splits
+    float2* pml;   // [t nh][nsp]: the prefix's splits, of the rows of decode sequences
     float* pacc;   // [t nh][nsp][hd]
-    float2* tml;   // [t nh][nst]: the splits of a long sequence's own keys
-    float* tacc;
-    int dblocks, nct, dr, nsp, nst;  // decode blocks, their column tiles; rows (tokens x G) up to which a sequence decodes; splits
-    bool final_tiles;              // the tile kernel writes out itself (one split, no prefix)
+    int* plan;     // long sequences (null: none): PlanHead, then a Tile each
+    int* drows;    // with a plan and a prefix: the rows of decode sequences
+    float2* tml;   // [2 tblocks][128]: the pieces of tiles that more than one block computes
+    float* tacc;   // [2 tblocks][128][hd]
+    int dblocks, nct, dr, nsp, tblocks;  // decode blocks, their column tiles; rows (tokens x G) up to which a sequence decodes
 };
 
 // ---------------- sequences ----------------
@@ -68,19 +69,38 @@ __device__ __forceinline__ void own_range(const PagedAttn& a, int pos, int len, 
     lo = a.win > 0 ? (int)max((long long)pos + 1 - a.win - P, 0ll) : 0;
 }
 
-// One query row again by a wave in float32 over the keys lo .. hi alone, for rows near a value that is not finite: acc, max and
-// sum of its softmax (the max in log2 units). Built for few registers, not for speed.
+// The keys of a sequence as one list: virtual key v < 64 np lies in the prefix (key v, none from P on), v >= 64 np is own key
+// v - 64 np, np = ceil(P / 64) tiles of 64.
+struct Keys {
+    const int* prefix;
+    const int* own;
+    int P, np, len;
+};
+// Virtual keys that a row at position pos sees: lo .. hi (none: hi = -1, lo past it).
+__device__ __forceinline__ void row_range(const PagedAttn& a, const Keys& k, int pos, int& lo, int& hi) {
+    const long long own = min((long long)pos - k.P, (long long)k.len - 1);
+    const int first = a.win > 0 ? (int)max((long long)pos + 1 - a.win, 0ll) : 0;
+    hi = own >= 0 ? 64 * k.np + (int)own : min(pos, k.P - 1);
+    lo = first < k.P ? first : 64 * k.np + (first - k.P);
+    if (hi < lo) hi = -1, lo = INT_MAX;
+}
+
+// One query row again by a wave in float32 over the virtual keys lo .. hi alone, for rows near a value that is not finite: acc,
+// max and sum of its softmax (the max in log2 units). Built for few registers, not for speed.
 template <int HD>
-__device__ void paged_row_again(const PagedAttn& a, const float* q, int g, const int* table, int lo, int hi, float (&acc)[HD / 64],
+__device__ void paged_row_again(const PagedAttn& a, const Keys& ks, const float* q, int g, int lo, int hi, float (&acc)[HD / 64],
                                 float& m, float& l) {
     const int lane = threadIdx.x & 63;
     const uint64_t kvd = (uint64_t)a.nkv * HD;
-    auto row = [&](int j) {  // the key's cache row, or -1
-        const int pg = table[j >> a.page_shift];
+    auto row = [&](int v) {  // the key's cache row, or -1
+        const bool pre = v < 64 * ks.np;
+        const int j = pre ? v : v - 64 * ks.np;
+        if (pre && j >= ks.P) return (int64_t)-1;
+        const int pg = (pre ? ks.prefix : ks.own)[j >> a.page_shift];
         return pg >= 0 && pg < a.n_pages ? ((int64_t)pg << a.page_shift) + (j & ((1 << a.page_shift) - 1)) : (int64_t)-1;
     };
-    auto score = [&](int j) {
-        const int64_t r = row(j);
+    auto score = [&](int v) {
+        const int64_t r = row(v);
         if (r < 0) return -INFINITY;
         float s = 0.0f;
 #pragma unroll 1
@@ -96,7 +116,7 @@ __device__ void paged_row_again(const PagedAttn& a, const float* q, int g, const
 #pragma unroll
     for (int c = 0; c < HD / 64; c++) acc[c] = 0.0f;
 #pragma unroll 1
-    for (int j = lo + lane; j <= hi; j += 64) m = fmaxf(m, score(j));
+    for (int v = lo + lane; v <= hi; v += 64) m = fmaxf(m, score(v));
     m = wave_max64(m);
     if (m == -INFINITY) return;
 #pragma unroll 1
@@ -113,57 +133,6 @@ __device__ void paged_row_again(const PagedAttn& a, const float* q, int g, const
         }
     }
     l = wave_sum64(l);
-}
-
-// The exclusive prefix sums of f(s), s < n <= SERVE_MAX_SEQ, into cum by a block of 256 threads; the total (and the largest
-// f(s)) to every thread. cum[n - 1] + f(n - 1) is the total.
-template <typename F>
-__device__ __forceinline__ int scan_seqs(int n, F&& f, int* cum, int* ws, int& largest) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, per = (n + 255) / 256;
-    int sum = 0, big = 0;
-    for (int i = 0; i < per; i++) {
-        const int s = tid * per + i;
-        if (s < n) {
-            const int v = f(s);
-            cum[s] = sum;
-            sum += v;
-            big = max(big, v);
-        }
-    }
-    int inc = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(inc, o, 64);
-        if (lane >= o) inc += u;
-        big = max(big, __shfl_xor(big, o, 64));
-    }
-    if (lane == 63) {
-        ws[wave] = inc;
-        ws[4 + wave] = big;
-    }
-    __syncthreads();
-    int base = inc - sum, total = 0;
-    largest = 0;
-#pragma unroll
-    for (int w = 0; w < 4; w++) {
-        if (w < wave) base += ws[w];
-        total += ws[w];
-        largest = max(largest, ws[4 + w]);
-    }
-    for (int i = 0; i < per; i++)
-        if (tid * per + i < n) cum[tid * per + i] += base;
-    __syncthreads();
-    return total;
-}
-// The last i < n with cum[i] <= v.
-__device__ __forceinline__ int seq_of(const int* cum, int n, int v) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (cum[mid] <= v) lo = mid;
-        else hi = mid;
-    }
-    return lo;
 }
 
 // The scaled hi and lo f16 parts of 8 query values.
@@ -509,7 +478,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attn_paged_dec_kernel(Pa
                 int klo, khi;
                 own_range(a, a.pos[q.q0 + tok], q.len, P, klo, khi);
                 float ac[HD / 64], mm, ll;
-                paged_row_again<HD>(a, a.q + ((uint64_t)(q.q0 + tok) * a.nh + g * G + cb % G) * HD, g, table, max(klo, DEC_CHUNK * c0),
+                paged_row_again<HD>(a, Keys{nullptr, table, 0, 0, q.len}, a.q + ((uint64_t)(q.q0 + tok) * a.nh + g * G + cb % G) * HD, g, max(klo, DEC_CHUNK * c0),
                                     min(khi, DEC_CHUNK * c1 - 1), ac, mm, ll);
                 const uint64_t r = (uint64_t)(b + pair) * w.dr + cb;
 #pragma unroll
@@ -522,63 +491,33 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attn_paged_dec_kernel(Pa
 }
 
 // ---------------- many rows over the same keys ----------------
-// A block of 4 waves takes 128 query rows of one KV head (128 / G tokens x G heads, 32 rows a wave) over a split of the keys
-// that they see, in tiles of 64 keys as attn_prefill_kernel of attn.hip does, on v_mfma_f32_32x32x16_f16. PRE: tiles of the
-// call's rows whatever their sequence, over the prefix's keys: K and V of the prefix are read once a tile of 128 / G tokens
-// rather than once a token. Else: tiles of the rows of each sequence that is too long for the decode kernel, over its own
-// keys. Blocks are numbered so that the tiles over the same keys run on one XCD (its L2 holds a split's K and V).
-template <int HD, bool PRE>
-__global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedAttn a, PagedWs w, int tiles) {
-    using L = PfLayout<HD>;
-    constexpr int KS = HD / 16, DT = HD / 32, ND = HD / 8, BK = 64;
-    constexpr int KB = BK * L::KP * 2, VB = HD * L::VP * 2;
-    static_assert(KB + VB >= SERVE_MAX_SEQ * 4, "the prefix sums use the tiles' LDS");
-    __shared__ __align__(16) uint8_t lds[KB + VB];
-    __shared__ int ws[8];
-    uint16_t* ks = (uint16_t*)lds;
-    uint16_t* vs = (uint16_t*)(lds + KB);
+// A block of 4 waves takes 128 query rows of one KV head (128 / G tokens x G heads, 32 rows a wave) over tiles of 64 keys, on
+// v_mfma_f32_32x32x16_f16 as attn_prefill_kernel of attn.hip does: S^T (32 keys x 32 rows, two sub-tiles) = K Q^T hi and lo,
+// an online softmax a column, O^T (32 dims x 32 rows) += V^T P^T hi and lo with V's rows read transposed from LDS. K and V
+// tiles alternate between two LDS buffers: while one is computed the next one's registers go to the other and the one after
+// is requested, so a tile costs one barrier.
+template <int HD>
+struct PagedTile {
+    static constexpr int BK = 64, KP = HD + 8, VP = HD + 32;  // halves a row: K's 16-byte reads, V's transposed reads spread over the banks
+    static constexpr int KB = BK * KP * 2, BUF = KB + BK * VP * 2;
+};
+
+// The softmax sums of a lane's row (column l32 of wave `wave`) over key tiles kb .. ke - 1.
+template <int HD>
+struct TileSums {
+    f16v o[HD / 32];
+    float m, l;
+};
+// live: the lane has a row; qr: its query; lo, hi: the virtual keys that it sees.
+template <int HD>
+__device__ __forceinline__ void tile_run(const PagedAttn& a, const Keys& keys, uint8_t* lds, int g, int kb, int ke, bool live, const float* qr,
+                                         int lo, int hi, TileSums<HD>& r) {
+    using L = PagedTile<HD>;
+    typedef unsigned v4u __attribute__((ext_vector_type(4)));
+    constexpr int KS = HD / 16, DT = HD / 32, ND = HD / 8, BK = 64, NP = BK * ND / 256, ST = 256 / ND;  // chunks a thread, keys apart
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l32 = lane & 31, hf = lane >> 5;
-    const int G = a.nh / a.nkv, gs = 31 - __builtin_clz(G), TT = 128 >> gs, P = prefix_len(a);
-    const int ns = PRE ? w.nsp : w.nst, nc = a.nkv * ns;
-    // block x: combination (KV head, split) c on XCD c % 8, tile tt
-    const int x = blockIdx.x, c = (x & 7) + 8 * ((x >> 3) / tiles);
-    int tt = (x >> 3) % tiles;
-    if (c >= nc) return;
-    const int g = c % a.nkv, split = c / a.nkv;
-    // the tile's first row, its tokens, the keys' table and number
-    int t0, nt, len;
-    const int* table;
-    if constexpr (PRE) {
-        t0 = tt * TT;
-        nt = min(TT, min(max(a.q_start[a.nseq], 0), a.t) - t0);
-        len = P;
-        table = a.prefix;
-        if (nt <= 0) return;
-    } else {
-        int* cum = (int*)lds;
-        int largest;
-        const int total = scan_seqs(a.nseq, [&](int i) {
-            const SeqInfo q = seq_info<false>(a, i, G, w.dr, P);
-            return q.qn * G > w.dr ? (q.qn + TT - 1) / TT : 0;
-        }, cum, ws, largest);
-        tt = total - 1 - tt;  // (a sequence's last, longest tiles first)
-        if (tt < 0) return;
-        const int s = seq_of(cum, a.nseq, tt);
-        const int j = tt - cum[s];
-        __syncthreads();
-        const SeqInfo q = seq_info<true>(a, __builtin_amdgcn_readfirstlane(s), G, w.dr, P);
-        t0 = q.q0 + j * TT;
-        nt = min(TT, q.qn - j * TT);
-        len = q.len;
-        table = a.tables + (uint64_t)s * a.max_pages;
-    }
-    // this lane's row (a query column), the keys it sees, and those that the wave's and the block's rows see
-    const int r = 32 * wave + l32, tok = r >> gs, h = g * G + (r & (G - 1));
-    const bool live = tok < nt;
-    int lo = INT_MAX, hi = -1;
-    if (live) own_range(a, a.pos[t0 + tok], len, PRE ? 0 : P, lo, hi);
-    if (hi < lo) hi = -1, lo = INT_MAX;
-    int wlo = lo, whi = hi, maxlo = hi < 0 ? -1 : lo, minhi = live ? hi : INT_MAX;
+    // the keys that the wave's rows see: outside of wlo .. whi none, inside maxlo .. minhi all of them all
+    int wlo = live ? lo : INT_MAX, whi = live ? hi : -1, maxlo = live && hi >= 0 ? lo : -1, minhi = live ? hi : INT_MAX;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         wlo = min(wlo, __shfl_xor(wlo, o, 64));
@@ -590,18 +529,57 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedAttn a, Pa
     whi = __builtin_amdgcn_readfirstlane(whi);
     maxlo = __builtin_amdgcn_readfirstlane(maxlo);
     minhi = __builtin_amdgcn_readfirstlane(minhi);
-    if (lane == 0) {
-        ws[wave] = wlo;
-        ws[4 + wave] = whi;
+    const int kk = tid / ND, col = 8 * (tid % ND);
+    const uint32_t kvd2 = 2 * a.nkv * HD, col2 = 2 * col;
+    const uint64_t kg = (uint64_t)(a.kc + g * HD), vg = (uint64_t)(a.vc + g * HD);
+    // Pages of a tile's four groups of 16 keys (a group lies in one page); past the last key its group's; a page outside the
+    // pool is read as page 0 and its keys hidden.
+    auto pages = [&](int kt, int (&pg)[4]) __attribute__((always_inline)) {
+        kt = min(kt, ke - 1);
+        const bool pre = kt < keys.np;
+        const int k0 = BK * (pre ? kt : kt - keys.np), n = pre ? keys.P : keys.len;
+        const int* table = pre ? keys.prefix : keys.own;
+#pragma unroll
+        for (int u = 0; u < 4; u++) pg[u] = sload(table + (min(k0 + 16 * u, (n - 1) & ~15) >> a.page_shift));
+    };
+    v4u kr[NP], vr[NP];
+    auto fetch = [&](int kt, const int (&pg)[4]) __attribute__((always_inline)) {
+        const bool pre = kt < keys.np;
+        const int k0 = BK * (pre ? kt : kt - keys.np), lim = (pre ? keys.P : keys.len) - 1 - k0;  // (keys past the last read its row)
+#pragma unroll
+        for (int u = 0; u < NP; u++) {
+            const int grp = ND == 16 ? u : 2 * u + (wave >> 1), g16 = min(16 * grp, lim & ~15);
+            const int p = grp == 0 ? pg[0] : grp == 1 ? pg[1] : grp == 2 ? pg[2] : pg[3];
+            const uint64_t at = (((uint64_t)((uint32_t)p < (uint32_t)a.n_pages ? p : 0) << a.page_shift) + ((k0 + g16) & ((1 << a.page_shift) - 1))) * kvd2;
+            const uint32_t off = __umul24(min(ST * u + kk, lim) - g16, kvd2) + col2;
+            kr[u] = *gptr<v4u>(kg + at + off);
+            vr[u] = *gptr<v4u>(vg + at + off);
+        }
+    };
+    auto stage = [&](int buf) __attribute__((always_inline)) {
+        uint16_t* ks = (uint16_t*)(lds + buf * L::BUF);
+        uint16_t* vs = (uint16_t*)(lds + buf * L::BUF + L::KB);
+#pragma unroll
+        for (int u = 0; u < NP; u++) {
+            *(v4u*)&ks[(kk + ST * u) * L::KP + col] = kr[u];
+            *(v4u*)&vs[(kk + ST * u) * L::VP + col] = vr[u];
+        }
+    };
+    auto holes = [&](const int (&pg)[4]) __attribute__((always_inline)) {
+        int h = 0;
+#pragma unroll
+        for (int u = 0; u < 4; u++) h |= ((uint32_t)pg[u] >= (uint32_t)a.n_pages) << u;
+        return h;
+    };
+    int pg[4], hole = 0, hole1 = 0;
+    if (kb < ke) {
+        pages(kb, pg);
+        fetch(kb, pg);
+        hole = holes(pg);
+        pages(kb + 1, pg);
     }
-    __syncthreads();
-    const int blo = min(min(ws[0], ws[1]), min(ws[2], ws[3])), bhi = max(max(ws[4], ws[5]), max(ws[6], ws[7]));
-    // the split's tiles of 64 keys: kb .. ke - 1
-    const int kt0 = bhi < 0 ? 0 : blo / BK, kt1 = bhi < 0 ? 0 : bhi / BK + 1, per = (kt1 - kt0 + ns - 1) / ns;
-    const int kb = min(kt0 + split * per, kt1), ke = min(kb + per, kt1);
     h8 qh[KS], ql[KS];
     float usc;
-    const float* qr = a.q + ((uint64_t)(t0 + (live ? tok : 0)) * a.nh + h) * HD;
     {
         f4 v[2 * KS];
         float mx = 0.0f;
@@ -624,329 +602,524 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedAttn a, Pa
 #pragma unroll
         for (int k = 0; k < KS; k++) split_q8(v[2 * k], v[2 * k + 1], up, qh[k], ql[k]);
     }
-    f16v o[DT];
 #pragma unroll
     for (int d = 0; d < DT; d++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) o[d][i] = 0.0f;
+        for (int i = 0; i < 16; i++) r.o[d][i] = 0.0f;
     float m = -INFINITY, l = 0.0f;
-    constexpr int NPK = BK * ND / 256, NPV = BK / 2 * ND / 256;
-    typedef unsigned v4u __attribute__((ext_vector_type(4)));
-    v4u kr[NPK], vr[NPV][2];
-    const int kk = tid / ND, kcol = 8 * (tid % ND);
-    const int vk = 2 * (((tid >> 3) & 7) + 8 * (wave / (ND / 8))), vcol = 8 * ((tid & 7) + 8 * (wave % (ND / 8)));
-    constexpr int KST = 256 / ND, VST = 64 / (ND / 8);
-    const uint64_t kvd2 = 2 * (uint64_t)a.nkv * HD;
-    const uint32_t kc2 = 2 * (g * HD + kcol), vc2 = 2 * (g * HD + vcol);
-    // Pages of a tile's four groups of 16 keys (a group lies in one page); past the last key its group's, a page outside the
-    // pool is read as page 0 and its keys hidden.
-    auto pages = [&](int k0, int (&pg)[4]) __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < 4; u++) pg[u] = sload(table + (min(k0 + 16 * u, (len - 1) & ~15) >> a.page_shift));
-    };
-    auto fetch = [&](int k0, const int (&pg)[4]) __attribute__((always_inline)) {
-        const int lim = len - 1 - k0;  // (keys past the last read its row)
-        auto at = [&](int i, int grp, uint32_t col) __attribute__((always_inline)) {  // cache bytes of key min(i, lim), in group grp
-            const int g16 = min(16 * grp, lim & ~15), p = grp == 0 ? pg[0] : grp == 1 ? pg[1] : grp == 2 ? pg[2] : pg[3];
-            const uint64_t row = ((uint64_t)(p >= 0 && p < a.n_pages ? p : 0) << a.page_shift) + ((k0 + g16) & ((1 << a.page_shift) - 1));
-            return row * kvd2 + (__umul24((uint32_t)(min(i, lim) - g16), (uint32_t)kvd2) + col);
-        };
-#pragma unroll
-        for (int u = 0; u < NPK; u++) kr[u] = *gptr<v4u>((uint64_t)a.kc + at(KST * u + kk, ND == 16 ? u : 2 * u + (wave >> 1), kc2));
-#pragma unroll
-        for (int u = 0; u < NPV; u++)
-#pragma unroll
-            for (int e = 0; e < 2; e++)
-                vr[u][e] = *gptr<v4u>((uint64_t)a.vc + at(VST * u + e + vk, ND == 16 ? 2 * u + (wave >> 1) : wave, vc2));
-    };
-    int pg[4], pn[4];
     if (kb < ke) {
-        pages(BK * kb, pg);
-        fetch(BK * kb, pg);
-        pages(min(BK * (kb + 1), (len - 1) & ~63), pn);
+        stage(0);
+        if (kb + 1 < ke) {
+            fetch(kb + 1, pg);
+            hole1 = holes(pg);
+            pages(kb + 2, pg);
+        }
+        lds_barrier();
     }
     for (int kt = kb; kt < ke; kt++) {
-        const int k0 = BK * kt;
-        __syncthreads();
-#pragma unroll
-        for (int u = 0; u < NPK; u++) *(v4u*)&ks[(kk + KST * u) * L::KP + kcol] = kr[u];
-#pragma unroll
-        for (int u = 0; u < NPV; u++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const uint32_t va = vr[u][0][e], vb = vr[u][1][e];
-                *(uint32_t*)&vs[(vcol + 2 * e) * L::VP + vk + VST * u] = __builtin_amdgcn_perm(vb, va, 0x05040100u);
-                *(uint32_t*)&vs[(vcol + 2 * e + 1) * L::VP + vk + VST * u] = __builtin_amdgcn_perm(vb, va, 0x07060302u);
-            }
-        __syncthreads();
-        int hole = 0;  // groups without a page
-#pragma unroll
-        for (int u = 0; u < 4; u++) hole |= (pg[u] < 0 || pg[u] >= a.n_pages) << u;
+        const int buf = (kt - kb) & 1;
+        const int now = hole;
         if (kt + 1 < ke) {
-#pragma unroll
-            for (int u = 0; u < 4; u++) pg[u] = pn[u];
-            fetch(k0 + BK, pg);
-            pages(min(k0 + 2 * BK, (len - 1) & ~63), pn);
+            stage(buf ^ 1);
+            hole = hole1;
+            if (kt + 2 < ke) {
+                fetch(kt + 2, pg);
+                hole1 = holes(pg);
+                pages(kt + 3, pg);
+            }
         }
-        if (k0 > whi || k0 + BK - 1 < wlo) continue;
-        f16v s[2], z;
+        const int k0 = BK * kt;
+        if (k0 <= whi && k0 + BK - 1 >= wlo) {
+            const uint16_t* ks = (const uint16_t*)(lds + buf * L::BUF);
+            const uint16_t* vs = (const uint16_t*)(lds + buf * L::BUF + L::KB);
+            f16v s[2], z;
 #pragma unroll
-        for (int i = 0; i < 16; i++) z[i] = 0.0f;
+            for (int i = 0; i < 16; i++) z[i] = 0.0f;
 #pragma unroll
-        for (int k = 0; k < KS; k++) {
-            const h8 k0f = *(const h8*)&ks[l32 * L::KP + 16 * k + 8 * hf], k1f = *(const h8*)&ks[(32 + l32) * L::KP + 16 * k + 8 * hf];
-            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0f, qh[k], k ? s[0] : z, 0, 0, 0);
-            s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1f, qh[k], k ? s[1] : z, 0, 0, 0);
-            s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0f, ql[k], s[0], 0, 0, 0);
-            s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1f, ql[k], s[1], 0, 0, 0);
-        }
-        if (k0 + BK - 1 > minhi || k0 < maxlo || hole) {
+            for (int k = 0; k < KS; k++) {
+                const h8 k0f = *(const h8*)&ks[l32 * L::KP + 16 * k + 8 * hf], k1f = *(const h8*)&ks[(32 + l32) * L::KP + 16 * k + 8 * hf];
+                s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0f, qh[k], k ? s[0] : z, 0, 0, 0);
+                s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1f, qh[k], k ? s[1] : z, 0, 0, 0);
+                s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0f, ql[k], s[0], 0, 0, 0);
+                s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1f, ql[k], s[1], 0, 0, 0);
+            }
+            const bool tail = kt < keys.np && k0 + BK > keys.P;  // (the prefix's last tile, where it is not whole)
+            if (k0 + BK - 1 > minhi || k0 < maxlo || now || tail) {
+                const int top = tail ? min(hi, keys.P - 1) : hi;
+#pragma unroll
+                for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const int kp = 32 * mt + 8 * (i >> 2) + 4 * hf + (i & 3);
+                        if (k0 + kp > top || k0 + kp < lo || ((now >> (kp >> 4)) & 1)) s[mt][i] = -INFINITY;
+                    }
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[mt][i]);
+            mx = max_half(mx);
+            const float mxs = mx * usc;
+            if (__ballot(mxs > m + 1.0f)) {  // (m follows the maximum when a weight would pass 2, column by column)
+                const float mnew = mxs > m + 1.0f ? mxs : m, alpha = m == -INFINITY ? 0.0f : exp2_hw(m - mnew);
+                l *= alpha;
+#pragma unroll
+                for (int d = 0; d < DT; d++) r.o[d] *= alpha;
+                m = mnew;
+            }
+            const float mref = m == -INFINITY ? 0.0f : m;
+            float sum = 0.0f;
 #pragma unroll
             for (int mt = 0; mt < 2; mt++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const int kp = 32 * mt + 8 * (i >> 2) + 4 * hf + (i & 3);
-                    if (k0 + kp > hi || k0 + kp < lo || ((hole >> (kp >> 4)) & 1)) s[mt][i] = -INFINITY;
+                    const float p = exp2_hw(__builtin_fmaf(s[mt][i], usc, -mref));
+                    s[mt][i] = p;
+                    sum += p;
+                }
+            l += sum;
+#pragma unroll
+            for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    float p[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) p[e] = s[mt][8 * u + e];
+                    h8 ph, pl;
+                    split_w8(p, ph, pl);
+                    h8 vf[DT];
+#pragma unroll
+                    for (int d = 0; d < DT; d++) {
+                        const uint16_t* vp = &vs[(32 * mt + 16 * u + 4 * hf + ((lane & 15) >> 2)) * L::VP + 32 * d + (lane & 16) + 4 * (lane & 3)];
+                        const h4 v0 = read_tr(vp), v1 = read_tr(vp + 8 * L::VP);
+                        vf[d] = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+                    }
+#pragma unroll
+                    for (int d = 0; d < DT; d++) r.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d], ph, r.o[d], 0, 0, 0);
+#pragma unroll
+                    for (int d = 0; d < DT; d++) r.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d], pl, r.o[d], 0, 0, 0);
                 }
         }
-        float mx = -INFINITY;
-#pragma unroll
-        for (int mt = 0; mt < 2; mt++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[mt][i]);
-        mx = max_half(mx);
-        const float mxs = mx * usc;
-        if (__ballot(mxs > m + 1.0f)) {  // (m follows the maximum when a weight would pass 2, column by column)
-            const float mnew = mxs > m + 1.0f ? mxs : m, alpha = m == -INFINITY ? 0.0f : exp2_hw(m - mnew);
-            l *= alpha;
-#pragma unroll
-            for (int d = 0; d < DT; d++) o[d] *= alpha;
-            m = mnew;
-        }
-        const float mref = m == -INFINITY ? 0.0f : m;
-        float sum = 0.0f;
-#pragma unroll
-        for (int mt = 0; mt < 2; mt++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const float p = exp2_hw(__builtin_fmaf(s[mt][i], usc, -mref));
-                s[mt][i] = p;
-                sum += p;
-            }
-        l += sum;
-#pragma unroll
-        for (int mt = 0; mt < 2; mt++)
-#pragma unroll
-            for (int u = 0; u < 2; u++) {
-                float p[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) p[e] = s[mt][8 * u + e];
-                h8 ph, pl;
-                split_w8(p, ph, pl);
-                h8 vf[DT];
-#pragma unroll
-                for (int d = 0; d < DT; d++) {
-                    const uint16_t* vp = &vs[(32 * d + l32) * L::VP + 32 * mt + 16 * u + 4 * hf];
-                    const uint2 a0 = *(const uint2*)vp, a1 = *(const uint2*)(vp + 8);
-                    vf[d] = __builtin_bit_cast(h8, make_uint4(a0.x, a0.y, a1.x, a1.y));
-                }
-#pragma unroll
-                for (int d = 0; d < DT; d++) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d], ph, o[d], 0, 0, 0);
-#pragma unroll
-                for (int d = 0; d < DT; d++) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d], pl, o[d], 0, 0, 0);
-            }
+        lds_barrier();
     }
-    l += __shfl_xor(l, 32, 64);
-    // rows with finite scores whose sums are not finite: again, over the keys that they see alone
+    r.l = l + __shfl_xor(l, 32, 64);
+    r.m = m;
+}
+
+// The rows of a wave whose sums may owe a value that is not finite to a key that they do not see (finite scores, sums that are
+// not): bit l32.
+template <int HD>
+__device__ __forceinline__ uint32_t tile_again(const TileSums<HD>& r, bool live) {
     float nf = 0.0f;
 #pragma unroll
-    for (int d = 0; d < DT; d++)
+    for (int d = 0; d < HD / 32; d++)
 #pragma unroll
-        for (int i = 0; i < 16; i++) nf = __builtin_fmaf(o[d][i], 0.0f, nf);
-    const uint64_t nfb = __ballot(nf != 0.0f && l - l == 0.0f && live);
-    uint32_t again = (uint32_t)nfb | (uint32_t)(nfb >> 32);
-    const uint64_t row = (uint64_t)(t0 + tok) * a.nh + h;
-    const bool fin = !PRE && w.final_tiles;
-    float2* ml = PRE ? w.pml : w.tml;
-    float* accp = PRE ? w.pacc : w.tacc;
-    // the scale that turns sums into an output (final: normalized by the sum and the sink), and its gate
-    auto norm = [&](int hh, float mm, float ll) {
-        const float sk = a.sink ? a.sink[hh] * LOG2E : -INFINITY, M = fmaxf(mm, sk);
-        const float sc = mm == -INFINITY ? 0.0f : exp2_hw(mm - M);
-        const float den = ll * sc + (sk == -INFINITY ? 0.0f : exp2_hw(sk - M));
-        return den == 0.0f ? 0.0f : sc / den;  // (not a number where a score is)
-    };
-    if (live && !((again >> l32) & 1)) {
-        const float f = (fin ? norm(h, m, l) : 1.0f) * (1.0f / PF_SCALE);
-        float* dst = fin ? a.out + row * HD : accp + (row * ns + split) * HD;
-        const float* gate = fin && a.qg ? a.qg + row * 2 * HD + HD : nullptr;
-        if (fin || m != -INFINITY) {
+        for (int i = 0; i < 16; i++) nf = __builtin_fmaf(r.o[d][i], 0.0f, nf);
+    const uint64_t b = __ballot(nf != 0.0f && r.l - r.l == 0.0f && live);
+    return (uint32_t)b | (uint32_t)(b >> 32);
+}
+// The factor that turns a row's sums into its output: over the sum and the sink (0 for a row without keys, not a number where a
+// score is not).
+__device__ __forceinline__ float out_factor(const PagedAttn& a, int h, float m, float l) {
+    const float sk = a.sink ? a.sink[h] * LOG2E : -INFINITY, M = fmaxf(m, sk);
+    const float sc = m == -INFINITY ? 0.0f : exp2_hw(m - M);
+    const float den = l * sc + (sk == -INFINITY ? 0.0f : exp2_hw(sk - M));
+    return den == 0.0f ? 0.0f : sc / den;
+}
+// This lane's half of its row: times f into dst, through the gate.
+template <int HD>
+__device__ __forceinline__ void tile_store(const TileSums<HD>& r, float f, float* dst, const float* gate) {
+    const int hf = (threadIdx.x >> 5) & 1;
 #pragma unroll
-            for (int d = 0; d < DT; d++)
+    for (int d = 0; d < HD / 32; d++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const int col = 32 * d + 8 * j + 4 * hf;
-                    float4 v = make_float4(o[d][4 * j] * f, o[d][4 * j + 1] * f, o[d][4 * j + 2] * f, o[d][4 * j + 3] * f);
-                    if (gate) {
-                        v.x *= sigmoid_f(gate[col]); v.y *= sigmoid_f(gate[col + 1]);
-                        v.z *= sigmoid_f(gate[col + 2]); v.w *= sigmoid_f(gate[col + 3]);
-                    }
-                    *(float4*)(dst + col) = v;
-                }
+        for (int j = 0; j < 4; j++) {
+            const int col = 32 * d + 8 * j + 4 * hf;
+            float4 v = make_float4(r.o[d][4 * j] * f, r.o[d][4 * j + 1] * f, r.o[d][4 * j + 2] * f, r.o[d][4 * j + 3] * f);
+            if (gate) {
+                v.x *= sigmoid_f(gate[col]); v.y *= sigmoid_f(gate[col + 1]);
+                v.z *= sigmoid_f(gate[col + 2]); v.w *= sigmoid_f(gate[col + 3]);
+            }
+            *(float4*)(dst + col) = v;
         }
-        if (!fin && hf == 0) ml[row * ns + split] = make_float2(m, l);
+}
+
+// The prefix for the rows of decode sequences: tiles of the call's rows (of the plan's list of them, where there is a plan)
+// whatever their sequence, so that the prefix's K and V are read once a tile of 128 / G tokens rather than once a token; a
+// block takes a split of the prefix's keys. Blocks are numbered so that the tiles over the same keys run on one XCD (its L2
+// holds a split's K and V).
+template <int HD>
+__global__ __launch_bounds__(256, 2) void attn_paged_prefix_kernel(PagedAttn a, PagedWs w, int tiles) {
+    __shared__ __align__(16) uint8_t lds[2 * PagedTile<HD>::BUF];
+    __shared__ int ws[8];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l32 = lane & 31;
+    const int G = a.nh / a.nkv, gs = 31 - __builtin_clz(G), TT = 128 >> gs, ns = w.nsp;
+    const Keys keys{a.prefix, nullptr, prefix_len(a), (prefix_len(a) + 63) / 64, 0};
+    // block x: combination (KV head, split) c on XCD c % 8, tile tt
+    const int x = blockIdx.x, c = (x & 7) + 8 * ((x >> 3) / tiles), tt = (x >> 3) % tiles;
+    if (c >= a.nkv * ns || !keys.P) return;
+    const int g = c % a.nkv, split = c / a.nkv;
+    const int nrows = w.drows ? sload(w.plan + 2) : min(max(sload(a.q_start + a.nseq), 0), a.t), nt = min(TT, nrows - tt * TT);
+    if (nt <= 0) return;
+    const int rr = 32 * wave + l32, tok = rr >> gs, h = g * G + (rr & (G - 1));
+    const bool live = tok < nt;
+    auto row_of = [&](int t) { return w.drows ? w.drows[tt * TT + t] : tt * TT + t; };
+    const int t = row_of(live ? tok : 0);
+    int lo, hi;
+    row_range(a, keys, a.pos[t], lo, hi);
+    // the tiles that the block's rows see
+    int blo = live ? lo : INT_MAX, bhi = live ? hi : -1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        blo = min(blo, __shfl_xor(blo, o, 64));
+        bhi = max(bhi, __shfl_xor(bhi, o, 64));
+    }
+    if (lane == 0) {
+        ws[wave] = blo;
+        ws[4 + wave] = bhi;
+    }
+    __syncthreads();
+    blo = __builtin_amdgcn_readfirstlane(min(min(ws[0], ws[1]), min(ws[2], ws[3])));
+    bhi = __builtin_amdgcn_readfirstlane(max(max(ws[4], ws[5]), max(ws[6], ws[7])));
+    const int kt0 = bhi < 0 ? 0 : blo / 64, kt1 = bhi < 0 ? 0 : bhi / 64 + 1, per = (kt1 - kt0 + ns - 1) / ns;
+    const int kb = min(kt0 + split * per, kt1), ke = min(kb + per, kt1);
+    const uint64_t row = (uint64_t)t * a.nh + h;
+    TileSums<HD> r;
+    tile_run<HD>(a, keys, lds, g, kb, ke, live, a.q + row * HD, lo, hi, r);
+    uint32_t again = tile_again<HD>(r, live);
+    if (live && !((again >> l32) & 1)) {
+        if (r.m != -INFINITY) tile_store<HD>(r, 1.0f / PF_SCALE, w.pacc + (row * ns + split) * HD, nullptr);
+        if (lane < 32) w.pml[row * ns + split] = make_float2(r.m, r.l);
     }
     for (; again; again &= again - 1) {
-        const int rb = 32 * wave + __builtin_ctz(again), hb = g * G + (rb & (G - 1)), tb = t0 + (rb >> gs);
-        const uint64_t rowb = (uint64_t)tb * a.nh + hb;
-        int klo, khi;
-        own_range(a, a.pos[tb], len, PRE ? 0 : P, klo, khi);
+        const int rb = 32 * wave + __builtin_ctz(again), tb = row_of(rb >> gs);
+        const uint64_t rowb = (uint64_t)tb * a.nh + g * G + (rb & (G - 1));
+        row_range(a, keys, a.pos[tb], lo, hi);
         float ac[HD / 64], mm, ll;
-        paged_row_again<HD>(a, a.q + rowb * HD, g, table, max(klo, BK * kb), min(khi, BK * ke - 1), ac, mm, ll);
-        const float f = fin ? norm(hb, mm, ll) : 1.0f;
-        float* dst = fin ? a.out + rowb * HD : accp + (rowb * ns + split) * HD;
+        paged_row_again<HD>(a, keys, a.q + rowb * HD, g, max(lo, 64 * kb), min(hi, 64 * ke - 1), ac, mm, ll);
 #pragma unroll
-        for (int d = 0; d < HD / 64; d++) {
-            const int col = lane + 64 * d;
-            const float v = ac[d] * f;
-            dst[col] = fin && a.qg ? v * sigmoid_f(a.qg[rowb * 2 * HD + HD + col]) : v;
-        }
-        if (!fin && lane == 0) ml[rowb * ns + split] = make_float2(mm, ll);
+        for (int d = 0; d < HD / 64; d++) w.pacc[(rowb * ns + split) * HD + lane + 64 * d] = ac[d];
+        if (lane == 0) w.pml[rowb * ns + split] = make_float2(mm, ll);
     }
 }
 
-// ---------------- the join ----------------
-// The sequence of row r < q_start[nseq]: the last s with q_start[s] <= r, by a wave in rounds of 64 loads (q_start does not
-// decrease; nseq <= 4096).
-__device__ __forceinline__ int row_seq(const PagedAttn& a, int r) {
+// Long sequences. The plan: for each tile of 128 / G tokens of each of them its rows and the tiles of 64 virtual keys that they
+// see, and the prefix sums of those; the work is the list of all (KV head, tile, key tile), key tile fastest, and a block takes
+// an equal run of it, so chunks at any depth of their contexts load the CUs evenly. A tile that lies in one run is finished by
+// its block; of one cut by a run's end each block leaves its sums (the piece from a tile's start at slot 2 b + 1, one that goes
+// on from the run before at 2 b), and attn_paged_join_kernel joins them.
+struct PlanTile {
+    int s, t0, nt, kt0, cum, nkt;  // sequence, first row, rows; first key tile, key tiles before this tile's, its key tiles
+};
+constexpr int PLAN_HEAD = 4;  // tiles, key tiles of all, rows of decode sequences
+
+// One block of 1024 threads: the sequences' tiles by a scan in LDS, then the tiles' keys and their scan, 1024 tiles at a time.
+__global__ __launch_bounds__(1024) void attn_paged_plan_kernel(PagedAttn a, PagedWs w, int tiles) {
+    __shared__ int start[SERVE_MAX_SEQ], dstart[SERVE_MAX_SEQ], ws[17];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, G = a.nh / a.nkv, TT = 128 / G, P = prefix_len(a), np = (P + 63) / 64;
+    auto scan = [&](int v, int& total) {  // exclusive, over the block
+        int inc = v;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(inc, o, 64);
+            if (lane >= o) inc += u;
+        }
+        __syncthreads();
+        if (lane == 63) ws[wave] = inc;
+        __syncthreads();
+        int before = inc - v;
+        total = 0;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            if (i < wave) before += ws[i];
+            total += ws[i];
+        }
+        return before;
+    };
+    int nt[4], nd[4], sum = 0, dsum = 0, ntiles, ndec;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int s = 4 * tid + i;
+        nt[i] = nd[i] = 0;
+        if (s < a.nseq) {
+            const int q0 = min(max(a.q_start[s], 0), a.t), qn = min(max(a.q_start[s + 1], q0), a.t) - q0;
+            if (qn * G > w.dr) nt[i] = (qn + TT - 1) / TT;
+            else nd[i] = qn;
+        }
+        sum += nt[i];
+        dsum += nd[i];
+    }
+    int at = scan(sum, ntiles), dat = scan(dsum, ndec);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if (4 * tid + i < a.nseq) {
+            start[4 * tid + i] = at;
+            dstart[4 * tid + i] = dat;
+        }
+        at += nt[i];
+        dat += nd[i];
+    }
+    __syncthreads();
+    auto find = [&](const int* v, int x) {  // the last sequence with v[s] <= x
+        int lo = 0, hi = a.nseq;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (v[mid] <= x) lo = mid;
+            else hi = mid;
+        }
+        return lo;
+    };
+    ntiles = min(ntiles, tiles);
+    ndec = min(ndec, a.t);
+    if (w.drows)
+        for (int i = tid; i < ndec; i += 1024) {
+            const int s = find(dstart, i);
+            w.drows[i] = min(max(a.q_start[s], 0) + i - dstart[s], a.t - 1);
+        }
+    PlanTile* plan = (PlanTile*)(w.plan + PLAN_HEAD);
+    int cum = 0;
+    for (int i0 = 0; i0 < ntiles; i0 += 1024) {
+        const int i = i0 + tid;
+        PlanTile p{};
+        if (i < ntiles) {
+            p.s = find(start, i);
+            const int q0 = min(max(a.q_start[p.s], 0), a.t), q1 = min(max(a.q_start[p.s + 1], q0), a.t);
+            p.t0 = q0 + (i - start[p.s]) * TT;
+            p.nt = min(TT, q1 - p.t0);
+            const Keys keys{nullptr, nullptr, P, np, (int)min((long long)max(a.len[p.s], 0), (long long)a.max_pages << a.page_shift)};
+            int first = INT_MAX, last = -1;
+            for (int t = 0; t < p.nt; t++) {
+                int lo, hi;
+                row_range(a, keys, a.pos[p.t0 + t], lo, hi);
+                first = min(first, lo);
+                last = max(last, hi);
+            }
+            p.kt0 = last < 0 ? 0 : first / 64;
+            p.nkt = last < 0 ? 1 : last / 64 + 1 - p.kt0;  // (rows without keys are written too: a tile that nothing of is computed)
+        }
+        int total;
+        p.cum = cum + scan(p.nkt, total);
+        cum += total;
+        if (i < ntiles) plan[i] = p;
+    }
+    if (tid == 0) {
+        w.plan[0] = ntiles;
+        w.plan[1] = cum;
+        w.plan[2] = ndec;
+    }
+}
+
+// The tile whose key tiles hold x (0 <= x < all), by a wave in rounds of 64 loads.
+__device__ __forceinline__ int tile_of(const PlanTile* plan, int n, int x) {
     const int lane = threadIdx.x & 63;
-    int lo = 0, n = a.nseq;
+    int lo = 0;
     while (n > 1) {
         const int step = (n + 63) / 64, i = lane * step;
-        const uint64_t le = __ballot(i < n && a.q_start[lo + i] <= r);
+        const uint64_t le = __ballot(i < n && plan[lo + min(i, n - 1)].cum <= x);
         const int k = le ? 63 - __builtin_clzll(le) : 0;
         lo += k * step;
         n = min(step, n - k * step);
     }
-    return lo;
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+__device__ __forceinline__ PlanTile plan_tile(const PlanTile* p) {
+    return PlanTile{sload(&p->s), sload(&p->t0), sload(&p->nt), sload(&p->kt0), sload(&p->cum), sload(&p->nkt)};
+}
+// The key tiles a block takes (at least 2: a piece costs its rows' sums).
+__device__ __forceinline__ long long tile_share(long long all, int blocks) { return max((all + blocks - 1) / blocks, 2ll); }
+
+template <int HD>
+__global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedAttn a, PagedWs w) {
+    __shared__ __align__(16) uint8_t lds[2 * PagedTile<HD>::BUF];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l32 = lane & 31;
+    const int G = a.nh / a.nkv, gs = 31 - __builtin_clz(G), P = prefix_len(a);
+    const PlanTile* plan = (const PlanTile*)(w.plan + PLAN_HEAD);
+    const int n = sload(w.plan), cost = sload(w.plan + 1);
+    const long long all = (long long)cost * a.nkv;
+    // block b takes the b-th run; neighbours in the list, which share keys, run on one XCD
+    const int b = (blockIdx.x & 7) * (w.tblocks / 8) + (blockIdx.x >> 3);
+    const long long share = tile_share(all, w.tblocks), W0 = b * share, W1 = min(W0 + share, all);
+    if (W0 >= W1) return;
+    int g = (int)(W0 / cost), i = tile_of(plan, n, (int)(W0 % cost));
+    for (long long at = W0; at < W1;) {
+        const PlanTile p = plan_tile(plan + i);
+        const long long start = (long long)g * cost + p.cum;
+        const int f = (int)(at - start), k = (int)min((long long)p.nkt - f, W1 - at);
+        const bool whole = k == p.nkt;
+        const Keys keys{a.prefix, a.tables + (uint64_t)p.s * a.max_pages, P, (P + 63) / 64,
+                        (int)min((long long)max(sload(a.len + p.s), 0), (long long)a.max_pages << a.page_shift)};
+        const int rr = 32 * wave + l32, tok = rr >> gs, h = g * G + (rr & (G - 1)), t = p.t0 + (tok < p.nt ? tok : 0);
+        const bool live = tok < p.nt;
+        int lo, hi;
+        row_range(a, keys, a.pos[t], lo, hi);
+        const uint64_t row = (uint64_t)t * a.nh + h;
+        const int kb = p.kt0 + f, ke = keys.P || keys.len ? kb + k : kb;
+        TileSums<HD> r;
+        tile_run<HD>(a, keys, lds, g, kb, ke, live, a.q + row * HD, lo, hi, r);
+        uint32_t again = tile_again<HD>(r, live);
+        const uint64_t slot = (uint64_t)(2 * b + (f == 0)) * 128;
+        if (live && !((again >> l32) & 1)) {
+            if (whole) {
+                tile_store<HD>(r, out_factor(a, h, r.m, r.l) * (1.0f / PF_SCALE), a.out + row * HD, a.qg ? a.qg + row * 2 * HD + HD : nullptr);
+            } else {
+                if (r.m != -INFINITY) tile_store<HD>(r, 1.0f / PF_SCALE, w.tacc + (slot + rr) * HD, nullptr);
+                if (lane < 32) w.tml[slot + rr] = make_float2(r.m, r.l);
+            }
+        }
+        for (; again; again &= again - 1) {
+            const int rb = 32 * wave + __builtin_ctz(again), tb = p.t0 + (rb >> gs), hb = g * G + (rb & (G - 1));
+            const uint64_t rowb = (uint64_t)tb * a.nh + hb;
+            row_range(a, keys, a.pos[tb], lo, hi);
+            float ac[HD / 64], mm, ll;
+            paged_row_again<HD>(a, keys, a.q + rowb * HD, g, max(lo, 64 * kb), min(hi, 64 * ke - 1), ac, mm, ll);
+            const float fo = whole ? out_factor(a, hb, mm, ll) : 1.0f;
+            float* dst = whole ? a.out + rowb * HD : w.tacc + (slot + rb) * HD;
+#pragma unroll
+            for (int d = 0; d < HD / 64; d++) {
+                const int col = lane + 64 * d;
+                dst[col] = whole && a.qg ? ac[d] * fo * sigmoid_f(a.qg[rowb * 2 * HD + HD + col]) : ac[d] * fo;
+            }
+            if (!whole && lane == 0) w.tml[slot + rb] = make_float2(mm, ll);
+        }
+        at += k;
+        if (f + k == p.nkt && ++i == n) i = 0, g++;
+    }
 }
 
-// Row r, query head h from its partial sums: out = sum_i acc_i 2^(m_i - M) / (sum_i l_i 2^(m_i - M) + 2^(sink - M)). Block
-// (x, heads y) of MW waves a head: wave v of a head takes partials v, v + MW, .. (the prefix's splits, then the own keys'
-// pieces or splits), their maxima a lane each, then the weighted rows with the loads of 8 in flight. DEC: x is row x % per of
-// sequence x / per, the sequences of the decode kernel; else x is a row, those of the tile kernel.
-template <int HD, int MW, bool DEC>
-__global__ __launch_bounds__(256) void attn_paged_merge_kernel(PagedAttn a, PagedWs w, int per) {
-    constexpr int DL = HD / 64, HPB = 4 / MW;
-    __shared__ float sm[HPB][MW], sl[HPB][MW], so[HPB][MW][HD];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int G = a.nh / a.nkv, P = prefix_len(a);
-    int s, r;
-    if constexpr (DEC) {
-        s = blockIdx.x / per;
-    } else {
-        r = blockIdx.x;
-        if (r >= a.q_start[a.nseq]) return;
-        s = __builtin_amdgcn_readfirstlane(row_seq(a, r));
-    }
-    const SeqInfo q = seq_info<true>(a, s, G, w.dr, P);
-    if constexpr (DEC) r = q.q0 + blockIdx.x % per;
-    const bool dec = q.qn * G <= w.dr;
-    if (r < q.q0 || r >= q.q0 + q.qn || dec != DEC) return;
-    const int hi = wave / MW, v = wave % MW;
-    for (int h = blockIdx.y * HPB + hi; h < a.nh; h += gridDim.y * HPB) {
-        const int g = h / G;
-        const uint64_t row = (uint64_t)r * a.nh + h;
-        const int np = P > 0 ? w.nsp : 0;
-        int no = 0;
-        uint64_t first = 0, step = 1;  // partial i >= np: row first + (i - np) step of (ml, acc)
-        const float2* oml = DEC ? w.dml : w.tml;
-        const float* oacc = DEC ? w.dacc : w.tacc;
-        if constexpr (DEC) {
-            if (q.nc > 0) {
-                const int2 mp = w.map[s * a.nkv + g];
-                no = mp.y;
-                first = (uint64_t)(mp.x + s * a.nkv + g) * w.dr + (r - q.q0) * G + h % G;
-                step = w.dr;
-            }
-        } else {
-            no = w.nst;
-            first = row * w.nst;
-        }
-        const int n = np + no;
+// Block b joins the tile that begins in block b's run and goes on past it: the pieces' sums of its 128 rows, a wave a row.
+template <int HD>
+__global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedAttn a, PagedWs w) {
+    constexpr int DL = HD / 64;
+    const PlanTile* plan = (const PlanTile*)(w.plan + PLAN_HEAD);
+    const int n = sload(w.plan), cost = sload(w.plan + 1), b = blockIdx.x;
+    const long long all = (long long)cost * a.nkv, share = tile_share(all, w.tblocks), W0 = b * share, W1 = W0 + share;
+    if (W1 >= all) return;
+    const int g = (int)(W1 / cost), i = tile_of(plan, n, (int)(W1 % cost));
+    const PlanTile p = plan_tile(plan + i);
+    const long long start = (long long)g * cost + p.cum;
+    if (start == W1 || start < W0) return;
+    const int last = (int)((start + p.nkt - 1) / share), lane = threadIdx.x & 63;  // pieces in blocks b .. last
+    const int G = a.nh / a.nkv, gs = 31 - __builtin_clz(G);
+    for (int rr = blockIdx.y * 4 + (threadIdx.x >> 6); rr < p.nt * G; rr += 4 * gridDim.y) {
         float M = -INFINITY, L = 0.0f, acc[DL];
 #pragma unroll
         for (int d = 0; d < DL; d++) acc[d] = 0.0f;
-        for (int i0 = v; i0 < n; i0 += 64 * MW) {
-            const int i = i0 + MW * lane;
-            float2 ml = make_float2(-INFINITY, 0.0f);
-            if (i < n) ml = i < np ? w.pml[row * np + i] : oml[first + (uint64_t)(i - np) * step];
-            const float mnew = fmaxf(M, wave_max64(ml.x));
-            const float e = ml.x == -INFINITY ? 0.0f : exp2_hw(ml.x - mnew), f = M == -INFINITY ? 0.0f : exp2_hw(M - mnew);
-            L = L * f + wave_sum64(ml.y * e);
+        for (int c = b; c <= last; c++) {
+            const uint64_t at = (uint64_t)(2 * c + (c == b)) * 128 + rr;
+            const float2 ml = w.tml[at];
+            float v[DL];
 #pragma unroll
-            for (int d = 0; d < DL; d++) acc[d] *= f;
+            for (int d = 0; d < DL; d++) v[d] = w.tacc[at * HD + DL * lane + d];
+            const float mnew = fmaxf(M, ml.x), f = M == -INFINITY ? 0.0f : exp2_hw(M - mnew), e = ml.x == -INFINITY ? 0.0f : exp2_hw(ml.x - mnew);
+            L = L * f + ml.y * (ml.x == -INFINITY ? 1.0f : e);  // (a piece without a maximum has a sum of 0, or not a number)
+#pragma unroll
+            for (int d = 0; d < DL; d++) acc[d] = acc[d] * f + (ml.x == -INFINITY ? 0.0f : v[d] * e);
             M = mnew;
-            const uint64_t some = __ballot(ml.x != -INFINITY);
-            const int cnt = some ? 64 - __builtin_clzll(some) : 0;
-            for (int j0 = 0; j0 < cnt; j0 += 8) {
-                float av[8][DL];
+        }
+        const int h = g * G + (rr & (G - 1));
+        const uint64_t row = (uint64_t)(p.t0 + (rr >> gs)) * a.nh + h;
+        const float f = out_factor(a, h, M, L);
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int ii = i0 + MW * (j0 + j);
-                    const bool has = j0 + j < 64 && ((some >> ((j0 + j) & 63)) & 1);
-                    const float* src = ii < np ? w.pacc + (row * np + ii) * HD : oacc + (first + (uint64_t)(ii - np) * step) * HD;
+        for (int d = 0; d < DL; d++) {
+            const int col = DL * lane + d;
+            const float x = acc[d] * f;
+            a.out[row * HD + col] = a.qg ? x * sigmoid_f(a.qg[row * 2 * HD + HD + col]) : x;
+        }
+    }
+}
+
+// ---------------- the join of a decode sequence's rows ----------------
+// Row x % per of sequence x / per, query head y from its partial sums: out = sum_i acc_i 2^(m_i - M) / (sum_i l_i 2^(m_i - M) +
+// 2^(sink - M)), the prefix's splits, then the own keys' pieces. Wave v of 4 takes partials v, v + 4, ..: the maxima a lane
+// each and the rows of the first 8 requested together (a launch is a chain of trips to memory: the sequence, then these).
+template <int HD>
+__global__ __launch_bounds__(256) void attn_paged_merge_kernel(PagedAttn a, PagedWs w, int per) {
+    constexpr int DL = HD / 64, MW = 4, U = 8;
+    __shared__ float sm[MW], sl[MW], so[MW][HD];
+    const int v = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int G = a.nh / a.nkv, s = blockIdx.x / per, h = blockIdx.y, g = h / G;
+    const int2* mp = w.map + s * a.nkv + g;
+    const int first = sload(&mp->x), pieces = sload(&mp->y), P = prefix_len(a);  // (not set, and not used, without own keys)
+    const SeqInfo q = seq_info<true>(a, s, G, w.dr, P);
+    const int r = q.q0 + blockIdx.x % per;
+    if (r >= q.q0 + q.qn || q.qn * G > w.dr) return;
+    const uint64_t row = (uint64_t)r * a.nh + h;
+    const int np = P > 0 ? w.nsp : 0, n = np + (q.nc > 0 ? pieces : 0);
+    const uint64_t own = (uint64_t)(first + s * a.nkv + g) * w.dr + (r - q.q0) * G + h % G;  // piece i of the own keys: own + i dr
+    auto at = [&](int i) { return i < np ? row * np + i : own + (uint64_t)(i - np) * w.dr; };
+    float M = -INFINITY, L = 0.0f, acc[DL];
 #pragma unroll
-                    for (int d = 0; d < DL; d++) av[j][d] = has ? src[DL * lane + d] : 0.0f;
-                }
+    for (int d = 0; d < DL; d++) acc[d] = 0.0f;
+    for (int i0 = v; i0 < n; i0 += 64 * MW) {
+        const int i = i0 + MW * lane;
+        float2 ml = make_float2(-INFINITY, 0.0f);
+        if (i < n) ml = (i < np ? w.pml : w.dml)[at(i)];
+        const int cnt = min((n - i0 + MW - 1) / MW, 64);
+        for (int j0 = 0; j0 < cnt; j0 += U) {
+            float av[U][DL];
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float es = __shfl(e, (j0 + j) & 63, 64);
+            for (int j = 0; j < U; j++) {  // (past the last partial: the first one again, with no weight)
+                const int ii = j0 + j < cnt ? i0 + MW * (j0 + j) : i0;
+                const float* src = (ii < np ? w.pacc : w.dacc) + at(ii) * HD;
 #pragma unroll
-                    for (int d = 0; d < DL; d++) acc[d] += av[j][d] * es;
-                }
+                for (int d = 0; d < DL; d++) av[j][d] = src[DL * lane + d];
+            }
+            if (j0 == 0) {
+                const float mnew = fmaxf(M, wave_max64(ml.x)), f = M == -INFINITY ? 0.0f : exp2_hw(M - mnew);
+                const float e = ml.x == -INFINITY ? 1.0f : exp2_hw(ml.x - mnew);  // (a partial without a maximum has a sum of 0, or not a number)
+                L = L * f + wave_sum64(ml.y * e);
+#pragma unroll
+                for (int d = 0; d < DL; d++) acc[d] *= f;
+                M = mnew;
+            }
+            const float e = exp2_hw(ml.x - M);
+            const uint64_t some = __ballot(ml.x != -INFINITY);  // (an empty partial's row is not written)
+#pragma unroll
+            for (int j = 0; j < U; j++) {
+                const float es = __shfl(e, (j0 + j) & 63, 64);
+                const bool has = j0 + j < cnt && ((some >> ((j0 + j) & 63)) & 1);
+#pragma unroll
+                for (int d = 0; d < DL; d++) acc[d] += has ? av[j][d] * es : 0.0f;
             }
         }
-        if constexpr (MW > 1) {
-            if (lane == 0) {
-                sm[hi][v] = M;
-                sl[hi][v] = L;
-            }
+    }
+    if (lane == 0) {
+        sm[v] = M;
+        sl[v] = L;
+    }
 #pragma unroll
-            for (int d = 0; d < DL; d++) so[hi][v][DL * lane + d] = acc[d];
-            __syncthreads();
-            float Mb = -INFINITY;
+    for (int d = 0; d < DL; d++) so[v][DL * lane + d] = acc[d];
+    __syncthreads();
+    if (v) return;
+    M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+    L = 0.0f;
 #pragma unroll
-            for (int u = 0; u < MW; u++) Mb = fmaxf(Mb, sm[hi][u]);
-            L = 0.0f;
+    for (int d = 0; d < DL; d++) acc[d] = 0.0f;
 #pragma unroll
-            for (int d = 0; d < DL; d++) acc[d] = 0.0f;
+    for (int u = 0; u < MW; u++) {
+        const float f = sm[u] == -INFINITY ? 1.0f : exp2_hw(sm[u] - M);
+        L += sl[u] * f;
 #pragma unroll
-            for (int u = 0; u < MW; u++) {
-                const float f = sm[hi][u] == -INFINITY ? 0.0f : exp2_hw(sm[hi][u] - Mb);
-                L += sl[hi][u] * f;
+        for (int d = 0; d < DL; d++) acc[d] += so[u][DL * lane + d] * f;
+    }
+    const float f = out_factor(a, h, M, L);
 #pragma unroll
-                for (int d = 0; d < DL; d++) acc[d] += so[hi][u][DL * lane + d] * f;
-            }
-            M = Mb;
-            __syncthreads();
-        }
-        if (MW == 1 || v == 0) {
-            const float sk = a.sink ? a.sink[h] * LOG2E : -INFINITY, Ms = fmaxf(M, sk);
-            const float sc = M == -INFINITY ? 0.0f : exp2_hw(M - Ms);
-            const float den = L * sc + (sk == -INFINITY ? 0.0f : exp2_hw(sk - Ms)), f = den == 0.0f ? 0.0f : sc / den;
-#pragma unroll
-            for (int d = 0; d < DL; d++) {
-                float x = acc[d] * f;
-                if (a.qg) x *= sigmoid_f(a.qg[row * 2 * HD + HD + DL * lane + d]);
-                a.out[row * HD + DL * lane + d] = x;
-            }
-        }
+    for (int d = 0; d < DL; d++) {
+        float x = acc[d] * f;
+        if (a.qg) x *= sigmoid_f(a.qg[row * 2 * HD + HD + DL * lane + d]);
+        a.out[row * HD + DL * lane + d] = x;
     }
 }
 
 // ---------------- launches ----------------
 static int div_up(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+// Tiles of the long sequences at most: each of them has more than dr / G rows.
+static int max_tiles(const PagedAttn& a, const PagedWs& w) {
+    const int G = a.nh / a.nkv;
+    return a.t / (128 / G) + std::min(a.nseq, a.t / (w.dr / G + 1)) + 1;
+}
 
 // The split plan and the workspace's layout from `at`; the end of the layout in *end.
 static PagedWs plan(const PagedAttn& a, uint8_t* at, size_t* end) {
@@ -959,15 +1132,10 @@ static PagedWs plan(const PagedAttn& a, uint8_t* at, size_t* end) {
     w.dr = (int)std::min<long long>(16 * w.nct, most_rows);
     const long long most = (long long)a.nseq * a.nkv * (((long long)a.max_pages << a.page_shift) / DEC_CHUNK + 1);
     w.dblocks = (int)std::min<long long>(most, w.nct == 1 ? 512 : 256);  // the blocks that run at once
-    // splits of the tile kernels: enough blocks for two a CU
-    auto splits = [&](long long tiles, long long keys) {
-        const long long blocks = tiles * a.nkv, want = div_up(512, std::max(blocks, 1ll));
-        return (int)std::max<long long>(1, std::min<long long>({want, (keys + 127) / 128, 64}));
-    };
-    w.nsp = splits(div_up(rows, 128), a.max_prefix);
-    const bool tiles = most_rows > w.dr;
-    w.nst = splits(div_up(rows, 128), (long long)a.max_pages << a.page_shift);
-    w.final_tiles = w.nst == 1 && !a.max_prefix;
+    // splits of the prefix: enough blocks for two a CU, of at least 128 keys
+    const long long blocks = std::max<long long>((long long)div_up(rows, 128) * a.nkv, 1);
+    w.nsp = (int)std::max<long long>(1, std::min<long long>({div_up(512, blocks), div_up(a.max_prefix, 128), 64}));
+    w.tblocks = 512;
     size_t o = 0;
     auto take = [&](size_t bytes) {
         uint8_t* p = at + o;
@@ -982,9 +1150,11 @@ static PagedWs plan(const PagedAttn& a, uint8_t* at, size_t* end) {
         w.pml = (float2*)take(out_rows * w.nsp * sizeof(float2));
         w.pacc = (float*)take(out_rows * w.nsp * a.hd * sizeof(float));
     }
-    if (tiles && !w.final_tiles) {
-        w.tml = (float2*)take(out_rows * w.nst * sizeof(float2));
-        w.tacc = (float*)take(out_rows * w.nst * a.hd * sizeof(float));
+    if (most_rows > w.dr) {
+        w.plan = (int*)take((PLAN_HEAD + (size_t)max_tiles(a, w) * (sizeof(PlanTile) / 4)) * 4);
+        if (a.max_prefix) w.drows = (int*)take((size_t)a.t * 4);
+        w.tml = (float2*)take((size_t)2 * w.tblocks * 128 * sizeof(float2));
+        w.tacc = (float*)take((size_t)2 * w.tblocks * 128 * a.hd * sizeof(float));
     }
     *end = o;
     return w;
@@ -998,24 +1168,21 @@ size_t paged_attn_ws_bytes(const PagedAttn& a) {
 
 template <int HD>
 static void launch_t(const PagedAttn& a, const PagedWs& w, hipStream_t s) {
-    const int G = a.nh / a.nkv, TT = 128 / G;
-    auto grid = [&](int tiles, int ns) { return dim3((unsigned)(8 * div_up((long long)a.nkv * ns, 8) * (long long)tiles)); };
-    if (a.max_prefix) {
-        const int tiles = div_up(a.t, TT);
-        attn_paged_tile_kernel<HD, true><<<grid(tiles, w.nsp), dim3(256), 0, s>>>(a, w, tiles);
+    const int G = a.nh / a.nkv, TT = 128 / G, per = w.dr / G;
+    if (w.plan) {
+        attn_paged_plan_kernel<<<dim3(1), dim3(1024), 0, s>>>(a, w, max_tiles(a, w));
+        attn_paged_tile_kernel<HD><<<dim3((unsigned)w.tblocks), dim3(256), 0, s>>>(a, w);
+        attn_paged_join_kernel<HD><<<dim3((unsigned)w.tblocks, 8), dim3(256), 0, s>>>(a, w);
     }
-    if ((long long)a.max_q * G > w.dr) {
-        // tiles of the long sequences: each has more than dr / G rows
-        const int tiles = (int)std::min<long long>((long long)a.t / TT + std::min<long long>(a.nseq, a.t / (w.dr / G + 1)), INT_MAX);
-        attn_paged_tile_kernel<HD, false><<<grid(std::max(tiles, 1), w.nst), dim3(256), 0, s>>>(a, w, std::max(tiles, 1));
+    if (a.max_prefix) {
+        const int tiles = div_up(w.plan ? std::min((long long)a.t, (long long)a.nseq * per) : a.t, TT);
+        attn_paged_prefix_kernel<HD><<<dim3((unsigned)(8 * div_up((long long)a.nkv * w.nsp, 8) * (long long)tiles)), dim3(256), 0, s>>>(a, w, tiles);
     }
     if (w.nct == 2)
         attn_paged_dec_kernel<HD, 2><<<dim3((unsigned)w.dblocks), dim3(256), 0, s>>>(a, w);
     else
         attn_paged_dec_kernel<HD, 1><<<dim3((unsigned)w.dblocks), dim3(256), 0, s>>>(a, w);
-    const int per = w.dr / G;
-    attn_paged_merge_kernel<HD, 4, true><<<dim3((unsigned)(a.nseq * per), (unsigned)a.nh), dim3(256), 0, s>>>(a, w, per);
-    if (w.tml) attn_paged_merge_kernel<HD, 1, false><<<dim3((unsigned)a.t, (unsigned)((a.nh + 3) / 4)), dim3(256), 0, s>>>(a, w, 0);
+    attn_paged_merge_kernel<HD><<<dim3((unsigned)(a.nseq * per), (unsigned)a.nh), dim3(256), 0, s>>>(a, w, per);
 }
 
 hipError_t launch_attn_paged(const PagedAttn& a, hipStream_t s) {
