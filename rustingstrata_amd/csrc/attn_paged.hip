@@ -493,44 +493,33 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attn_paged_dec_kernel(Pa
 // ---------------- many rows over the same keys ----------------
 // A block of 4 waves takes 128 query rows of one KV head (128 / G tokens x G heads, 32 rows a wave) over tiles of 64 keys, on
 // v_mfma_f32_32x32x16_f16 as attn_prefill_kernel of attn.hip does: S^T (32 keys x 32 rows, two sub-tiles) = K Q^T hi and lo,
-// an online softmax a column, O^T (32 dims x 32 rows) += V^T P^T hi and lo with V's rows read transposed from LDS. K and V
-// tiles alternate between two LDS buffers: while one is computed the next one's registers go to the other and the one after
-// is requested, so a tile costs one barrier.
+// an online softmax a column, O^T (32 dims x 32 rows) += V^T P^T hi and lo with V's rows read transposed from LDS.
+// The scores of a tile are computed beside the softmax of the one before, whose vector instructions fill the matrix
+// instructions' shadow; a tile costs one barrier. K and V go from memory straight to LDS (no registers hold them), two buffers
+// each: while tile t's V and tile t + 1's K are used, the next of each land.
+// Rows in LDS are HD halves apart without padding; 16-byte chunk c of row r sits at c ^ swz(r), which spreads both the score
+// fragments' reads (a chunk of 32 rows) and the transposed reads (4 chunks of 8 rows) over all banks.
 template <int HD>
 struct PagedTile {
-    static constexpr int BK = 64, KP = HD + 8, VP = HD + 32;  // halves a row: K's 16-byte reads, V's transposed reads spread over the banks
-    static constexpr int KB = BK * KP * 2, BUF = KB + BK * VP * 2;
+    static constexpr int BK = 64, ROW = 2 * HD, KB = BK * ROW, BUF = 2 * KB;  // bytes a row, of K's (or V's) tile, of both
+    __device__ static __forceinline__ int swz(int r) { return HD == 128 ? ((r & 3) << 2) | ((r >> 2) & 3) : ((r & 2) << 1) | ((r >> 2) & 3); }
 };
 
-// The softmax sums of a lane's row (column l32 of wave `wave`) over key tiles kb .. ke - 1.
+// The softmax sums of a lane's row (column l32 of wave `wave`) over key tiles kb .. ke - 1; o and l times TILE_SCALE.
+constexpr float TILE_SCALE = 16384.0f;
 template <int HD>
 struct TileSums {
     f16v o[HD / 32];
     float m, l;
 };
-// live: the lane has a row; qr: its query; lo, hi: the virtual keys that it sees.
+// live: the lane has a row; qr: its query; pos: its position.
 template <int HD>
 __device__ __forceinline__ void tile_run(const PagedAttn& a, const Keys& keys, uint8_t* lds, int g, int kb, int ke, bool live, const float* qr,
-                                         int lo, int hi, TileSums<HD>& r) {
+                                         int pos, TileSums<HD>& r) {
     using L = PagedTile<HD>;
-    typedef unsigned v4u __attribute__((ext_vector_type(4)));
-    constexpr int KS = HD / 16, DT = HD / 32, ND = HD / 8, BK = 64, NP = BK * ND / 256, ST = 256 / ND;  // chunks a thread, keys apart
+    constexpr int KS = HD / 16, DT = HD / 32, BK = 64, LPR = HD / 8, RPI = 64 / LPR, NJ = 16 / RPI;  // lanes a row, rows a load, loads
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l32 = lane & 31, hf = lane >> 5;
-    // the keys that the wave's rows see: outside of wlo .. whi none, inside maxlo .. minhi all of them all
-    int wlo = live ? lo : INT_MAX, whi = live ? hi : -1, maxlo = live && hi >= 0 ? lo : -1, minhi = live ? hi : INT_MAX;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        wlo = min(wlo, __shfl_xor(wlo, o, 64));
-        whi = max(whi, __shfl_xor(whi, o, 64));
-        maxlo = max(maxlo, __shfl_xor(maxlo, o, 64));
-        minhi = min(minhi, __shfl_xor(minhi, o, 64));
-    }
-    wlo = __builtin_amdgcn_readfirstlane(wlo);
-    whi = __builtin_amdgcn_readfirstlane(whi);
-    maxlo = __builtin_amdgcn_readfirstlane(maxlo);
-    minhi = __builtin_amdgcn_readfirstlane(minhi);
-    const int kk = tid / ND, col = 8 * (tid % ND);
-    const uint32_t kvd2 = 2 * a.nkv * HD, col2 = 2 * col;
+    const uint32_t kvd2 = 2 * a.nkv * HD;
     const uint64_t kg = (uint64_t)(a.kc + g * HD), vg = (uint64_t)(a.vc + g * HD);
     // Pages of a tile's four groups of 16 keys (a group lies in one page); past the last key its group's; a page outside the
     // pool is read as page 0 and its keys hidden.
@@ -542,57 +531,58 @@ __device__ __forceinline__ void tile_run(const PagedAttn& a, const Keys& keys, u
 #pragma unroll
         for (int u = 0; u < 4; u++) pg[u] = sload(table + (min(k0 + 16 * u, (n - 1) & ~15) >> a.page_shift));
     };
-    v4u kr[NP], vr[NP];
-    auto fetch = [&](int kt, const int (&pg)[4]) __attribute__((always_inline)) {
-        const bool pre = kt < keys.np;
-        const int k0 = BK * (pre ? kt : kt - keys.np), lim = (pre ? keys.P : keys.len) - 1 - k0;  // (keys past the last read its row)
-#pragma unroll
-        for (int u = 0; u < NP; u++) {
-            const int grp = ND == 16 ? u : 2 * u + (wave >> 1), g16 = min(16 * grp, lim & ~15);
-            const int p = grp == 0 ? pg[0] : grp == 1 ? pg[1] : grp == 2 ? pg[2] : pg[3];
-            const uint64_t at = (((uint64_t)((uint32_t)p < (uint32_t)a.n_pages ? p : 0) << a.page_shift) + ((k0 + g16) & ((1 << a.page_shift) - 1))) * kvd2;
-            const uint32_t off = __umul24(min(ST * u + kk, lim) - g16, kvd2) + col2;
-            kr[u] = *gptr<v4u>(kg + at + off);
-            vr[u] = *gptr<v4u>(vg + at + off);
-        }
-    };
-    auto stage = [&](int buf) __attribute__((always_inline)) {
-        uint16_t* ks = (uint16_t*)(lds + buf * L::BUF);
-        uint16_t* vs = (uint16_t*)(lds + buf * L::BUF + L::KB);
-#pragma unroll
-        for (int u = 0; u < NP; u++) {
-            *(v4u*)&ks[(kk + ST * u) * L::KP + col] = kr[u];
-            *(v4u*)&vs[(kk + ST * u) * L::VP + col] = vr[u];
-        }
-    };
     auto holes = [&](const int (&pg)[4]) __attribute__((always_inline)) {
         int h = 0;
 #pragma unroll
         for (int u = 0; u < 4; u++) h |= ((uint32_t)pg[u] >= (uint32_t)a.n_pages) << u;
         return h;
     };
-    int pg[4], hole = 0, hole1 = 0;
+    // A tile's rows of K (or V) into LDS: this wave its 16-key group `wave`, load j rows RPI j .. of it; past the last key its row
+    auto load = [&](int kt, const int (&pg)[4], uint64_t src, uint8_t* dst) __attribute__((always_inline)) {
+        const bool pre = kt < keys.np;
+        const int k0 = BK * (pre ? kt : kt - keys.np), lim = (pre ? keys.P : keys.len) - 1 - k0, g16 = min(16 * wave, lim & ~15);
+        const int p = wave == 0 ? pg[0] : wave == 1 ? pg[1] : wave == 2 ? pg[2] : pg[3];
+        const uint64_t at = src + (((uint64_t)((uint32_t)p < (uint32_t)a.n_pages ? p : 0) << a.page_shift) + ((k0 + g16) & ((1 << a.page_shift) - 1))) * kvd2;
+        uint32_t ln = lane;
+        asm volatile("" : "+v"(ln));
+#pragma unroll
+        for (int j = 0; j < NJ; j++) {
+            const int row = RPI * j + ln / LPR;  // of the group
+            const uint32_t off = __umul24(min(16 * wave + row, lim) - g16, kvd2) + 16 * ((ln % LPR) ^ L::swz(row));
+            load_lds16_so(at, off, dst + (16 * wave + RPI * j) * L::ROW);
+        }
+    };
+    // (the query's loads before the tiles', which the loop's first wait covers)
+    f4 qv[2 * KS];
+#pragma unroll
+    for (int k = 0; k < KS; k++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) qv[2 * k + e] = *(const f4*)(qr + 16 * k + 8 * hf + 4 * e);
+    uint8_t *kbuf = lds, *vbuf = lds + L::BUF;
+    int pg[4], hole = 0, hole1 = 0;  // pg: of the next tile to request; holes of the tiles whose scores are next, and after it
     if (kb < ke) {
         pages(kb, pg);
-        fetch(kb, pg);
+        load(kb, pg, kg, kbuf);
+        load(kb, pg, vg, vbuf);
         hole = holes(pg);
-        pages(kb + 1, pg);
+        if (kb + 1 < ke) {
+            pages(kb + 1, pg);
+            load(kb + 1, pg, kg, kbuf + L::KB);
+            hole1 = holes(pg);
+        }
     }
+    int lo, hi;  // the virtual keys that the lane's row sees
+    row_range(a, keys, pos, lo, hi);
     h8 qh[KS], ql[KS];
     float usc;
     {
-        f4 v[2 * KS];
         float mx = 0.0f;
 #pragma unroll
-        for (int k = 0; k < KS; k++)
+        for (int k = 0; k < 2 * KS; k++)
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                v[2 * k + e] = *(const f4*)(qr + 16 * k + 8 * hf + 4 * e);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    v[2 * k + e][i] = live ? v[2 * k + e][i] : 0.0f;
-                    mx = fmaxf(mx, fabsf(v[2 * k + e][i]));
-                }
+            for (int i = 0; i < 4; i++) {
+                qv[k][i] = live ? qv[k][i] : 0.0f;
+                mx = fmaxf(mx, fabsf(qv[k][i]));
             }
         mx = max_half(mx);
         int ex = 0;
@@ -600,108 +590,168 @@ __device__ __forceinline__ void tile_run(const PagedAttn& a, const Keys& keys, u
         const float up = ldexpf(1.0f, 14 - ex);
         usc = ldexpf(a.scale * LOG2E, ex - 14);
 #pragma unroll
-        for (int k = 0; k < KS; k++) split_q8(v[2 * k], v[2 * k + 1], up, qh[k], ql[k]);
+        for (int k = 0; k < KS; k++) split_q8(qv[2 * k], qv[2 * k + 1], up, qh[k], ql[k]);
     }
 #pragma unroll
     for (int d = 0; d < DT; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) r.o[d][i] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    if (kb < ke) {
-        stage(0);
-        if (kb + 1 < ke) {
-            fetch(kb + 1, pg);
-            hole1 = holes(pg);
-            pages(kb + 2, pg);
+    float m = -INFINITY, l = 0.0f, one = 1.0f;
+    asm("" : "+s"(one));  // (a product with it stays a mixed-precision multiply-add)
+    // this lane's addresses: K's fragment of sub-tile 0, k-step 0, V's transposed reads of dim tile 0 (opaque in each tile, so
+    // that the exclusive-ors of the other steps' are not kept in registers)
+    auto opaque = [](uint32_t v) __attribute__((always_inline)) {
+        asm volatile("" : "+v"(v));
+        return v;
+    };
+    const uint32_t kf0 = l32 * L::ROW + 16 * (hf ^ L::swz(l32));
+    const int i16 = lane & 15;
+    const uint32_t vf0 = (4 * hf + (i16 >> 2)) * L::ROW + 16 * ((((lane & 16) >> 3) + ((i16 & 3) >> 1)) ^ L::swz(4 * hf + (i16 >> 2))) + 8 * (i16 & 1);
+    // all of the wave's rows see keys maxlo .. minhi (both halves of a wave hold the same rows)
+    int maxlo = live && hi >= 0 ? lo : -1, minhi = live ? hi : INT_MAX;
+    static_for<0, 5>([&](auto S) {
+        constexpr int st = decltype(S)::value;
+        maxlo = max(maxlo, xl32<st>(maxlo));
+        minhi = min(minhi, xl32<st>(minhi));
+    });
+    maxlo = __builtin_amdgcn_readfirstlane(maxlo);
+    minhi = __builtin_amdgcn_readfirstlane(minhi);
+    f16v s[2];
+    float mx = -INFINITY;
+    auto scores = [&](int buf, f16v (&x)[2]) __attribute__((always_inline)) {
+        const uint8_t* kt = kbuf + buf * L::KB;
+        const uint32_t kf0o = opaque(kf0);
+        f16v z;
+#pragma unroll
+        for (int i = 0; i < 16; i++) z[i] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            const h8 f0 = *(const h8*)(kt + (kf0o ^ (32 * k))), f1 = *(const h8*)(kt + 32 * L::ROW + (kf0o ^ (32 * k)));
+            x[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f0, qh[k], k ? x[0] : z, 0, 0, 0);
+            x[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f1, qh[k], k ? x[1] : z, 0, 0, 0);
+            x[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f0, ql[k], x[0], 0, 0, 0);
+            x[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f1, ql[k], x[1], 0, 0, 0);
         }
-        lds_barrier();
-    }
-    for (int kt = kb; kt < ke; kt++) {
-        const int buf = (kt - kb) & 1;
-        const int now = hole;
-        if (kt + 1 < ke) {
-            stage(buf ^ 1);
-            hole = hole1;
-            if (kt + 2 < ke) {
-                fetch(kt + 2, pg);
-                hole1 = holes(pg);
-                pages(kt + 3, pg);
-            }
-        }
+    };
+    // keys that a row does not see (where a tile has such), and the column's largest score
+    auto mask = [&](int kt, int hole, f16v (&x)[2]) __attribute__((always_inline)) {
         const int k0 = BK * kt;
-        if (k0 <= whi && k0 + BK - 1 >= wlo) {
-            const uint16_t* ks = (const uint16_t*)(lds + buf * L::BUF);
-            const uint16_t* vs = (const uint16_t*)(lds + buf * L::BUF + L::KB);
-            f16v s[2], z;
-#pragma unroll
-            for (int i = 0; i < 16; i++) z[i] = 0.0f;
-#pragma unroll
-            for (int k = 0; k < KS; k++) {
-                const h8 k0f = *(const h8*)&ks[l32 * L::KP + 16 * k + 8 * hf], k1f = *(const h8*)&ks[(32 + l32) * L::KP + 16 * k + 8 * hf];
-                s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0f, qh[k], k ? s[0] : z, 0, 0, 0);
-                s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1f, qh[k], k ? s[1] : z, 0, 0, 0);
-                s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k0f, ql[k], s[0], 0, 0, 0);
-                s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k1f, ql[k], s[1], 0, 0, 0);
-            }
-            const bool tail = kt < keys.np && k0 + BK > keys.P;  // (the prefix's last tile, where it is not whole)
-            if (k0 + BK - 1 > minhi || k0 < maxlo || now || tail) {
-                const int top = tail ? min(hi, keys.P - 1) : hi;
-#pragma unroll
-                for (int mt = 0; mt < 2; mt++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int kp = 32 * mt + 8 * (i >> 2) + 4 * hf + (i & 3);
-                        if (k0 + kp > top || k0 + kp < lo || ((now >> (kp >> 4)) & 1)) s[mt][i] = -INFINITY;
-                    }
-            }
-            float mx = -INFINITY;
-#pragma unroll
-            for (int mt = 0; mt < 2; mt++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) mx = fmaxf(mx, s[mt][i]);
-            mx = max_half(mx);
-            const float mxs = mx * usc;
-            if (__ballot(mxs > m + 1.0f)) {  // (m follows the maximum when a weight would pass 2, column by column)
-                const float mnew = mxs > m + 1.0f ? mxs : m, alpha = m == -INFINITY ? 0.0f : exp2_hw(m - mnew);
-                l *= alpha;
-#pragma unroll
-                for (int d = 0; d < DT; d++) r.o[d] *= alpha;
-                m = mnew;
-            }
-            const float mref = m == -INFINITY ? 0.0f : m;
-            float sum = 0.0f;
+        const bool tail = kt < keys.np && k0 + BK > keys.P;  // (the prefix's last tile, where it is not whole)
+        if (k0 + BK - 1 > minhi || k0 < maxlo || hole || tail) {
+            const int top = tail ? min(hi, keys.P - 1) : hi;
 #pragma unroll
             for (int mt = 0; mt < 2; mt++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const float p = exp2_hw(__builtin_fmaf(s[mt][i], usc, -mref));
-                    s[mt][i] = p;
-                    sum += p;
-                }
-            l += sum;
-#pragma unroll
-            for (int mt = 0; mt < 2; mt++)
-#pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    float p[8];
-#pragma unroll
-                    for (int e = 0; e < 8; e++) p[e] = s[mt][8 * u + e];
-                    h8 ph, pl;
-                    split_w8(p, ph, pl);
-                    h8 vf[DT];
-#pragma unroll
-                    for (int d = 0; d < DT; d++) {
-                        const uint16_t* vp = &vs[(32 * mt + 16 * u + 4 * hf + ((lane & 15) >> 2)) * L::VP + 32 * d + (lane & 16) + 4 * (lane & 3)];
-                        const h4 v0 = read_tr(vp), v1 = read_tr(vp + 8 * L::VP);
-                        vf[d] = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
-                    }
-#pragma unroll
-                    for (int d = 0; d < DT; d++) r.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d], ph, r.o[d], 0, 0, 0);
-#pragma unroll
-                    for (int d = 0; d < DT; d++) r.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d], pl, r.o[d], 0, 0, 0);
+                    const int kp = 32 * mt + 8 * (i >> 2) + 4 * hf + (i & 3);
+                    if (k0 + kp > top || k0 + kp < lo || ((hole >> (kp >> 4)) & 1)) x[mt][i] = -INFINITY;
                 }
         }
+    };
+    auto largest = [&](const f16v (&x)[2]) __attribute__((always_inline)) {
+        float v = -INFINITY;
+#pragma unroll
+        for (int mt = 0; mt < 2; mt++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) v = fmaxf(v, x[mt][i]);
+        return max_half(v);
+    };
+    // one tile: its softmax beside the next one's scores, then its V products; NEXT: there is a next one
+    auto tile = [&](int kt, auto NEXT) __attribute__((always_inline)) {
+        constexpr bool next = decltype(NEXT)::value;
+        const int buf = (kt - kb) & 1;
+        if constexpr (next) {
+            // (pg: tile kt + 1's pages; its V, and the K of the one after)
+            load(kt + 1, pg, vg, vbuf + (buf ^ 1) * L::KB);
+            if (kt + 2 < ke) {
+                pages(kt + 2, pg);
+                load(kt + 2, pg, kg, kbuf + buf * L::KB);
+            }
+        }
+        const float mxs = mx * usc;
+        if (__ballot(mxs > m + 1.0f)) {  // (m follows the maximum when a weight would pass 2, column by column)
+            const float mnew = mxs > m + 1.0f ? mxs : m, alpha = m == -INFINITY ? 0.0f : exp2_hw(m - mnew);
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; d++) r.o[d] *= alpha;
+            m = mnew;
+        }
+        const float mref = (m == -INFINITY ? 0.0f : m) - 14.0f;  // (the weights times TILE_SCALE)
+        // the softmax of this tile's 32 values, 32 / KS a step, beside the four matrix instructions of a step of the next one's
+        // scores, whose fragments are read a step ahead
+        f16v x[2];
+        h8 ph[4], pl[4], kf[2][2];
+        const uint8_t* kn = kbuf + (buf ^ 1) * L::KB;
+        const uint32_t kf0o = opaque(kf0);
+        auto frag = [&](int k) __attribute__((always_inline)) {
+            kf[k & 1][0] = *(const h8*)(kn + (kf0o ^ (32 * k)));
+            kf[k & 1][1] = *(const h8*)(kn + 32 * L::ROW + (kf0o ^ (32 * k)));
+        };
+        if constexpr (next) {
+            frag(0);
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[0][i] = x[1][i] = 0.0f;
+        }
+#pragma unroll
+        for (int k = 0; k < KS; k++) {
+            if constexpr (next) {
+                if (k + 1 < KS) frag(k + 1);
+                x[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k & 1][0], qh[k], x[0], 0, 0, 0);
+                x[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k & 1][1], qh[k], x[1], 0, 0, 0);
+                x[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k & 1][0], ql[k], x[0], 0, 0, 0);
+                x[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[k & 1][1], ql[k], x[1], 0, 0, 0);
+            }
+#pragma unroll
+            for (int v = 32 / KS * k; v < 32 / KS * (k + 1); v += 2) {
+                const int b = v >> 3, e = v & 7;
+                const float p0 = exp2_hw(__builtin_fmaf(s[b >> 1][8 * (b & 1) + e], usc, -mref));
+                const float p1 = exp2_hw(__builtin_fmaf(s[b >> 1][8 * (b & 1) + e + 1], usc, -mref));
+                l += p0;
+                l += p1;
+                const auto h = __builtin_amdgcn_cvt_pkrtz(p0, p1);
+                ph[b][e] = (_Float16)h[0];
+                ph[b][e + 1] = (_Float16)h[1];
+                pl[b][e] = (_Float16)__builtin_fmaf(p0, one, -(float)h[0]);
+                pl[b][e + 1] = (_Float16)__builtin_fmaf(p1, one, -(float)h[1]);
+            }
+        }
+        const uint8_t* vt = vbuf + buf * L::KB;
+        const uint32_t vf0o = opaque(vf0);
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+            h8 vf[DT];
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                const h4 v0 = read_tr((const uint16_t*)(vt + 16 * b * L::ROW + (vf0o ^ (64 * d))));
+                const h4 v1 = read_tr((const uint16_t*)(vt + (16 * b + 8) * L::ROW + (vf0o ^ (64 * d) ^ 32)));
+                vf[d] = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+#pragma unroll
+            for (int d = 0; d < DT; d++) r.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d], ph[b], r.o[d], 0, 0, 0);
+#pragma unroll
+            for (int d = 0; d < DT; d++) r.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[d], pl[b], r.o[d], 0, 0, 0);
+        }
+        if constexpr (next) {
+            s[0] = x[0];
+            s[1] = x[1];
+            wait_loads();
+            lds_barrier();
+            mask(kt + 1, hole1, s);
+            hole1 = holes(pg);
+            mx = largest(s);
+        }
+    };
+    if (kb < ke) {
+        wait_loads();
         lds_barrier();
+        scores(0, s);
+        mask(kb, hole, s);
+        mx = largest(s);
+        // (the K of tile kb has been read by all waves before tile kb + 2's may land on it)
+        lds_barrier();
+        for (int kt = kb; kt + 1 < ke; kt++) tile(kt, std::integral_constant<bool, true>{});
+        tile(ke - 1, std::integral_constant<bool, false>{});
+        lds_barrier();  // (the buffers are free for what comes next)
     }
     r.l = l + __shfl_xor(l, 32, 64);
     r.m = m;
@@ -727,22 +777,33 @@ __device__ __forceinline__ float out_factor(const PagedAttn& a, int h, float m, 
     const float den = l * sc + (sk == -INFINITY ? 0.0f : exp2_hw(sk - M));
     return den == 0.0f ? 0.0f : sc / den;
 }
-// This lane's half of its row: times f into dst, through the gate.
-template <int HD>
-__device__ __forceinline__ void tile_store(const TileSums<HD>& r, float f, float* dst, const float* gate) {
-    const int hf = (threadIdx.x >> 5) & 1;
+// The wave's rows times their factors f, from the fragments' layout (16 bytes of a row a lane) through LDS (free of tiles) to
+// whole rows: row r (0 .. 31, a bit of `rows`) to dst(r), through gate(r) where there is one. Chunk c of row r sits at c ^ r.
+template <int HD, typename D, typename G>
+__device__ __forceinline__ void tile_store(const TileSums<HD>& r, int tid, float f, uint8_t* lds, uint32_t rows, D&& dst, G&& gate) {
+    constexpr int NC = HD / 4, RPL = 64 / NC;  // chunks a row, rows a load
+    const int lane = tid & 63, l32 = lane & 31, hf = lane >> 5;
+    uint8_t* mine = lds + (tid >> 6) * (32 * 4 * HD);
 #pragma unroll
     for (int d = 0; d < HD / 32; d++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const int col = 32 * d + 8 * j + 4 * hf;
-            float4 v = make_float4(r.o[d][4 * j] * f, r.o[d][4 * j + 1] * f, r.o[d][4 * j + 2] * f, r.o[d][4 * j + 3] * f);
-            if (gate) {
-                v.x *= sigmoid_f(gate[col]); v.y *= sigmoid_f(gate[col + 1]);
-                v.z *= sigmoid_f(gate[col + 2]); v.w *= sigmoid_f(gate[col + 3]);
+        for (int j = 0; j < 4; j++)
+            *(float4*)(mine + l32 * 4 * HD + 16 * ((8 * d + 2 * j + hf) ^ (l32 & (NC - 1)))) =
+                make_float4(r.o[d][4 * j] * f, r.o[d][4 * j + 1] * f, r.o[d][4 * j + 2] * f, r.o[d][4 * j + 3] * f);
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 4
+    for (int i = 0; i < 32 / RPL; i++) {
+        const int row = RPL * i + lane / NC, c = (lane % NC) ^ (row & (NC - 1));
+        if ((rows >> row) & 1) {
+            float4 v = *(const float4*)(mine + row * 4 * HD + 16 * (lane % NC));
+            if (const float* gt = gate(row)) {
+                const float4 x = *(const float4*)(gt + 4 * c);
+                v.x *= sigmoid_f(x.x); v.y *= sigmoid_f(x.y); v.z *= sigmoid_f(x.z); v.w *= sigmoid_f(x.w);
             }
-            *(float4*)(dst + col) = v;
+            *(float4*)(dst(row) + 4 * c) = v;
         }
+    }
+    __builtin_amdgcn_wave_barrier();
 }
 
 // The prefix for the rows of decode sequences: tiles of the call's rows (of the plan's list of them, where there is a plan)
@@ -766,15 +827,16 @@ __global__ __launch_bounds__(256, 2) void attn_paged_prefix_kernel(PagedAttn a, 
     const bool live = tok < nt;
     auto row_of = [&](int t) { return w.drows ? w.drows[tt * TT + t] : tt * TT + t; };
     const int t = row_of(live ? tok : 0);
+    const int pos = a.pos[t];
     int lo, hi;
-    row_range(a, keys, a.pos[t], lo, hi);
+    row_range(a, keys, pos, lo, hi);
     // the tiles that the block's rows see
     int blo = live ? lo : INT_MAX, bhi = live ? hi : -1;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        blo = min(blo, __shfl_xor(blo, o, 64));
-        bhi = max(bhi, __shfl_xor(bhi, o, 64));
-    }
+    static_for<0, 5>([&](auto S) {
+        constexpr int st = decltype(S)::value;
+        blo = min(blo, xl32<st>(blo));
+        bhi = max(bhi, xl32<st>(bhi));
+    });
     if (lane == 0) {
         ws[wave] = blo;
         ws[4 + wave] = bhi;
@@ -786,12 +848,14 @@ __global__ __launch_bounds__(256, 2) void attn_paged_prefix_kernel(PagedAttn a, 
     const int kb = min(kt0 + split * per, kt1), ke = min(kb + per, kt1);
     const uint64_t row = (uint64_t)t * a.nh + h;
     TileSums<HD> r;
-    tile_run<HD>(a, keys, lds, g, kb, ke, live, a.q + row * HD, lo, hi, r);
+    tile_run<HD>(a, keys, lds, g, kb, ke, live, a.q + row * HD, pos, r);
     uint32_t again = tile_again<HD>(r, live);
-    if (live && !((again >> l32) & 1)) {
-        if (r.m != -INFINITY) tile_store<HD>(r, 1.0f / PF_SCALE, w.pacc + (row * ns + split) * HD, nullptr);
-        if (lane < 32) w.pml[row * ns + split] = make_float2(r.m, r.l);
-    }
+    const uint32_t rows = (uint32_t)__ballot(live) & ~again;
+    tile_store<HD>(r, tid, 1.0f / TILE_SCALE, lds, rows, [&](int i) {
+        const int rb = 32 * wave + i;
+        return w.pacc + (((uint64_t)row_of(rb >> gs) * a.nh + g * G + (rb & (G - 1))) * ns + split) * HD;
+    }, [](int) { return (const float*)nullptr; });
+    if (lane < 32 && ((rows >> l32) & 1)) w.pml[row * ns + split] = make_float2(r.m, r.l * (1.0f / TILE_SCALE));
     for (; again; again &= again - 1) {
         const int rb = 32 * wave + __builtin_ctz(again), tb = row_of(rb >> gs);
         const uint64_t rowb = (uint64_t)tb * a.nh + g * G + (rb & (G - 1));
@@ -810,9 +874,12 @@ __global__ __launch_bounds__(256, 2) void attn_paged_prefix_kernel(PagedAttn a, 
 // its block; of one cut by a run's end each block leaves its sums (the piece from a tile's start at slot 2 b + 1, one that goes
 // on from the run before at 2 b), and attn_paged_join_kernel joins them.
 struct PlanTile {
-    int s, t0, nt, kt0, cum, nkt;  // sequence, first row, rows; first key tile, key tiles before this tile's, its key tiles
+    int s, t0, nt, len;  // sequence, first row, rows, own keys
+    int kt0, nkt, cum, pad;  // first key tile, key tiles; work of the tiles before
 };
-constexpr int PLAN_HEAD = 4;  // tiles, key tiles of all, rows of decode sequences
+constexpr int PLAN_HEAD = 4;  // tiles, their work, rows of decode sequences
+// A tile's work in key tiles: those it has, and what it takes to begin and end one (9 + 4 us beside 4 a key tile).
+constexpr int TILE_EXTRA = 3;
 
 // One block of 1024 threads: the sequences' tiles by a scan in LDS, then the tiles' keys and their scan, 1024 tiles at a time.
 __global__ __launch_bounds__(1024) void attn_paged_plan_kernel(PagedAttn a, PagedWs w, int tiles) {
@@ -887,19 +954,26 @@ __global__ __launch_bounds__(1024) void attn_paged_plan_kernel(PagedAttn a, Page
             const int q0 = min(max(a.q_start[p.s], 0), a.t), q1 = min(max(a.q_start[p.s + 1], q0), a.t);
             p.t0 = q0 + (i - start[p.s]) * TT;
             p.nt = min(TT, q1 - p.t0);
-            const Keys keys{nullptr, nullptr, P, np, (int)min((long long)max(a.len[p.s], 0), (long long)a.max_pages << a.page_shift)};
+            p.len = (int)min((long long)max(a.len[p.s], 0), (long long)a.max_pages << a.page_shift);
+            const Keys keys{nullptr, nullptr, P, np, p.len};
             int first = INT_MAX, last = -1;
-            for (int t = 0; t < p.nt; t++) {
-                int lo, hi;
-                row_range(a, keys, a.pos[p.t0 + t], lo, hi);
-                first = min(first, lo);
-                last = max(last, hi);
+            for (int t = 0; t < p.nt; t += 16) {
+                int pos[16];
+#pragma unroll
+                for (int e = 0; e < 16; e++) pos[e] = a.pos[p.t0 + min(t + e, p.nt - 1)];
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    int lo, hi;
+                    row_range(a, keys, pos[e], lo, hi);
+                    first = min(first, lo);
+                    last = max(last, hi);
+                }
             }
             p.kt0 = last < 0 ? 0 : first / 64;
             p.nkt = last < 0 ? 1 : last / 64 + 1 - p.kt0;  // (rows without keys are written too: a tile that nothing of is computed)
         }
         int total;
-        p.cum = cum + scan(p.nkt, total);
+        p.cum = cum + scan(i < ntiles ? p.nkt + TILE_EXTRA : 0, total);
         cum += total;
         if (i < ntiles) plan[i] = p;
     }
@@ -910,7 +984,7 @@ __global__ __launch_bounds__(1024) void attn_paged_plan_kernel(PagedAttn a, Page
     }
 }
 
-// The tile whose key tiles hold x (0 <= x < all), by a wave in rounds of 64 loads.
+// The tile whose work holds x (0 <= x < all), by a wave in rounds of 64 loads.
 __device__ __forceinline__ int tile_of(const PlanTile* plan, int n, int x) {
     const int lane = threadIdx.x & 63;
     int lo = 0;
@@ -924,52 +998,71 @@ __device__ __forceinline__ int tile_of(const PlanTile* plan, int n, int x) {
     return __builtin_amdgcn_readfirstlane(lo);
 }
 __device__ __forceinline__ PlanTile plan_tile(const PlanTile* p) {
-    return PlanTile{sload(&p->s), sload(&p->t0), sload(&p->nt), sload(&p->kt0), sload(&p->cum), sload(&p->nkt)};
+    return PlanTile{sload(&p->s), sload(&p->t0), sload(&p->nt), sload(&p->len), sload(&p->kt0), sload(&p->nkt), sload(&p->cum), 0};
 }
-// The key tiles a block takes (at least 2: a piece costs its rows' sums).
-__device__ __forceinline__ long long tile_share(long long all, int blocks) { return max((all + blocks - 1) / blocks, 2ll); }
+// Where block b's run of the list begins: at b times an equal share of the work, moved to the tile's border where no more than
+// an eighth of the share, and no more than 3 key tiles, lie between: a tile that is not cut costs no sums.
+struct RunAt {
+    long long at;  // in the list of all tiles' work
+    int g, i, f;   // the KV head, the tile, the key tile of it
+};
+__device__ __forceinline__ RunAt run_at(const PlanTile* plan, int n, int cost, int nkv, int b, int blocks) {
+    const long long all = (long long)cost * nkv, share = max((all + blocks - 1) / blocks, 2ll);
+    RunAt r{min(b * share, all), nkv, 0, 0};
+    if (r.at == all) return r;
+    r.g = (int)(r.at / cost);
+    const int x = (int)(r.at - (long long)r.g * cost), near = (int)min(share / 8, 3ll);
+    r.i = tile_of(plan, n, x);
+    const int cum = sload(&plan[r.i].cum), nkt = sload(&plan[r.i].nkt), f = x - cum - TILE_EXTRA;
+    if (f <= near) {
+        r.at -= x - cum;
+    } else if (nkt - f <= near) {
+        r.at += cum + TILE_EXTRA + nkt - x;
+        if (++r.i == n) r.i = 0, r.g++;
+    } else {
+        r.f = f;
+    }
+    return r;
+}
 
 template <int HD>
 __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedAttn a, PagedWs w) {
     __shared__ __align__(16) uint8_t lds[2 * PagedTile<HD>::BUF];
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l32 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int G = a.nh / a.nkv, gs = 31 - __builtin_clz(G), P = prefix_len(a);
     const PlanTile* plan = (const PlanTile*)(w.plan + PLAN_HEAD);
     const int n = sload(w.plan), cost = sload(w.plan + 1);
-    const long long all = (long long)cost * a.nkv;
+    if (!n) return;
     // block b takes the b-th run; neighbours in the list, which share keys, run on one XCD
     const int b = (blockIdx.x & 7) * (w.tblocks / 8) + (blockIdx.x >> 3);
-    const long long share = tile_share(all, w.tblocks), W0 = b * share, W1 = min(W0 + share, all);
-    if (W0 >= W1) return;
-    int g = (int)(W0 / cost), i = tile_of(plan, n, (int)(W0 % cost));
-    for (long long at = W0; at < W1;) {
+    const RunAt from = run_at(plan, n, cost, a.nkv, b, w.tblocks), to = run_at(plan, n, cost, a.nkv, b + 1, w.tblocks);
+    for (int g = from.g, i = from.i, f = from.f; g < to.g || (g == to.g && (i < to.i || (i == to.i && f < to.f)));) {
         const PlanTile p = plan_tile(plan + i);
-        const long long start = (long long)g * cost + p.cum;
-        const int f = (int)(at - start), k = (int)min((long long)p.nkt - f, W1 - at);
+        const int k = (g == to.g && i == to.i ? to.f : p.nkt) - f;
         const bool whole = k == p.nkt;
-        const Keys keys{a.prefix, a.tables + (uint64_t)p.s * a.max_pages, P, (P + 63) / 64,
-                        (int)min((long long)max(sload(a.len + p.s), 0), (long long)a.max_pages << a.page_shift)};
-        const int rr = 32 * wave + l32, tok = rr >> gs, h = g * G + (rr & (G - 1)), t = p.t0 + (tok < p.nt ? tok : 0);
-        const bool live = tok < p.nt;
-        int lo, hi;
-        row_range(a, keys, a.pos[t], lo, hi);
-        const uint64_t row = (uint64_t)t * a.nh + h;
+        const Keys keys{a.prefix, a.tables + (uint64_t)p.s * a.max_pages, P, (P + 63) / 64, p.len};
         const int kb = p.kt0 + f, ke = keys.P || keys.len ? kb + k : kb;
         TileSums<HD> r;
-        tile_run<HD>(a, keys, lds, g, kb, ke, live, a.q + row * HD, lo, hi, r);
+        {
+            const int rr = 32 * wave + (threadIdx.x & 31), tok = rr >> gs, h = g * G + (rr & (G - 1)), t = p.t0 + (tok < p.nt ? tok : 0);
+            tile_run<HD>(a, keys, lds, g, kb, ke, tok < p.nt, a.q + ((uint64_t)t * a.nh + h) * HD, a.pos[t], r);
+        }
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));  // (nothing of this lane's row waits in registers while the tiles run)
+        const int lane = tid & 63, l32 = lane & 31, rr = 32 * wave + l32, h = g * G + (rr & (G - 1));
+        const bool live = (rr >> gs) < p.nt;
         uint32_t again = tile_again<HD>(r, live);
         const uint64_t slot = (uint64_t)(2 * b + (f == 0)) * 128;
-        if (live && !((again >> l32) & 1)) {
-            if (whole) {
-                tile_store<HD>(r, out_factor(a, h, r.m, r.l) * (1.0f / PF_SCALE), a.out + row * HD, a.qg ? a.qg + row * 2 * HD + HD : nullptr);
-            } else {
-                if (r.m != -INFINITY) tile_store<HD>(r, 1.0f / PF_SCALE, w.tacc + (slot + rr) * HD, nullptr);
-                if (lane < 32) w.tml[slot + rr] = make_float2(r.m, r.l);
-            }
-        }
+        const uint32_t rows = (uint32_t)__ballot(live) & ~again;
+        auto row_at = [&](int i) { return (uint64_t)(p.t0 + ((32 * wave + i) >> gs)) * a.nh + g * G + (i & (G - 1)); };
+        tile_store<HD>(r, tid, (whole ? out_factor(a, h, r.m, r.l * (1.0f / TILE_SCALE)) : 1.0f) * (1.0f / TILE_SCALE), lds, rows,
+                       [&](int i) { return whole ? a.out + row_at(i) * HD : w.tacc + (slot + 32 * wave + i) * HD; },
+                       [&](int i) { return whole && a.qg ? a.qg + row_at(i) * 2 * HD + HD : (const float*)nullptr; });
+        if (!whole && lane < 32 && ((rows >> l32) & 1)) w.tml[slot + rr] = make_float2(r.m, r.l * (1.0f / TILE_SCALE));
         for (; again; again &= again - 1) {
             const int rb = 32 * wave + __builtin_ctz(again), tb = p.t0 + (rb >> gs), hb = g * G + (rb & (G - 1));
             const uint64_t rowb = (uint64_t)tb * a.nh + hb;
+            int lo, hi;
             row_range(a, keys, a.pos[tb], lo, hi);
             float ac[HD / 64], mm, ll;
             paged_row_again<HD>(a, keys, a.q + rowb * HD, g, max(lo, 64 * kb), min(hi, 64 * ke - 1), ac, mm, ll);
@@ -982,50 +1075,75 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedAttn a, Pa
             }
             if (!whole && lane == 0) w.tml[slot + rb] = make_float2(mm, ll);
         }
-        at += k;
-        if (f + k == p.nkt && ++i == n) i = 0, g++;
+        f += k;
+        if (f == p.nkt) {
+            f = 0;
+            if (++i == n) i = 0, g++;
+        }
+        lds_barrier();  // (the rows have left LDS)
     }
 }
 
-// Block b joins the tile that begins in block b's run and goes on past it: the pieces' sums of its 128 rows, a wave a row.
+// Block b joins the tile that begins in block b's run and goes on past it: the pieces' sums of its 128 rows, 4 rows a wave at a
+// time with their loads in flight together.
 template <int HD>
 __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedAttn a, PagedWs w) {
-    constexpr int DL = HD / 64;
+    constexpr int NC = HD / 4, RPW = 64 / NC, U = 4;  // lanes a row (16 bytes each), rows a wave and load, loads
     const PlanTile* plan = (const PlanTile*)(w.plan + PLAN_HEAD);
-    const int n = sload(w.plan), cost = sload(w.plan + 1), b = blockIdx.x;
-    const long long all = (long long)cost * a.nkv, share = tile_share(all, w.tblocks), W0 = b * share, W1 = W0 + share;
-    if (W1 >= all) return;
-    const int g = (int)(W1 / cost), i = tile_of(plan, n, (int)(W1 % cost));
-    const PlanTile p = plan_tile(plan + i);
-    const long long start = (long long)g * cost + p.cum;
-    if (start == W1 || start < W0) return;
-    const int last = (int)((start + p.nkt - 1) / share), lane = threadIdx.x & 63;  // pieces in blocks b .. last
-    const int G = a.nh / a.nkv, gs = 31 - __builtin_clz(G);
-    for (int rr = blockIdx.y * 4 + (threadIdx.x >> 6); rr < p.nt * G; rr += 4 * gridDim.y) {
-        float M = -INFINITY, L = 0.0f, acc[DL];
+    const int n = sload(w.plan), cost = sload(w.plan + 1), b = blockIdx.x, lane = threadIdx.x & 63;
+    if (!n) return;
+    const RunAt end = run_at(plan, n, cost, a.nkv, b + 1, w.tblocks);
+    if (end.g >= a.nkv || end.f == 0) return;  // (no tile is cut there)
+    const RunAt from = run_at(plan, n, cost, a.nkv, b, w.tblocks);
+    if (from.g == end.g && from.i == end.i && from.f > 0) return;  // (it began before this block's run)
+    const PlanTile p = plan_tile(plan + end.i);
+    int last = b + 1;  // pieces in blocks b .. last
+    for (RunAt to; to = run_at(plan, n, cost, a.nkv, last + 1, w.tblocks), to.g == end.g && to.i == end.i;) last++;
+    const int G = a.nh / a.nkv, gs = 31 - __builtin_clz(G), nr = p.nt * G, col = 4 * (lane % NC);
+    const int r0 = (blockIdx.y * 4 + (threadIdx.x >> 6)) * U * RPW + lane / NC;
+    float M[U], L[U];
+    float4 acc[U];
 #pragma unroll
-        for (int d = 0; d < DL; d++) acc[d] = 0.0f;
-        for (int c = b; c <= last; c++) {
-            const uint64_t at = (uint64_t)(2 * c + (c == b)) * 128 + rr;
-            const float2 ml = w.tml[at];
-            float v[DL];
+    for (int u = 0; u < U; u++) {
+        M[u] = -INFINITY;
+        L[u] = 0.0f;
+        acc[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    for (int c = b; c <= last; c++) {
+        float2 ml[U];
+        float4 v[U];
 #pragma unroll
-            for (int d = 0; d < DL; d++) v[d] = w.tacc[at * HD + DL * lane + d];
-            const float mnew = fmaxf(M, ml.x), f = M == -INFINITY ? 0.0f : exp2_hw(M - mnew), e = ml.x == -INFINITY ? 0.0f : exp2_hw(ml.x - mnew);
-            L = L * f + ml.y * (ml.x == -INFINITY ? 1.0f : e);  // (a piece without a maximum has a sum of 0, or not a number)
-#pragma unroll
-            for (int d = 0; d < DL; d++) acc[d] = acc[d] * f + (ml.x == -INFINITY ? 0.0f : v[d] * e);
-            M = mnew;
+        for (int u = 0; u < U; u++) {
+            const uint64_t at = (uint64_t)(2 * c + (c == b)) * 128 + min(r0 + u * RPW, nr - 1);
+            ml[u] = w.tml[at];
+            v[u] = *(const float4*)(w.tacc + at * HD + col);
         }
-        const int h = g * G + (rr & (G - 1));
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const float mnew = fmaxf(M[u], ml[u].x), f = M[u] == -INFINITY ? 0.0f : exp2_hw(M[u] - mnew);
+            const bool none = ml[u].x == -INFINITY;  // (a piece without a maximum has a sum of 0, or not a number)
+            const float e = none ? 0.0f : exp2_hw(ml[u].x - mnew);
+            L[u] = L[u] * (M[u] == -INFINITY ? 1.0f : f) + (none ? ml[u].y : ml[u].y * e);
+            acc[u].x = acc[u].x * f + (none ? 0.0f : v[u].x * e);
+            acc[u].y = acc[u].y * f + (none ? 0.0f : v[u].y * e);
+            acc[u].z = acc[u].z * f + (none ? 0.0f : v[u].z * e);
+            acc[u].w = acc[u].w * f + (none ? 0.0f : v[u].w * e);
+            M[u] = mnew;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int rr = r0 + u * RPW;
+        if (rr >= nr) continue;
+        const int h = end.g * G + (rr & (G - 1));
         const uint64_t row = (uint64_t)(p.t0 + (rr >> gs)) * a.nh + h;
-        const float f = out_factor(a, h, M, L);
-#pragma unroll
-        for (int d = 0; d < DL; d++) {
-            const int col = DL * lane + d;
-            const float x = acc[d] * f;
-            a.out[row * HD + col] = a.qg ? x * sigmoid_f(a.qg[row * 2 * HD + HD + col]) : x;
+        const float f = out_factor(a, h, M[u], L[u]);
+        float4 x = make_float4(acc[u].x * f, acc[u].y * f, acc[u].z * f, acc[u].w * f);
+        if (a.qg) {
+            const float* gt = a.qg + row * 2 * HD + HD + col;
+            x.x *= sigmoid_f(gt[0]); x.y *= sigmoid_f(gt[1]); x.z *= sigmoid_f(gt[2]); x.w *= sigmoid_f(gt[3]);
         }
+        *(float4*)(a.out + row * HD + col) = x;
     }
 }
 
@@ -1172,7 +1290,7 @@ static void launch_t(const PagedAttn& a, const PagedWs& w, hipStream_t s) {
     if (w.plan) {
         attn_paged_plan_kernel<<<dim3(1), dim3(1024), 0, s>>>(a, w, max_tiles(a, w));
         attn_paged_tile_kernel<HD><<<dim3((unsigned)w.tblocks), dim3(256), 0, s>>>(a, w);
-        attn_paged_join_kernel<HD><<<dim3((unsigned)w.tblocks, 8), dim3(256), 0, s>>>(a, w);
+        attn_paged_join_kernel<HD><<<dim3((unsigned)w.tblocks, HD / 32), dim3(256), 0, s>>>(a, w);
     }
     if (a.max_prefix) {
         const int tiles = div_up(w.plan ? std::min((long long)a.t, (long long)a.nseq * per) : a.t, TT);
