@@ -218,18 +218,20 @@ hipError_t launch_pages_step(const PagesStep& a, hipStream_t s) {
 // For token v of a row, with c its count among the history's tokens at index >= from and seen whether the history (its last
 // `last` tokens) holds it:
 //   y = x; seen: y = y > 0 ? y / rep : y * rep; y = y - freq * c; c > 0: y = y - pres; y = y + bias; not allowed: -inf
-// one rounding a step, in this order. A block takes LP_CHUNK tokens of a row: it counts the history's tokens of its chunk and
-// marks the biases in LDS (integer atomics, so the order does not matter; of a token's biases the largest index counts), then
-// passes once over its logits. Bound by the logits' bytes for many rows (64 rows of 151936 from x into out 60 us, 1.3 TB/s), by
-// latency for one (10 us). Every block of a row reads the row's history again, from L2.
-constexpr int LP_T = 256;
+// one rounding a step, in this order. A block takes 4 NU tokens a thread of a row. One table of a word a token in LDS serves
+// twice (a table each left half the waves: 27.5 us for the 22 below): first the biases (of a token's the largest index counts),
+// which go to the registers of the token's thread, then the history's counts (integer atomics, so the order does not matter);
+// then one pass over the logits, which were requested at the start. Every block of a row reads the row's history again, from
+// L2. 64 rows of 151936 from x into out, histories of 4096, 100 biases and a mask: 22 us, 3.6 TB/s; one row, bound by the chain
+// of its loads: 4.4 us. The rows' choices follow in logits_choose_kernel (4.0 and 1.5 us).
+constexpr int LP_T = 512;
 constexpr uint32_t LP_SEEN = 0x80000000u;
 
 // NU: tokens a thread / 4. VEC: rows that are 16-byte aligned in x and out, 4 consecutive tokens a load; else a token a load.
 template <int NU, bool VEC>
 __global__ __launch_bounds__(LP_T) void logits_process_kernel(LogitsProcess a) {
     constexpr int CHUNK = 4 * NU * LP_T;
-    __shared__ __align__(16) uint32_t cnt[CHUNK], bix[CHUNK];
+    __shared__ __align__(16) uint32_t tab[CHUNK];
     __shared__ uint64_t sk[LP_T / 64];
     const int r = blockIdx.y, base = blockIdx.x * CHUNK, tid = threadIdx.x, m = min(CHUNK, a.n - base);
     const float* x = a.x + (uint64_t)r * a.x_stride + base;
@@ -274,54 +276,70 @@ __global__ __launch_bounds__(LP_T) void logits_process_kernel(LogitsProcess a) {
         b0 = min(max(a.bias_start[r], 0), a.n_bias);
         b1 = min(max(a.bias_start[r + 1], b0), a.n_bias);
     }
-    if (a.pen) {
-#pragma unroll
-        for (int u = 0; u < NU; u++) *(uint4*)&cnt[4 * (u * LP_T + tid)] = make_uint4(0, 0, 0, 0);
-    }
-    if (a.bias_start) {
-#pragma unroll
-        for (int u = 0; u < NU; u++) *(uint4*)&bix[4 * (u * LP_T + tid)] = make_uint4(0, 0, 0, 0);
-    }
     const bool pen = h1 > h0, bias = b1 > b0;
-    if (pen || bias) __syncthreads();
-    if (pen) {
-        const int* hr = a.hist + (uint64_t)r * a.hist_stride;
-        constexpr int HU = 8;  // history loads in flight
-        for (int i0 = h0 + tid; i0 < h1; i0 += HU * LP_T) {
-            int tok[HU];
+    const int* hr = a.hist + (uint64_t)r * a.hist_stride;
+    constexpr int HU = 8;  // history loads in flight
+    int tok[HU];
+    auto history = [&](int i0) {
 #pragma unroll
-            for (int k = 0; k < HU; k++) tok[k] = i0 + k * LP_T < h1 ? hr[i0 + k * LP_T] : -1;
+        for (int k = 0; k < HU; k++) tok[k] = i0 + k * LP_T < h1 ? hr[i0 + k * LP_T] : -1;
+    };
+    if (pen) history(h0 + tid);
+    auto clear = [&] {  // this thread's words
+#pragma unroll
+        for (int u = 0; u < NU; u++) {
+            if constexpr (VEC) *(uint4*)&tab[at(u, 0)] = make_uint4(0, 0, 0, 0);
+            else
+#pragma unroll
+                for (int e = 0; e < 4; e++) tab[at(u, e)] = 0;
+        }
+    };
+    auto words = [&](int u, uint32_t (&w)[4]) {
+        if constexpr (VEC) *(uint4*)w = *(const uint4*)&tab[at(u, 0)];
+        else
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = tab[at(u, e)];
+    };
+    uint32_t bv[NU][4] = {};
+    if (pen || bias) {
+        clear();
+        __syncthreads();
+    }
+    if (bias) {
+        for (int e = b0 + tid; e < b1; e += LP_T) {
+            const unsigned v = (unsigned)a.bias_ids[e] - (unsigned)base;
+            if (v < (unsigned)m) atomicMax(&tab[v], (uint32_t)(e + 1));
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < NU; u++) words(u, bv[u]);
+        if (pen) {
+            clear();  // (the words that this thread has just read)
+            __syncthreads();
+        }
+    }
+    if (pen) {
+        for (int i0 = h0 + tid;;) {
 #pragma unroll
             for (int k = 0; k < HU; k++) {
                 const unsigned v = (unsigned)tok[k] - (unsigned)base;
                 if (v < (unsigned)m) {  // (no id below 0: base + m is at most 2^31 - 1)
-                    if (i0 + k * LP_T >= from) atomicAdd(&cnt[v], 1u);
-                    else atomicOr(&cnt[v], LP_SEEN);
+                    if (i0 + k * LP_T >= from) atomicAdd(&tab[v], 1u);
+                    else atomicOr(&tab[v], LP_SEEN);
                 }
             }
+            i0 += HU * LP_T;
+            if (i0 >= h1) break;
+            history(i0);
         }
+        __syncthreads();
     }
-    if (bias)
-        for (int e = b0 + tid; e < b1; e += LP_T) {
-            const unsigned v = (unsigned)a.bias_ids[e] - (unsigned)base;
-            if (v < (unsigned)m) atomicMax(&bix[v], (uint32_t)(e + 1));
-        }
-    if (pen || bias) __syncthreads();
     const bool place = x == out;
     uint64_t best = 0;
 #pragma unroll
     for (int u = 0; u < NU; u++) {
-        uint32_t cv[4] = {}, bv[4] = {};
-        if constexpr (VEC) {
-            if (pen) *(uint4*)cv = *(const uint4*)&cnt[at(u, 0)];
-            if (bias) *(uint4*)bv = *(const uint4*)&bix[at(u, 0)];
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if (pen) cv[e] = cnt[at(u, e)];
-                if (bias) bv[e] = bix[at(u, e)];
-            }
-        }
+        uint32_t cv[4] = {};
+        if (pen) words(u, cv);
         bool changed = !place;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -333,7 +351,7 @@ __global__ __launch_bounds__(LP_T) void logits_process_kernel(LogitsProcess a) {
                 v = v - freq * (float)k;
                 v = v - pres;
             }
-            if (bv[e]) v = v + a.bias_vals[bv[e] - 1];
+            if (bv[u][e]) v = v + a.bias_vals[bv[u][e] - 1];
             const bool ok = VEC ? (mw[u][0] >> e) & 1u : mw[u][VEC ? 0 : e] & 1u;
             if (!ok) v = -INFINITY;
             changed |= __float_as_uint(v) != __float_as_uint(x0);
@@ -363,28 +381,26 @@ __global__ __launch_bounds__(LP_T) void logits_process_kernel(LogitsProcess a) {
 
 // A row's choice from its chunks' keys (a key is 0 only where no token of the chunk is allowed), and the history's next token.
 __global__ __launch_bounds__(64) void logits_choose_kernel(LogitsProcess a, int parts) {
-    const int r = blockIdx.x, lane = threadIdx.x;
+    const int r = blockIdx.x, lane = threadIdx.x, k = a.append ? a.hist_len[r] : -1;  // (waits with the keys)
     uint64_t best = 0;
     for (int i = lane; i < parts; i += 64) {
-        const uint64_t k = a.keys[(uint64_t)r * parts + i];
-        best = k > best ? k : best;
+        const uint64_t key = a.keys[(uint64_t)r * parts + i];
+        best = key > best ? key : best;
     }
     best = wave_max_u64(best);
     if (lane == 0) {
         const int id = best ? (int)(0xFFFFFFFFu - (uint32_t)best) : -1;
         a.ids[r] = id;
-        if (a.append && id >= 0) {
-            const int k = a.hist_len[r];
-            if (k >= 0 && (uint64_t)k < a.hist_stride) {
-                a.hist[(uint64_t)r * a.hist_stride + k] = id;
-                a.hist_len[r] = k + 1;
-            }
+        if (id >= 0 && k >= 0 && (uint64_t)k < a.hist_stride) {
+            a.hist[(uint64_t)r * a.hist_stride + k] = id;
+            a.hist_len[r] = k + 1;
         }
     }
 }
 
-// Tokens a block: 4096, or 1024 where the larger blocks leave CUs idle.
-static int logits_nu(int n, int rows) { return (long long)rows * ((n + 16 * LP_T - 1) / (16 * LP_T)) >= 512 ? 4 : 1; }
+// Tokens a block: 4096, or 2048 where the larger blocks would be fewer than two a CU (64 rows of 151936: 22.0 against 26.2 us; one
+// row 5.2 against 4.3).
+static int logits_nu(int n, int rows) { return (long long)rows * ((n + 8 * LP_T - 1) / (8 * LP_T)) >= 512 ? 2 : 1; }
 static int logits_parts(int n, int nu) { return (n + 4 * nu * LP_T - 1) / (4 * nu * LP_T); }
 size_t logits_key_bytes(int n, int rows) { return (size_t)rows * logits_parts(n, logits_nu(n, rows)) * sizeof(uint64_t); }
 
@@ -392,8 +408,8 @@ hipError_t launch_logits_process(const LogitsProcess& a, hipStream_t s) {
     const int nu = logits_nu(a.n, a.rows), parts = logits_parts(a.n, nu);
     const dim3 grid((unsigned)parts, (unsigned)a.rows);
     const bool vec = ((uintptr_t)a.x | (uintptr_t)a.out) % 16 == 0 && (a.rows == 1 || (a.x_stride | a.out_stride) % 4 == 0);
-    if (nu == 4 && vec) logits_process_kernel<4, true><<<grid, dim3(LP_T), 0, s>>>(a);
-    else if (nu == 4) logits_process_kernel<4, false><<<grid, dim3(LP_T), 0, s>>>(a);
+    if (nu == 2 && vec) logits_process_kernel<2, true><<<grid, dim3(LP_T), 0, s>>>(a);
+    else if (nu == 2) logits_process_kernel<2, false><<<grid, dim3(LP_T), 0, s>>>(a);
     else if (vec) logits_process_kernel<1, true><<<grid, dim3(LP_T), 0, s>>>(a);
     else logits_process_kernel<1, false><<<grid, dim3(LP_T), 0, s>>>(a);
     if (a.ids) logits_choose_kernel<<<dim3((unsigned)a.rows), dim3(64), 0, s>>>(a, parts);
