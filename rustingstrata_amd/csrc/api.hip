@@ -1105,7 +1105,7 @@ int strata_attn_paged(strata_ctx* c, uint64_t q, uint64_t kc, uint64_t vc, uint6
     if (max_prefix && (!prefix || !prefix_len)) return set_error("paged attention: null prefix or its length");
     if (t > (1ull << 20) || !max_q || max_q > t) return set_error("paged attention: " + std::to_string(t) + " rows (at most 2^20), at most " + std::to_string(max_q) + " a sequence");
     if (max_prefix > (1ull << 30) || win >= (1ull << 31) || nkv > 65535 || nh > 65535) return set_error("paged attention: too large");
-    if (nseq * nkv * (max_pages * page / 64 + 1) >= (1ull << 31)) return set_error("paged attention: more than 2^31 chunks of keys (sequences x KV heads x positions / 64)");
+    if (nseq * nkv * (max_pages * page / 64 + 32) >= (1ull << 31)) return set_error("paged attention: more than 2^31 chunks of keys (sequences x KV heads x positions / 64)");
     if ((t / (128 / (nh / nkv)) + nseq + 1) * ((max_prefix + max_pages * page) / 64 + 3) >= (1ull << 31))
         return set_error("paged attention: more than 2^31 tiles of rows and keys (rows x group / 128 + sequences, times positions / 64)");
     if (q % 16 || out % 16 || kc % 16 || vc % 16) return set_error("paged attention: q, out and the caches must be 16-byte aligned");
@@ -1133,7 +1133,7 @@ int strata_logits_process(strata_ctx* c, uint64_t x, uint64_t x_stride, uint64_t
     if (rows > 1 && (x_stride < n || out_stride < n)) return set_error("logits_process: a row stride shorter than " + std::to_string(n));
     if (x == out && x_stride != out_stride && rows > 1) return set_error("logits_process: in place with two row strides");
     if ((pen || append) && (!hist || !hist_len)) return set_error("logits_process: penalties or append without a history");
-    if (hist_stride >= (1ull << 31) || last >= (1ull << 31) || n_bias >= (1ull << 31)) return set_error("logits_process: too large");
+    if (hist_stride > (1ull << 30) || last >= (1ull << 31) || n_bias >= (1ull << 31)) return set_error("logits_process: too large");
     if (bias_start && n_bias && (!bias_ids || !bias_vals)) return set_error("logits_process: null bias_ids or bias_vals");
     if (mask && rows > 1 && mask_stride < (n + 31) / 32) return set_error("logits_process: a mask row shorter than " + std::to_string((n + 31) / 32) + " words");
     if (append && !ids) return set_error("logits_process: append without ids");

@@ -30,6 +30,7 @@ struct PagedWs {
     float* pacc;   // [t nh][nsp][hd]
     int* plan;     // long sequences (null: none): PlanHead, then a Tile each
     int* drows;    // with a plan and a prefix: the rows of decode sequences
+    int4* cut;     // [tblocks] KV head and tile that block b's run cuts, and the last block of its pieces (below 0: none)
     float2* tml;   // [2 tblocks][128]: the pieces of tiles that more than one block computes
     float* tacc;   // [2 tblocks][128][hd]
     int dblocks, nct, dr, nsp, tblocks;  // decode blocks, their column tiles; rows (tokens x G) up to which a sequence decodes
@@ -173,16 +174,15 @@ struct PagedDec {
     static constexpr int BYTES = DEC_WAVES * WAVE > MERGE ? DEC_WAVES * WAVE : MERGE;
 };
 template <int HD, int NT>
-__global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attn_paged_dec_kernel(PagedAttn a, PagedWs w) {
+__device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, int b, uint8_t* lds) {
     using L = PagedDec<HD>;
     typedef unsigned v4u __attribute__((ext_vector_type(4)));
     constexpr int KS = HD / 32, DT = HD / 16, LPR = HD / 8, RPI = 64 / LPR, NV = 32 / RPI;  // lanes a V row, rows a load, loads
-    __shared__ __align__(16) uint8_t lds[L::BYTES];
     __shared__ int ws[8];
     __shared__ SeqInfo sq;
     __shared__ int sb[2];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
-    const int G = a.nh / a.nkv, P = prefix_len(a), b = blockIdx.x;
+    const int G = a.nh / a.nkv, P = prefix_len(a);
     // this block's run of the list: the thread that holds the sequence of its start says which it is
     int W0, W1, share;
     {
@@ -217,7 +217,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attn_paged_dec_kernel(Pa
         }
         total *= a.nkv;
         // (at most 128 pieces a pair: the merge's work)
-        share = max((total + (int)gridDim.x - 1) / (int)gridDim.x, (big + 127) / 128);
+        share = max((total + w.dblocks - 1) / w.dblocks, (big + 127) / 128);
         W0 = (int)min((long long)b * share, (long long)total);
         W1 = (int)min((long long)W0 + share, (long long)total);
         if (W0 >= W1) return;
@@ -811,14 +811,13 @@ __device__ __forceinline__ void tile_store(const TileSums<HD>& r, int tid, float
 // block takes a split of the prefix's keys. Blocks are numbered so that the tiles over the same keys run on one XCD (its L2
 // holds a split's K and V).
 template <int HD>
-__global__ __launch_bounds__(256, 2) void attn_paged_prefix_kernel(PagedAttn a, PagedWs w, int tiles) {
-    __shared__ __align__(16) uint8_t lds[2 * PagedTile<HD>::BUF];
+__device__ __forceinline__ void prefix_block(const PagedAttn& a, const PagedWs& w, int x, int tiles, uint8_t* lds) {
     __shared__ int ws[8];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l32 = lane & 31;
     const int G = a.nh / a.nkv, gs = 31 - __builtin_clz(G), TT = 128 >> gs, ns = w.nsp;
     const Keys keys{a.prefix, nullptr, prefix_len(a), (prefix_len(a) + 63) / 64, 0};
     // block x: combination (KV head, split) c on XCD c % 8, tile tt
-    const int x = blockIdx.x, c = (x & 7) + 8 * ((x >> 3) / tiles), tt = (x >> 3) % tiles;
+    const int c = (x & 7) + 8 * ((x >> 3) / tiles), tt = (x >> 3) % tiles;
     if (c >= a.nkv * ns || !keys.P) return;
     const int g = c % a.nkv, split = c / a.nkv;
     const int nrows = w.drows ? sload(w.plan + 2) : min(max(sload(a.q_start + a.nseq), 0), a.t), nt = min(TT, nrows - tt * TT);
@@ -1005,13 +1004,16 @@ __device__ __forceinline__ PlanTile plan_tile(const PlanTile* p) {
 struct RunAt {
     long long at;  // in the list of all tiles' work
     int g, i, f;   // the KV head, the tile, the key tile of it
+    long long share;
+    int near;
 };
 __device__ __forceinline__ RunAt run_at(const PlanTile* plan, int n, int cost, int nkv, int b, int blocks) {
     const long long all = (long long)cost * nkv, share = max((all + blocks - 1) / blocks, 2ll);
-    RunAt r{min(b * share, all), nkv, 0, 0};
+    const int near = (int)min(share / 8, 3ll);
+    RunAt r{min(b * share, all), nkv, 0, 0, share, near};
     if (r.at == all) return r;
     r.g = (int)(r.at / cost);
-    const int x = (int)(r.at - (long long)r.g * cost), near = (int)min(share / 8, 3ll);
+    const int x = (int)(r.at - (long long)r.g * cost);
     r.i = tile_of(plan, n, x);
     const int cum = sload(&plan[r.i].cum), nkt = sload(&plan[r.i].nkt), f = x - cum - TILE_EXTRA;
     if (f <= near) {
@@ -1026,16 +1028,28 @@ __device__ __forceinline__ RunAt run_at(const PlanTile* plan, int n, int cost, i
 }
 
 template <int HD>
-__global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedAttn a, PagedWs w) {
-    __shared__ __align__(16) uint8_t lds[2 * PagedTile<HD>::BUF];
+__device__ __forceinline__ void tile_block(const PagedAttn& a, const PagedWs& w, int x, uint8_t* lds) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int G = a.nh / a.nkv, gs = 31 - __builtin_clz(G), P = prefix_len(a);
     const PlanTile* plan = (const PlanTile*)(w.plan + PLAN_HEAD);
     const int n = sload(w.plan), cost = sload(w.plan + 1);
-    if (!n) return;
-    // block b takes the b-th run; neighbours in the list, which share keys, run on one XCD
-    const int b = (blockIdx.x & 7) * (w.tblocks / 8) + (blockIdx.x >> 3);
+    // the b-th run; neighbours in the list, which share keys, run on one XCD
+    const int b = (x & 7) * (w.tblocks / 8) + (x >> 3);
+    if (!n) {
+        if (threadIdx.x == 0) w.cut[b] = make_int4(0, 0, -1, 0);
+        return;
+    }
     const RunAt from = run_at(plan, n, cost, a.nkv, b, w.tblocks), to = run_at(plan, n, cost, a.nkv, b + 1, w.tblocks);
+    if (threadIdx.x == 0) {
+        // the tile that begins in this run and goes on past it: the last block of its pieces (run_at's borders)
+        int last = -1;
+        if (to.f && (from.g != to.g || from.i != to.i || !from.f)) {
+            const PlanTile p = plan_tile(plan + to.i);
+            const long long end = (long long)cost * to.g + p.cum + TILE_EXTRA + p.nkt;
+            last = (int)min((end - to.near - 1) / to.share, (long long)w.tblocks - 1);
+        }
+        w.cut[b] = make_int4(to.g, to.i, last, 0);
+    }
     for (int g = from.g, i = from.i, f = from.f; g < to.g || (g == to.g && (i < to.i || (i == to.i && f < to.f)));) {
         const PlanTile p = plan_tile(plan + i);
         const int k = (g == to.g && i == to.i ? to.f : p.nkt) - f;
@@ -1084,23 +1098,17 @@ __global__ __launch_bounds__(256, 2) void attn_paged_tile_kernel(PagedAttn a, Pa
     }
 }
 
-// Block b joins the tile that begins in block b's run and goes on past it: the pieces' sums of its 128 rows, 4 rows a wave at a
-// time with their loads in flight together.
+// A tile that begins in block b's run and goes on past it, joined: the pieces' sums of its 128 rows, 4 rows a wave at a time
+// with their loads in flight together; y of HD / 32 blocks.
 template <int HD>
-__global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedAttn a, PagedWs w) {
+__device__ __forceinline__ void join_block(const PagedAttn& a, const PagedWs& w, int b, int y) {
     constexpr int NC = HD / 4, RPW = 64 / NC, U = 4;  // lanes a row (16 bytes each), rows a wave and load, loads
-    const PlanTile* plan = (const PlanTile*)(w.plan + PLAN_HEAD);
-    const int n = sload(w.plan), cost = sload(w.plan + 1), b = blockIdx.x, lane = threadIdx.x & 63;
-    if (!n) return;
-    const RunAt end = run_at(plan, n, cost, a.nkv, b + 1, w.tblocks);
-    if (end.g >= a.nkv || end.f == 0) return;  // (no tile is cut there)
-    const RunAt from = run_at(plan, n, cost, a.nkv, b, w.tblocks);
-    if (from.g == end.g && from.i == end.i && from.f > 0) return;  // (it began before this block's run)
-    const PlanTile p = plan_tile(plan + end.i);
-    int last = b + 1;  // pieces in blocks b .. last
-    for (RunAt to; to = run_at(plan, n, cost, a.nkv, last + 1, w.tblocks), to.g == end.g && to.i == end.i;) last++;
+    const int lane = threadIdx.x & 63, last = sload(&w.cut[b].z);
+    if (last < 0) return;
+    struct { int g, i; } end{sload(&w.cut[b].x), sload(&w.cut[b].y)};
+    const PlanTile p = plan_tile((const PlanTile*)(w.plan + PLAN_HEAD) + end.i);
     const int G = a.nh / a.nkv, gs = 31 - __builtin_clz(G), nr = p.nt * G, col = 4 * (lane % NC);
-    const int r0 = (blockIdx.y * 4 + (threadIdx.x >> 6)) * U * RPW + lane / NC;
+    const int r0 = (y * 4 + (threadIdx.x >> 6)) * U * RPW + lane / NC;
     float M[U], L[U];
     float4 acc[U];
 #pragma unroll
@@ -1148,27 +1156,34 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedAttn a, Paged
 }
 
 // ---------------- the join of a decode sequence's rows ----------------
-// Row x % per of sequence x / per, query head y from its partial sums: out = sum_i acc_i 2^(m_i - M) / (sum_i l_i 2^(m_i - M) +
-// 2^(sink - M)), the prefix's splits, then the own keys' pieces. Wave v of 4 takes partials v, v + 4, ..: the maxima a lane
-// each and the rows of the first 8 requested together (a launch is a chain of trips to memory: the sequence, then these).
+// Item x (of [sequence][row of it][query head]) from its partial sums: out = sum_i acc_i 2^(m_i - M) / (sum_i l_i 2^(m_i - M) +
+// 2^(sink - M)), the prefix's splits, then the own keys' pieces. Two waves an item, two items a block: wave v takes partials
+// v, v + 2, .., their maxima a lane each and 4 rows requested together (a launch is a chain of trips to memory: the sequence,
+// then these). 2048 items of 64 sequences of 200 .. 6000 keys: 5.7 us (four waves 7.1, one 5.4); 768 of 4 .. 16 partials
+// 6.6 us (four waves 8.4, one 8.2).
+constexpr int MERGE_WAVES = 2, MERGE_ITEMS = 2;
 template <int HD>
-__global__ __launch_bounds__(256) void attn_paged_merge_kernel(PagedAttn a, PagedWs w, int per) {
-    constexpr int DL = HD / 64, MW = 4, U = 8;
-    __shared__ float sm[MW], sl[MW], so[MW][HD];
-    const int v = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int G = a.nh / a.nkv, s = blockIdx.x / per, h = blockIdx.y, g = h / G;
+__device__ __forceinline__ void merge_block(const PagedAttn& a, const PagedWs& w, int x, int per) {
+    constexpr int DL = HD / 64, MW = MERGE_WAVES, U = 4;
+    __shared__ float sm[MERGE_ITEMS][MW], sl[MERGE_ITEMS][MW], so[MERGE_ITEMS][MW][HD];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), v = wave % MW, it = wave / MW, lane = threadIdx.x & 63;
+    x = MERGE_ITEMS * x + it;
+    const int G = a.nh / a.nkv, h = x % a.nh, g = h / G, s = min(x / a.nh / per, a.nseq - 1);
     const int2* mp = w.map + s * a.nkv + g;
     const int first = sload(&mp->x), pieces = sload(&mp->y), P = prefix_len(a);  // (not set, and not used, without own keys)
     const SeqInfo q = seq_info<true>(a, s, G, w.dr, P);
-    const int r = q.q0 + blockIdx.x % per;
-    if (r >= q.q0 + q.qn || q.qn * G > w.dr) return;
+    const int r = q.q0 + x / a.nh % per;
+    const bool live = x < a.nseq * per * a.nh && r < q.q0 + q.qn && q.qn * G <= w.dr;
     const uint64_t row = (uint64_t)r * a.nh + h;
-    const int np = P > 0 ? w.nsp : 0, n = np + (q.nc > 0 ? pieces : 0);
+    const int np = P > 0 ? w.nsp : 0, n = live ? np + (q.nc > 0 ? pieces : 0) : 0;
     const uint64_t own = (uint64_t)(first + s * a.nkv + g) * w.dr + (r - q.q0) * G + h % G;  // piece i of the own keys: own + i dr
     auto at = [&](int i) { return i < np ? row * np + i : own + (uint64_t)(i - np) * w.dr; };
-    float M = -INFINITY, L = 0.0f, acc[DL];
+    float M = -INFINITY, L = 0.0f, acc[DL], gt[DL];
 #pragma unroll
-    for (int d = 0; d < DL; d++) acc[d] = 0.0f;
+    for (int d = 0; d < DL; d++) {
+        acc[d] = 0.0f;
+        gt[d] = live && a.qg ? a.qg[row * 2 * HD + HD + DL * lane + d] : 0.0f;
+    }
     for (int i0 = v; i0 < n; i0 += 64 * MW) {
         const int i = i0 + MW * lane;
         float2 ml = make_float2(-INFINITY, 0.0f);
@@ -1203,34 +1218,61 @@ __global__ __launch_bounds__(256) void attn_paged_merge_kernel(PagedAttn a, Page
         }
     }
     if (lane == 0) {
-        sm[v] = M;
-        sl[v] = L;
+        sm[it][v] = M;
+        sl[it][v] = L;
     }
 #pragma unroll
-    for (int d = 0; d < DL; d++) so[v][DL * lane + d] = acc[d];
+    for (int d = 0; d < DL; d++) so[it][v][DL * lane + d] = acc[d];
     __syncthreads();
-    if (v) return;
-    M = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+    if (v || !live) return;
+    M = sm[it][0];
+#pragma unroll
+    for (int u = 1; u < MW; u++) M = fmaxf(M, sm[it][u]);
     L = 0.0f;
 #pragma unroll
     for (int d = 0; d < DL; d++) acc[d] = 0.0f;
 #pragma unroll
     for (int u = 0; u < MW; u++) {
-        const float f = sm[u] == -INFINITY ? 1.0f : exp2_hw(sm[u] - M);
-        L += sl[u] * f;
+        const float f = sm[it][u] == -INFINITY ? 1.0f : exp2_hw(sm[it][u] - M);
+        L += sl[it][u] * f;
 #pragma unroll
-        for (int d = 0; d < DL; d++) acc[d] += so[u][DL * lane + d] * f;
+        for (int d = 0; d < DL; d++) acc[d] += so[it][u][DL * lane + d] * f;
     }
     const float f = out_factor(a, h, M, L);
 #pragma unroll
     for (int d = 0; d < DL; d++) {
-        float x = acc[d] * f;
-        if (a.qg) x *= sigmoid_f(a.qg[row * 2 * HD + HD + DL * lane + d]);
-        a.out[row * HD + DL * lane + d] = x;
+        float o = acc[d] * f;
+        if (a.qg) o *= sigmoid_f(gt[d]);
+        a.out[row * HD + DL * lane + d] = o;
     }
 }
 
 // ---------------- launches ----------------
+// The pieces: blocks of the long sequences' tiles (TILE), of the prefix for the rows of decode sequences (PRE) and of their own
+// keys, in one launch.
+template <int HD, int NT, bool TILE, bool PRE>
+__global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attn_paged_kernel(PagedAttn a, PagedWs w, int pblocks, int tiles) {
+    constexpr int TB = TILE || PRE ? 2 * PagedTile<HD>::BUF : 0;
+    __shared__ __align__(16) uint8_t lds[PagedDec<HD>::BYTES > TB ? PagedDec<HD>::BYTES : TB];
+    int b = blockIdx.x;
+    if constexpr (TILE) {
+        if (b < w.tblocks) return tile_block<HD>(a, w, b, lds);
+        b -= w.tblocks;
+    }
+    if constexpr (PRE) {
+        if (b < pblocks) return prefix_block<HD>(a, w, b, tiles, lds);
+        b -= pblocks;
+    }
+    dec_block<HD, NT>(a, w, b, lds);
+}
+// The joins: of the tiles in pieces, and of the rows of decode sequences.
+template <int HD>
+__global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedAttn a, PagedWs w, int jblocks, int per) {
+    const int b = blockIdx.x;
+    if (b < jblocks) return join_block<HD>(a, w, b / (HD / 32), b % (HD / 32));
+    merge_block<HD>(a, w, b - jblocks, per);
+}
+
 static int div_up(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 // Tiles of the long sequences at most: each of them has more than dr / G rows.
@@ -1249,10 +1291,10 @@ static PagedWs plan(const PagedAttn& a, uint8_t* at, size_t* end) {
     w.nct = most_rows > 16 && most_rows <= 32 ? 2 : 1;
     w.dr = (int)std::min<long long>(16 * w.nct, most_rows);
     const long long most = (long long)a.nseq * a.nkv * (((long long)a.max_pages << a.page_shift) / DEC_CHUNK + 1);
-    w.dblocks = (int)std::min<long long>(most, w.nct == 1 ? 512 : 256);  // the blocks that run at once
+    w.dblocks = (int)std::min<long long>(most, w.nct == 1 && (!a.max_prefix || most_rows > w.dr) ? 512 : 256);  // the blocks that run at once
     // splits of the prefix: enough blocks for two a CU, of at least 128 keys
     const long long blocks = std::max<long long>((long long)div_up(rows, 128) * a.nkv, 1);
-    w.nsp = (int)std::max<long long>(1, std::min<long long>({div_up(512, blocks), div_up(a.max_prefix, 128), 64}));
+    w.nsp = (int)std::max<long long>(1, std::min<long long>({div_up(256, blocks), div_up(a.max_prefix, 128), 64}));
     w.tblocks = 512;
     size_t o = 0;
     auto take = [&](size_t bytes) {
@@ -1271,6 +1313,7 @@ static PagedWs plan(const PagedAttn& a, uint8_t* at, size_t* end) {
     if (most_rows > w.dr) {
         w.plan = (int*)take((PLAN_HEAD + (size_t)max_tiles(a, w) * (sizeof(PlanTile) / 4)) * 4);
         if (a.max_prefix) w.drows = (int*)take((size_t)a.t * 4);
+        w.cut = (int4*)take((size_t)w.tblocks * sizeof(int4));
         w.tml = (float2*)take((size_t)2 * w.tblocks * 128 * sizeof(float2));
         w.tacc = (float*)take((size_t)2 * w.tblocks * 128 * a.hd * sizeof(float));
     }
@@ -1287,20 +1330,25 @@ size_t paged_attn_ws_bytes(const PagedAttn& a) {
 template <int HD>
 static void launch_t(const PagedAttn& a, const PagedWs& w, hipStream_t s) {
     const int G = a.nh / a.nkv, TT = 128 / G, per = w.dr / G;
-    if (w.plan) {
-        attn_paged_plan_kernel<<<dim3(1), dim3(1024), 0, s>>>(a, w, max_tiles(a, w));
-        attn_paged_tile_kernel<HD><<<dim3((unsigned)w.tblocks), dim3(256), 0, s>>>(a, w);
-        attn_paged_join_kernel<HD><<<dim3((unsigned)w.tblocks, HD / 32), dim3(256), 0, s>>>(a, w);
-    }
+    int tiles = 0, pblocks = 0;
+    if (w.plan) attn_paged_plan_kernel<<<dim3(1), dim3(1024), 0, s>>>(a, w, max_tiles(a, w));
     if (a.max_prefix) {
-        const int tiles = div_up(w.plan ? std::min((long long)a.t, (long long)a.nseq * per) : a.t, TT);
-        attn_paged_prefix_kernel<HD><<<dim3((unsigned)(8 * div_up((long long)a.nkv * w.nsp, 8) * (long long)tiles)), dim3(256), 0, s>>>(a, w, tiles);
+        tiles = div_up(w.plan ? std::min((long long)a.t, (long long)a.nseq * per) : a.t, TT);
+        pblocks = 8 * div_up((long long)a.nkv * w.nsp, 8) * tiles;
     }
-    if (w.nct == 2)
-        attn_paged_dec_kernel<HD, 2><<<dim3((unsigned)w.dblocks), dim3(256), 0, s>>>(a, w);
-    else
-        attn_paged_dec_kernel<HD, 1><<<dim3((unsigned)w.dblocks), dim3(256), 0, s>>>(a, w);
-    attn_paged_merge_kernel<HD><<<dim3((unsigned)(a.nseq * per), (unsigned)a.nh), dim3(256), 0, s>>>(a, w, per);
+    const dim3 grid((unsigned)((w.plan ? w.tblocks : 0) + pblocks + w.dblocks)), block(256);
+    if (w.nct == 2) {
+        if (a.max_prefix) attn_paged_kernel<HD, 2, false, true><<<grid, block, 0, s>>>(a, w, pblocks, tiles);
+        else attn_paged_kernel<HD, 2, false, false><<<grid, block, 0, s>>>(a, w, pblocks, tiles);
+    } else if (w.plan) {
+        if (a.max_prefix) attn_paged_kernel<HD, 1, true, true><<<grid, block, 0, s>>>(a, w, pblocks, tiles);
+        else attn_paged_kernel<HD, 1, true, false><<<grid, block, 0, s>>>(a, w, pblocks, tiles);
+    } else {
+        if (a.max_prefix) attn_paged_kernel<HD, 1, false, true><<<grid, block, 0, s>>>(a, w, pblocks, tiles);
+        else attn_paged_kernel<HD, 1, false, false><<<grid, block, 0, s>>>(a, w, pblocks, tiles);
+    }
+    const int jblocks = w.plan ? w.tblocks * (HD / 32) : 0;
+    attn_paged_join_kernel<HD><<<dim3((unsigned)(jblocks + div_up((long long)a.nseq * per * a.nh, MERGE_ITEMS))), block, 0, s>>>(a, w, jblocks, per);
 }
 
 hipError_t launch_attn_paged(const PagedAttn& a, hipStream_t s) {
