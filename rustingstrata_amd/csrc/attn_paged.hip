@@ -170,7 +170,7 @@ template <int HD>
 struct PagedDec {
     static constexpr int VP = HD + 16;             // halves a V row in LDS (32 bytes on: the transposed reads' 16 rows spread)
     static constexpr int WAVE = 32 * VP * 2;
-    static constexpr int MERGE = DEC_WAVES * (HD * 16 + 32) * 4;
+    static constexpr int MERGE = DEC_WAVES * (HD * 17 + 32) * 4;
     static constexpr int BYTES = DEC_WAVES * WAVE > MERGE ? DEC_WAVES * WAVE : MERGE;
 };
 template <int HD, int NT>
@@ -430,9 +430,10 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
             l[u] += __shfl_xor(l[u], 16, 64);
             l[u] += __shfl_xor(l[u], 32, 64);
         }
-        // the waves' sums meet in LDS, 16 rows at a time
+        // the waves' sums meet in LDS, 16 rows at a time (a dim's 16 rows 17 words apart: the reads of 4 rows x 64 dims hit all
+        // banks once)
         float* ow = (float*)lds;
-        float* mw = ow + DEC_WAVES * HD * 16;
+        float* mw = ow + DEC_WAVES * HD * 17;
         float* lw = mw + DEC_WAVES * 16;
 #pragma unroll
         for (int u = 0; u < NT; u++) {
@@ -440,14 +441,14 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
 #pragma unroll
             for (int d = 0; d < DT; d++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) ow[(wave * HD + 16 * d + 4 * lg + i) * 16 + l16] = o[u][d][i];
+                for (int i = 0; i < 4; i++) ow[(wave * HD + 16 * d + 4 * lg + i) * 17 + l16] = o[u][d][i];
             if (lg == 0) {
                 mw[wave * 16 + l16] = m[u];
                 lw[wave * 16 + l16] = l[u];
             }
             __syncthreads();
             constexpr int DPT = HD / 16;
-            const int rr = tid >> 4, dd0 = (tid & 15) * DPT, c = 16 * u + rr;
+            const int rr = tid >> 4, d4 = 4 * (tid & 15), c = 16 * u + rr;  // dims d4 .. d4 + 3 of each 64
             const bool live = c < q.qn * G;
             const uint64_t at_row = (uint64_t)(b + pair) * w.dr + c;
             float M = -INFINITY, e[DEC_WAVES], sum = 0.0f, acc[DPT], nf = 0.0f;
@@ -462,12 +463,14 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
             for (int d = 0; d < DPT; d++) {
                 acc[d] = 0.0f;
 #pragma unroll
-                for (int v = 0; v < DEC_WAVES; v++) acc[d] += ow[(v * HD + dd0 + d) * 16 + rr] * e[v];
+                for (int v = 0; v < DEC_WAVES; v++) acc[d] += ow[(v * HD + (d & ~3) * 16 + d4 + (d & 3)) * 17 + rr] * e[v];
                 nf = __builtin_fmaf(acc[d], 0.0f, nf);
             }
             if (live) {
 #pragma unroll
-                for (int d = 0; d < DPT; d++) w.dacc[at_row * HD + dd0 + d] = acc[d] * (1.0f / PF_SCALE);
+                for (int d = 0; d < DPT; d += 4)
+                    *(float4*)(w.dacc + at_row * HD + 16 * d + d4) = make_float4(acc[d] * (1.0f / PF_SCALE), acc[d + 1] * (1.0f / PF_SCALE),
+                                                                                 acc[d + 2] * (1.0f / PF_SCALE), acc[d + 3] * (1.0f / PF_SCALE));
                 if ((tid & 15) == 0) w.dml[at_row] = make_float2(M, sum);
             }
             // A row with finite scores whose sums are not may owe it to a key that it does not see (0 times a value that is not
