@@ -1106,7 +1106,7 @@ int strata_attn_paged(strata_ctx* c, uint64_t q, uint64_t kc, uint64_t vc, uint6
     if (t > (1ull << 20) || !max_q || max_q > t) return set_error("paged attention: " + std::to_string(t) + " rows (at most 2^20), at most " + std::to_string(max_q) + " a sequence");
     if (max_prefix > (1ull << 30) || win >= (1ull << 31) || nkv > 65535 || nh > 65535) return set_error("paged attention: too large");
     if (nseq * nkv * (max_pages * page / 64 + 32) >= (1ull << 31)) return set_error("paged attention: more than 2^31 chunks of keys (sequences x KV heads x positions / 64)");
-    if ((t / (128 / (nh / nkv)) + nseq + 1) * ((max_prefix + max_pages * page) / 64 + 3) >= (1ull << 31))
+    if ((t / (128 / (nh / nkv)) + nseq + 1) * ((max_prefix + max_pages * page) / 64 + 5) >= (1ull << 31))
         return set_error("paged attention: more than 2^31 tiles of rows and keys (rows x group / 128 + sequences, times positions / 64)");
     if (q % 16 || out % 16 || kc % 16 || vc % 16) return set_error("paged attention: q, out and the caches must be 16-byte aligned");
     PagedAttn a;

@@ -103,9 +103,9 @@ def rows_of(pool, table, n, page):
     return pool[np.where(ok, pg, 0) * page + j % page].astype(np.float64), ok
 
 
-def attn(q, kc, vc, pos, q_start, length, tables, page, prefix, P, scale, win=0, sink=None, gate=None):
+def attn(q, kc, vc, pos, q_start, length, tables, page, prefix, P, scale, win=0, sink=None, gate=None, rows=None):
     """q [t, nh, hd]; kc, vc [slots, nkv, hd]. Returns out (rows from q_start[-1] on NaN) and each row and head's largest
-    score magnitude (of the keys it sees)."""
+    score magnitude (of the keys it sees). rows: only these (the others NaN)."""
     t, nh, hd = q.shape
     nkv = kc.shape[1]
     out, top = np.full((t, nh, hd), np.nan), np.zeros((t, nh))
@@ -118,6 +118,8 @@ def attn(q, kc, vc, pos, q_start, length, tables, page, prefix, P, scale, win=0,
         k, v, ok = np.concatenate([pk, k]), np.concatenate([pv, v]), np.concatenate([pok, ok])
         at = np.arange(P + n)
         for r in range(q_start[s], q_start[s + 1]):
+            if rows is not None and r not in rows:
+                continue
             see = ok & (at <= pos[r]) & ((at > pos[r] - win) if win else True)
             for h in range(nh):
                 g = h // (nh // nkv)

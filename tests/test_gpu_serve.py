@@ -386,15 +386,15 @@ class Batch:
     def get(self):
         return self.hip.get(self.out, np.float32, self.q.size).reshape(self.q.shape)
 
-    def want(self, win=0):
+    def want(self, win=0, rows=None):
         return V.attn(self.q, self.kc, self.vc, self.pos, self.q_start, self.n, self.tables, self.page, self.prefix, self.P, self.scale, win=win, sink=self.sink,
-                      gate=self.gate[:, :, 1] if self.gate is not None else None)
+                      gate=self.gate[:, :, 1] if self.gate is not None else None, rows=rows)
 
     def check(self, got, win=0, rows=None):
         """Each row and head within 2^-23 (14 + max |s|) of its norm: a float32 score is off by 2^-24 |s| in its sum and again in
         the exponent, which is its weight's relative error; the exps, the splits (2^-22), the sums and the two joins of partial
         sums (an exp, a product and a sum each) add fourteen times 2^-23 at most."""
-        want, top = self.want(win)
+        want, top = self.want(win, rows if rows is None else set(rows))
         m = self.q_start[-1]
         assert (got[m:] == 6.5).all()
         for r in range(m) if rows is None else rows:
@@ -452,6 +452,55 @@ def test_attn_paged_long(hip):
         b = Batch(hip, [1, 2, 1], [3, 2, 100], nh, nkv, hd, 64, P=30011, seed=2).upload()
         b.launch()
         b.check(b.get())
+
+
+@pytest.mark.parametrize("nh,nkv,hd,q,n,P,win", [
+    (2, 2, 128, [300, 1, 40], [20000, 9000, 40], 0, 0), (2, 2, 64, [140, 260], [12000, 260], 4100, 0), (8, 1, 128, [100, 1, 1, 1, 90], [15000, 700, 1, 64, 90], 3001, 0),
+    (8, 1, 64, [33, 1], [25000, 25000], 0, 9000), (4, 2, 128, [700], [700], 0, 0), (2, 1, 128, [9, 10, 8, 9], [3000, 10, 5000, 64], 0, 0)])
+def test_attn_paged_deep_chunks(hip, nh, nkv, hd, q, n, P, win):
+    """Prompt chunks deep in their contexts, whose tiles many blocks share, beside decoding sequences; rows at the borders of
+    tiles and sequences."""
+    b = Batch(hip, q, n, nh, nkv, hd, 64, P=P, seed=sum(q)).upload()
+    b.launch(win)
+    TT = 128 * nkv // nh
+    rows = {r for s, m in zip(b.q_start, q) for r in [*range(s, s + m, TT), s + m - 1, s + m // 2, min(s + TT - 1, s + m - 1)]}
+    b.check(b.get(), win, rows=sorted(rows)[:40])
+
+
+@pytest.mark.parametrize("nseq", [257, 1030, 4096])
+@pytest.mark.parametrize("P", [0, 33])
+def test_attn_paged_many_sequences(hip, nseq, P):
+    """Hundreds to thousands of sequences: of no rows, decoding ones and short chunks, more tiles than a block plans at once."""
+    rng = np.random.default_rng(nseq)
+    q = rng.choice([0, 1, 2, 8, 9, 17], nseq, p=[0.1, 0.2, 0.1, 0.1, 0.3, 0.2])
+    n = q + rng.integers(0, 40, nseq) * (rng.random(nseq) < 0.7)
+    b = Batch(hip, q.tolist(), n.tolist(), 2, 1, 64, 16, P=P, seed=nseq, extra=5).upload()
+    b.launch()
+    rows = sorted({0, int(b.q_start[-1]) - 1} | set(rng.integers(0, b.q_start[-1], 400).tolist()))
+    got = b.get()
+    b.check(got, rows=rows)
+    assert np.isfinite(got).all()
+
+
+def test_attn_paged_two_graphs_of_one_context(hip):
+    """Two recorded calls of one context share its workspace, which a larger eager call between them replaces."""
+    a = Batch(hip, [1] * 4, [300, 3, 64, 900], 8, 2, 64, 16, P=70, seed=1).upload()
+    c = Batch(hip, [60, 1, 3], [300, 80, 3], 8, 2, 64, 16, P=30, seed=2).upload()
+    a.launch(), c.launch()
+    wa, wc = a.get(), c.get()
+    a.check(wa), c.check(wc)
+    ga = hip.record_graph(a.launch, keep=[a])
+    d = Batch(hip, [1] * 200, [100] * 200, 8, 8, 128, 16, P=300, seed=3).upload()
+    d.launch()
+    gc = hip.record_graph(c.launch, keep=[c])
+    for _ in range(4):
+        for b, g, w in ((a, ga, wa), (c, gc, wc)):
+            hip.htod(np.full(b.q.size, 6.5, np.float32), b.out)
+            g.launch()
+            np.testing.assert_array_equal(b.get().view(np.uint32), w.view(np.uint32))
+        d.launch()
+    d.check(d.get(), rows=[0, 57, 199])
+    ga.close(), gc.close()
 
 
 def test_attn_paged_offsets_past_32_bits(hip):
@@ -594,3 +643,148 @@ def test_attn_paged_refused_arguments(hip):
             hip.attn_paged(**{**ok, **bad})
     hip.attn_paged(**{**ok, "t": 0})
     hip.attn_paged(**{**ok, "nseq": 0})
+
+
+# ---------------- the operators together ----------------
+class Server:
+    """A decode layer served with these operators: a step brings tokens of several sequences, whose q, k and v come from a table by
+    token id; the attention's output row is its sequence's row of logits."""
+    NH, NKV, HD, PAGE, NSEQ, MAX_PAGES, N_PAGES, T, CAP, P = 8, 2, 64, 16, 4, 6, 17, 70, 90, 21
+
+    def __init__(self, hip, rng):
+        self.hip, self.vocab = hip, self.NH * self.HD
+        f = lambda *s: rng.standard_normal(s).astype(np.float32)  # noqa: E731
+        self.tq, self.tk, self.tv = f(self.vocab, self.NH, self.HD), f(self.vocab, self.NKV, self.HD), f(self.vocab, self.NKV, self.HD)
+        self.qw, self.kw = 1 + 0.1 * f(self.HD), 1 + 0.1 * f(self.HD)
+        self.pre = rng.integers(0, self.vocab, self.P)
+        kvd = self.NKV * self.HD
+        self.kc, self.vc = (up(hip, np.full(self.N_PAGES * self.PAGE * kvd, np.nan, np.float16)) for _ in range(2))
+        self.q, self.k, self.v = (hip.alloc(4 * self.T * n * self.HD) for n in (self.NH, self.NKV, self.NKV))
+        self.qo, self.out = (hip.alloc(4 * self.T * self.vocab) for _ in range(2))
+        self.qwb, self.kwb = up(hip, self.qw), up(hip, self.kw)
+        self.tables = up(hip, np.full((self.NSEQ, self.MAX_PAGES), -1, np.int32))
+        self.prefix = i32(hip, [self.N_PAGES - 1, self.N_PAGES - 2])  # the prefix on two pages that are never free
+        self.free = i32(hip, rng.permutation(self.N_PAGES - 2))
+        self.n_free, self.n_free0 = i32(hip, [self.N_PAGES - 2]), self.N_PAGES - 2
+        self.add, self.len, self.err, self.plen = i32(hip, [0] * self.NSEQ), i32(hip, [0] * self.NSEQ), i32(hip, [0]), i32(hip, [0])
+        self.q_start, self.pos, self.slots = (hip.alloc(4 * (self.T + 8)) for _ in range(3))
+        self.hist, self.hlen, self.ids = hip.alloc(4 * self.NSEQ * self.CAP), i32(hip, [0] * self.NSEQ), i32(hip, [0] * self.NSEQ)
+        self.pen = up(hip, np.tile(np.array([1.3, 0.2, 0.1], np.float32), (self.NSEQ, 1)))
+        self.logits = hip.alloc(4 * self.NSEQ * self.vocab)
+
+    def norm_rope(self, t, pos, slots):
+        H = self.HD
+        self.hip.rms_norm_rope_qk_paged(self.q, self.NH * H, H, self.qwb, self.qo, self.NH, self.k, self.NKV * H, self.kwb, self.NKV, H, 1e-6, H, pos, 1e4,
+                                        self.v, self.NKV * H, self.kc, self.vc, slots, self.N_PAGES * self.PAGE, t)
+
+    def inputs(self, tokens):
+        for b, tab in ((self.q, self.tq), (self.k, self.tk), (self.v, self.tv)):
+            self.hip.htod(np.ascontiguousarray(tab[tokens]), b)
+
+    def cache_prefix(self):
+        self.inputs(self.pre)
+        pages = [self.N_PAGES - 1, self.N_PAGES - 2]
+        self.norm_rope(self.P, i32(self.hip, np.arange(self.P)), i32(self.hip, [pages[i // self.PAGE] * self.PAGE + i % self.PAGE for i in range(self.P)]))
+        self.hip.htod(np.array([self.P], np.int32), self.plen)
+
+    def layer(self, t, max_q):
+        self.hip.kv_pages_step(self.NSEQ, self.add, self.len, self.tables, self.MAX_PAGES, self.PAGE, self.free, self.N_PAGES, self.n_free, t, self.q_start,
+                               self.pos, self.slots, self.len, self.n_free, prefix_len=self.plen, err=self.err)
+        self.norm_rope(t, self.pos, self.slots)
+        self.hip.attn_paged(self.qo, self.kc, self.vc, 0, self.out, t, max_q, self.pos, self.q_start, self.len, self.NSEQ, self.tables, self.MAX_PAGES, self.PAGE,
+                            self.N_PAGES, self.NH, self.NKV, self.HD, self.HD ** -0.5, prefix=self.prefix, prefix_len=self.plen, max_prefix=2 * self.PAGE)
+
+    def choose(self, x):
+        self.hip.logits_process(x, self.vocab, self.logits, self.vocab, self.vocab, self.NSEQ, hist=self.hist, hist_stride=self.CAP, hist_len=self.hlen,
+                                pen=self.pen, ids=self.ids, append=True)
+
+    def check(self, toks, add):
+        """The device's state after a layer against each sequence's tokens: keys and values at their slots, and the attention's rows
+        from the cached values and roped queries in float64."""
+        hip, H = self.hip, self.HD
+        pool = lambda b: hip.get(b, np.float16, self.N_PAGES * self.PAGE * self.NKV * H).reshape(-1, self.NKV, H)  # noqa: E731
+        kc, vc, tables = pool(self.kc), pool(self.vc), get_i32(hip, self.tables, self.NSEQ * self.MAX_PAGES).reshape(self.NSEQ, -1)
+        prefix, length = get_i32(hip, self.prefix, 2), [len(x) for x in toks]
+        for s, x in enumerate(toks):
+            all_ = np.concatenate([self.pre, np.array(x, np.int64)]).astype(np.int64)
+            got = [np.concatenate([V.rows_of(c, prefix, self.P, self.PAGE)[0], V.rows_of(c, tables[s], len(x), self.PAGE)[0]]) for c in (kc, vc)]
+            np.testing.assert_array_equal(got[1], self.tv[all_].astype(np.float16))
+            k = V.norm_rope(self.tk[all_].astype(np.float64), self.kw, 1e-6, H, np.arange(len(all_))[:, None], 1e4)
+            # half a step of f16, and angles below 128 in float32 (their frequency's rounding, the product's, and sin and cos: 4 half
+            # steps of 2^-24 times 128) turn a pair of values by 2^-15 of its length
+            pair = np.hypot(k[..., :H // 2], k[..., H // 2:])
+            assert (np.abs(got[0] - k) <= 2.0 ** -11 * np.abs(k) + 2.0 ** -15 * np.concatenate([pair, pair], -1) + 2.0 ** -25).all(), s
+        rows = [max(a, 0) for a in add]
+        q_start = np.concatenate([[0], np.cumsum(rows)])
+        assert get_i32(hip, self.q_start, self.NSEQ + 1).tolist() == q_start.tolist()
+        t = q_start[-1]
+        qo, out = (hip.get(b, np.float32, self.T * self.vocab).reshape(self.T, self.NH, H)[:t] for b in (self.qo, self.out))
+        pos = np.concatenate([self.P + n - m + np.arange(m) for n, m in zip(length, rows)])
+        assert get_i32(hip, self.pos, t).tolist() == pos.tolist()
+        want, top = V.attn(qo, kc, vc, pos, q_start, length, tables, self.PAGE, prefix, self.P, self.HD ** -0.5)
+        for r in range(t):
+            for h in range(self.NH):
+                assert rel_l2(out[r, h], want[r, h]) <= 2.0 ** -23 * (14 + top[r, h]), (add, r, h)  # (Batch.check's bound)
+
+
+def test_serving_a_batch(hip):
+    """Prompts, chunks, decode steps, sequences that end and begin: every step's state and rows, pages back at the end."""
+    rng = np.random.default_rng(5)
+    sv = Server(hip, rng)
+    sv.cache_prefix()
+    toks = [[] for _ in range(sv.NSEQ)]  # cached tokens of each sequence
+    # a step's new tokens a sequence (-1: it ends): prompts, a chunk beside decoding ones, decoding, an end, another's begin
+    steps = [[20, 0, 3, 0], [1, 40, 1, 0], [1, 1, 1, 25], [1, 1, 1, 1], [1, 1, -1, 1], [1, 1, 0, 1], [1, 1, 17, 1]] + [[1, 1, 1, 1]] * 3 + [[-1, 1, 1, 1], [5, 1, 1, 1], [-1] * 4]
+    for add in steps:
+        new = [rng.integers(0, sv.vocab, max(a, 0)) for a in add]
+        flat = np.concatenate(new).astype(np.int64)
+        if len(flat):
+            sv.inputs(flat)
+        hip.htod(np.array(add, np.int32), sv.add)
+        sv.layer(max(len(flat), 1), max(max(add), 1))
+        for s, a in enumerate(add):
+            toks[s] = [] if a < 0 else toks[s] + new[s].tolist()
+        assert get_i32(hip, sv.len, sv.NSEQ).tolist() == [len(t) for t in toks]
+        assert get_i32(hip, sv.n_free, 1)[0] == sv.n_free0 - sum(-(-len(t) // sv.PAGE) for t in toks)
+        sv.check(toks, add)
+    assert get_i32(hip, sv.err, 1)[0] == 0
+
+
+def test_serving_steps_recorded(hip):
+    """A recorded decode step (pages, keys and values, attention, choice, histories) replayed over page borders gives the bits of
+    the same steps launched one by one."""
+    runs = []
+    for graph in (False, True):
+        rng = np.random.default_rng(6)
+        sv = Server(hip, rng)
+        sv.cache_prefix()
+        flat = rng.integers(0, sv.vocab, 35)
+        sv.inputs(flat)
+        hip.htod(np.array([16, 3, 15, 1], np.int32), sv.add)
+        sv.layer(35, 16)
+        sv.inputs(rng.integers(0, sv.vocab, sv.NSEQ))
+        hip.htod(np.array([1] * sv.NSEQ, np.int32), sv.add)
+        got = []
+
+        def step():
+            sv.layer(sv.NSEQ, 1)
+            sv.choose(sv.out)
+
+        if graph:
+            save = [(b, hip.get(b, np.int32, n)) for b, n in ((sv.len, sv.NSEQ), (sv.n_free, 1), (sv.hlen, sv.NSEQ))]
+            step()  # (sizes the workspace)
+            for b, x in save:
+                hip.htod(x, b)
+            g = hip.record_graph(step, keep=[sv])
+        for k in range(40):
+            g.launch() if graph else step()
+            got.append((hip.get(sv.logits, np.uint32, sv.NSEQ * sv.vocab), get_i32(hip, sv.ids, sv.NSEQ), get_i32(hip, sv.len, sv.NSEQ)))
+        runs.append(got)
+        assert get_i32(hip, sv.err, 1)[0] == 0
+        assert get_i32(hip, sv.len, sv.NSEQ).tolist() == [56, 43, 55, 41]
+        if graph:
+            g.close()
+    for k, (a, b) in enumerate(zip(*runs)):
+        for x, y in zip(a, b):
+            np.testing.assert_array_equal(x, y, err_msg=str(k))
+    assert len({tuple(i) for _, i, _ in runs[0]}) > 3  # (the penalties move the choices)
