@@ -540,7 +540,8 @@ __device__ __forceinline__ void tile_run(const PagedAttn& a, const Keys& keys, u
         for (int u = 0; u < 4; u++) h |= ((uint32_t)pg[u] >= (uint32_t)a.n_pages) << u;
         return h;
     };
-    // A tile's rows of K (or V) into LDS: this wave its 16-key group `wave`, load j rows RPI j .. of it; past the last key its row
+    // A tile's rows of K (or V) into LDS: this wave its 16-key group `wave`, load j rows RPI j .. of it; past the last key its
+    // row. Rows RPI j further on, a chunk's place differs by the bits of swz(RPI j) alone (row addresses are multiples of 64 bytes).
     auto load = [&](int kt, const int (&pg)[4], uint64_t src, uint8_t* dst) __attribute__((always_inline)) {
         const bool pre = kt < keys.np;
         const int k0 = BK * (pre ? kt : kt - keys.np), lim = (pre ? keys.P : keys.len) - 1 - k0, g16 = min(16 * wave, lim & ~15);
@@ -548,11 +549,17 @@ __device__ __forceinline__ void tile_run(const PagedAttn& a, const Keys& keys, u
         const uint64_t at = src + (((uint64_t)((uint32_t)p < (uint32_t)a.n_pages ? p : 0) << a.page_shift) + ((k0 + g16) & ((1 << a.page_shift) - 1))) * kvd2;
         uint32_t ln = lane;
         asm volatile("" : "+v"(ln));
+        const uint32_t c16 = 16 * ((ln % LPR) ^ L::swz(ln / LPR));
+        if (lim >= BK - 1) {
+            const uint32_t off = __umul24(ln / LPR, kvd2) + c16;
 #pragma unroll
-        for (int j = 0; j < NJ; j++) {
-            const int row = RPI * j + ln / LPR;  // of the group
-            const uint32_t off = __umul24(min(16 * wave + row, lim) - g16, kvd2) + 16 * ((ln % LPR) ^ L::swz(row));
-            load_lds16_so(at, off, dst + (16 * wave + RPI * j) * L::ROW);
+            for (int j = 0; j < NJ; j++) load_lds16_so(at + RPI * j * kvd2, off ^ (16 * L::swz(RPI * j)), dst + (16 * wave + RPI * j) * L::ROW);
+        } else {
+#pragma unroll
+            for (int j = 0; j < NJ; j++) {
+                const int row = RPI * j + ln / LPR;  // of the group
+                load_lds16_so(at, __umul24(min(16 * wave + row, lim) - g16, kvd2) + (c16 ^ (16 * L::swz(RPI * j))), dst + (16 * wave + RPI * j) * L::ROW);
+            }
         }
     };
     // (the query's loads before the tiles', which the loop's first wait covers)
@@ -642,13 +649,16 @@ __device__ __forceinline__ void tile_run(const PagedAttn& a, const Keys& keys, u
         const bool tail = kt < keys.np && k0 + BK > keys.P;  // (the prefix's last tile, where it is not whole)
         if (k0 + BK - 1 > minhi || k0 < maxlo || hole || tail) {
             const int top = tail ? min(hi, keys.P - 1) : hi;
+            // (one unsigned comparison a key: 0 <= key - lo <= top - lo)
+            const uint32_t from = k0 + 4 * hf - (top < lo ? INT_MAX : lo), span = top < lo ? 0 : top - lo;
 #pragma unroll
             for (int mt = 0; mt < 2; mt++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int kp = 32 * mt + 8 * (i >> 2) + 4 * hf + (i & 3);
-                    if (k0 + kp > top || k0 + kp < lo || ((hole >> (kp >> 4)) & 1)) x[mt][i] = -INFINITY;
-                }
+                for (int i = 0; i < 16; i++) x[mt][i] = from + (32 * mt + 8 * (i >> 2) + (i & 3)) <= span ? x[mt][i] : -INFINITY;
+            if (hole)
+#pragma unroll
+                for (int v = 0; v < 32; v++)
+                    if ((hole >> (v >> 3)) & 1) x[v >> 4][v & 15] = -INFINITY;
         }
     };
     auto largest = [&](const f16v (&x)[2]) __attribute__((always_inline)) {
