@@ -391,7 +391,8 @@ int strata_rms_norm_rope_qk_paged(strata_ctx* ctx, uint64_t q, uint64_t q_tstrid
  * prefix[0 ..], computed once for all rows, and the sequence's own len[s] (new ones included), as strata_attn_decode_gq and
  * strata_attn_prefill_m compute it: sigmoid gates qg, per-head sink logits, head_dim 64 or 128, nh / nkv 1, 2, 4 or 8. No
  * prefix: max_prefix 0. A row that sees no key is 0; the keys of a page id outside 0 .. n_pages - 1 are not seen; values of
- * keys that a row does not see do not reach it, not even infinities and NaN. Rows from q_start[nseq] on stay as they were. */
+ * keys that a row does not see do not reach it, not even infinities and NaN. Rows from q_start[nseq] on stay as they were. q, qg, out and the caches are 16-byte aligned; out
+ * lies over no input. */
 int strata_attn_paged(strata_ctx* ctx, uint64_t q, uint64_t kc, uint64_t vc, uint64_t qg, uint64_t out, uint64_t t,
                       uint64_t max_q, uint64_t pos, uint64_t q_start, uint64_t len, uint64_t nseq, uint64_t tables,
                       uint64_t max_pages, uint64_t page, uint64_t n_pages, uint64_t prefix, uint64_t prefix_len,

@@ -1108,7 +1108,8 @@ int strata_attn_paged(strata_ctx* c, uint64_t q, uint64_t kc, uint64_t vc, uint6
     if (nseq * nkv * (max_pages * page / 64 + 32) >= (1ull << 31)) return set_error("paged attention: more than 2^31 chunks of keys (sequences x KV heads x positions / 64)");
     if ((t / (128 / (nh / nkv)) + nseq + 1) * ((max_prefix + max_pages * page) / 64 + 5) >= (1ull << 31))
         return set_error("paged attention: more than 2^31 tiles of rows and keys (rows x group / 128 + sequences, times positions / 64)");
-    if (q % 16 || out % 16 || kc % 16 || vc % 16) return set_error("paged attention: q, out and the caches must be 16-byte aligned");
+    if (q % 16 || out % 16 || kc % 16 || vc % 16 || qg % 16) return set_error("paged attention: q, qg, out and the caches must be 16-byte aligned");
+    if (out == q || out == qg) return set_error("paged attention: out over an input");
     PagedAttn a;
     a.q = (const float*)q; a.kc = (const uint16_t*)kc; a.vc = (const uint16_t*)vc; a.qg = (const float*)qg; a.out = (float*)out;
     a.t = (int)t; a.max_q = (int)max_q; a.pos = (const int*)pos; a.q_start = (const int*)q_start; a.len = (const int*)len;

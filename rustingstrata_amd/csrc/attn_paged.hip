@@ -7,10 +7,14 @@
 // over the keys at positions <= pos[r] (with a window the last `win` of them). A row that sees no key gives 0; a page outside
 // 0 .. n_pages - 1 holds no keys.
 //
-// Three kernels: attn_paged_dec_kernel takes the sequences of few rows (a decode step: bound by their K and V bytes),
-// attn_paged_tile_kernel the keys that many rows share (the prefix for all rows, or a prompt chunk's own keys: bound by the
-// matrix cores), and attn_paged_merge_kernel joins their softmax sums. Numerics as in attn.hip: q and the softmax weights as
-// f16 hi + lo parts, K and V exact in f16, all sums in f32, log2 units.
+// One launch does the work in blocks of three kinds (attn_paged_kernel), a second one joins its partial sums:
+//   dec_block     the own keys of sequences of few rows (a decode step): bound by their K and V bytes;
+//   prefix_block  the prefix for those sequences' rows, whatever their sequence: K and V read once a tile of rows;
+//   tile_block    the prefix and own keys of sequences of many rows (prompt chunks), from attn_paged_plan_kernel's list of their
+//                 tiles: bound by the matrix cores and the softmax's vector instructions, which add up.
+// The kinds are bound by different things and run beside each other (in launches of their own: 64 sequences over a prefix of 16000
+// 71 us a call for 59, 24 of 4 tokens over one of 6001 35 for 22). Numerics as in attn.hip: q and the softmax weights as f16 hi
+// + lo parts (2^-22 of a value), K and V exact in f16, all sums in f32, log2 units.
 #include <algorithm>
 #include <climits>
 
@@ -21,7 +25,7 @@ namespace strata {
 
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 
-// A call's workspace and split plan (launch_attn_paged).
+// A call's workspace and split plan (plan() below).
 struct PagedWs {
     int2* map;     // [nseq nkv] first block and pieces of a decode sequence's KV head
     float2* dml;   // [slots][dr] max and sum of a piece's rows
@@ -166,6 +170,8 @@ __device__ __forceinline__ h4 read_tr(const uint16_t* p) {
 //   wave's LDS, read transposed).
 // The next chunk's V is requested when this one's has gone to LDS, its K when the scores are done: both fly during the softmax
 // and the V products without more registers. The four waves meet in LDS at the piece's end.
+// 64 sequences of 100 to 24000 keys (32 heads of 128 over 4, 539 MB): 114 us, 4.7 TB/s, a copy's rate; one of 550 keys 9 us, a chain
+// of the run's search (2), the loads (2.5), the products (1.2) and the waves' meeting (2).
 template <int HD>
 struct PagedDec {
     static constexpr int VP = HD + 16;             // halves a V row in LDS (32 bytes on: the transposed reads' 16 rows spread)
@@ -500,6 +506,9 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
 // The scores of a tile are computed beside the softmax of the one before, whose vector instructions fill the matrix
 // instructions' shadow; a tile costs one barrier. K and V go from memory straight to LDS (no registers hold them), two buffers
 // each: while tile t's V and tile t + 1's K are used, the next of each land.
+// 1024 rows over 16384 keys (32 heads of 128 over 4): 500 us, 533 TFLOP/s of the formula's operations, twice that on the matrix
+// cores for the hi and lo parts. A wave's tile costs its 64 matrix instructions and about 270 vector ones and 33 exps one after
+// the other (each part left out alone saves its own share); without loads or over one page it takes as long.
 // Rows in LDS are HD halves apart without padding; 16-byte chunk c of row r sits at c ^ swz(r), which spreads both the score
 // fragments' reads (a chunk of 32 rows) and the transposed reads (4 chunks of 8 rows) over all banks.
 template <int HD>
@@ -822,7 +831,7 @@ __device__ __forceinline__ void tile_store(const TileSums<HD>& r, int tid, float
 // The prefix for the rows of decode sequences: tiles of the call's rows (of the plan's list of them, where there is a plan)
 // whatever their sequence, so that the prefix's K and V are read once a tile of 128 / G tokens rather than once a token; a
 // block takes a split of the prefix's keys. Blocks are numbered so that the tiles over the same keys run on one XCD (its L2
-// holds a split's K and V).
+// holds a split's K and V). 64 rows of 32 heads over 16000 keys, own keys beside them: 52 us.
 template <int HD>
 __device__ __forceinline__ void prefix_block(const PagedAttn& a, const PagedWs& w, int x, int tiles, uint8_t* lds) {
     __shared__ int ws[8];
@@ -890,7 +899,8 @@ struct PlanTile {
     int kt0, nkt, cum, pad;  // first key tile, key tiles; work of the tiles before
 };
 constexpr int PLAN_HEAD = 4;  // tiles, their work, rows of decode sequences
-// A tile's work in key tiles: those it has, and what it takes to begin and end one (9 + 4 us beside 4 a key tile).
+// A tile's work in key tiles: those it has, and what it takes to begin and end one (9 + 4 us beside 4 a key tile). With 0 here
+// chunks of 2501 tokens take 174 us for 132, long contexts the same.
 constexpr int TILE_EXTRA = 3;
 
 // One block of 1024 threads: the sequences' tiles by a scan in LDS, then the tiles' keys and their scan, 1024 tiles at a time.
@@ -1299,13 +1309,18 @@ static PagedWs plan(const PagedAttn& a, uint8_t* at, size_t* end) {
     PagedWs w{};
     const int G = a.nh / a.nkv;
     const long long rows = (long long)a.t * G;
-    // a sequence decodes up to 16 rows (one column tile), up to 32 where the longest has no more
+    // a sequence decodes up to 16 rows (one column tile), up to 32 where the longest has no more (64 sequences of 4 tokens, 8 heads a
+    // KV head, over 2048 keys: 70 us, as tiles of 128 rows 97)
     const long long most_rows = (long long)a.max_q * G;
     w.nct = most_rows > 16 && most_rows <= 32 ? 2 : 1;
     w.dr = (int)std::min<long long>(16 * w.nct, most_rows);
     const long long most = (long long)a.nseq * a.nkv * (((long long)a.max_pages << a.page_shift) / DEC_CHUNK + 1);
-    w.dblocks = (int)std::min<long long>(most, w.nct == 1 && (!a.max_prefix || most_rows > w.dr) ? 512 : 256);  // the blocks that run at once
-    // splits of the prefix: enough blocks for two a CU, of at least 128 keys
+    // the blocks that run at once: two a CU (64 ragged sequences 117 us against 122, 300 of 700 keys 104 against 116; a few long ones
+    // gain 3 to 5% from one), one where their columns or the prefix's blocks take the other's place (24 of 4 tokens over a prefix
+    // 24.2 us against 26.4, 64 over one of 4096 33 against 41)
+    w.dblocks = (int)std::min<long long>(most, w.nct == 1 && (!a.max_prefix || most_rows > w.dr) ? 512 : 256);
+    // splits of the prefix, of at least 128 keys: a block a CU (64 sequences over a prefix of 4096 31 us, for two a CU 46; of 16000 56
+    // and 59): more of them cost more sums than they hide
     const long long blocks = std::max<long long>((long long)div_up(rows, 128) * a.nkv, 1);
     w.nsp = (int)std::max<long long>(1, std::min<long long>({div_up(256, blocks), div_up(a.max_prefix, 128), 64}));
     w.tblocks = 512;

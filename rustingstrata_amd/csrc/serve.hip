@@ -20,7 +20,8 @@ namespace strata {
 // a thread sums 4 consecutive sequences, the waves' totals meet in LDS, and the tokens find their sequence by a binary search
 // of q_start in LDS. Bound by latency (two rounds of loads and three barriers of scans): 8 sequences, one token each 6.6 us, 512
 // with 8192 new tokens 11.6.
-// More than PAGES_ONE tokens take a second launch over many blocks that searches q_start in memory.
+// More than PAGES_ONE tokens take a second launch over many blocks that searches q_start in memory (4096 tokens 9.6 us in one block,
+// 10.0 in two launches; 2048 7.8 and 9.8; 8192 13.1 and 10.0).
 constexpr int PAGES_ONE = 4096;
 constexpr unsigned SAT = 1u << 30;
 __device__ __forceinline__ unsigned sat_add(unsigned a, unsigned b) { return min(a + b, SAT); }  // a, b <= SAT

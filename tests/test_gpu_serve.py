@@ -633,12 +633,12 @@ def test_attn_paged_matches_the_contiguous_forms(hip):
 
 
 def test_attn_paged_refused_arguments(hip):
-    x = hip.alloc(1 << 16)
-    ok = dict(q=x, kc=x, vc=x, qg=0, out=x, t=2, max_q=1, pos=x, q_start=x, length=x, nseq=2, tables=x, max_pages=4, page=16, n_pages=8, nh=8, nkv=2, hd=64, scale=0.125)
+    x, y = hip.alloc(1 << 16), hip.alloc(1 << 16)
+    ok = dict(q=x, kc=x, vc=x, qg=0, out=y, t=2, max_q=1, pos=x, q_start=x, length=x, nseq=2, tables=x, max_pages=4, page=16, n_pages=8, nh=8, nkv=2, hd=64, scale=0.125)
     for bad in (dict(hd=96), dict(nh=6), dict(nh=32), dict(nkv=0), dict(nseq=4097), dict(page=24), dict(page=8), dict(n_pages=0), dict(n_pages=1 << 27), dict(max_pages=0),
                 dict(max_pages=1 << 27), dict(q=0), dict(kc=0), dict(vc=0), dict(out=0), dict(pos=0), dict(q_start=0), dict(length=0), dict(tables=0), dict(max_q=0), dict(max_q=3),
                 dict(t=(1 << 20) + 1), dict(max_prefix=5), dict(max_prefix=5, prefix=x), dict(max_prefix=5, prefix_len=x), dict(max_prefix=(1 << 30) + 1, prefix=x, prefix_len=x),
-                dict(win=1 << 31), dict(q=int(x) + 4), dict(out=int(x) + 8), dict(kc=int(x) + 2), dict(vc=int(x) + 8), dict(nseq=4096, max_pages=1 << 26)):
+                dict(win=1 << 31), dict(q=int(x) + 4), dict(qg=int(x) + 4), dict(out=int(y) + 8), dict(out=x), dict(qg=y), dict(kc=int(x) + 2), dict(vc=int(x) + 8), dict(nseq=4096, max_pages=1 << 26)):
         with pytest.raises(S.StrataError, match="paged attention"):
             hip.attn_paged(**{**ok, **bad})
     hip.attn_paged(**{**ok, "t": 0})
