@@ -1022,8 +1022,9 @@ __device__ __forceinline__ int tile_of(const PlanTile* plan, int n, int x) {
 __device__ __forceinline__ PlanTile plan_tile(const PlanTile* p) {
     return PlanTile{sload(&p->s), sload(&p->t0), sload(&p->nt), sload(&p->len), sload(&p->kt0), sload(&p->nkt), sload(&p->cum), 0};
 }
-// Where block b's run of the list begins: at b times an equal share of the work, moved to the tile's border where no more than
-// an eighth of the share, and no more than 3 key tiles, lie between: a tile that is not cut costs no sums.
+// Where block b's run of the list begins: at b times an equal share of the work, moved to the tile's border where one key tile, and
+// no more than an eighth of the share, lies between: a tile that is not cut costs no sums, but the run becomes longer (up to 3 key
+// tiles: chunks of 2501 tokens 132 us for 130, up to 5 134).
 struct RunAt {
     long long at;  // in the list of all tiles' work
     int g, i, f;   // the KV head, the tile, the key tile of it
@@ -1032,7 +1033,7 @@ struct RunAt {
 };
 __device__ __forceinline__ RunAt run_at(const PlanTile* plan, int n, int cost, int nkv, int b, int blocks) {
     const long long all = (long long)cost * nkv, share = max((all + blocks - 1) / blocks, 2ll);
-    const int near = (int)min(share / 8, 3ll);
+    const int near = (int)min(share / 8, 1ll);
     RunAt r{min(b * share, all), nkv, 0, 0, share, near};
     if (r.at == all) return r;
     r.g = (int)(r.at / cost);
