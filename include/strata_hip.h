@@ -365,7 +365,7 @@ int strata_attn_decode_gq(strata_ctx* ctx, uint64_t q, uint64_t kc, uint64_t vc,
  * add[s] < 0: it ends; its pages go back on the stack of free pages (free_pages: n_pages entries, *n_free of them in use, the
  * top last) in order of sequence and page, before any page is taken. Then, in order of sequence, new pages come from the
  * top of the stack into the tables. Writes q_start[nseq + 1], for each row t < q_start[nseq] its position pos[t] (*prefix_len
- * more than its own one; prefix_len may be 0) and its slot slots[t], -1 in both for the rows up to t_max behind them, and len_out
+ * more than its own one, nothing where that is below 0; prefix_len may be 0) and its slot slots[t], -1 in both for the rows up to t_max behind them, and len_out
  * and *n_free_out (which may be len and n_free). A sequence is refused where its positions exceed max_pages pages, its rows
  * exceed t_max, the stack holds too few pages for it and the sequences before it, or len[s] is below 0: its length, table and
  * the stack stay as they are, its rows keep their places (q_start is cut at t_max, positions at 2^31 - 1) and have slot -1, and *err (device int32,
@@ -392,7 +392,7 @@ int strata_rms_norm_rope_qk_paged(strata_ctx* ctx, uint64_t q, uint64_t q_tstrid
  * strata_attn_prefill_m compute it: sigmoid gates qg, per-head sink logits, head_dim 64 or 128, nh / nkv 1, 2, 4 or 8. No
  * prefix: max_prefix 0. A row that sees no key is 0; the keys of a page id outside 0 .. n_pages - 1 are not seen; values of
  * keys that a row does not see do not reach it, not even infinities and NaN. Rows from q_start[nseq] on stay as they were. q, qg, out and the caches are 16-byte aligned; out
- * lies over no input. */
+ * lies over no input; scale is above 0. */
 int strata_attn_paged(strata_ctx* ctx, uint64_t q, uint64_t kc, uint64_t vc, uint64_t qg, uint64_t out, uint64_t t,
                       uint64_t max_q, uint64_t pos, uint64_t q_start, uint64_t len, uint64_t nseq, uint64_t tables,
                       uint64_t max_pages, uint64_t page, uint64_t n_pages, uint64_t prefix, uint64_t prefix_len,

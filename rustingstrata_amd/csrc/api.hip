@@ -1,6 +1,7 @@
 // The C ABI (include/strata_hip.h): context, memory, argument checks, and the launch sequences of the hot-path
 // Backend methods (src/backend.rs:98-443, CUDA implementation src/cuda/mod.rs:748-1242).
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <map>
 #include <mutex>
@@ -1110,6 +1111,7 @@ int strata_attn_paged(strata_ctx* c, uint64_t q, uint64_t kc, uint64_t vc, uint6
         return set_error("paged attention: more than 2^31 tiles of rows and keys (rows x group / 128 + sequences, times positions / 64)");
     if (q % 16 || out % 16 || kc % 16 || vc % 16 || qg % 16) return set_error("paged attention: q, qg, out and the caches must be 16-byte aligned");
     if (out == q || out == qg) return set_error("paged attention: out over an input");
+    if (!(scale > 0.0f) || std::isinf(scale)) return set_error("paged attention: a scale of " + std::to_string(scale) + " (above 0)");
     PagedAttn a;
     a.q = (const float*)q; a.kc = (const uint16_t*)kc; a.vc = (const uint16_t*)vc; a.qg = (const float*)qg; a.out = (float*)out;
     a.t = (int)t; a.max_q = (int)max_q; a.pos = (const int*)pos; a.q_start = (const int*)q_start; a.len = (const int*)len;

@@ -106,7 +106,7 @@ __global__ __launch_bounds__(1024) void pages_plan_kernel(PagesStep a) {
         len[k] = s < a.nseq ? a.len[s] : 0;
         v[k] = add[k] < 0 && len[k] > 0 ? (unsigned)((min(len[k], limit) + (long long)page - 1) >> a.page_shift) : 0u;
     }
-    const int held = min(max(*a.n_free, 0), a.n_pages), P = a.prefix_len ? *a.prefix_len : 0;
+    const int held = min(max(*a.n_free, 0), a.n_pages), P = a.prefix_len ? max(*a.prefix_len, 0) : 0;
     // sequences that end: their pages on the stack, entry i by thread i
     const unsigned back = scan4(v, ex, ws);
 #pragma unroll

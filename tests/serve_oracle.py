@@ -5,7 +5,7 @@ import numpy as np
 
 def pages_step(add, length, tables, max_pages, page, free, n_pages, n_free, P, t_max):
     """What kv_pages_step leaves: q_start, pos, slots, len_out, n_free_out, tables, free, refused."""
-    tables, free = tables.copy(), free.copy()
+    tables, free, P = tables.copy(), free.copy(), max(P, 0)
     limit = max_pages * page
     stack = list(free[:min(max(n_free, 0), n_pages)])
     refused, lost = 0, False

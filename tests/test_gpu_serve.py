@@ -467,6 +467,20 @@ def test_attn_paged_deep_chunks(hip, nh, nkv, hd, q, n, P, win):
     b.check(b.get(), win, rows=sorted(rows)[:40])
 
 
+@pytest.mark.parametrize("q,P", [([1] * 9, 0), ([1, 4, 2, 1], 70), ([60, 1, 17, 2, 33], 0), ([60, 1, 17, 2, 33], 130)])
+@pytest.mark.parametrize("win", [0, 1, 37, 2**31 - 1])
+def test_attn_paged_positions_in_any_order(hip, q, P, win):
+    """Rows at any positions in any order: before the first key, past the last, twice the same; windows of one key and of all; a
+    bound max_q of all rows."""
+    rng = np.random.default_rng(win % 100 + P)
+    n = rng.integers(0, 500, len(q)).tolist()
+    b = Batch(hip, q, n, 8, 2, 64, 16, P=P, seed=P + 3, sink=True, gate=True)
+    for s in range(len(q)):
+        b.pos[b.q_start[s]:b.q_start[s + 1]] = rng.integers(-3, P + n[s] + 6, q[s])
+    b.upload().launch(win, max_q=b.t)
+    b.check(b.get(), win)
+
+
 @pytest.mark.parametrize("nseq", [257, 1030, 4096])
 @pytest.mark.parametrize("P", [0, 33])
 def test_attn_paged_many_sequences(hip, nseq, P):
@@ -638,7 +652,8 @@ def test_attn_paged_refused_arguments(hip):
     for bad in (dict(hd=96), dict(nh=6), dict(nh=32), dict(nkv=0), dict(nseq=4097), dict(page=24), dict(page=8), dict(n_pages=0), dict(n_pages=1 << 27), dict(max_pages=0),
                 dict(max_pages=1 << 27), dict(q=0), dict(kc=0), dict(vc=0), dict(out=0), dict(pos=0), dict(q_start=0), dict(length=0), dict(tables=0), dict(max_q=0), dict(max_q=3),
                 dict(t=(1 << 20) + 1), dict(max_prefix=5), dict(max_prefix=5, prefix=x), dict(max_prefix=5, prefix_len=x), dict(max_prefix=(1 << 30) + 1, prefix=x, prefix_len=x),
-                dict(win=1 << 31), dict(q=int(x) + 4), dict(qg=int(x) + 4), dict(out=int(y) + 8), dict(out=x), dict(qg=y), dict(kc=int(x) + 2), dict(vc=int(x) + 8), dict(nseq=4096, max_pages=1 << 26)):
+                dict(win=1 << 31), dict(q=int(x) + 4), dict(qg=int(x) + 4), dict(out=int(y) + 8), dict(out=x), dict(qg=y), dict(scale=0.0), dict(scale=-1.0), dict(scale=np.nan),
+                dict(scale=np.inf), dict(kc=int(x) + 2), dict(vc=int(x) + 8), dict(nseq=4096, max_pages=1 << 26)):
         with pytest.raises(S.StrataError, match="paged attention"):
             hip.attn_paged(**{**ok, **bad})
     hip.attn_paged(**{**ok, "t": 0})
