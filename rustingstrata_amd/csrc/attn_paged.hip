@@ -905,7 +905,7 @@ constexpr int TILE_EXTRA = 3;
 
 // One block of 1024 threads: the sequences' tiles by a scan in LDS, then the tiles' keys and their scan, 1024 tiles at a time.
 __global__ __launch_bounds__(1024) void attn_paged_plan_kernel(PagedAttn a, PagedWs w, int tiles) {
-    __shared__ int start[SERVE_MAX_SEQ], dstart[SERVE_MAX_SEQ], ws[17];
+    __shared__ int start[SERVE_MAX_SEQ], dstart[SERVE_MAX_SEQ], row0[SERVE_MAX_SEQ + 1], ws[16];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, G = a.nh / a.nkv, TT = 128 / G, P = prefix_len(a), np = (P + 63) / 64;
     auto scan = [&](int v, int& total) {  // exclusive, over the block
         int inc = v;
@@ -926,20 +926,21 @@ __global__ __launch_bounds__(1024) void attn_paged_plan_kernel(PagedAttn a, Page
         }
         return before;
     };
-    int nt[4], nd[4], sum = 0, dsum = 0, ntiles, ndec;
+    int nt[4], nd[4], q[5], sum = 0, dsum = 0, ntiles, ndec = 0;
+#pragma unroll
+    for (int i = 0; i < 5; i++) q[i] = 4 * tid + i <= a.nseq ? a.q_start[4 * tid + i] : 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const int s = 4 * tid + i;
-        nt[i] = nd[i] = 0;
-        if (s < a.nseq) {
-            const int q0 = min(max(a.q_start[s], 0), a.t), qn = min(max(a.q_start[s + 1], q0), a.t) - q0;
-            if (qn * G > w.dr) nt[i] = (qn + TT - 1) / TT;
-            else nd[i] = qn;
-        }
+        const int s = 4 * tid + i, q0 = min(max(q[i], 0), a.t), qn = s < a.nseq ? min(max(q[i + 1], q0), a.t) - q0 : 0;
+        const bool dec = qn * G <= w.dr;
+        nt[i] = dec ? 0 : (qn + TT - 1) / TT;
+        nd[i] = dec ? qn : 0;
+        if (s <= a.nseq) row0[s] = q0;
         sum += nt[i];
         dsum += nd[i];
     }
-    int at = scan(sum, ntiles), dat = scan(dsum, ndec);
+    if (tid == 1023 && a.nseq == SERVE_MAX_SEQ) row0[SERVE_MAX_SEQ] = min(max(q[4], 0), a.t);
+    int at = scan(sum, ntiles), dat = w.drows ? scan(dsum, ndec) : 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         if (4 * tid + i < a.nseq) {
@@ -964,7 +965,7 @@ __global__ __launch_bounds__(1024) void attn_paged_plan_kernel(PagedAttn a, Page
     if (w.drows)
         for (int i = tid; i < ndec; i += 1024) {
             const int s = find(dstart, i);
-            w.drows[i] = min(max(a.q_start[s], 0) + i - dstart[s], a.t - 1);
+            w.drows[i] = min(row0[s] + i - dstart[s], a.t - 1);
         }
     PlanTile* plan = (PlanTile*)(w.plan + PLAN_HEAD);
     int cum = 0;
@@ -973,7 +974,7 @@ __global__ __launch_bounds__(1024) void attn_paged_plan_kernel(PagedAttn a, Page
         PlanTile p{};
         if (i < ntiles) {
             p.s = find(start, i);
-            const int q0 = min(max(a.q_start[p.s], 0), a.t), q1 = min(max(a.q_start[p.s + 1], q0), a.t);
+            const int q0 = row0[p.s], q1 = max(row0[p.s + 1], q0);
             p.t0 = q0 + (i - start[p.s]) * TT;
             p.nt = min(TT, q1 - p.t0);
             p.len = (int)min((long long)max(a.len[p.s], 0), (long long)a.max_pages << a.page_shift);
