@@ -368,16 +368,15 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
                 for (int u = 0; u < NT; u++)
 #pragma unroll
                     for (int t = 0; t < 2; t++) sv[u][t] = (f4){0.0f, 0.0f, 0.0f, 0.0f};
+                // (the lo parts first: their sums are small, so only the hi parts' steps round at the score's size)
 #pragma unroll
-                for (int k = 0; k < KS; k++)
+                for (int k = 0; k < 2 * KS; k++)
 #pragma unroll
                     for (int u = 0; u < NT; u++)
 #pragma unroll
-                        for (int t = 0; t < 2; t++) {
-                            const h8 kv = __builtin_bit_cast(h8, kf[t][k]);
-                            sv[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, qh[u][k], sv[u][t], 0, 0, 0);
-                            sv[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kv, ql[u][k], sv[u][t], 0, 0, 0);
-                        }
+                        for (int t = 0; t < 2; t++)
+                            sv[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, kf[t][k % KS]), k < KS ? ql[u][k % KS] : qh[u][k % KS],
+                                                                              sv[u][t], 0, 0, 0);
             }
             if (more) {
                 if (cur.ok) load_k(cur);

@@ -391,8 +391,8 @@ class Batch:
                       gate=self.gate[:, :, 1] if self.gate is not None else None, rows=rows)
 
     def check(self, got, win=0, rows=None):
-        """Each row and head within 2^-23 (14 + max |s|) of its norm: a float32 score is off by 2^-24 |s| in its sum and again in
-        the exponent, which is its weight's relative error; the exps, the splits (2^-22), the sums and the two joins of partial
+        """Each row and head within 2^-23 (14 + max |s|) of its norm: a float32 score is off by 2^-24 |s| in its sum (of some
+        hd / 8 steps, whose roundings mostly cancel) and again in the exponent, which is its weight's relative error; the exps, the splits (2^-22), the sums and the two joins of partial
         sums (an exp, a product and a sum each) add fourteen times 2^-23 at most."""
         want, top = self.want(win, rows if rows is None else set(rows))
         m = self.q_start[-1]
