@@ -1275,7 +1275,7 @@ __device__ __forceinline__ void merge_block(const PagedAttn& a, const PagedWs& w
 // The pieces: blocks of the long sequences' tiles (TILE), of the prefix for the rows of decode sequences (PRE) and of their own
 // keys, in one launch.
 template <int HD, int NT, bool TILE, bool PRE>
-__global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void attn_paged_kernel(PagedAttn a, PagedWs w, int pblocks, int tiles) {
+__global__ __launch_bounds__(256, NT == 1 || HD == 64 ? 2 : 1) void attn_paged_kernel(PagedAttn a, PagedWs w, int pblocks, int tiles) {
     constexpr int TB = TILE || PRE ? 2 * PagedTile<HD>::BUF : 0;
     __shared__ __align__(16) uint8_t lds[PagedDec<HD>::BYTES > TB ? PagedDec<HD>::BYTES : TB];
     int b = blockIdx.x;
@@ -1317,9 +1317,10 @@ static PagedWs plan(const PagedAttn& a, uint8_t* at, size_t* end) {
     w.dr = (int)std::min<long long>(16 * w.nct, most_rows);
     const long long most = (long long)a.nseq * a.nkv * (((long long)a.max_pages << a.page_shift) / DEC_CHUNK + 1);
     // the blocks that run at once: two a CU (64 ragged sequences 117 us against 122, 300 of 700 keys 104 against 116; a few long ones
-    // gain 3 to 5% from one), one where their columns or the prefix's blocks take the other's place (24 of 4 tokens over a prefix
-    // 24.2 us against 26.4, 64 over one of 4096 33 against 41)
-    w.dblocks = (int)std::min<long long>(most, w.nct == 1 && (!a.max_prefix || most_rows > w.dr) ? 512 : 256);
+    // gain 3 to 5% from one), one where two column tiles of 128 values fill a CU's registers (of 64 values two: 100 sequences of 4
+    // tokens 169 us against 211) or the prefix's blocks take the other's place (24 of 4 tokens over a prefix 24.2 us against 26.4, 64
+    // over one of 4096 33 against 41)
+    w.dblocks = (int)std::min<long long>(most, (w.nct == 1 || a.hd == 64) && (!a.max_prefix || most_rows > w.dr) ? 512 : 256);
     // splits of the prefix, of at least 128 keys: a block a CU (64 sequences over a prefix of 4096 31 us, for two a CU 46; of 16000 56
     // and 59): more of them cost more sums than they hide
     const long long blocks = std::max<long long>((long long)div_up(rows, 128) * a.nkv, 1);
