@@ -27,7 +27,8 @@ typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 
 // A call's workspace and split plan (plan() below).
 struct PagedWs {
-    int2* map;     // [nseq nkv] first block and pieces of a decode sequence's KV head
+    int2* map;     // decode sequences: [nseq nkv] first block and pieces of a KV head; direct: [dblocks] the (sequence, KV head)
+                   // that begins in a block and goes on past it, and its pieces (0: none)
     float2* dml;   // [slots][dr] max and sum of a piece's rows
     float* dacc;   // [slots][dr][hd]
     float2* pml;   // [t nh][nsp]: the prefix's splits, of the rows of decode sequences
@@ -37,6 +38,7 @@ struct PagedWs {
     int4* cut;     // [tblocks] KV head and tile that block b's run cuts, and the last block of its pieces (below 0: none)
     float2* tml;   // [2 tblocks][128]: the pieces of tiles that more than one block computes
     float* tacc;   // [2 tblocks][128][hd]
+    int direct;    // a (sequence, KV head) that one block holds is finished there, and the join takes those that a block cuts
     int dblocks, nct, dr, nsp, tblocks;  // decode blocks, their column tiles; rows (tokens x G) up to which a sequence decodes
 };
 
@@ -157,20 +159,31 @@ __device__ __forceinline__ h4 read_tr(const uint16_t* p) {
     return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4*)p));
 }
 
+// The factor that turns a row's sums into its output: over the sum and the sink (0 for a row without keys, not a number where a
+// score is not).
+__device__ __forceinline__ float out_factor(const PagedAttn& a, int h, float m, float l) {
+    const float sk = a.sink ? a.sink[h] * LOG2E : -INFINITY, M = fmaxf(m, sk);
+    const float sc = m == -INFINITY ? 0.0f : exp2_hw(m - M);
+    const float den = l * sc + (sk == -INFINITY ? 0.0f : exp2_hw(sk - M));
+    return den == 0.0f ? 0.0f : sc / den;
+}
+
 // ---------------- few rows a sequence ----------------
 // The work is the list of all (sequence, KV head, chunk of DEC_CHUNK own keys), chunk fastest; a block takes an equal run of
 // it, so contexts of any lengths load the CUs evenly. A run covers pieces of one or more (sequence, KV head) pairs; block b's
 // piece of pair i leaves its softmax sums at slot b + i (along the list either b or i goes up by one, so slots are distinct).
-// The block that holds a pair's first chunk notes which blocks follow.
+// The block that holds a pair's first chunk notes which blocks follow; with many pairs (DIRECT) one that holds a whole pair
+// finishes its rows.
 // Inside a piece, wave w takes keys 32 w .. 32 w + 31 of each chunk with its own online softmax for all rows (16 NT columns:
 // token c / G, head c % G), on f16 MFMA with f32 accuracy:
 //   S^T (2 tiles of 16 keys x 16 columns) = K Q^T (v_mfma_f32_16x16x32_f16; A: the key rows, read straight from memory in the
 //   fragments' layout, 16 rows x 64 bytes a load; B: q's hi and lo parts);
 //   O^T (16 dims x 16 columns, DT tiles) += V^T P^T (K = 32; B: the lane's own 8 weights, hi and lo; A: V's rows through the
 //   wave's LDS, read transposed).
-// The next chunk's V is requested when this one's has gone to LDS, its K when the scores are done: both fly during the softmax
-// and the V products without more registers. The four waves meet in LDS at the piece's end.
-// 64 sequences of 100 to 24000 keys (32 heads of 128 over 4, 539 MB): 114 us, 4.7 TB/s, a copy's rate; one of 550 keys 9 us, a chain
+// The next chunk's V (the next piece's, at the end of one) is requested when this one's has gone to LDS, its K when the scores are
+// done: both fly during the softmax and the V products without more registers. The four waves meet in LDS at the piece's end,
+// while the next one's queries arrive.
+// 64 sequences of 100 to 24000 keys (32 heads of 128 over 4, 539 MB): 112 us, 4.8 TB/s, a copy's rate; 1000 of 300 138 us, 4.5 TB/s; one of 550 keys 9 us, a chain
 // of the run's search (2), the loads (2.5), the products (1.2) and the waves' meeting (2).
 template <int HD>
 struct PagedDec {
@@ -179,7 +192,7 @@ struct PagedDec {
     static constexpr int MERGE = DEC_WAVES * (HD * 17 + 32) * 4;
     static constexpr int BYTES = DEC_WAVES * WAVE > MERGE ? DEC_WAVES * WAVE : MERGE;
 };
-template <int HD, int NT>
+template <int HD, int NT, bool DIRECT>
 __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, int b, uint8_t* lds) {
     using L = PagedDec<HD>;
     typedef unsigned v4u __attribute__((ext_vector_type(4)));
@@ -226,6 +239,7 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
         share = max((total + w.dblocks - 1) / w.dblocks, (big + 127) / 128);
         W0 = (int)min((long long)b * share, (long long)total);
         W1 = (int)min((long long)W0 + share, (long long)total);
+        if (DIRECT && tid == 0) w.map[b] = make_int2(0, 0);
         if (W0 >= W1) return;
         if (W0 >= at * a.nkv && W0 < (at + sum) * a.nkv)
             for (int i = 0; i < per && tid * per + i < a.nseq; i++) {
@@ -247,69 +261,100 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
     const uint32_t kvd2 = 2 * a.nkv * HD;
     const int vr = lane / LPR, vcol = 8 * (lane % LPR);
     const uint32_t vcol2 = 2 * vcol;
-    for (int at = W0; at < W1;) {
+    const uint64_t kb = (uint64_t)a.kc, vb0 = (uint64_t)a.vc;
+    // a piece: chunks c0 .. c1 - 1 of sequence s and KV head g
+    struct Piece {
+        SeqInfo q;
+        int s, g, c0, c1, head;  // head: if it holds the pair's first chunk, the blocks that share the pair (else 0)
+    };
+    int at = W0;
+    auto next_piece = [&](Piece& p) __attribute__((always_inline)) {
+        if (at >= W1) return false;
         while (at - base >= q.nc * a.nkv) {  // the next sequence that has work
             base += q.nc * a.nkv;
-            if (++s >= a.nseq) return;
+            if (++s >= a.nseq) return false;
             q = seq_info<true>(a, s, G, w.dr, P);
         }
         const int g = (at - base) / q.nc, f = (at - base) % q.nc, n = min(q.nc - f, W1 - at);
-        const int pair = s * a.nkv + g;
-        if (f == 0 && tid == 0) w.map[pair] = make_int2(b, (at + q.nc - 1) / share - b + 1);
+        p = Piece{q, s, g, q.c0 + f, q.c0 + f + n, f == 0 ? (at + q.nc - 1) / share - b + 1 : 0};
         at += n;
-        const int* table = a.tables + (uint64_t)s * a.max_pages;
-        const uint64_t kg = (uint64_t)(a.kc + g * HD), vg = (uint64_t)(a.vc + g * HD);
-        // The wave's two groups of 16 keys of chunk c (each in one page): their cache rows; ok: bit t where group t has keys. A
-        // group without keys reads the other's rows.
-        struct Rows {
-            uint64_t at[2];  // bytes into either cache
-            int last[2], ok;
-        };
-        auto pages = [&](int c, int (&pg)[2]) __attribute__((always_inline)) {
+        return true;
+    };
+    // The wave's two groups of 16 keys of chunk c (each in one page): their cache rows; ok: bit t where group t has keys. A
+    // group without keys reads the other's rows.
+    struct Rows {
+        uint64_t at[2];  // bytes into either cache
+        int last[2], ok;
+    };
+    auto pages = [&](const Piece& p, int c, int (&pg)[2]) __attribute__((always_inline)) {
+        const int* table = a.tables + (uint64_t)p.s * a.max_pages;
 #pragma unroll
-            for (int t = 0; t < 2; t++) pg[t] = sload(table + (min(DEC_CHUNK * c + 32 * wave + 16 * t, q.len - 1) >> a.page_shift));
-        };
-        auto rows = [&](int c, const int (&pg)[2]) __attribute__((always_inline)) {
-            Rows r;
-            r.ok = 0;
+        for (int t = 0; t < 2; t++) pg[t] = sload(table + (min(DEC_CHUNK * c + 32 * wave + 16 * t, p.q.len - 1) >> a.page_shift));
+    };
+    auto rows = [&](const Piece& p, int c, const int (&pg)[2]) __attribute__((always_inline)) {
+        Rows r;
+        r.ok = 0;
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const int k0 = DEC_CHUNK * c + 32 * wave + 16 * t;
-                r.at[t] = (((uint64_t)(uint32_t)pg[t] << a.page_shift) + (k0 & ((1 << a.page_shift) - 1))) * kvd2;
-                r.last[t] = min(q.len - 1 - k0, 15);
-                r.ok |= (r.last[t] >= 0 && (uint32_t)pg[t] < (uint32_t)a.n_pages) << t;
-            }
-            if (r.ok == 1) r.at[1] = r.at[0], r.last[1] = r.last[0];
-            if (r.ok == 2) r.at[0] = r.at[1], r.last[0] = r.last[1];
-            return r;
-        };
-        // (a group's rows: a scalar base and a lane's 32-bit offset)
-        v4u kf[2][KS], vb[NV];
-        auto load_v = [&](const Rows& r) __attribute__((always_inline)) {
-#pragma unroll
-            for (int u = 0; u < NV; u++) {
-                const int t = u * RPI / 16, k = (u * RPI) % 16 + vr;  // key k of group t
-                const uint32_t off = __umul24(min(k, r.last[t]), kvd2) + vcol2;
-                vb[u] = *gptr<v4u>(vg + r.at[t] + off);
-            }
-        };
-        auto load_k = [&](const Rows& r) __attribute__((always_inline)) {
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                const uint32_t off = __umul24(min(l16, r.last[t]), kvd2) + 16 * lg;
-#pragma unroll
-                for (int k = 0; k < KS; k++) kf[t][k] = *gptr<v4u>(kg + r.at[t] + off + 64 * k);
-            }
-        };
-        const int c0 = q.c0 + f, c1 = c0 + n;
-        int pg[2];
-        pages(c0, pg);
-        Rows cur = rows(c0, pg);
-        if (cur.ok) {
-            load_v(cur);
-            load_k(cur);
+        for (int t = 0; t < 2; t++) {
+            const int k0 = DEC_CHUNK * c + 32 * wave + 16 * t;
+            r.at[t] = (((uint64_t)(uint32_t)pg[t] << a.page_shift) + (k0 & ((1 << a.page_shift) - 1))) * kvd2 + 2 * HD * p.g;
+            r.last[t] = min(p.q.len - 1 - k0, 15);
+            r.ok |= (r.last[t] >= 0 && (uint32_t)pg[t] < (uint32_t)a.n_pages) << t;
         }
-        if (n > 1) pages(c0 + 1, pg);
+        if (r.ok == 1) r.at[1] = r.at[0], r.last[1] = r.last[0];
+        if (r.ok == 2) r.at[0] = r.at[1], r.last[0] = r.last[1];
+        return r;
+    };
+    // (a group's rows: a scalar base and a lane's 32-bit offset)
+    v4u kf[2][KS], vb[NV];
+    auto load_v = [&](const Rows& r) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < NV; u++) {
+            const int t = u * RPI / 16, k = (u * RPI) % 16 + vr;  // key k of group t
+            const uint32_t off = __umul24(min(k, r.last[t]), kvd2) + vcol2;
+            vb[u] = *gptr<v4u>(vb0 + r.at[t] + off);
+        }
+    };
+    auto load_k = [&](const Rows& r) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const uint32_t off = __umul24(min(l16, r.last[t]), kvd2) + 16 * lg;
+#pragma unroll
+            for (int k = 0; k < KS; k++) kf[t][k] = *gptr<v4u>(kb + r.at[t] + off + 64 * k);
+        }
+    };
+    // a piece's queries and positions, row 16 u + l16
+    f4 qv[NT][2 * KS];
+    int qpos[NT];
+    auto load_q = [&](const Piece& p) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < NT; u++) {
+            const int c = 16 * u + l16, tok = c / G < p.q.qn ? c / G : 0, h = p.g * G + c % G;
+            const float* qr = a.q + ((uint64_t)(p.q.q0 + tok) * a.nh + h) * HD;
+            qpos[u] = a.pos[p.q.q0 + tok];
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) qv[u][2 * k + e] = *(const f4*)(qr + 32 * k + 8 * lg + 4 * e);
+        }
+    };
+    Piece pc, nx;
+    if (!next_piece(pc)) return;
+    int pg[2];
+    pages(pc, pc.c0, pg);
+    Rows cur = rows(pc, pc.c0, pg);
+    if (cur.ok) {
+        load_v(cur);
+        load_k(cur);
+    }
+    load_q(pc);
+    for (bool more_pieces = true; more_pieces; pc = nx) {
+        const int c0 = pc.c0, c1 = pc.c1, pair = pc.s * a.nkv + pc.g;
+        const bool whole = DIRECT && pc.head == 1;  // no other partial sums: this block writes the rows
+        if (pc.head && !whole && tid == 0) w.map[DIRECT ? b : pair] = make_int2(DIRECT ? pair : b, pc.head);
+        more_pieces = next_piece(nx);
+        if (c0 + 1 < c1) pages(pc, c0 + 1, pg);
+        else if (more_pieces) pages(nx, nx.c0, pg);
         // the rows' queries and the keys they see
         h8 qh[NT][KS], ql[NT][KS];
         float usc[NT], m[NT], l[NT];
@@ -317,26 +362,18 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
         f4 o[NT][DT];
 #pragma unroll
         for (int u = 0; u < NT; u++) {
-            const int c = 16 * u + l16, tok = c / G, h = g * G + c % G;
-            const bool live = tok < q.qn;
-            f4 qv[2 * KS];
+            const bool live = (16 * u + l16) / G < pc.q.qn;
             float mx = 0.0f;
-            const float* qr = a.q + ((uint64_t)(q.q0 + (live ? tok : 0)) * a.nh + h) * HD;
-            const int pos = a.pos[q.q0 + (live ? tok : 0)];
 #pragma unroll
-            for (int k = 0; k < KS; k++)
+            for (int k = 0; k < 2 * KS; k++)
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    qv[2 * k + e] = *(const f4*)(qr + 32 * k + 8 * lg + 4 * e);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        qv[2 * k + e][i] = live ? qv[2 * k + e][i] : 0.0f;
-                        mx = fmaxf(mx, fabsf(qv[2 * k + e][i]));
-                    }
+                for (int i = 0; i < 4; i++) {
+                    qv[u][k][i] = live ? qv[u][k][i] : 0.0f;
+                    mx = fmaxf(mx, fabsf(qv[u][k][i]));
                 }
             lo[u] = 1;
             hi[u] = 0;
-            if (live) own_range(a, pos, q.len, P, lo[u], hi[u]);
+            if (live) own_range(a, qpos[u], pc.q.len, P, lo[u], hi[u]);
             mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
             int ex = 0;
@@ -344,7 +381,7 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
             const float up = ldexpf(1.0f, 14 - ex);
             usc[u] = ldexpf(a.scale * LOG2E, ex - 14);
 #pragma unroll
-            for (int k = 0; k < KS; k++) split_q8(qv[2 * k], qv[2 * k + 1], up, qh[u][k], ql[u][k]);
+            for (int k = 0; k < KS; k++) split_q8(qv[u][2 * k], qv[u][2 * k + 1], up, qh[u][k], ql[u][k]);
             m[u] = -INFINITY;
             l[u] = 0.0f;
 #pragma unroll
@@ -357,9 +394,9 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
                 for (int u = 0; u < NV; u++) *(v4u*)&vs[(u * RPI + vr) * L::VP + vcol] = vb[u];
             }
             __builtin_amdgcn_wave_barrier();
-            const bool more = c + 1 < c1;
+            const bool same = c + 1 < c1, more = same || more_pieces;  // the next chunk: of this piece, or the next one's first
             if (more) {
-                cur = rows(c + 1, pg);
+                cur = same ? rows(pc, c + 1, pg) : rows(nx, nx.c0, pg);
                 if (cur.ok) load_v(cur);
             }
             f4 sv[NT][2];
@@ -380,7 +417,8 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
             }
             if (more) {
                 if (cur.ok) load_k(cur);
-                if (c + 2 < c1) pages(c + 2, pg);
+                if (c + 2 < c1) pages(pc, c + 2, pg);
+                else if (same && more_pieces) pages(nx, nx.c0, pg);
             }
             if (!r.ok) continue;
             const int k0 = DEC_CHUNK * c + 32 * wave;
@@ -430,6 +468,7 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
             }
             __builtin_amdgcn_wave_barrier();
         }
+        if (more_pieces) load_q(nx);
 #pragma unroll
         for (int u = 0; u < NT; u++) {
             l[u] += __shfl_xor(l[u], 16, 64);
@@ -454,7 +493,7 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
             __syncthreads();
             constexpr int DPT = HD / 16;
             const int rr = tid >> 4, d4 = 4 * (tid & 15), c = 16 * u + rr;  // dims d4 .. d4 + 3 of each 64
-            const bool live = c < q.qn * G;
+            const bool live = c < pc.q.qn * G;
             const uint64_t at_row = (uint64_t)(b + pair) * w.dr + c;
             float M = -INFINITY, e[DEC_WAVES], sum = 0.0f, acc[DPT], nf = 0.0f;
 #pragma unroll
@@ -472,11 +511,20 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
                 nf = __builtin_fmaf(acc[d], 0.0f, nf);
             }
             if (live) {
+                const int h = pc.g * G + c % G;
+                const uint64_t row = (uint64_t)(pc.q.q0 + c / G) * a.nh + h;
+                const float f = (whole ? out_factor(a, h, M, sum) : 1.0f) * (1.0f / PF_SCALE);
+                float* dst = whole ? a.out + row * HD : w.dacc + at_row * HD;
 #pragma unroll
-                for (int d = 0; d < DPT; d += 4)
-                    *(float4*)(w.dacc + at_row * HD + 16 * d + d4) = make_float4(acc[d] * (1.0f / PF_SCALE), acc[d + 1] * (1.0f / PF_SCALE),
-                                                                                 acc[d + 2] * (1.0f / PF_SCALE), acc[d + 3] * (1.0f / PF_SCALE));
-                if ((tid & 15) == 0) w.dml[at_row] = make_float2(M, sum);
+                for (int d = 0; d < DPT; d += 4) {
+                    float4 x = make_float4(acc[d] * f, acc[d + 1] * f, acc[d + 2] * f, acc[d + 3] * f);
+                    if (whole && a.qg) {
+                        const float4 gt = *(const float4*)(a.qg + row * 2 * HD + HD + 16 * d + d4);
+                        x.x *= sigmoid_f(gt.x); x.y *= sigmoid_f(gt.y); x.z *= sigmoid_f(gt.z); x.w *= sigmoid_f(gt.w);
+                    }
+                    *(float4*)(dst + 16 * d + d4) = x;
+                }
+                if (!whole && (tid & 15) == 0) w.dml[at_row] = make_float2(M, sum);
             }
             // A row with finite scores whose sums are not may owe it to a key that it does not see (0 times a value that is not
             // finite): again, over its own keys alone
@@ -484,14 +532,20 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
                 const int ln = __builtin_ctzll(bad), rb = (64 * wave + ln) >> 4, cb = 16 * u + rb, tok = cb / G;
                 bad &= ~(0xFFFFull << (ln & 48));
                 int klo, khi;
-                own_range(a, a.pos[q.q0 + tok], q.len, P, klo, khi);
+                own_range(a, a.pos[pc.q.q0 + tok], pc.q.len, P, klo, khi);
                 float ac[HD / 64], mm, ll;
-                paged_row_again<HD>(a, Keys{nullptr, table, 0, 0, q.len}, a.q + ((uint64_t)(q.q0 + tok) * a.nh + g * G + cb % G) * HD, g, max(klo, DEC_CHUNK * c0),
+                paged_row_again<HD>(a, Keys{nullptr, a.tables + (uint64_t)pc.s * a.max_pages, 0, 0, pc.q.len},
+                                    a.q + ((uint64_t)(pc.q.q0 + tok) * a.nh + pc.g * G + cb % G) * HD, pc.g, max(klo, DEC_CHUNK * c0),
                                     min(khi, DEC_CHUNK * c1 - 1), ac, mm, ll);
-                const uint64_t r = (uint64_t)(b + pair) * w.dr + cb;
+                const uint64_t r = (uint64_t)(b + pair) * w.dr + cb, row = (uint64_t)(pc.q.q0 + tok) * a.nh + pc.g * G + cb % G;
+                const float f = whole ? out_factor(a, pc.g * G + cb % G, mm, ll) : 1.0f;
+                float* dst = whole ? a.out + row * HD : w.dacc + r * HD;
 #pragma unroll
-                for (int d = 0; d < HD / 64; d++) w.dacc[r * HD + lane + 64 * d] = ac[d];
-                if (lane == 0) w.dml[r] = make_float2(mm, ll);
+                for (int d = 0; d < HD / 64; d++) {
+                    const int col = lane + 64 * d;
+                    dst[col] = whole && a.qg ? ac[d] * f * sigmoid_f(a.qg[row * 2 * HD + HD + col]) : ac[d] * f;
+                }
+                if (!whole && lane == 0) w.dml[r] = make_float2(mm, ll);
             }
         }
         __syncthreads();  // the tiles are rewritten by the next piece
@@ -789,14 +843,6 @@ __device__ __forceinline__ uint32_t tile_again(const TileSums<HD>& r, bool live)
         for (int i = 0; i < 16; i++) nf = __builtin_fmaf(r.o[d][i], 0.0f, nf);
     const uint64_t b = __ballot(nf != 0.0f && r.l - r.l == 0.0f && live);
     return (uint32_t)b | (uint32_t)(b >> 32);
-}
-// The factor that turns a row's sums into its output: over the sum and the sink (0 for a row without keys, not a number where a
-// score is not).
-__device__ __forceinline__ float out_factor(const PagedAttn& a, int h, float m, float l) {
-    const float sk = a.sink ? a.sink[h] * LOG2E : -INFINITY, M = fmaxf(m, sk);
-    const float sc = m == -INFINITY ? 0.0f : exp2_hw(m - M);
-    const float den = l * sc + (sk == -INFINITY ? 0.0f : exp2_hw(sk - M));
-    return den == 0.0f ? 0.0f : sc / den;
 }
 // The wave's rows times their factors f, from the fragments' layout (16 bytes of a row a lane) through LDS (free of tiles) to
 // whole rows: row r (0 .. 31, a bit of `rows`) to dst(r), through gate(r) where there is one. Chunk c of row r sits at c ^ r.
@@ -1186,18 +1232,34 @@ __device__ __forceinline__ void join_block(const PagedAttn& a, const PagedWs& w,
 // then these). 2048 items of 64 sequences of 200 .. 6000 keys: 5.7 us (four waves 7.1, one 5.4); 768 of 4 .. 16 partials
 // 6.6 us (four waves 8.4, one 8.2).
 constexpr int MERGE_WAVES = 2, MERGE_ITEMS = 2;
-template <int HD>
+template <int HD, bool DIRECT>
 __device__ __forceinline__ void merge_block(const PagedAttn& a, const PagedWs& w, int x, int per) {
     constexpr int DL = HD / 64, MW = MERGE_WAVES, U = 4;
     __shared__ float sm[MERGE_ITEMS][MW], sl[MERGE_ITEMS][MW], so[MERGE_ITEMS][MW][HD];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), v = wave % MW, it = wave / MW, lane = threadIdx.x & 63;
-    x = MERGE_ITEMS * x + it;
-    const int G = a.nh / a.nkv, h = x % a.nh, g = h / G, s = min(x / a.nh / per, a.nseq - 1);
-    const int2* mp = w.map + s * a.nkv + g;
-    const int first = sload(&mp->x), pieces = sload(&mp->y), P = prefix_len(a);  // (not set, and not used, without own keys)
-    const SeqInfo q = seq_info<true>(a, s, G, w.dr, P);
-    const int r = q.q0 + x / a.nh % per;
-    const bool live = x < a.nseq * per * a.nh && r < q.q0 + q.qn && q.qn * G <= w.dr;
+    const int G = a.nh / a.nkv, P = prefix_len(a);
+    const int y = MERGE_ITEMS * x + it;
+    int s = min(y / a.nh / per, a.nseq - 1), h = y % a.nh, i = y / a.nh % per, first, pieces;
+    SeqInfo q;
+    if constexpr (!DIRECT) {
+        const int2* mp = w.map + s * a.nkv + h / G;
+        first = sload(&mp->x), pieces = sload(&mp->y);  // (not set, and not used, without own keys)
+        q = seq_info<true>(a, s, G, w.dr, P);
+    } else {
+        if (x < a.nseq) {  // sequence x without own keys: its rows are 0
+            q = seq_info<true>(a, x, G, w.dr, P);
+            if (q.nc == 0 && q.qn * G <= w.dr)
+                for (int j = threadIdx.x; j < q.qn * a.nh * (HD / 4); j += 256)
+                    *(float4*)(a.out + (uint64_t)q.q0 * a.nh * HD + 4 * j) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        first = min(y / w.dr, w.dblocks - 1);
+        const int pair = sload(&w.map[first].x), c = y % w.dr;
+        pieces = sload(&w.map[first].y);
+        s = pair / a.nkv, h = pair % a.nkv * G + c % G, i = c / G;
+        q = seq_info<true>(a, s, G, w.dr, P);
+    }
+    const int g = h / G, r = q.q0 + i;
+    const bool live = (DIRECT ? pieces > 0 && y < w.dblocks * w.dr : y < a.nseq * per * a.nh) && i < q.qn && q.qn * G <= w.dr;
     const uint64_t row = (uint64_t)r * a.nh + h;
     const int np = P > 0 ? w.nsp : 0, n = live ? np + (q.nc > 0 ? pieces : 0) : 0;
     const uint64_t own = (uint64_t)(first + s * a.nkv + g) * w.dr + (r - q.q0) * G + h % G;  // piece i of the own keys: own + i dr
@@ -1274,7 +1336,7 @@ __device__ __forceinline__ void merge_block(const PagedAttn& a, const PagedWs& w
 // ---------------- launches ----------------
 // The pieces: blocks of the long sequences' tiles (TILE), of the prefix for the rows of decode sequences (PRE) and of their own
 // keys, in one launch.
-template <int HD, int NT, bool TILE, bool PRE>
+template <int HD, int NT, bool TILE, bool PRE, bool DIRECT>
 __global__ __launch_bounds__(256, NT == 1 || HD == 64 ? 2 : 1) void attn_paged_kernel(PagedAttn a, PagedWs w, int pblocks, int tiles) {
     constexpr int TB = TILE || PRE ? 2 * PagedTile<HD>::BUF : 0;
     __shared__ __align__(16) uint8_t lds[PagedDec<HD>::BYTES > TB ? PagedDec<HD>::BYTES : TB];
@@ -1287,14 +1349,14 @@ __global__ __launch_bounds__(256, NT == 1 || HD == 64 ? 2 : 1) void attn_paged_k
         if (b < pblocks) return prefix_block<HD>(a, w, b, tiles, lds);
         b -= pblocks;
     }
-    dec_block<HD, NT>(a, w, b, lds);
+    dec_block<HD, NT, DIRECT>(a, w, b, lds);
 }
 // The joins: of the tiles in pieces, and of the rows of decode sequences.
-template <int HD>
+template <int HD, bool DIRECT>
 __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedAttn a, PagedWs w, int jblocks, int per) {
     const int b = blockIdx.x;
     if (b < jblocks) return join_block<HD>(a, w, b / (HD / 32), b % (HD / 32));
-    merge_block<HD>(a, w, b - jblocks, per);
+    merge_block<HD, DIRECT>(a, w, b - jblocks, per);
 }
 
 static int div_up(long long a, long long b) { return (int)((a + b - 1) / b); }
@@ -1321,6 +1383,9 @@ static PagedWs plan(const PagedAttn& a, uint8_t* at, size_t* end) {
     // tokens 169 us against 211) or the prefix's blocks take the other's place (24 of 4 tokens over a prefix 24.2 us against 26.4, 64
     // over one of 4096 33 against 41)
     w.dblocks = (int)std::min<long long>(most, (w.nct == 1 || a.hd == 64) && (!a.max_prefix || most_rows > w.dr) ? 512 : 256);
+    // where no more (sequence, KV head) than blocks are there, most are cut and each of their rows is joined (64 sequences of 2000
+    // keys over 4 KV heads 49 us, direct 53); else most are not (256: 196 and 187; 1000 of 300 keys 177 and 139)
+    w.direct = !a.max_prefix && (long long)a.nseq * a.nkv >= w.dblocks;
     // splits of the prefix, of at least 128 keys: a block a CU (64 sequences over a prefix of 4096 31 us, for two a CU 46; of 16000 56
     // and 59): more of them cost more sums than they hide
     const long long blocks = std::max<long long>((long long)div_up(rows, 128) * a.nkv, 1);
@@ -1333,7 +1398,7 @@ static PagedWs plan(const PagedAttn& a, uint8_t* at, size_t* end) {
         return (void*)p;
     };
     const size_t slots = (size_t)w.dblocks + (size_t)a.nseq * a.nkv, out_rows = (size_t)a.t * a.nh;
-    w.map = (int2*)take((size_t)a.nseq * a.nkv * sizeof(int2));
+    w.map = (int2*)take(std::max((size_t)a.nseq * a.nkv, (size_t)w.dblocks) * sizeof(int2));
     w.dml = (float2*)take(slots * w.dr * sizeof(float2));
     w.dacc = (float*)take(slots * w.dr * a.hd * sizeof(float));
     if (a.max_prefix) {
@@ -1367,18 +1432,31 @@ static void launch_t(const PagedAttn& a, const PagedWs& w, hipStream_t s) {
         pblocks = 8 * div_up((long long)a.nkv * w.nsp, 8) * tiles;
     }
     const dim3 grid((unsigned)((w.plan ? w.tblocks : 0) + pblocks + w.dblocks)), block(256);
+    auto launch = [&](auto NT, auto TILE, auto PRE, auto DIRECT) {
+        attn_paged_kernel<HD, decltype(NT)::value, decltype(TILE)::value, decltype(PRE)::value, decltype(DIRECT)::value><<<grid, block, 0, s>>>(a, w, pblocks, tiles);
+    };
+    constexpr std::integral_constant<int, 1> one;
+    constexpr std::integral_constant<int, 2> two;
+    constexpr std::true_type yes;
+    constexpr std::false_type no;
     if (w.nct == 2) {
-        if (a.max_prefix) attn_paged_kernel<HD, 2, false, true><<<grid, block, 0, s>>>(a, w, pblocks, tiles);
-        else attn_paged_kernel<HD, 2, false, false><<<grid, block, 0, s>>>(a, w, pblocks, tiles);
+        if (a.max_prefix) launch(two, no, yes, no);
+        else if (w.direct) launch(two, no, no, yes);
+        else launch(two, no, no, no);
     } else if (w.plan) {
-        if (a.max_prefix) attn_paged_kernel<HD, 1, true, true><<<grid, block, 0, s>>>(a, w, pblocks, tiles);
-        else attn_paged_kernel<HD, 1, true, false><<<grid, block, 0, s>>>(a, w, pblocks, tiles);
+        if (a.max_prefix) launch(one, yes, yes, no);
+        else if (w.direct) launch(one, yes, no, yes);
+        else launch(one, yes, no, no);
     } else {
-        if (a.max_prefix) attn_paged_kernel<HD, 1, false, true><<<grid, block, 0, s>>>(a, w, pblocks, tiles);
-        else attn_paged_kernel<HD, 1, false, false><<<grid, block, 0, s>>>(a, w, pblocks, tiles);
+        if (a.max_prefix) launch(one, no, yes, no);
+        else if (w.direct) launch(one, no, no, yes);
+        else launch(one, no, no, no);
     }
     const int jblocks = w.plan ? w.tblocks * (HD / 32) : 0;
-    attn_paged_join_kernel<HD><<<dim3((unsigned)(jblocks + div_up((long long)a.nseq * per * a.nh, MERGE_ITEMS))), block, 0, s>>>(a, w, jblocks, per);
+    const int mblocks = w.direct ? std::max(div_up(w.dblocks * w.dr, MERGE_ITEMS), a.nseq) : div_up((long long)a.nseq * per * a.nh, MERGE_ITEMS);
+    const dim3 jgrid((unsigned)(jblocks + mblocks));
+    if (w.direct) attn_paged_join_kernel<HD, true><<<jgrid, block, 0, s>>>(a, w, jblocks, per);
+    else attn_paged_join_kernel<HD, false><<<jgrid, block, 0, s>>>(a, w, jblocks, per);
 }
 
 hipError_t launch_attn_paged(const PagedAttn& a, hipStream_t s) {

@@ -496,6 +496,32 @@ def test_attn_paged_many_sequences(hip, nseq, P):
     assert np.isfinite(got).all()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("most", [1, 2, 4, 40])
+@pytest.mark.parametrize("win,bad", [(0, False), (30, True)])
+def test_attn_paged_rows_finished_in_one_launch(hip, hd, most, win, bad):
+    """More (sequence, KV head) pairs than blocks: those that one block holds are finished there, others are joined; sinks, gates,
+    sequences without keys or rows, and values that are not finite at keys that a sequence's earlier rows do not see."""
+    rng = np.random.default_rng(most)
+    nseq = 300
+    q = rng.integers(0, min(most, 4) + 1, nseq)
+    if most > 4:
+        q[[7, 200]] = most
+    n = np.where(rng.random(nseq) < 0.1, 0, q + rng.integers(0, 400, nseq))
+    b = Batch(hip, q.tolist(), n.tolist(), 8, 2, hd, 16, seed=most, sink=True, gate=True, extra=2)
+    rows = sorted(set(rng.integers(0, b.q_start[-1], 150).tolist()))
+    want = b.want(win, set(rows))
+    if bad:
+        for s in range(nseq):
+            if q[s] > 1 and n[s]:
+                j = n[s] - 1
+                b.vc[b.tables[s][j // 16] * 16 + j % 16] = np.inf
+                rows = [r for r in rows if r != b.q_start[s + 1] - 1]
+    b.want = lambda *a: want
+    b.upload().launch(win)
+    b.check(b.get(), win, rows=rows)
+
+
 def test_attn_paged_two_graphs_of_one_context(hip):
     """Two recorded calls of one context share its workspace, which a larger eager call between them replaces."""
     a = Batch(hip, [1] * 4, [300, 3, 64, 900], 8, 2, 64, 16, P=70, seed=1).upload()
