@@ -235,7 +235,7 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
             big = max(big, ws[4 + v]);
         }
         total *= a.nkv;
-        // (at most 128 pieces a pair: the merge's work)
+        // (at most 128 pieces a pair, the join's work: 131072 keys over one KV head 29 us, up to 64 40; up to 256, joined by two waves, 38 for 33)
         share = max((total + w.dblocks - 1) / w.dblocks, (big + 127) / 128);
         W0 = (int)min((long long)b * share, (long long)total);
         W1 = (int)min((long long)W0 + share, (long long)total);
@@ -1226,19 +1226,19 @@ __device__ __forceinline__ void join_block(const PagedAttn& a, const PagedWs& w,
 }
 
 // ---------------- the join of a decode sequence's rows ----------------
-// Item x (of [sequence][row of it][query head]) from its partial sums: out = sum_i acc_i 2^(m_i - M) / (sum_i l_i 2^(m_i - M) +
-// 2^(sink - M)), the prefix's splits, then the own keys' pieces. Two waves an item, two items a block: wave v takes partials
-// v, v + 2, .., their maxima a lane each and 4 rows requested together (a launch is a chain of trips to memory: the sequence,
-// then these). 2048 items of 64 sequences of 200 .. 6000 keys: 5.7 us (four waves 7.1, one 5.4); 768 of 4 .. 16 partials
-// 6.6 us (four waves 8.4, one 8.2).
-constexpr int MERGE_WAVES = 2, MERGE_ITEMS = 2;
-template <int HD, bool DIRECT>
+// An item is a row and query head, of all rows or (DIRECT) of the pairs that blocks cut, from its partial sums: out = sum_i acc_i
+// 2^(m_i - M) / (sum_i l_i 2^(m_i - M) + 2^(sink - M)), the prefix's splits, then the own keys' pieces. Wave v of an item's MW takes
+// partials v, v + MW, .., their maxima a lane each and 4 rows requested together (a launch is a chain of trips to memory: the
+// sequence, then these). Two waves an item: 2048 items of 64 sequences of 200 .. 6000 keys 5.7 us (four waves 7.1, one 5.4); 768 of
+// 4 .. 16 partials 6.6 us (8.4, 8.2). Four waves up to 512 items (a call with one sequence of 32768 keys and one KV head, 128
+// pieces, 17 us, with two 21.5; of 131072 keys and four 52 and 57).
+template <int HD, bool DIRECT, int MW>
 __device__ __forceinline__ void merge_block(const PagedAttn& a, const PagedWs& w, int x, int per) {
-    constexpr int DL = HD / 64, MW = MERGE_WAVES, U = 4;
-    __shared__ float sm[MERGE_ITEMS][MW], sl[MERGE_ITEMS][MW], so[MERGE_ITEMS][MW][HD];
+    constexpr int DL = HD / 64, ITEMS = 4 / MW, U = 4;
+    __shared__ float sm[ITEMS][MW], sl[ITEMS][MW], so[ITEMS][MW][HD];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), v = wave % MW, it = wave / MW, lane = threadIdx.x & 63;
     const int G = a.nh / a.nkv, P = prefix_len(a);
-    const int y = MERGE_ITEMS * x + it;
+    const int y = ITEMS * x + it;
     int s = min(y / a.nh / per, a.nseq - 1), h = y % a.nh, i = y / a.nh % per, first, pieces;
     SeqInfo q;
     if constexpr (!DIRECT) {
@@ -1352,11 +1352,11 @@ __global__ __launch_bounds__(256, NT == 1 || HD == 64 ? 2 : 1) void attn_paged_k
     dec_block<HD, NT, DIRECT>(a, w, b, lds);
 }
 // The joins: of the tiles in pieces, and of the rows of decode sequences.
-template <int HD, bool DIRECT>
+template <int HD, bool DIRECT, int MW>
 __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedAttn a, PagedWs w, int jblocks, int per) {
     const int b = blockIdx.x;
     if (b < jblocks) return join_block<HD>(a, w, b / (HD / 32), b % (HD / 32));
-    merge_block<HD, DIRECT>(a, w, b - jblocks, per);
+    merge_block<HD, DIRECT, MW>(a, w, b - jblocks, per);
 }
 
 static int div_up(long long a, long long b) { return (int)((a + b - 1) / b); }
@@ -1453,10 +1453,15 @@ static void launch_t(const PagedAttn& a, const PagedWs& w, hipStream_t s) {
         else launch(one, no, no, no);
     }
     const int jblocks = w.plan ? w.tblocks * (HD / 32) : 0;
-    const int mblocks = w.direct ? std::max(div_up(w.dblocks * w.dr, MERGE_ITEMS), a.nseq) : div_up((long long)a.nseq * per * a.nh, MERGE_ITEMS);
-    const dim3 jgrid((unsigned)(jblocks + mblocks));
-    if (w.direct) attn_paged_join_kernel<HD, true><<<jgrid, block, 0, s>>>(a, w, jblocks, per);
-    else attn_paged_join_kernel<HD, false><<<jgrid, block, 0, s>>>(a, w, jblocks, per);
+    const long long items = w.direct ? (long long)w.dblocks * w.dr : (long long)a.nseq * per * a.nh;
+    if (w.direct) {
+        const dim3 jgrid((unsigned)(jblocks + std::max(div_up(items, 2), a.nseq)));
+        attn_paged_join_kernel<HD, true, 2><<<jgrid, block, 0, s>>>(a, w, jblocks, per);
+    } else if (items > 512) {
+        attn_paged_join_kernel<HD, false, 2><<<dim3((unsigned)(jblocks + div_up(items, 2))), block, 0, s>>>(a, w, jblocks, per);
+    } else {
+        attn_paged_join_kernel<HD, false, 4><<<dim3((unsigned)(jblocks + items)), block, 0, s>>>(a, w, jblocks, per);
+    }
 }
 
 hipError_t launch_attn_paged(const PagedAttn& a, hipStream_t s) {
