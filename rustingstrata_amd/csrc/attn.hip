@@ -209,10 +209,9 @@ __global__ __launch_bounds__(64 * DEC_WAVES) void attn_decode_kernel(const float
                     for (int e = 0; e < 4; e++) mx = fmaxf(mx, fabsf(qv[k][e]));
                 mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
                 mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-                int ex = 0;
-                if (mx > 0.0f) (void)frexpf(mx, &ex);  // mx < 2^ex
-                const float up = ldexpf(1.0f, 14 - ex);
-                usc = ldexpf(scale * LOG2E, ex - 14);  // scores in log2 units: the softmax's exps are exp2s
+                float up;
+                query_scale(mx, scale, up, usc);  // scores in log2 units: the softmax's exps are exp2s
+                if (scale >= 0.0f) usc = fmaxf(usc, USC_MIN);
 #pragma unroll
                 for (int k = 0; k < KS; k++)
 #pragma unroll
@@ -599,10 +598,9 @@ __global__ __launch_bounds__(64 * PF_W, 2) void attn_prefill_kernel(const float*
             for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(v[k][e]));
         }
         mx = max_half(mx);
-        int ex = 0;
-        if (mx > 0.0f) (void)frexpf(mx, &ex);  // mx < 2^ex
-        const float up = ldexpf(1.0f, 14 - ex);
-        usc = ldexpf(scale * LOG2E, ex - 14);  // scores in log2 units: the softmax's exps are exp2s
+        float up;
+        query_scale(mx, scale, up, usc);  // scores in log2 units: the softmax's exps are exp2s
+        if (scale >= 0.0f) usc = fmaxf(usc, USC_MIN);
 #pragma unroll
         for (int k = 0; k < KS; k++)
 #pragma unroll

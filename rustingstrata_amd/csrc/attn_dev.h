@@ -63,6 +63,18 @@ struct DecLayout {
 
 typedef float f16v __attribute__((ext_vector_type(16)));
 
+// A query head, whose largest magnitude is mx, goes to f16 hi and lo parts times `up`, the power of two that puts mx in [2^13,
+// 2^14), so that the lo parts stay normal numbers; usc undoes it, times `scale` and log2(e). Below 2^-112 `up` stays at 2^126, as
+// 2^127 is the last that float32 has (2^(14 - ex) was infinite for heads below 2^-114, their scores not numbers).
+__device__ __forceinline__ void query_scale(float mx, float scale, float& up, float& usc) {
+    const int e = max((int)(__float_as_uint(mx) >> 23), 14);  // 2^(e - 127) <= mx, which is not below 0
+    up = __uint_as_float((uint32_t)(267 - e) << 23);
+    usc = scale * LOG2E * __uint_as_float((uint32_t)(e - 13) << 23);
+}
+// usc is kept at this at least (for a scale not below 0), so that a masked score of -inf stays one times usc. A score s of the
+// scaled parts is below 2^37: with usc at this or less its exp2 is 1.
+constexpr float USC_MIN = 0x1p-126f;
+
 // Eight softmax weights p (at most 2) times PF_SCALE as f16 hi and lo parts for the P V MFMA: hi = f16(p c), lo the exact
 // remainder p c - hi rounded likewise, both to nearest, so hi + lo carries each weight to 2^-22 of its value and the lo
 // parts stay normal f16 numbers for weights down to 2^-17. (2^14 is the largest scale that p = 2 leaves in f16, hence the

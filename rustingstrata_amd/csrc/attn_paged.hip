@@ -376,10 +376,9 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
             if (live) own_range(a, qpos[u], pc.q.len, P, lo[u], hi[u]);
             mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            int ex = 0;
-            if (mx > 0.0f) (void)frexpf(mx, &ex);
-            const float up = ldexpf(1.0f, 14 - ex);
-            usc[u] = ldexpf(a.scale * LOG2E, ex - 14);
+            float up;
+            query_scale(mx, a.scale, up, usc[u]);
+            usc[u] = fmaxf(usc[u], USC_MIN);
 #pragma unroll
             for (int k = 0; k < KS; k++) split_q8(qv[u][2 * k], qv[u][2 * k + 1], up, qh[u][k], ql[u][k]);
             m[u] = -INFINITY;
@@ -657,10 +656,9 @@ __device__ __forceinline__ void tile_run(const PagedAttn& a, const Keys& keys, u
                 mx = fmaxf(mx, fabsf(qv[k][i]));
             }
         mx = max_half(mx);
-        int ex = 0;
-        if (mx > 0.0f) (void)frexpf(mx, &ex);
-        const float up = ldexpf(1.0f, 14 - ex);
-        usc = ldexpf(a.scale * LOG2E, ex - 14);
+        float up;
+        query_scale(mx, a.scale, up, usc);
+        usc = fmaxf(usc, USC_MIN);
 #pragma unroll
         for (int k = 0; k < KS; k++) split_q8(qv[2 * k], qv[2 * k + 1], up, qh[k], ql[k]);
     }

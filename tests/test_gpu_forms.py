@@ -257,6 +257,30 @@ def test_attn_prefill_non_finite(hip, nh, nkv, hd):
     assert same(got, clean)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("size", [3e-35, 1e-36, 1e-38, 1e-44])
+@pytest.mark.parametrize("t,pos", [(1, 130), (70, 40)])
+def test_attn_of_tiny_queries(hip, hd, size, t, pos):
+    """Queries down to the smallest float beside ordinary ones (the decode form takes the last row alone, the prefill form all of
+    them): scores near 0, so the mean of the values that a row sees. Tolerance as in the test of rows and chunks."""
+    nh, nkv, n = 8, 2, pos + t
+    q, k, v = normal((t, nh, hd), seed=1), normal((n, nkv, hd), seed=2).astype(np.float16), normal((n, nkv, hd), seed=3).astype(np.float16)
+    q[::2] *= np.float32(size)
+    q[:, 5] *= np.float32(size)
+    q[-1, 3] *= np.float32(size)
+    kb, vb, out, part = up(hip, k), up(hip, v), hip.alloc(t * nh * hd * 4), hip.alloc(4 * hip.attn_part_floats(nh, hd))
+    scale = 1.0 / np.sqrt(hd)
+    hip.attn_prefill(up(hip, q), kb, vb, 0, out, up(hip, np.array([pos, 0], np.int32)), t, nh, nkv, hd, scale)
+    got = hip.get(out, np.float32, t * nh * hd).reshape(t, nh, hd)
+    hip.attn_decode(up(hip, q[-1]), kb, vb, 0, out, part, up(hip, np.array([n - 1, 0], np.int32)), nh, nkv, hd, scale, 1)
+    for o, i in [(got[i], i) for i in range(t)] + [(hip.get(out, np.float32, nh * hd).reshape(nh, hd), t - 1)]:
+        for h in range(nh):
+            kk, vv = (a[:pos + i + 1, h // 4].astype(np.float64) for a in (k, v))
+            s = kk @ q[i, h].astype(np.float64) * scale
+            w = np.exp(s - s.max())
+            assert rel_l2(o[h], w @ vv / w.sum()) <= 2.0 ** -23 * (8 + np.abs(s).max()), (i, h)
+
+
 @pytest.mark.parametrize("nh,nkv,hd,win,extra", [(8, 8, 128, 0, False), (8, 2, 64, 0, True), (8, 1, 128, 40, True), (4, 2, 64, 150, False)])
 @pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
 def test_attn_prefill_non_finite_values(hip, nh, nkv, hd, win, extra, bad):

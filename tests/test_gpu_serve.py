@@ -587,6 +587,24 @@ def test_attn_paged_non_finite(hip, bad):
                 assert np.isfinite(ok).all() and ok.max() <= 1e-5, (q, key, what)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("q,n,P,win", [([1, 1, 1, 2], [200, 1, 70, 33], 0, 0), ([1, 2, 1], [70, 40, 9], 130, 60), ([60, 1], [90, 50], 65, 0), ([4], [300], 0, 20)])
+@pytest.mark.parametrize("size,scale", [(3e-35, None), (1e-36, None), (1e-38, None), (1e-44, None), (1.0, 1e-38), (1.0, 1e-45), (1e-38, 1e37)])
+def test_attn_paged_tiny_queries(hip, hd, q, n, P, win, size, scale):
+    """Queries down to the smallest float, in all heads of a row and in one, beside ordinary ones, and scales as small: the weights
+    are those of scores near 0, not numbers that are not (decode rows, prefix and tiles; Batch.check's bound)."""
+    b = Batch(hip, q, n, 8, 2, hd, 16, P=P, seed=sum(n), sink=True)
+    if scale:
+        b.scale = float(np.float32(scale))
+        b.q *= np.float32(size)
+    else:
+        b.q[::2] *= np.float32(size)
+        b.q[:, 5] *= np.float32(size)
+    assert np.isfinite(b.q).all() and b.q[0].any()
+    b.upload().launch(win)
+    b.check(b.get(), win)
+
+
 def test_attn_paged_holes(hip):
     """Page ids outside the pool hold no keys, in tables and prefix; a sequence of holes alone gives 0."""
     for q in ([1, 1, 1], [40, 3, 50]):
