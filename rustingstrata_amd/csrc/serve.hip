@@ -399,10 +399,10 @@ __global__ __launch_bounds__(64) void logits_choose_kernel(LogitsProcess a, int 
     }
 }
 
+static int logits_parts(int n, int nu) { return (int)(((long long)n + 4 * nu * LP_T - 1) / (4 * nu * LP_T)); }
 // Tokens a block: 4096, or 2048 where the larger blocks would be fewer than two a CU (64 rows of 151936: 22.0 against 26.2 us; one
 // row 5.2 against 4.3).
-static int logits_nu(int n, int rows) { return (long long)rows * ((n + 8 * LP_T - 1) / (8 * LP_T)) >= 512 ? 2 : 1; }
-static int logits_parts(int n, int nu) { return (n + 4 * nu * LP_T - 1) / (4 * nu * LP_T); }
+static int logits_nu(int n, int rows) { return (long long)rows * logits_parts(n, 2) >= 512 ? 2 : 1; }
 size_t logits_key_bytes(int n, int rows) { return (size_t)rows * logits_parts(n, logits_nu(n, rows)) * sizeof(uint64_t); }
 
 hipError_t launch_logits_process(const LogitsProcess& a, hipStream_t s) {

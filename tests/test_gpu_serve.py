@@ -268,6 +268,22 @@ def test_logits_refused_arguments(hip):
     hip.logits_process(0, 0, 0, 0, 0, 0)  # no rows: nothing to do
 
 
+def test_logits_of_the_longest_row(hip):
+    """A row of 2^31 - 1 logits in place: the choice and its place in the history at its far end, the rest as it was."""
+    n = 2**31 - 1
+    x = hip.alloc(4 * n)
+    hip.memset(x)
+    for at, v in ((0, -1.0), (n // 2, 0.5), (n - 2, 2.0), (n - 1, 3.0)):
+        hip.htod(np.array([v], np.float32), x, off=4 * at)
+    h, lens, ids = i32(hip, [n - 1, n - 1, 0]), i32(hip, [2]), i32(hip, [GUARD, GUARD])
+    hip.logits_process(x, n, x, n, n, 1, hist=h, hist_stride=3, hist_len=lens, pen=up(hip, np.array([[2.0, 0.25, 0.5]], np.float32)), ids=ids, append=True)
+    assert get_i32(hip, ids, 2).tolist() == [n - 2, GUARD] and get_i32(hip, h, 3).tolist() == [n - 1, n - 1, n - 2] and get_i32(hip, lens, 1)[0] == 3
+    for at, want in ((0, [-1.0, 0.0]), (n // 2 - 1, [0.0, 0.5, 0.0]), (n - 3, [0.0, 2.0, 3.0 / 2 - 0.25 * 2 - 0.5])):
+        got = np.zeros(len(want), np.float32)
+        hip.dtoh(x, 4 * at, got)
+        assert got.tolist() == want
+
+
 # ---------------- q/k norms and rope into pages ----------------
 @pytest.mark.parametrize("t,nh,nkv,hd,n_rot", [(1, 32, 4, 128, 128), (5, 8, 8, 64, 64), (7, 4, 1, 96, 32), (16, 16, 2, 128, 128), (333, 32, 4, 128, 128), (700, 4, 4, 64, 32),
                                                  (3, 64, 8, 128, 128), (2, 40, 40, 64, 0), (9, 3, 2, 64, 64)])
