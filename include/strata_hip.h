@@ -390,7 +390,7 @@ int strata_rms_norm_rope_qk_paged(strata_ctx* ctx, uint64_t q, uint64_t q_tstrid
  * positions up to pos[r] (of them the last `win` when win > 0): the prefix's *prefix_len (at most max_prefix) on the pages
  * prefix[0 ..], computed once for all rows, and the sequence's own len[s] (new ones included), as strata_attn_decode_gq and
  * strata_attn_prefill_m compute it: sigmoid gates qg, per-head sink logits, head_dim 64 or 128, nh / nkv 1, 2, 4 or 8. No
- * prefix: max_prefix 0. A row that sees no key is 0; the keys of a page id outside 0 .. n_pages - 1 are not seen; values of
+ * prefix: max_prefix 0. max_prefix + max_pages page is at most 2^31 - 1024. A row that sees no key is 0; the keys of a page id outside 0 .. n_pages - 1 are not seen; values of
  * keys that a row does not see do not reach it, not even infinities and NaN. Rows from q_start[nseq] on stay as they were. q, qg, out and the caches are 16-byte aligned; out
  * lies over no input; scale is above 0. */
 int strata_attn_paged(strata_ctx* ctx, uint64_t q, uint64_t kc, uint64_t vc, uint64_t qg, uint64_t out, uint64_t t,

@@ -1106,6 +1106,8 @@ int strata_attn_paged(strata_ctx* c, uint64_t q, uint64_t kc, uint64_t vc, uint6
     if (max_prefix && (!prefix || !prefix_len)) return set_error("paged attention: null prefix or its length");
     if (t > (1ull << 20) || !max_q || max_q > t) return set_error("paged attention: " + std::to_string(t) + " rows (at most 2^20), at most " + std::to_string(max_q) + " a sequence");
     if (max_prefix > (1ull << 30) || win >= (1ull << 31) || nkv > 65535 || nh > 65535) return set_error("paged attention: too large");
+    if (max_prefix + max_pages * page > PAGED_ATTN_KEYS)
+        return set_error("paged attention: " + std::to_string(max_prefix + max_pages * page) + " positions of a prefix and a sequence (at most 2^31 - 1024)");
     if (nseq * nkv * (max_pages * page / 64 + 32) >= (1ull << 31)) return set_error("paged attention: more than 2^31 chunks of keys (sequences x KV heads x positions / 64)");
     if ((t / (128 / (nh / nkv)) + nseq + 1) * ((max_prefix + max_pages * page) / 64 + 5) >= (1ull << 31))
         return set_error("paged attention: more than 2^31 tiles of rows and keys (rows x group / 128 + sequences, times positions / 64)");

@@ -32,6 +32,10 @@ struct LogitsProcess {
 size_t logits_key_bytes(int n, int rows);
 hipError_t launch_logits_process(const LogitsProcess& a, hipStream_t s);
 
+// Positions of a prefix and a sequence's own keys behind it: the attention numbers both in one int32 list, with up to 63 places
+// between them and a tile and a wave's step past its end.
+constexpr uint64_t PAGED_ATTN_KEYS = (1ull << 31) - 1024;
+
 // Attention of a ragged batch over pages (strata_attn_paged). ws: paged_attn_ws_bytes() bytes of workspace.
 struct PagedAttn {
     const float* q = nullptr; const uint16_t* kc = nullptr; const uint16_t* vc = nullptr; const float* qg = nullptr;

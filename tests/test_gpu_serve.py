@@ -720,6 +720,22 @@ def test_attn_paged_refused_arguments(hip):
     hip.attn_paged(**{**ok, "nseq": 0})
 
 
+def test_attn_paged_positions_up_to_31_bits(hip):
+    """Bounds on a prefix and a sequence that pass 2^31 - 1024 positions together are refused; at that sum, a call whose device
+    lengths are small is computed (a decoding row; a tile of rows)."""
+    x, y = hip.alloc(1 << 16), hip.alloc(1 << 16)
+    ok = dict(q=x, kc=x, vc=x, qg=0, out=y, t=1, max_q=1, pos=x, q_start=x, length=x, nseq=1, tables=x, max_pages=1 << 26, page=16, n_pages=8, nh=8, nkv=2, hd=64, scale=0.125,
+              prefix=x, prefix_len=x)
+    for P in (1 << 30, (1 << 30) - 1023):
+        with pytest.raises(S.StrataError, match="positions of a prefix and a sequence"):
+            hip.attn_paged(**{**ok, "max_prefix": P})
+    for q in (1, 20):
+        b = Batch(hip, [q], [50], 8, 2, 64, 16, P=70, seed=q, extra=1).upload()
+        b.max_pages = 1 << 26
+        b.launch(max_prefix=(1 << 30) - 1024)
+        b.check(b.get())
+
+
 # ---------------- the operators together ----------------
 class Server:
     """A decode layer served with these operators: a step brings tokens of several sequences, whose q, k and v come from a table by
