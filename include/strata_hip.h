@@ -406,7 +406,8 @@ int strata_attn_paged(strata_ctx* ctx, uint64_t q, uint64_t kc, uint64_t vc, uin
  * mask_stride apart) y = -inf, whatever it was, where bit v % 32 of word v / 32 is 0. Each step rounds to f32 once, in this
  * order. Ids outside 0 .. n - 1 are ignored. ids (not 0): the greatest allowed token of each row, the first on ties, as
  * strata_argmax_rows orders them; -1 if none is allowed. append: it also goes to the end of the row's history (when that has
- * room: hist_len < hist_stride), so that a recorded step sees it when it is replayed. */
+ * room: hist_len < hist_stride), so that a recorded step sees it when it is replayed; -1 does not, so a mask row of zeros keeps
+ * the history of a sequence that chooses nothing in this step as it is. */
 int strata_logits_process(strata_ctx* ctx, uint64_t x, uint64_t x_stride, uint64_t out, uint64_t out_stride, uint64_t n,
                           uint64_t rows, uint64_t hist, uint64_t hist_stride, uint64_t hist_len, uint64_t hist_from,
                           uint64_t last, uint64_t pen, uint64_t bias_start, uint64_t bias_ids, uint64_t bias_vals,

@@ -879,3 +879,124 @@ def test_serving_steps_recorded(hip):
         for x, y in zip(a, b):
             np.testing.assert_array_equal(x, y, err_msg=str(k))
     assert len({tuple(i) for _, i, _ in runs[0]}) > 3  # (the penalties move the choices)
+
+
+class Loop:
+    """The steps of a server around one Server, as they are documented: each sequence's history is its prompt and what it has
+    chosen, a step's new tokens are the history's next ones, and a sequence chooses with the row of its history's last token.
+    Rows of the others are masked; a refused sequence's choice is taken back."""
+
+    def __init__(self, hip, seed):
+        self.hip, self.rng = hip, np.random.default_rng(seed)
+        self.sv = sv = Server(hip, self.rng)
+        sv.cache_prefix()
+        self.rows, self.mask = up(hip, np.zeros((sv.NSEQ, sv.vocab), np.float32)), hip.alloc(sv.NSEQ * sv.vocab // 8)
+        self.cached, self.hist = [0] * sv.NSEQ, [[] for _ in range(sv.NSEQ)]
+        self.pen, self.err, self.refusals = np.tile(np.array([1.3, 0.2, 0.1], np.float32), (sv.NSEQ, 1)), 0, 0
+
+    def begin(self, s, n):
+        self.hist[s] = self.rng.integers(0, self.sv.vocab, n).tolist()
+        self.hip.htod(np.array(self.hist[s], np.int32), self.sv.hist, off=4 * s * self.sv.CAP)
+        self.hip.htod(np.array([n], np.int32), self.sv.hlen, off=4 * s)
+
+    def step(self, add, graph=None):
+        """add[s] > 0 (or 0 to wait, -1 to end). graph: a recorded step of one token of each sequence. Returns who was refused."""
+        hip, sv, n = self.hip, self.sv, self.sv.NSEQ
+        new = [h[c:c + max(a, 0)] for h, c, a in zip(self.hist, self.cached, add)]
+        assert [len(x) for x in new] == [max(a, 0) for a in add]
+        chooses = np.array([a > 0 and c + a == len(h) for h, c, a in zip(self.hist, self.cached, add)])
+        lens, hist = np.array([len(h) for h in self.hist]), np.zeros((n, sv.CAP), np.int64)
+        for s, h in enumerate(self.hist):
+            hist[s, :len(h)] = h
+        if any(new):
+            sv.inputs(np.concatenate(new).astype(np.int64))
+        hip.htod(np.array(add, np.int32), sv.add)
+        ok = np.repeat(chooses[:, None], sv.vocab, 1)
+        if graph:
+            graph.launch()
+            rows = hip.get(sv.out, np.float32, n * sv.vocab).reshape(n, -1)
+        else:
+            sv.layer(max(sum(map(len, new)), 1), max(max(add), 1))
+            for s, end in enumerate(np.cumsum([len(x) for x in new])):
+                if chooses[s]:
+                    hip.dtod(sv.out, 4 * sv.vocab * int(end - 1), self.rows, 4 * sv.vocab * s, 4 * sv.vocab)
+            hip.htod(words(ok), self.mask)
+            hip.logits_process(self.rows, sv.vocab, sv.logits, sv.vocab, sv.vocab, n, hist=sv.hist, hist_stride=sv.CAP, hist_len=sv.hlen, pen=sv.pen,
+                               mask=self.mask, mask_stride=sv.vocab // 32, ids=sv.ids, append=True)
+            rows = hip.get(self.rows, np.float32, n * sv.vocab).reshape(n, -1)
+        ids, length = get_i32(hip, sv.ids, n), get_i32(hip, sv.len, n)
+        y, want = V.logits_process(rows, hist, lens, None, 0, self.pen, None, ok)
+        same_bits(hip.get(sv.logits, np.float32, n * sv.vocab).reshape(n, -1), y)
+        np.testing.assert_array_equal(ids, want)
+        assert (ids[~chooses] == -1).all() and np.isfinite(rows).all()
+        refused = [s for s, a in enumerate(add) if a > 0 and length[s] == self.cached[s]]
+        for s, a in enumerate(add):
+            if a < 0:
+                self.cached[s] = 0
+                self.begin(s, 0)
+            elif s in refused:
+                hip.htod(np.array([len(self.hist[s])], np.int32), sv.hlen, off=4 * s)
+            else:
+                self.cached[s] += a
+                self.hist[s] += [int(ids[s])] if chooses[s] else []
+        err = get_i32(hip, sv.err, 1)[0]
+        assert err - self.err == len(refused)
+        self.err, self.refusals = err, self.refusals + len(refused)
+        # cached lengths and histories have not parted: lengths, tokens, and the cached rows of the histories' tokens
+        assert get_i32(hip, sv.len, n).tolist() == self.cached
+        assert get_i32(hip, sv.hlen, n).tolist() == [len(h) for h in self.hist]
+        device = get_i32(hip, sv.hist, n * sv.CAP).reshape(n, sv.CAP)
+        for s, h in enumerate(self.hist):
+            assert device[s, :len(h)].tolist() == h, s
+        if not refused:
+            sv.check([h[:c] for h, c in zip(self.hist, self.cached)], add)
+        return refused
+
+
+def test_serving_mixed_steps(hip):
+    """Steps in which some sequences decode, some wait, end or bring a part of a prompt, and one finds no room: only the sequences
+    whose last token is in get another, and the refused one's step can be made again."""
+    lp = Loop(hip, 7)
+    lp.begin(0, 20), lp.begin(1, 50), lp.begin(2, 3)
+    for add in ([20, 30, 3, 0], [1, 20, 0, 0], [0, 0, 1, 0], [1, 1, 1, 0]):
+        assert not lp.step(add)
+    assert [len(h) for h in lp.hist] == [23, 52, 6, 0]
+    lp.begin(3, 60)
+    for add in ([0, 0, 0, 59], [1, 1, 1, 1]):
+        assert not lp.step(add)
+    for _ in range(5):  # (sequence 3 takes its fifth page)
+        assert not lp.step([0, 1, 0, 1])
+    assert not lp.step([1, 0, -1, 0])
+    lp.begin(2, 66)
+    for _ in range(2):
+        assert lp.step([1, 1, 66, 0]) == [2]
+    assert lp.hist[2] and len(lp.hist[2]) == 66
+    assert not lp.step([0, -1, 0, 0])
+    assert not lp.step([1, 0, 66, 1])
+    assert len(lp.hist[2]) == 67 and lp.refusals == 2
+    assert not lp.step([-1, 0, -1, -1])
+    assert get_i32(hip, lp.sv.n_free, 1)[0] == lp.sv.n_free0
+
+
+def test_serving_recorded_steps_refused(hip):
+    """A recorded decode step replayed until sequences find no room, whose choices are taken back until another's end makes room:
+    tokens as if nothing had been refused."""
+    lp = Loop(hip, 8)
+    for s, n in enumerate((50, 30, 62, 45)):
+        lp.begin(s, n)
+    assert not lp.step([50, 0, 0, 0]) and not lp.step([0, 30, 0, 0]) and not lp.step([0, 0, 62, 0]) and not lp.step([0, 0, 0, 45])
+
+    def step():
+        lp.sv.layer(lp.sv.NSEQ, 1)
+        lp.sv.choose(lp.sv.out)
+
+    g = hip.record_graph(step, keep=[lp])
+    refused = [lp.step([1] * 4, graph=g) for _ in range(7)]
+    assert refused == [[]] * 3 + [[3]] * 4
+    assert not lp.step([-1, 0, 0, 0])
+    lp.begin(0, 4)
+    assert not lp.step([4, 0, 0, 0])
+    for _ in range(5):
+        assert not lp.step([1] * 4, graph=g)
+    assert lp.refusals == 4 and [len(h) for h in lp.hist] == [lp.cached[s] + 1 for s in range(4)]
+    g.close()
