@@ -12,8 +12,9 @@
 //   prefix_block  the prefix for those sequences' rows, whatever their sequence: K and V read once a tile of rows;
 //   tile_block    the prefix and own keys of sequences of many rows (prompt chunks), from attn_paged_plan_kernel's list of their
 //                 tiles: bound by the matrix cores and the softmax's vector instructions, which add up.
-// The kinds are bound by different things and run beside each other (in launches of their own: 64 sequences over a prefix of 16000
-// 71 us a call for 59, 24 of 4 tokens over one of 6001 35 for 22). Numerics as in attn.hip: q and the softmax weights as f16 hi
+// The prefix and the own keys are bound by different things and run beside each other (in launches of their own: 64 sequences over a
+// prefix of 16000 71 us a call for 59, 24 of 4 tokens over one of 6001 35 for 22). Beside tiles, whose blocks come first and fill the
+// CUs, they start as those end (2500 tokens of three chunks over a prefix of 16000 1265 us, with 60 decoding sequences 1293). Numerics as in attn.hip: q and the softmax weights as f16 hi
 // + lo parts (2^-22 of a value), K and V exact in f16, all sums in f32, log2 units.
 #include <algorithm>
 #include <climits>
@@ -31,15 +32,16 @@ struct PagedWs {
                    // that begins in a block and goes on past it, and its pieces (0: none)
     float2* dml;   // [slots][dr] max and sum of a piece's rows
     float* dacc;   // [slots][dr][hd]
-    float2* pml;   // [t nh][nsp]: the prefix's splits, of the rows of decode sequences
-    float* pacc;   // [t nh][nsp][hd]
+    float2* pml;   // [prows nh][nsp]: the prefix's splits, of the rows of decode sequences (without a plan of all rows)
+    float* pacc;   // [prows nh][nsp][hd]
     int* plan;     // long sequences (null: none): PlanHead, then a Tile each
-    int* drows;    // with a plan and a prefix: the rows of decode sequences
+    int* drows;    // with a plan and a prefix: the rows of decode sequences, one sequence's behind the other's
+    int* dstart;   // and where sequence s's begin in that list
     int4* cut;     // [tblocks] KV head and tile that block b's run cuts, and the last block of its pieces (below 0: none)
     float2* tml;   // [2 tblocks][128]: the pieces of tiles that more than one block computes
     float* tacc;   // [2 tblocks][128][hd]
     int direct;    // a (sequence, KV head) that one block holds is finished there, and the join takes those that a block cuts
-    int dblocks, nct, dr, nsp, tblocks;  // decode blocks, their column tiles; rows (tokens x G) up to which a sequence decodes
+    int dblocks, nct, dr, nsp, prows, tblocks;  // decode blocks, their column tiles; rows (tokens x G) up to which a sequence decodes
 };
 
 // ---------------- sequences ----------------
@@ -878,7 +880,8 @@ __device__ __forceinline__ void tile_store(const TileSums<HD>& r, int tid, float
 template <int HD>
 __device__ __forceinline__ void prefix_block(const PagedAttn& a, const PagedWs& w, int x, int tiles, uint8_t* lds) {
     __shared__ int ws[8];
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l32 = lane & 31;
+    int tid = threadIdx.x;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int G = a.nh / a.nkv, gs = 31 - __builtin_clz(G), TT = 128 >> gs, ns = w.nsp;
     const Keys keys{a.prefix, nullptr, prefix_len(a), (prefix_len(a) + 63) / 64, 0};
     // block x: combination (KV head, split) c on XCD c % 8, tile tt
@@ -887,21 +890,21 @@ __device__ __forceinline__ void prefix_block(const PagedAttn& a, const PagedWs& 
     const int g = c % a.nkv, split = c / a.nkv;
     const int nrows = w.drows ? sload(w.plan + 2) : min(max(sload(a.q_start + a.nseq), 0), a.t), nt = min(TT, nrows - tt * TT);
     if (nt <= 0) return;
-    const int rr = 32 * wave + l32, tok = rr >> gs, h = g * G + (rr & (G - 1));
-    const bool live = tok < nt;
+    auto tok_of = [&](int i) { return (32 * wave + i) >> gs; };  // of the wave's row i, and its head
+    auto head_of = [&](int i) { return g * G + (i & (G - 1)); };
     auto row_of = [&](int t) { return w.drows ? w.drows[tt * TT + t] : tt * TT + t; };
-    const int t = row_of(live ? tok : 0);
-    const int pos = a.pos[t];
+    auto sums_of = [&](int i) { return ((uint64_t)(tt * TT + tok_of(i)) * a.nh + head_of(i)) * ns + split; };
+    const int t = row_of(tok_of(tid & 31) < nt ? tok_of(tid & 31) : 0), pos = a.pos[t];
     int lo, hi;
     row_range(a, keys, pos, lo, hi);
     // the tiles that the block's rows see
-    int blo = live ? lo : INT_MAX, bhi = live ? hi : -1;
+    int blo = tok_of(tid & 31) < nt ? lo : INT_MAX, bhi = tok_of(tid & 31) < nt ? hi : -1;
     static_for<0, 5>([&](auto S) {
         constexpr int st = decltype(S)::value;
         blo = min(blo, xl32<st>(blo));
         bhi = max(bhi, xl32<st>(bhi));
     });
-    if (lane == 0) {
+    if ((tid & 63) == 0) {
         ws[wave] = blo;
         ws[4 + wave] = bhi;
     }
@@ -910,25 +913,23 @@ __device__ __forceinline__ void prefix_block(const PagedAttn& a, const PagedWs& 
     bhi = __builtin_amdgcn_readfirstlane(max(max(ws[4], ws[5]), max(ws[6], ws[7])));
     const int kt0 = bhi < 0 ? 0 : blo / 64, kt1 = bhi < 0 ? 0 : bhi / 64 + 1, per = (kt1 - kt0 + ns - 1) / ns;
     const int kb = min(kt0 + split * per, kt1), ke = min(kb + per, kt1);
-    const uint64_t row = (uint64_t)t * a.nh + h;
     TileSums<HD> r;
-    tile_run<HD>(a, keys, lds, g, kb, ke, live, a.q + row * HD, pos, r);
+    tile_run<HD>(a, keys, lds, g, kb, ke, tok_of(tid & 31) < nt, a.q + ((uint64_t)t * a.nh + head_of(tid & 31)) * HD, pos, r);
+    asm volatile("" : "+v"(tid));  // (nothing of this lane's row waits in registers while the tiles run)
+    const int lane = tid & 63, l32 = lane & 31;
+    const bool live = tok_of(l32) < nt;
     uint32_t again = tile_again<HD>(r, live);
     const uint32_t rows = (uint32_t)__ballot(live) & ~again;
-    tile_store<HD>(r, tid, 1.0f / TILE_SCALE, lds, rows, [&](int i) {
-        const int rb = 32 * wave + i;
-        return w.pacc + (((uint64_t)row_of(rb >> gs) * a.nh + g * G + (rb & (G - 1))) * ns + split) * HD;
-    }, [](int) { return (const float*)nullptr; });
-    if (lane < 32 && ((rows >> l32) & 1)) w.pml[row * ns + split] = make_float2(r.m, r.l * (1.0f / TILE_SCALE));
+    tile_store<HD>(r, tid, 1.0f / TILE_SCALE, lds, rows, [&](int i) { return w.pacc + sums_of(i) * HD; }, [](int) { return (const float*)nullptr; });
+    if (lane < 32 && ((rows >> l32) & 1)) w.pml[sums_of(l32)] = make_float2(r.m, r.l * (1.0f / TILE_SCALE));
     for (; again; again &= again - 1) {
-        const int rb = 32 * wave + __builtin_ctz(again), tb = row_of(rb >> gs);
-        const uint64_t rowb = (uint64_t)tb * a.nh + g * G + (rb & (G - 1));
+        const int i = __builtin_ctz(again), tb = row_of(tok_of(i));
         row_range(a, keys, a.pos[tb], lo, hi);
         float ac[HD / 64], mm, ll;
-        paged_row_again<HD>(a, keys, a.q + rowb * HD, g, max(lo, 64 * kb), min(hi, 64 * ke - 1), ac, mm, ll);
+        paged_row_again<HD>(a, keys, a.q + ((uint64_t)tb * a.nh + head_of(i)) * HD, g, max(lo, 64 * kb), min(hi, 64 * ke - 1), ac, mm, ll);
 #pragma unroll
-        for (int d = 0; d < HD / 64; d++) w.pacc[(rowb * ns + split) * HD + lane + 64 * d] = ac[d];
-        if (lane == 0) w.pml[rowb * ns + split] = make_float2(mm, ll);
+        for (int d = 0; d < HD / 64; d++) w.pacc[sums_of(i) * HD + lane + 64 * d] = ac[d];
+        if (lane == 0) w.pml[sums_of(i)] = make_float2(mm, ll);
     }
 }
 
@@ -989,6 +990,7 @@ __global__ __launch_bounds__(1024) void attn_paged_plan_kernel(PagedAttn a, Page
         if (4 * tid + i < a.nseq) {
             start[4 * tid + i] = at;
             dstart[4 * tid + i] = dat;
+            if (w.drows) w.dstart[4 * tid + i] = dat;
         }
         at += nt[i];
         dat += nd[i];
@@ -1261,7 +1263,10 @@ __device__ __forceinline__ void merge_block(const PagedAttn& a, const PagedWs& w
     const uint64_t row = (uint64_t)r * a.nh + h;
     const int np = P > 0 ? w.nsp : 0, n = live ? np + (q.nc > 0 ? pieces : 0) : 0;
     const uint64_t own = (uint64_t)(first + s * a.nkv + g) * w.dr + (r - q.q0) * G + h % G;  // piece i of the own keys: own + i dr
-    auto at = [&](int i) { return i < np ? row * np + i : own + (uint64_t)(i - np) * w.dr; };
+    // (a place past the list's room belongs to no row that the call's q_start allows)
+    const int pr = !DIRECT && w.drows ? min(sload(w.dstart + s) + i, w.prows - 1) : r;
+    const uint64_t pre = ((uint64_t)pr * a.nh + h) * np;
+    auto at = [&](int i) { return i < np ? pre + i : own + (uint64_t)(i - np) * w.dr; };
     float M = -INFINITY, L = 0.0f, acc[DL], gt[DL];
 #pragma unroll
     for (int d = 0; d < DL; d++) {
@@ -1369,7 +1374,6 @@ static int max_tiles(const PagedAttn& a, const PagedWs& w) {
 static PagedWs plan(const PagedAttn& a, uint8_t* at, size_t* end) {
     PagedWs w{};
     const int G = a.nh / a.nkv;
-    const long long rows = (long long)a.t * G;
     // a sequence decodes up to 16 rows (one column tile), up to 32 where the longest has no more (64 sequences of 4 tokens, 8 heads a
     // KV head, over 2048 keys: 70 us, as tiles of 128 rows 97)
     const long long most_rows = (long long)a.max_q * G;
@@ -1385,8 +1389,11 @@ static PagedWs plan(const PagedAttn& a, uint8_t* at, size_t* end) {
     // keys over 4 KV heads 49 us, direct 53); else most are not (256: 196 and 187; 1000 of 300 keys 177 and 139)
     w.direct = !a.max_prefix && (long long)a.nseq * a.nkv >= w.dblocks;
     // splits of the prefix, of at least 128 keys: a block a CU (64 sequences over a prefix of 4096 31 us, for two a CU 46; of 16000 56
-    // and 59): more of them cost more sums than they hide
-    const long long blocks = std::max<long long>((long long)div_up(rows, 128) * a.nkv, 1);
+    // and 59): more of them cost more sums than they hide. The rows that count are those of sequences that may decode (all t rows
+    // left the decode rows beside chunks with a few long splits: 512 tokens and 63 decoding sequences over 16000 511 us for 336,
+    // 1500 tokens and 4 over 2000 212 for 169)
+    w.prows = (int)(most_rows > w.dr ? std::min<long long>(a.t, (long long)a.nseq * (w.dr / G)) : a.t);
+    const long long blocks = std::max<long long>((long long)div_up((long long)w.prows * G, 128) * a.nkv, 1);
     w.nsp = (int)std::max<long long>(1, std::min<long long>({div_up(256, blocks), div_up(a.max_prefix, 128), 64}));
     w.tblocks = 512;
     size_t o = 0;
@@ -1395,7 +1402,7 @@ static PagedWs plan(const PagedAttn& a, uint8_t* at, size_t* end) {
         o += (bytes + 255) & ~(size_t)255;
         return (void*)p;
     };
-    const size_t slots = (size_t)w.dblocks + (size_t)a.nseq * a.nkv, out_rows = (size_t)a.t * a.nh;
+    const size_t slots = (size_t)w.dblocks + (size_t)a.nseq * a.nkv, out_rows = (size_t)w.prows * a.nh;
     w.map = (int2*)take(std::max((size_t)a.nseq * a.nkv, (size_t)w.dblocks) * sizeof(int2));
     w.dml = (float2*)take(slots * w.dr * sizeof(float2));
     w.dacc = (float*)take(slots * w.dr * a.hd * sizeof(float));
@@ -1405,7 +1412,10 @@ static PagedWs plan(const PagedAttn& a, uint8_t* at, size_t* end) {
     }
     if (most_rows > w.dr) {
         w.plan = (int*)take((PLAN_HEAD + (size_t)max_tiles(a, w) * (sizeof(PlanTile) / 4)) * 4);
-        if (a.max_prefix) w.drows = (int*)take((size_t)a.t * 4);
+        if (a.max_prefix) {
+            w.drows = (int*)take((size_t)a.t * 4);
+            w.dstart = (int*)take((size_t)a.nseq * 4);
+        }
         w.cut = (int4*)take((size_t)w.tblocks * sizeof(int4));
         w.tml = (float2*)take((size_t)2 * w.tblocks * 128 * sizeof(float2));
         w.tacc = (float*)take((size_t)2 * w.tblocks * 128 * a.hd * sizeof(float));
@@ -1426,7 +1436,7 @@ static void launch_t(const PagedAttn& a, const PagedWs& w, hipStream_t s) {
     int tiles = 0, pblocks = 0;
     if (w.plan) attn_paged_plan_kernel<<<dim3(1), dim3(1024), 0, s>>>(a, w, max_tiles(a, w));
     if (a.max_prefix) {
-        tiles = div_up(w.plan ? std::min((long long)a.t, (long long)a.nseq * per) : a.t, TT);
+        tiles = div_up(w.prows, TT);
         pblocks = 8 * div_up((long long)a.nkv * w.nsp, 8) * tiles;
     }
     const dim3 grid((unsigned)((w.plan ? w.tblocks : 0) + pblocks + w.dblocks)), block(256);

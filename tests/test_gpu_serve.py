@@ -559,6 +559,20 @@ def test_attn_paged_two_graphs_of_one_context(hip):
     ga.close(), gc.close()
 
 
+def test_attn_paged_prefix_sums_of_decoding_rows_alone(hip):
+    """Chunks of thousands of rows beside decoding sequences over a prefix: the context's scratch holds no sums of the prefix for the
+    chunks' rows (134 MB here for each split of it), and the rows of either kind are right."""
+    other = S.HipBackend(0)
+    b = Batch(other, [1, 8189, 2], [40, 8189, 3], 32, 4, 128, 64, P=500, seed=11).upload()
+    other.sync()
+    before = other.mem_info()[0]
+    b.launch()
+    got = b.get()
+    assert before - other.mem_info()[0] < 100 << 20  # (67 MB of cut tiles' sums, 4 of own keys', 6 of the prefix's)
+    b.check(got, rows=[0, 1, 700, 8189, 8190, 8191])
+    other.close()
+
+
 def test_attn_paged_offsets_past_32_bits(hip):
     """A pool of 2.4 GB a cache whose used pages lie at its far end."""
     nh, nkv, hd, page = 16, 16, 128, 64
