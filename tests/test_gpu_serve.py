@@ -211,6 +211,28 @@ def test_logits_process(hip, rows, n, hist, last, bias, mask, special):
             np.testing.assert_array_equal(gi, ids)
 
 
+@pytest.mark.parametrize("rows,n,hist,last,bias,mask", [
+    (4, 33, 5, 2, 3, True), (5, 4097, 700, 0, 30, True), (3, 8192, 100, 64, 0, True), (6, 32003, 300, 64, 20, False), (2, 151936, 9000, 0, 300, True), (64, 9000, 64, 1, 5, True)])
+@pytest.mark.parametrize("nan", [False, True])
+def test_logits_choices_among_special_values(hip, rows, n, hist, last, bias, mask, nan):
+    """Every row's choice among infinities, zeros of both signs, the lowest value and, with nan, values that are not numbers: the
+    greatest allowed one of the values that the call writes, by the total order of their bits, the first on ties; without nan
+    that of the restatement."""
+    x, h, lens, first, pen, b, ok = logits_case(rows, n, hist, seed=rows * n + nan, bias=bias, mask=mask, special=True)
+    if not nan:
+        x[np.isnan(x)] = 0.0
+    x[0] = np.where(np.arange(n) % 3 == 0, np.float32(-0.0), -np.inf)
+    x[1] = np.where(np.arange(n) % 5 == 2, np.finfo(np.float32).min, -np.inf)
+    want, ids = V.logits_process(x, h, lens, first, last, pen, b, ok)
+    allowed = ok if ok is not None else np.ones(x.shape, bool)
+    for kw in (dict(), dict(place=True), dict(stride=n + 5, pad=2)):
+        got, gi, _, _ = run_logits(hip, x, h, lens, first, last, pen, b, ok, **kw)
+        same_bits(got, want)
+        assert gi.tolist() == [V.argmax_total(np.ascontiguousarray(g), a) for g, a in zip(got, allowed)]
+        rest = [r for r in range(rows) if not np.isnan(want[r][allowed[r]]).any()]
+        assert (len(rest) == rows or nan) and gi[rest].tolist() == ids[rest].tolist()
+
+
 def test_logits_parts_alone(hip):
     """Nothing asked: a copy and the argmax; each part by itself; a mask that leaves nothing, one, or only -inf."""
     x, h, lens, first, pen, b, ok = logits_case(4, 5000, 50, seed=1, bias=6, mask=True)
@@ -635,6 +657,25 @@ def test_attn_paged_tiny_queries(hip, hd, q, n, P, win, size, scale):
     b.check(b.get(), win)
 
 
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_attn_paged_non_finite_queries(hip, bad):
+    """A query that is not finite spoils its own row of its head and no other bit: decode rows with and without a prefix, rows that a
+    block finishes itself, tiles whole and cut."""
+    for q, n, P in (([1, 2, 1], [300, 60, 5], 0), ([1, 2, 1], [300, 60, 5], 200), ([1] * 300, [20] * 300, 0), ([70, 1, 300], [900, 60, 300], 0), ([70, 1, 300], [900, 60, 300], 200)):
+        b = Batch(hip, q, n, 8, 2, 64, 16, P=P, seed=P + len(q), sink=True).upload()
+        b.launch()
+        clean = b.get()
+        for r, h in ((0, 3), (b.q_start[1] + q[1] - 1, 7), (b.t - 1, 0)):
+            x = b.q.copy()
+            x[r, h, 5] = bad
+            hip.htod(x, b.b["q"])
+            b.launch()
+            got = b.get()
+            assert not np.isfinite(got[r, h]).any(), (q[:3], P, r, h)
+            got[r, h] = clean[r, h]
+            np.testing.assert_array_equal(got.view(np.uint32), clean.view(np.uint32))
+
+
 def test_attn_paged_holes(hip):
     """Page ids outside the pool hold no keys, in tables and prefix; a sequence of holes alone gives 0."""
     for q in ([1, 1, 1], [40, 3, 50]):
@@ -677,6 +718,23 @@ def test_attn_paged_lengths_from_the_device(hip):
     b = Batch(hip, [40, 1], [40, 9], nh, nkv, hd, page, seed=1).upload()
     b.launch(max_q=1)
     b.check(b.get(), rows=[40])
+
+
+@pytest.mark.parametrize("q,max_q", [([1] * 5, 1), ([1, 40, 1, 17, 2], 40)])
+@pytest.mark.parametrize("win", [0, 50])
+def test_attn_paged_device_lengths_past_their_bounds(hip, q, max_q, win):
+    """Device lengths above max_pages pages and above max_prefix count as those, below 0 as 0."""
+    page, pages, P = 32, 6, 90
+    b = Batch(hip, q, [page * pages] * len(q), 8, 2, 64, page, P=P, seed=max_q + win, sink=True).upload()
+    assert b.max_pages == pages
+    for n, pl in ((2**31 - 1, 2**31 - 1), (page * pages + 1, P + 1), (-1, P), (-2**31, -2**31)):
+        b.n, b.P = [min(max(n, 0), page * pages)] * len(q), min(max(pl, 0), P)
+        hip.htod(np.array([n] * len(q), np.int32), b.b["length"])
+        hip.htod(np.array([pl], np.int32), b.pb["prefix_len"])
+        b.launch(win, max_prefix=P)
+        got = b.get()
+        b.check(got, win)
+        assert got.any() == (n > 0 or (pl > 0 and not win))
 
 
 def test_attn_paged_two_contexts(hip):
@@ -1014,3 +1072,22 @@ def test_serving_recorded_steps_refused(hip):
         assert not lp.step([1] * 4, graph=g)
     assert lp.refusals == 4 and [len(h) for h in lp.hist] == [lp.cached[s] + 1 for s in range(4)]
     g.close()
+
+
+def test_serving_cached_keys(hip):
+    """The cached keys after prompts and decode steps: float64 within half a step of f16 (2^-11 of the value, 2^-25 below the normal
+    range) and the float32 arithmetic of a rope pair: 64 roundings of the sum of squares, halved by the root, the root's, the
+    inverse's and two products' 4, and 3 each for the two terms of a turn whose sine and cosine are rounded once from double:
+    48 times 2^-24 of the pair's length."""
+    lp, H = Loop(hip, 9), Server.HD
+    sv = lp.sv
+    lp.begin(0, 30), lp.begin(2, 36)
+    for add in ([30, 0, 20, 0], [1, 0, 16, 0], [1, 0, 1, 0], [1, 0, 1, 0]):
+        assert not lp.step(add)
+    kc = hip.get(sv.kc, np.float16, sv.N_PAGES * sv.PAGE * sv.NKV * H).reshape(-1, sv.NKV, H)
+    tables, prefix = get_i32(hip, sv.tables, sv.NSEQ * sv.MAX_PAGES).reshape(sv.NSEQ, -1), get_i32(hip, sv.prefix, 2)
+    for rows, toks, p0 in ((V.rows_of(kc, prefix, sv.P, sv.PAGE)[0], sv.pre, 0), *((V.rows_of(kc, tables[s], lp.cached[s], sv.PAGE)[0], lp.hist[s][:lp.cached[s]], sv.P) for s in (0, 2))):
+        k = V.norm_rope(sv.tk[np.array(toks)].astype(np.float64), sv.kw.astype(np.float64), 1e-6, H, p0 + np.arange(len(toks))[:, None], 1e4)
+        pair = np.hypot(k[..., :H // 2], k[..., H // 2:])
+        f32 = 48 * 2.0 ** -24 * np.concatenate([pair, pair], -1)
+        assert len(rows) and (np.abs(rows - k) <= (2.0 ** -11 * np.abs(k) + 2.0 ** -25 + f32) * (1 + 2.0 ** -10)).all()
