@@ -20,6 +20,9 @@
 
 namespace strata {
 
+// Word i (0..3, a constant) of v.
+__device__ __forceinline__ uint32_t u4c(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
 // Positions of token t: base .. end (inclusive); a sliding window keeps the last `win`.
 __device__ __forceinline__ void att_range(const int* step, int t, int win, int& base, int& n_pos) {
     const int end = step[2 * t];
@@ -30,6 +33,12 @@ __device__ __forceinline__ void att_range(const int* step, int t, int win, int& 
 // ---------------- decode ----------------
 // Positions a split of a token with n_pos positions: at least one chunk of 64, so short contexts use few waves.
 __device__ __forceinline__ int split_len(int n_pos, int ns) { return max((n_pos + ns - 1) / ns, 64); }
+
+// Layout of the K tile ([key][dim]) and the V tile transposed ([dim][key]) in LDS, 64 keys.
+template <int HD> struct PfLayout {
+    static constexpr int KP = HD + 8;          // halves per K row in LDS (16-byte pad: rows start in spread banks)
+    static constexpr int VP = 64 + 4;          // halves per V^T row (8-byte pad)
+};
 
 // grid (ATT_SPLITS, nkv, nt), 4 waves a block. Block (s, g, t) serves the G = nh / nkv query heads of KV head g over
 // the s-th share of token t's positions, 64 keys a chunk, and wave w takes keys 16 w .. 16 w + 15 of each chunk with
@@ -46,6 +55,14 @@ __device__ __forceinline__ int split_len(int n_pos, int ns) { return max((n_pos 
 // arithmetic: the same bits), and the block whose split holds the token's own position also norms and ropes its key
 // head, stores the new key and value into the f16 caches and uses them for that position (no block reads it from the
 // cache): one launch in place of rms_norm_rope_qk + kv store + attention.
+template <int HD>
+struct DecLayout {
+    static constexpr int KP = HD + 8;    // halves per K row (16-byte pad: rows start in spread banks)
+    static constexpr int VP = 16 + 4;    // halves per V^T row of a wave's 16 keys (8-byte pad)
+    static constexpr int WAVE = 16 * KP * 2 + HD * VP * 2;  // bytes of one wave's K and V^T tiles
+    static constexpr int MERGE = DEC_WAVES * (HD * 16 + 32) * 4;  // the waves' o, m and l for the block merge
+    static constexpr int BYTES = DEC_WAVES * WAVE > MERGE ? DEC_WAVES * WAVE : MERGE;
+};
 template <int HD, int G, bool NR>
 __global__ __launch_bounds__(64 * DEC_WAVES) void attn_decode_kernel(const float* __restrict__ q,
                                                                      const uint16_t* __restrict__ kc,

@@ -1,5 +1,5 @@
 // Device pieces that the attention kernels share (attn.hip: one sequence's contiguous cache; attn_paged.hip: a batch over
-// pages): fragment types, wave reductions, the softmax's exp2, LDS layouts, the weights' f16 split.
+// pages): fragment types, wave reductions, the softmax's exp2, the f16 splits of queries and weights.
 #pragma once
 #include "xlane.h"
 
@@ -42,24 +42,7 @@ __device__ __forceinline__ float wave_sum64(float v) {
 constexpr float LOG2E = 1.44269504088896341f;
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Word i (0..3, a constant) of v.
-__device__ __forceinline__ uint32_t u4c(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-
-// Layout of the K tile ([key][dim]) and the V tile transposed ([dim][key]) in LDS, 64 keys.
-template <int HD> struct PfLayout {
-    static constexpr int KP = HD + 8;          // halves per K row in LDS (16-byte pad: rows start in spread banks)
-    static constexpr int VP = 64 + 4;          // halves per V^T row (8-byte pad)
-};
-
-constexpr int DEC_WAVES = 4;
-template <int HD>
-struct DecLayout {
-    static constexpr int KP = HD + 8;    // halves per K row (16-byte pad: rows start in spread banks)
-    static constexpr int VP = 16 + 4;    // halves per V^T row of a wave's 16 keys (8-byte pad)
-    static constexpr int WAVE = 16 * KP * 2 + HD * VP * 2;  // bytes of one wave's K and V^T tiles
-    static constexpr int MERGE = DEC_WAVES * (HD * 16 + 32) * 4;  // the waves' o, m and l for the block merge
-    static constexpr int BYTES = DEC_WAVES * WAVE > MERGE ? DEC_WAVES * WAVE : MERGE;
-};
+constexpr int DEC_WAVES = 4;  // of a block over few rows
 
 typedef float f16v __attribute__((ext_vector_type(16)));
 
