@@ -32,7 +32,7 @@ struct PagedWs {
                    // that begins in a block and goes on past it, and its pieces (0: none)
     float2* dml;   // [slots][dr] max and sum of a piece's rows
     float* dacc;   // [slots][dr][hd]
-    float2* pml;   // [prows nh][nsp]: the prefix's splits, of the rows of decode sequences (without a plan of all rows)
+    float2* pml;   // [prows nh][nsp]: the prefix's splits, of the rows of decode sequences (without a plan: of all rows)
     float* pacc;   // [prows nh][nsp][hd]
     int* plan;     // long sequences (null: none): PlanHead, then a Tile each
     int* drows;    // with a plan and a prefix: the rows of decode sequences, one sequence's behind the other's
