@@ -73,6 +73,14 @@ __device__ __forceinline__ void split_w8(const float* p, h8& hi, h8& lo) {
         lo[e] = (_Float16)__builtin_fmaf(p[e], PF_SCALE, -(float)hi[e]);
     }
 }
+// The wait states between a 32 x 32 x 16 product (8 passes) and a vector instruction that reads it. The compiler counts them along
+// one of the ways that lead to the reader, which need not be the shortest: where a branch follows at once, they are kept here (a
+// reader 6 states behind got the sums without the last product's part).
+__device__ __forceinline__ void mfma_wait() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 11");
+    __builtin_amdgcn_sched_barrier(0);
+}
 // The larger of this lane's value and that of the lane 32 away.
 __device__ __forceinline__ float max_half(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);

@@ -820,12 +820,14 @@ __device__ __forceinline__ void tile_run(const PagedAttn& a, const Keys& keys, u
         wait_loads();
         lds_barrier();
         scores(0, s);
+        mfma_wait();
         mask(kb, hole, s);
         mx = largest(s);
         // (the K of tile kb has been read by all waves before tile kb + 2's may land on it)
         lds_barrier();
         for (int kt = kb; kt + 1 < ke; kt++) tile(kt, std::integral_constant<bool, true>{});
         tile(ke - 1, std::integral_constant<bool, false>{});
+        mfma_wait();
         lds_barrier();  // (the buffers are free for what comes next)
     }
     r.l = l + __shfl_xor(l, 32, 64);
