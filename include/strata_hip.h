@@ -413,6 +413,70 @@ int strata_logits_process(strata_ctx* ctx, uint64_t x, uint64_t x_stride, uint64
                           uint64_t last, uint64_t pen, uint64_t bias_start, uint64_t bias_ids, uint64_t bias_vals,
                           uint64_t n_bias, uint64_t mask, uint64_t mask_stride, uint64_t ids, int append);
 
+/* ---- drafted trees and branching sequences over the same caches (no counterpart in the reference) ----
+ * A step may bring a tree of drafted tokens instead of a line: row 0 of a sequence's rows is the tree's root (the last chosen
+ * token), row i's parent is row parent[i] < i of the same sequence, -1 for the root. The rows' slots come from
+ * strata_kv_pages_step as for a line. `words` (1 to 8) is the mask words a row has: a sequence of up to 32 words rows is a tree,
+ * one of more rows a line of tokens (a prompt's chunk), its parents unread; both may be in one call. */
+
+/* The positions and ancestor masks of a step's trees: pos[r] = *prefix_len (at least 0; prefix_len may be 0) + the sequence's
+ * positions before its rows (len[s], which holds the rows, less them) + the number of row r's ancestors, cut at 2^31 - 1; bit j %
+ * 32 of mask[r words + j / 32] is set for row j of the same sequence that is r itself or above it. Rows of a line: consecutive
+ * positions, masks 0; rows from q_start[nseq] up to t: position -1, masks 0. A parent that is not below its row counts as -1, and
+ * *err (device int32, may be 0) goes up by one for each. q_start, parent, len: device int32, as strata_kv_pages_step leaves them. */
+int strata_tree_step(strata_ctx* ctx, uint64_t nseq, uint64_t q_start, uint64_t parent, uint64_t len, uint64_t prefix_len,
+                     uint64_t t, uint64_t words, uint64_t pos, uint64_t mask, uint64_t err);
+/* strata_attn_paged over trees: the arguments and limits of that call, and each row's mask (device uint32 words, rows of `words`
+ * words). A row of a tree sees the prefix, its sequence's own keys before its rows, and row j's key where bit j of its mask is
+ * set, j up to its own row; a row of a line sees what strata_attn_paged shows it. pos is used for lines and windows only; win
+ * is 0 or at least 32 words, so that a window hides no ancestor. A row that sees no key is 0. */
+int strata_attn_paged_tree(strata_ctx* ctx, uint64_t q, uint64_t kc, uint64_t vc, uint64_t qg, uint64_t out, uint64_t t,
+                           uint64_t max_q, uint64_t pos, uint64_t q_start, uint64_t len, uint64_t nseq, uint64_t tables,
+                           uint64_t max_pages, uint64_t page, uint64_t n_pages, uint64_t prefix, uint64_t prefix_len,
+                           uint64_t max_prefix, uint64_t nh, uint64_t nkv, uint64_t hd, float scale, uint64_t sink, uint64_t win,
+                           uint64_t mask, uint64_t words);
+/* The path of each tree that the model's choices confirm: tokens[r] is row r's drafted token, ids[r] the choice after it
+ * (strata_argmax_rows or strata_logits_process over all rows). The path begins with row 0 and goes on with the first child whose
+ * token is the choice after its parent, up to max_path rows (1 to 32 words); a choice below 0 ends it. n_path[s]: its rows;
+ * chosen[s max_path + i]: the choice after its row i, the step's new tokens, -1 behind them; last[s]: its last row (of all t);
+ * keep[s]: the sequence's positions that stay, those before its rows and the path's; runs[(s max_path + i) 3 ..]: slot of the path's
+ * row i, slot of the sequence's row i, 1, or three zeros where they are the same, for strata_kv_rows_move. A line: the choice after its
+ * last row, n_path 1, keep len[s], no runs. A sequence without rows, or whose first row has a slot below 0 (refused by
+ * strata_kv_pages_step): n_path 0, last -1, keep len[s]. */
+int strata_tree_accept(strata_ctx* ctx, uint64_t nseq, uint64_t q_start, uint64_t parent, uint64_t tokens, uint64_t ids,
+                       uint64_t len, uint64_t slots, uint64_t t, uint64_t words, uint64_t max_path, uint64_t n_path,
+                       uint64_t chosen, uint64_t last, uint64_t keep, uint64_t runs);
+/* Every sequence s becomes the first keep[s] positions (a value cut to 0 .. what there is; no array, keep = 0: all of them) of what
+ * sequence src[s] held before the call (no array, src = 0: itself): beams that go on from others, samples that branch, sequences cut
+ * back or, where keep[s] is 0, ended. Full
+ * pages are shared: refs (device int32, n_pages; 0 at first) holds the holders of each page but one. The page behind them, if keep
+ * ends inside it, stays with src[s] itself or else goes to the first sequence that goes on from it, where no other holds it; every
+ * other gets a new page from the top of the stack as it is before the call, in order of sequence, and runs[3 s ..] = first slot of
+ * the old page, of the new one, rows to copy (three zeros: none), for strata_kv_rows_move before the caches are written again. So a
+ * page that a sequence may still write is its own. Pages that nobody holds any more go on the stack in the order (sequence, place in
+ * its table) in which they are first met. Writes tables, free_pages, refs, runs, len_out (may be len) and *n_free_out (may be
+ * n_free). *err (device int32, may be 0) goes up by one for each sequence that is refused: one whose src is no sequence, and a cut
+ * that finds no page, stay as they are; a sequence that was to become another and finds no page is empty; and once for pages that
+ * the stack has no room for. Page ids outside 0 .. n_pages - 1 are handed on as they are. A sequence that holds shared pages ends here
+ * (keep[s] 0), not by add < 0 of strata_kv_pages_step, which gives its pages back whoever else holds them. */
+int strata_kv_pages_fork(strata_ctx* ctx, uint64_t nseq, uint64_t src, uint64_t keep, uint64_t len, uint64_t tables,
+                         uint64_t max_pages, uint64_t page, uint64_t free_pages, uint64_t n_pages, uint64_t n_free, uint64_t refs,
+                         uint64_t len_out, uint64_t n_free_out, uint64_t runs, uint64_t err);
+/* Rows of n_caches caches (device uint64 addresses, 16-byte aligned; the K and V caches of all layers) of row_bytes bytes (a
+ * multiple of 16) from slot to slot: `groups` groups of `per` (1 to 256) runs (from, to, rows) of consecutive rows, device int32. A
+ * group's runs are made in order; no run reads a row that the same or an earlier run of its group has written, and no group one that
+ * another group writes. A run with a row outside 0 .. n_slots - 1, or of no rows, is left out. */
+int strata_kv_rows_move(strata_ctx* ctx, uint64_t caches, uint64_t n_caches, uint64_t row_bytes, uint64_t n_slots, uint64_t runs,
+                        uint64_t groups, uint64_t per);
+/* Of rows of n logits (x_stride floats apart; x 4-byte aligned): logp[r m + i] = ln softmax(x_r)[ids[r m + i]] of m given tokens a row (up to
+ * 16; device int32; -inf for an id outside 0 .. n - 1), rank[r m + i] = 1 + the tokens ordered before it (0 for such an id), entropy[r]
+ * = -sum p ln p, and the k (up to 64) likeliest tokens in order with their log probabilities, top_ids and top_logp [rows][k] (-1
+ * and -inf behind the last where n < k). Tokens are ordered as strata_argmax_rows orders them, the first of equals first. Each of
+ * logp, rank, entropy, top_ids and top_logp may be 0. A row of -inf alone: log probabilities -inf, entropy 0; one that holds +inf or
+ * NaN: NaN. */
+int strata_logits_logprobs(strata_ctx* ctx, uint64_t x, uint64_t x_stride, uint64_t n, uint64_t rows, uint64_t ids, uint64_t m,
+                           uint64_t logp, uint64_t rank, uint64_t entropy, uint64_t k, uint64_t top_ids, uint64_t top_logp);
+
 /* Backend::add (src/backend.rs:282): x += y over n floats. */
 int strata_add(strata_ctx* ctx, uint64_t x, uint64_t y, uint64_t n);
 /* Backend::swiglu (src/backend.rs:284): g = silu(g) * u over n floats. */

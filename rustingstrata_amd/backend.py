@@ -117,6 +117,12 @@ SIGNATURES = {
     "strata_rms_norm_rope_qk_paged": [CTX] + [U64] * 11 + [F32, U64, U64, F32] + [U64] * 7,
     "strata_attn_paged": [CTX] + [U64] * 21 + [F32, U64, U64],
     "strata_logits_process": [CTX] + [U64] * 19 + [I32],
+    "strata_tree_step": [CTX] + [U64] * 10,
+    "strata_attn_paged_tree": [CTX] + [U64] * 21 + [F32] + [U64] * 4,
+    "strata_tree_accept": [CTX] + [U64] * 15,
+    "strata_kv_pages_fork": [CTX] + [U64] * 15,
+    "strata_kv_rows_move": [CTX] + [U64] * 7,
+    "strata_logits_logprobs": [CTX] + [U64] * 12,
     "strata_add": [CTX, U64, U64, U64],
     "strata_swiglu": [CTX, U64, U64, U64],
     "strata_get_rows": [CTX, TP, U64, U64, U64],
@@ -558,6 +564,44 @@ class HipBackend:
                                            hist_stride, int(hist_len), int(hist_from), last, int(pen), int(bias_start),
                                            int(bias_ids), int(bias_vals), n_bias, int(mask), mask_stride, int(ids),
                                            int(append)))
+
+    # ---- drafted trees and branching sequences ----
+    def tree_step(self, nseq, q_start, parent, length, t, words, pos, mask, prefix_len=0, err=0):
+        """Positions and ancestor masks (`words` uint32 a row) of a step's drafted trees from each row's parent."""
+        _check(lib().strata_tree_step(self._ctx, nseq, int(q_start), int(parent), int(length), int(prefix_len), t, words,
+                                      int(pos), int(mask), int(err)))
+
+    def attn_paged_tree(self, q, kc, vc, qg, out, t, max_q, pos, q_start, length, nseq, tables, max_pages, page, n_pages, nh,
+                        nkv, hd, scale, mask, words, prefix=0, prefix_len=0, max_prefix=0, sink=0, win=0):
+        """attn_paged whose rows are nodes of trees: of its step's keys a row sees those that its mask names."""
+        _check(lib().strata_attn_paged_tree(self._ctx, int(q), int(kc), int(vc), int(qg), int(out), t, max_q, int(pos),
+                                            int(q_start), int(length), nseq, int(tables), max_pages, page, n_pages,
+                                            int(prefix), int(prefix_len), max_prefix, nh, nkv, hd, scale, int(sink), win,
+                                            int(mask), words))
+
+    def tree_accept(self, nseq, q_start, parent, tokens, ids, length, slots, t, words, max_path, n_path, chosen, last, keep,
+                    runs):
+        """The path of each tree that the choices confirm, the positions that stay and the cache rows that have to move."""
+        _check(lib().strata_tree_accept(self._ctx, nseq, int(q_start), int(parent), int(tokens), int(ids), int(length),
+                                        int(slots), t, words, max_path, int(n_path), int(chosen), int(last), int(keep),
+                                        int(runs)))
+
+    def kv_pages_fork(self, nseq, src, keep, length, tables, max_pages, page, free, n_pages, n_free, refs, len_out,
+                      n_free_out, runs, err=0):
+        """Every sequence becomes the first keep[s] positions of what src[s] held: full pages shared, the last one taken
+        over or copied (runs), pages that nobody holds any more back on the stack. src 0: itself; keep 0: all."""
+        _check(lib().strata_kv_pages_fork(self._ctx, nseq, int(src), int(keep), int(length), int(tables), max_pages, page,
+                                          int(free), n_pages, int(n_free), int(refs), int(len_out), int(n_free_out),
+                                          int(runs), int(err)))
+
+    def kv_rows_move(self, caches, n_caches, row_bytes, n_slots, runs, groups, per):
+        """Runs of rows of all caches (an array of device addresses) from slot to slot."""
+        _check(lib().strata_kv_rows_move(self._ctx, int(caches), n_caches, row_bytes, n_slots, int(runs), groups, per))
+
+    def logits_logprobs(self, x, x_stride, n, rows, ids=0, m=0, logp=0, rank=0, entropy=0, k=0, top_ids=0, top_logp=0):
+        """Log probabilities of m given tokens a row with their ranks, the entropy, and the k likeliest tokens."""
+        _check(lib().strata_logits_logprobs(self._ctx, int(x), x_stride, n, rows, int(ids), m, int(logp), int(rank),
+                                            int(entropy), k, int(top_ids), int(top_logp)))
 
     def add(self, x, y, n):
         _check(lib().strata_add(self._ctx, int(x), int(y), n))

@@ -13,6 +13,7 @@
 #include "gemm.h"
 #include "decoder.h"
 #include "serve.h"
+#include "branch.h"
 #include "../../include/strata_hip.h"
 
 using namespace strata;
@@ -1096,31 +1097,43 @@ int strata_rms_norm_rope_qk_paged(strata_ctx* c, uint64_t q, uint64_t q_tstride,
     return 0;
 }
 
-int strata_attn_paged(strata_ctx* c, uint64_t q, uint64_t kc, uint64_t vc, uint64_t qg, uint64_t out, uint64_t t,
-                      uint64_t max_q, uint64_t pos, uint64_t q_start, uint64_t len, uint64_t nseq, uint64_t tables,
-                      uint64_t max_pages, uint64_t page, uint64_t n_pages, uint64_t prefix, uint64_t prefix_len,
-                      uint64_t max_prefix, uint64_t nh, uint64_t nkv, uint64_t hd, float scale, uint64_t sink, uint64_t win) {
-    if (check_ctx(c) || check_attn(nh, nkv, hd, "paged attention") || check_pages(nseq, max_pages, page, n_pages, "paged attention")) return -1;
+// Checks and arguments that both forms of paged attention share.
+static int paged_attn_args(strata_ctx* c, const char* what, PagedAttn& a, uint64_t q, uint64_t kc, uint64_t vc, uint64_t qg, uint64_t out, uint64_t t,
+                           uint64_t max_q, uint64_t pos, uint64_t q_start, uint64_t len, uint64_t nseq, uint64_t tables,
+                           uint64_t max_pages, uint64_t page, uint64_t n_pages, uint64_t prefix, uint64_t prefix_len,
+                           uint64_t max_prefix, uint64_t nh, uint64_t nkv, uint64_t hd, float scale, uint64_t sink, uint64_t win) {
+    const std::string w = what;
+    if (check_ctx(c) || check_attn(nh, nkv, hd, what) || check_pages(nseq, max_pages, page, n_pages, what)) return -1;
     if (!t || !nseq) return 0;
-    if (!q || !kc || !vc || !out || !pos || !q_start || !len || !tables) return set_error("paged attention: null argument");
-    if (max_prefix && (!prefix || !prefix_len)) return set_error("paged attention: null prefix or its length");
-    if (t > (1ull << 20) || !max_q || max_q > t) return set_error("paged attention: " + std::to_string(t) + " rows (at most 2^20), at most " + std::to_string(max_q) + " a sequence");
-    if (max_prefix > (1ull << 30) || win >= (1ull << 31) || nkv > 65535 || nh > 65535) return set_error("paged attention: too large");
+    if (!q || !kc || !vc || !out || !pos || !q_start || !len || !tables) return set_error(w + ": null argument");
+    if (max_prefix && (!prefix || !prefix_len)) return set_error(w + ": null prefix or its length");
+    if (t > (1ull << 20) || !max_q || max_q > t) return set_error(w + ": " + std::to_string(t) + " rows (at most 2^20), at most " + std::to_string(max_q) + " a sequence");
+    if (max_prefix > (1ull << 30) || win >= (1ull << 31) || nkv > 65535 || nh > 65535) return set_error(w + ": too large");
     if (max_prefix + max_pages * page > PAGED_ATTN_KEYS)
-        return set_error("paged attention: " + std::to_string(max_prefix + max_pages * page) + " positions of a prefix and a sequence (at most 2^31 - 1024)");
-    if (nseq * nkv * (max_pages * page / 64 + 32) >= (1ull << 31)) return set_error("paged attention: more than 2^31 chunks of keys (sequences x KV heads x positions / 64)");
+        return set_error(w + ": " + std::to_string(max_prefix + max_pages * page) + " positions of a prefix and a sequence (at most 2^31 - 1024)");
+    if (nseq * nkv * (max_pages * page / 64 + 32) >= (1ull << 31)) return set_error(w + ": more than 2^31 chunks of keys (sequences x KV heads x positions / 64)");
     if ((t / (128 / (nh / nkv)) + nseq + 1) * ((max_prefix + max_pages * page) / 64 + 5) >= (1ull << 31))
-        return set_error("paged attention: more than 2^31 tiles of rows and keys (rows x group / 128 + sequences, times positions / 64)");
-    if (q % 16 || out % 16 || kc % 16 || vc % 16 || qg % 16) return set_error("paged attention: q, qg, out and the caches must be 16-byte aligned");
-    if (out == q || out == qg) return set_error("paged attention: out over an input");
-    if (!(scale > 0.0f) || std::isinf(scale)) return set_error("paged attention: a scale of " + std::to_string(scale) + " (above 0)");
-    PagedAttn a;
+        return set_error(w + ": more than 2^31 tiles of rows and keys (rows x group / 128 + sequences, times positions / 64)");
+    if (q % 16 || out % 16 || kc % 16 || vc % 16 || qg % 16) return set_error(w + ": q, qg, out and the caches must be 16-byte aligned");
+    if (out == q || out == qg) return set_error(w + ": out over an input");
+    if (!(scale > 0.0f) || std::isinf(scale)) return set_error(w + ": a scale of " + std::to_string(scale) + " (above 0)");
     a.q = (const float*)q; a.kc = (const uint16_t*)kc; a.vc = (const uint16_t*)vc; a.qg = (const float*)qg; a.out = (float*)out;
     a.t = (int)t; a.max_q = (int)max_q; a.pos = (const int*)pos; a.q_start = (const int*)q_start; a.len = (const int*)len;
     a.nseq = (int)nseq; a.tables = (const int*)tables; a.max_pages = (int)max_pages; a.page_shift = log2_of(page);
     a.n_pages = (int)n_pages;
     if (max_prefix) { a.prefix = (const int*)prefix; a.prefix_len = (const int*)prefix_len; a.max_prefix = (int)max_prefix; }
     a.nh = (int)nh; a.nkv = (int)nkv; a.hd = (int)hd; a.scale = scale; a.sink = (const float*)sink; a.win = (int)win;
+    return 0;
+}
+
+int strata_attn_paged(strata_ctx* c, uint64_t q, uint64_t kc, uint64_t vc, uint64_t qg, uint64_t out, uint64_t t,
+                      uint64_t max_q, uint64_t pos, uint64_t q_start, uint64_t len, uint64_t nseq, uint64_t tables,
+                      uint64_t max_pages, uint64_t page, uint64_t n_pages, uint64_t prefix, uint64_t prefix_len,
+                      uint64_t max_prefix, uint64_t nh, uint64_t nkv, uint64_t hd, float scale, uint64_t sink, uint64_t win) {
+    PagedAttn a;
+    if (paged_attn_args(c, "paged attention", a, q, kc, vc, qg, out, t, max_q, pos, q_start, len, nseq, tables, max_pages, page, n_pages,
+                        prefix, prefix_len, max_prefix, nh, nkv, hd, scale, sink, win)) return -1;
+    if (!t || !nseq) return 0;
     STRATA_HIP(c->need(c->sv, paged_attn_ws_bytes(a)));
     a.ws = c->sv.p;
     STRATA_HIP(launch_attn_paged(a, c->stream));
@@ -1154,6 +1167,118 @@ int strata_logits_process(strata_ctx* c, uint64_t x, uint64_t x_stride, uint64_t
         a.keys = (uint64_t*)c->sv.p;
     }
     STRATA_HIP(launch_logits_process(a, c->stream));
+    return 0;
+}
+
+// ---- drafted trees and branching sequences ----
+
+static int check_words(uint64_t words, const char* what) {
+    if (!words || words > (uint64_t)TREE_MAX_WORDS)
+        return set_error(std::string(what) + ": masks of " + std::to_string(words) + " words (1 to " + std::to_string(TREE_MAX_WORDS) + ")");
+    return 0;
+}
+static int check_seqs(uint64_t nseq, uint64_t t, const char* what) {
+    if (nseq > (uint64_t)SERVE_MAX_SEQ)
+        return set_error(std::string(what) + ": " + std::to_string(nseq) + " sequences (at most " + std::to_string(SERVE_MAX_SEQ) + ")");
+    if (t > (1ull << 24)) return set_error(std::string(what) + ": " + std::to_string(t) + " tokens (at most 2^24)");
+    return 0;
+}
+
+int strata_tree_step(strata_ctx* c, uint64_t nseq, uint64_t q_start, uint64_t parent, uint64_t len, uint64_t prefix_len,
+                     uint64_t t, uint64_t words, uint64_t pos, uint64_t mask, uint64_t err) {
+    if (check_ctx(c) || check_seqs(nseq, t, "tree_step") || check_words(words, "tree_step")) return -1;
+    if (!t) return 0;
+    if (!q_start || (nseq && (!parent || !len)) || !pos || !mask) return set_error("tree_step: null argument");
+    TreeStep a;
+    a.nseq = (int)nseq; a.q_start = (const int*)q_start; a.parent = (const int*)parent; a.len = (const int*)len;
+    a.prefix_len = (const int*)prefix_len; a.t = (int)t; a.words = (int)words; a.pos = (int*)pos; a.mask = (uint32_t*)mask; a.err = (int*)err;
+    STRATA_HIP(launch_tree_step(a, c->stream));
+    return 0;
+}
+
+int strata_attn_paged_tree(strata_ctx* c, uint64_t q, uint64_t kc, uint64_t vc, uint64_t qg, uint64_t out, uint64_t t,
+                           uint64_t max_q, uint64_t pos, uint64_t q_start, uint64_t len, uint64_t nseq, uint64_t tables,
+                           uint64_t max_pages, uint64_t page, uint64_t n_pages, uint64_t prefix, uint64_t prefix_len,
+                           uint64_t max_prefix, uint64_t nh, uint64_t nkv, uint64_t hd, float scale, uint64_t sink, uint64_t win,
+                           uint64_t mask, uint64_t words) {
+    PagedAttn a;
+    if (paged_attn_args(c, "tree attention", a, q, kc, vc, qg, out, t, max_q, pos, q_start, len, nseq, tables, max_pages, page, n_pages,
+                        prefix, prefix_len, max_prefix, nh, nkv, hd, scale, sink, win) || check_words(words, "tree attention")) return -1;
+    if (!t || !nseq) return 0;
+    if (!mask) return set_error("tree attention: null mask");
+    if (win && win < 32 * words) return set_error("tree attention: a window of " + std::to_string(win) + " over trees of up to " + std::to_string(32 * words) + " rows");
+    a.mask = (const uint32_t*)mask; a.words = (int)words;
+    STRATA_HIP(c->need(c->sv, tree_attn_ws_bytes(a)));
+    a.ws = c->sv.p;
+    STRATA_HIP(launch_attn_tree(a, c->stream));
+    return 0;
+}
+
+int strata_tree_accept(strata_ctx* c, uint64_t nseq, uint64_t q_start, uint64_t parent, uint64_t tokens, uint64_t ids,
+                       uint64_t len, uint64_t slots, uint64_t t, uint64_t words, uint64_t max_path, uint64_t n_path,
+                       uint64_t chosen, uint64_t last, uint64_t keep, uint64_t runs) {
+    if (check_ctx(c) || check_seqs(nseq, t, "tree_accept") || check_words(words, "tree_accept")) return -1;
+    if (!max_path || max_path > 32 * words) return set_error("tree_accept: paths of " + std::to_string(max_path) + " rows (1 to " + std::to_string(32 * words) + ")");
+    if (!nseq) return 0;
+    if (!q_start || !len || !n_path || !chosen || !last || !keep || !runs || (t && (!parent || !tokens || !ids || !slots))) return set_error("tree_accept: null argument");
+    TreeAccept a;
+    a.nseq = (int)nseq; a.q_start = (const int*)q_start; a.parent = (const int*)parent; a.tokens = (const int*)tokens; a.ids = (const int*)ids;
+    a.len = (const int*)len; a.slots = (const int*)slots; a.t = (int)t; a.words = (int)words; a.max_path = (int)max_path;
+    a.n_path = (int*)n_path; a.chosen = (int*)chosen; a.last = (int*)last; a.keep = (int*)keep; a.runs = (int*)runs;
+    STRATA_HIP(launch_tree_accept(a, c->stream));
+    return 0;
+}
+
+int strata_kv_pages_fork(strata_ctx* c, uint64_t nseq, uint64_t src, uint64_t keep, uint64_t len, uint64_t tables,
+                         uint64_t max_pages, uint64_t page, uint64_t free_pages, uint64_t n_pages, uint64_t n_free, uint64_t refs,
+                         uint64_t len_out, uint64_t n_free_out, uint64_t runs, uint64_t err) {
+    if (check_ctx(c) || check_pages(nseq, max_pages, page, n_pages, "kv_pages_fork")) return -1;
+    if (!free_pages || !n_free || !refs || !n_free_out || (nseq && (!len || !tables || !len_out || !runs))) return set_error("kv_pages_fork: null argument");
+    if (nseq * max_pages >= (1ull << 31)) return set_error("kv_pages_fork: tables of more than 2^31 entries");
+    if (keep && (keep == len_out || keep == runs)) return set_error("kv_pages_fork: an output over keep");
+    PagesFork a;
+    a.nseq = (int)nseq; a.src = (const int*)src; a.keep = (const int*)keep; a.len = (const int*)len;
+    a.tables = (int*)tables; a.max_pages = (int)max_pages; a.page_shift = log2_of(page);
+    a.free_pages = (int*)free_pages; a.n_pages = (int)n_pages; a.n_free = (const int*)n_free; a.refs = (int*)refs;
+    a.len_out = (int*)len_out; a.n_free_out = (int*)n_free_out; a.runs = (int*)runs; a.err = (int*)err;
+    STRATA_HIP(c->need(c->sv, pages_fork_scratch_bytes(a)));
+    a.scratch = c->sv.p;
+    STRATA_HIP(launch_pages_fork(a, c->stream));
+    return 0;
+}
+
+int strata_kv_rows_move(strata_ctx* c, uint64_t caches, uint64_t n_caches, uint64_t row_bytes, uint64_t n_slots, uint64_t runs,
+                        uint64_t groups, uint64_t per) {
+    if (check_ctx(c)) return -1;
+    if (!row_bytes || row_bytes % 16 || row_bytes > (1ull << 24)) return set_error("kv_rows_move: rows of " + std::to_string(row_bytes) + " bytes (a multiple of 16, at most 2^24)");
+    if (!per || per > 256) return set_error("kv_rows_move: " + std::to_string(per) + " runs a group (1 to 256)");
+    if (!n_slots || n_slots >= (1ull << 31)) return set_error("kv_rows_move: " + std::to_string(n_slots) + " slots (1 to 2^31 - 1)");
+    if (groups > (1ull << 20) || n_caches > (1ull << 20) || groups * n_caches >= (1ull << 31)) return set_error("kv_rows_move: more than 2^31 groups of caches");
+    if (!groups || !n_caches) return 0;
+    if (!caches || !runs) return set_error("kv_rows_move: null argument");
+    RowsMove a;
+    a.caches = (const uint64_t*)caches; a.n_caches = (int)n_caches; a.row_bytes = row_bytes; a.n_slots = n_slots;
+    a.runs = (const int*)runs; a.groups = (int)groups; a.per = (int)per;
+    STRATA_HIP(launch_rows_move(a, c->stream));
+    return 0;
+}
+
+int strata_logits_logprobs(strata_ctx* c, uint64_t x, uint64_t x_stride, uint64_t n, uint64_t rows, uint64_t ids, uint64_t m,
+                           uint64_t logp, uint64_t rank, uint64_t entropy, uint64_t k, uint64_t top_ids, uint64_t top_logp) {
+    if (check_ctx(c)) return -1;
+    if (!rows) return 0;
+    if (!n || n >= (1ull << 31) || rows > (1ull << 20)) return set_error("logits_logprobs: " + std::to_string(rows) + " rows (at most 2^20) of " + std::to_string(n));
+    if (m > (uint64_t)LOGP_MAX_IDS || k > (uint64_t)LOGP_MAX_TOP)
+        return set_error("logits_logprobs: " + std::to_string(m) + " given tokens (at most " + std::to_string(LOGP_MAX_IDS) + "), " + std::to_string(k) + " likeliest (at most " + std::to_string(LOGP_MAX_TOP) + ")");
+    if (!x || x % 4 || (m && !ids)) return set_error("logits_logprobs: null or misaligned argument");
+    if (rows > 1 && x_stride < n) return set_error("logits_logprobs: a row stride shorter than " + std::to_string(n));
+    Logprobs a;
+    a.x = (const float*)x; a.x_stride = x_stride; a.n = (int)n; a.rows = (int)rows; a.ids = (const int*)ids; a.m = (int)m;
+    a.logp = (float*)logp; a.rank = (int*)rank; a.entropy = (float*)entropy;
+    a.k = top_ids || top_logp ? (int)k : 0; a.top_ids = (int*)top_ids; a.top_logp = (float*)top_logp;
+    STRATA_HIP(c->need(c->sv, logprobs_scratch_bytes(a)));
+    a.scratch = c->sv.p;
+    STRATA_HIP(launch_logprobs(a, c->stream));
     return 0;
 }
 

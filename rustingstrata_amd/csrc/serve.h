@@ -45,6 +45,7 @@ struct PagedAttn {
     const int* prefix = nullptr; const int* prefix_len = nullptr; int max_prefix = 0;
     int nh = 0, nkv = 0, hd = 0; float scale = 0; const float* sink = nullptr; int win = 0;
     void* ws = nullptr;
+    const uint32_t* mask = nullptr; int words = 0;  // of drafted trees (strata_attn_paged_tree): ancestor masks, words a row
 };
 size_t paged_attn_ws_bytes(const PagedAttn& a);
 hipError_t launch_attn_paged(const PagedAttn& a, hipStream_t s);
