@@ -46,6 +46,7 @@ struct PagedWs {
     float2* tml;   // [2 tblocks][128]: the pieces of tiles that more than one block computes
     float* tacc;   // [2 tblocks][128][hd]
     int direct;    // a (sequence, KV head) that one block holds is finished there, and the join takes those that a block cuts
+    int rt;        // TREE: row tiles of a sequence (above 1: of dr rows each, and all of them decode)
     int dblocks, nct, dr, nsp, prows, tblocks;  // decode blocks, their column tiles; rows (tokens x G) up to which a sequence decodes
 };
 
@@ -53,20 +54,35 @@ struct PagedWs {
 constexpr int DEC_CHUNK = 128;  // 32 keys a wave
 struct SeqInfo {
     int q0, qn;   // query rows
+    int seq, s0, sn;  // the sequence that they belong to, and all of its rows
     int len;      // own keys
     int c0, nc;   // the first chunk of DEC_CHUNK own keys that a row sees, and how many (decode sequences)
 };
 __device__ __forceinline__ int prefix_len(const PagedAttn& a) { return a.prefix_len ? min(max(sload(a.prefix_len), 0), a.max_prefix) : 0; }
-// UNI: s is the same in the whole wave (scalar loads, so that what follows from them stays in scalar registers).
-template <bool UNI>
-__device__ __forceinline__ SeqInfo seq_info(const PagedAttn& a, int s, int G, int dr, int P) {
+// UNI: s is the same in the whole wave (scalar loads, so that what follows from them stays in scalar registers). Of TREE's sequences in
+// row tiles, s counts the tiles, a sequence's one after the other.
+template <bool TREE, bool UNI>
+__device__ __forceinline__ SeqInfo seq_info(const PagedAttn& a, const PagedWs& w, int s, int G, int P) {
     auto ld = [](const int* p) { return UNI ? sload(p) : *p; };
     SeqInfo r;
+    int tile = 0;
+    if (TREE && w.rt > 1) {
+        tile = s % w.rt;
+        s /= w.rt;
+    }
+    r.seq = s;
     r.q0 = min(max(ld(a.q_start + s), 0), a.t);
     r.qn = min(max(ld(a.q_start + s + 1), r.q0), a.t) - r.q0;
     r.len = (int)min((long long)max(ld(a.len + s), 0), (long long)a.max_pages << a.page_shift);
+    r.s0 = r.q0;
+    r.sn = r.qn;
+    if (TREE && w.rt > 1) {
+        const int tr = w.dr / G, first = min(tile * tr, r.qn);
+        r.q0 += first;
+        r.qn = min(r.qn - first, tr);
+    }
     r.c0 = r.nc = 0;
-    if (r.qn > 0 && r.qn * G <= dr) {
+    if (r.qn > 0 && r.qn * G <= w.dr) {
         if (a.win > 0) {
             int first = INT_MAX;  // (a window hides keys before the first row's)
             for (int i = 0; i < r.qn; i++) first = min(first, ld(a.pos + r.q0 + i));
@@ -237,16 +253,16 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
     __shared__ SeqInfo sq;
     __shared__ int sb[2];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
-    const int G = a.nh / a.nkv, P = prefix_len(a);
+    const int G = a.nh / a.nkv, P = prefix_len(a), nseq = TREE ? a.nseq * w.rt : a.nseq;
     // this block's run of the list: the thread that holds the sequence of its start says which it is
     int W0, W1, share;
     {
-        const int per = (a.nseq + 255) / 256;
+        const int per = (nseq + 255) / 256;
         SeqInfo mine{};
         int sum = 0, big = 0;
         for (int i = 0; i < per; i++)
-            if (tid * per + i < a.nseq) {
-                mine = seq_info<false>(a, tid * per + i, G, w.dr, P);
+            if (tid * per + i < nseq) {
+                mine = seq_info<TREE, false>(a, w, tid * per + i, G, P);
                 sum += mine.nc;
                 big = max(big, mine.nc);
             }
@@ -278,8 +294,8 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
         if (DIRECT && tid == 0) w.map[b] = make_int2(0, 0);
         if (W0 >= W1) return;
         if (W0 >= at * a.nkv && W0 < (at + sum) * a.nkv)
-            for (int i = 0; i < per && tid * per + i < a.nseq; i++) {
-                const SeqInfo q = per == 1 ? mine : seq_info<false>(a, tid * per + i, G, w.dr, P);
+            for (int i = 0; i < per && tid * per + i < nseq; i++) {
+                const SeqInfo q = per == 1 ? mine : seq_info<TREE, false>(a, w, tid * per + i, G, P);
                 if (W0 >= at * a.nkv && W0 < (at + q.nc) * a.nkv) {
                     sq = q;
                     sb[0] = tid * per + i;
@@ -290,7 +306,7 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
         __syncthreads();
     }
     auto uni = [](int v) { return __builtin_amdgcn_readfirstlane(v); };
-    SeqInfo q{uni(sq.q0), uni(sq.qn), uni(sq.len), uni(sq.c0), uni(sq.nc)};
+    SeqInfo q{uni(sq.q0), uni(sq.qn), uni(sq.seq), uni(sq.s0), uni(sq.sn), uni(sq.len), uni(sq.c0), uni(sq.nc)};
     int s = uni(sb[0]), base = uni(sb[1]);
     W0 = uni(W0), W1 = uni(W1), share = uni(share);
     uint16_t* vs = (uint16_t*)(lds + wave * L::WAVE);
@@ -308,8 +324,8 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
         if (at >= W1) return false;
         while (at - base >= q.nc * a.nkv) {  // the next sequence that has work
             base += q.nc * a.nkv;
-            if (++s >= a.nseq) return false;
-            q = seq_info<true>(a, s, G, w.dr, P);
+            if (++s >= nseq) return false;
+            q = seq_info<TREE, true>(a, w, s, G, P);
         }
         const int g = (at - base) / q.nc, f = (at - base) % q.nc, n = min(q.nc - f, W1 - at);
         p = Piece{q, s, g, q.c0 + f, q.c0 + f + n, f == 0 ? (at + q.nc - 1) / share - b + 1 : 0};
@@ -323,7 +339,7 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
         int last[2], ok;
     };
     auto pages = [&](const Piece& p, int c, int (&pg)[2]) __attribute__((always_inline)) {
-        const int* table = a.tables + (uint64_t)p.s * a.max_pages;
+        const int* table = a.tables + (uint64_t)p.q.seq * a.max_pages;
 #pragma unroll
         for (int t = 0; t < 2; t++) pg[t] = sload(table + (min(DEC_CHUNK * c + 32 * wave + 16 * t, p.q.len - 1) >> a.page_shift));
     };
@@ -409,7 +425,7 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
                 }
             lo[u] = 1;
             hi[u] = 0;
-            if (live) own_range<TREE>(a, qpos[u], pc.q.len, P, node_of<TREE>(a, pc.q.q0 + (16 * u + l16) / G, pc.q.q0, pc.q.qn, pc.q.len), lo[u], hi[u]);
+            if (live) own_range<TREE>(a, qpos[u], pc.q.len, P, node_of<TREE>(a, pc.q.q0 + (16 * u + l16) / G, pc.q.s0, pc.q.sn, pc.q.len), lo[u], hi[u]);
             mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
             mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
             float up;
@@ -458,12 +474,12 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
             if (!r.ok) continue;
             const int k0 = DEC_CHUNK * c + 32 * wave;
             if constexpr (TREE) {
-                const int base = max(pc.q.len - pc.q.qn, 0);
-                if (k0 + 31 >= base) {  // (keys of the tree's rows)
+                const int base = max(pc.q.len - pc.q.sn, 0);
+                if (k0 + 31 >= base && pc.q.sn <= 32 * a.words) {  // (keys of the tree's rows)
 #pragma unroll
                     for (int u = 0; u < NT; u++) {
                         const int c = 16 * u + l16, tok = c / G < pc.q.qn ? c / G : 0;
-                        const uint64_t see = node_bits(node_of<TREE>(a, pc.q.q0 + tok, pc.q.q0, pc.q.qn, pc.q.len), a.words, k0 - base) >> (4 * lg);
+                        const uint64_t see = node_bits(node_of<TREE>(a, pc.q.q0 + tok, pc.q.s0, pc.q.sn, pc.q.len), a.words, k0 - base) >> (4 * lg);
 #pragma unroll
                         for (int t = 0; t < 2; t++)
 #pragma unroll
@@ -582,10 +598,10 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
                 const int ln = __builtin_ctzll(bad), rb = (64 * wave + ln) >> 4, cb = 16 * u + rb, tok = cb / G;
                 bad &= ~(0xFFFFull << (ln & 48));
                 int klo, khi;
-                const Node node = node_of<TREE>(a, pc.q.q0 + tok, pc.q.q0, pc.q.qn, pc.q.len);
+                const Node node = node_of<TREE>(a, pc.q.q0 + tok, pc.q.s0, pc.q.sn, pc.q.len);
                 own_range<TREE>(a, a.pos[pc.q.q0 + tok], pc.q.len, P, node, klo, khi);
                 float ac[HD / 64], mm, ll;
-                paged_row_again<TREE, HD>(a, Keys{nullptr, a.tables + (uint64_t)pc.s * a.max_pages, 0, 0, pc.q.len}, node,
+                paged_row_again<TREE, HD>(a, Keys{nullptr, a.tables + (uint64_t)pc.q.seq * a.max_pages, 0, 0, pc.q.len}, node,
                                     a.q + ((uint64_t)(pc.q.q0 + tok) * a.nh + pc.g * G + cb % G) * HD, pc.g, max(klo, DEC_CHUNK * c0),
                                     min(khi, DEC_CHUNK * c1 - 1), ac, mm, ll);
                 const uint64_t r = (uint64_t)(b + pair) * w.dr + cb, row = (uint64_t)(pc.q.q0 + tok) * a.nh + pc.g * G + cb % G;
@@ -1162,10 +1178,57 @@ __device__ __forceinline__ RunAt run_at(const PlanTile* plan, int n, int cost, i
     return r;
 }
 
+// Key tiles f .. f + k - 1 of tile p and KV head g, by block b: the rows' output where that is the whole tile, else their sums.
+template <bool TREE, int HD>
+__device__ __forceinline__ void tile_piece(const PagedAttn& a, const PagedWs& w, const PlanTile& p, int P, int g, int f, int k, int b, uint8_t* lds) {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), G = a.nh / a.nkv, gs = 31 - __builtin_clz(G);
+    const bool whole = k == p.nkt;
+    const Keys keys{a.prefix, a.tables + (uint64_t)p.s * a.max_pages, P, (P + 63) / 64, p.len};
+    const int kb = p.kt0 + f, ke = keys.P || keys.len ? kb + k : kb;
+    int q0 = 0, qn = 0;  // the sequence's rows
+    if constexpr (TREE) {
+        q0 = min(max(sload(a.q_start + p.s), 0), a.t);
+        qn = min(max(sload(a.q_start + p.s + 1), q0), a.t) - q0;
+    }
+    auto node_at = [&](int row) { return node_of<TREE>(a, row, q0, qn, p.len); };
+    TileSums<HD> r;
+    {
+        const int rr = 32 * wave + (threadIdx.x & 31), tok = rr >> gs, h = g * G + (rr & (G - 1)), t = p.t0 + (tok < p.nt ? tok : 0);
+        tile_run<TREE, HD>(a, keys, lds, g, kb, ke, tok < p.nt, a.q + ((uint64_t)t * a.nh + h) * HD, a.pos[t], node_at(t), r);
+    }
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // (nothing of this lane's row waits in registers while the tiles run)
+    const int lane = tid & 63, l32 = lane & 31, rr = 32 * wave + l32, h = g * G + (rr & (G - 1));
+    const bool live = (rr >> gs) < p.nt;
+    uint32_t again = tile_again<HD>(r, live);
+    const uint64_t slot = (uint64_t)(2 * b + (f == 0)) * 128;
+    const uint32_t rows = (uint32_t)__ballot(live) & ~again;
+    auto row_at = [&](int i) { return (uint64_t)(p.t0 + ((32 * wave + i) >> gs)) * a.nh + g * G + (i & (G - 1)); };
+    tile_store<HD>(r, tid, (whole ? out_factor(a, h, r.m, r.l * (1.0f / TILE_SCALE)) : 1.0f) * (1.0f / TILE_SCALE), lds, rows,
+                   [&](int i) { return whole ? a.out + row_at(i) * HD : w.tacc + (slot + 32 * wave + i) * HD; },
+                   [&](int i) { return whole && a.qg ? a.qg + row_at(i) * 2 * HD + HD : (const float*)nullptr; });
+    if (!whole && lane < 32 && ((rows >> l32) & 1)) w.tml[slot + rr] = make_float2(r.m, r.l * (1.0f / TILE_SCALE));
+    for (; again; again &= again - 1) {
+        const int rb = 32 * wave + __builtin_ctz(again), tb = p.t0 + (rb >> gs), hb = g * G + (rb & (G - 1));
+        const uint64_t rowb = (uint64_t)tb * a.nh + hb;
+        int lo, hi;
+        row_range<TREE>(a, keys, a.pos[tb], node_at(tb), lo, hi);
+        float ac[HD / 64], mm, ll;
+        paged_row_again<TREE, HD>(a, keys, node_at(tb), a.q + rowb * HD, g, max(lo, 64 * kb), min(hi, 64 * ke - 1), ac, mm, ll);
+        const float fo = whole ? out_factor(a, hb, mm, ll) : 1.0f;
+        float* dst = whole ? a.out + rowb * HD : w.tacc + (slot + rb) * HD;
+#pragma unroll
+        for (int d = 0; d < HD / 64; d++) {
+            const int col = lane + 64 * d;
+            dst[col] = whole && a.qg ? ac[d] * fo * sigmoid_f(a.qg[rowb * 2 * HD + HD + col]) : ac[d] * fo;
+        }
+        if (!whole && lane == 0) w.tml[slot + rb] = make_float2(mm, ll);
+    }
+}
+
 template <bool TREE, int HD>
 __device__ __forceinline__ void tile_block(const PagedAttn& a, const PagedWs& w, int x, uint8_t* lds) {
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int G = a.nh / a.nkv, gs = 31 - __builtin_clz(G), P = prefix_len(a);
+    const int P = prefix_len(a);
     const PlanTile* plan = (const PlanTile*)(w.plan + PLAN_HEAD);
     const int n = sload(w.plan), cost = sload(w.plan + 1);
     // the b-th run; neighbours in the list, which share keys, run on one XCD
@@ -1177,59 +1240,19 @@ __device__ __forceinline__ void tile_block(const PagedAttn& a, const PagedWs& w,
     const RunAt from = run_at(plan, n, cost, a.nkv, b, w.tblocks), to = run_at(plan, n, cost, a.nkv, b + 1, w.tblocks);
     if (threadIdx.x == 0) {
         // the tile that begins in this run and goes on past it: the last block of its pieces (run_at's borders)
-        int last = -1;
+        int4 cut = make_int4(to.g, to.i, -1, 0);
         if (to.f && (from.g != to.g || from.i != to.i || !from.f)) {
             const PlanTile p = plan_tile(plan + to.i);
             const long long end = (long long)cost * to.g + p.cum + TILE_EXTRA + p.nkt;
-            last = (int)min((end - to.near - 1) / to.share, (long long)w.tblocks - 1);
+            cut.z = (int)min((end - to.near - 1) / to.share, (long long)w.tblocks - 1);
+            if constexpr (TREE) cut.y = p.t0, cut.w = p.nt;
         }
-        w.cut[b] = make_int4(to.g, to.i, last, 0);
+        w.cut[b] = cut;
     }
     for (int g = from.g, i = from.i, f = from.f; g < to.g || (g == to.g && (i < to.i || (i == to.i && f < to.f)));) {
         const PlanTile p = plan_tile(plan + i);
         const int k = (g == to.g && i == to.i ? to.f : p.nkt) - f;
-        const bool whole = k == p.nkt;
-        const Keys keys{a.prefix, a.tables + (uint64_t)p.s * a.max_pages, P, (P + 63) / 64, p.len};
-        const int kb = p.kt0 + f, ke = keys.P || keys.len ? kb + k : kb;
-        int q0 = 0, qn = 0;  // the sequence's rows
-        if constexpr (TREE) {
-            q0 = min(max(sload(a.q_start + p.s), 0), a.t);
-            qn = min(max(sload(a.q_start + p.s + 1), q0), a.t) - q0;
-        }
-        auto node_at = [&](int row) { return node_of<TREE>(a, row, q0, qn, p.len); };
-        TileSums<HD> r;
-        {
-            const int rr = 32 * wave + (threadIdx.x & 31), tok = rr >> gs, h = g * G + (rr & (G - 1)), t = p.t0 + (tok < p.nt ? tok : 0);
-            tile_run<TREE, HD>(a, keys, lds, g, kb, ke, tok < p.nt, a.q + ((uint64_t)t * a.nh + h) * HD, a.pos[t], node_at(t), r);
-        }
-        int tid = threadIdx.x;
-        asm volatile("" : "+v"(tid));  // (nothing of this lane's row waits in registers while the tiles run)
-        const int lane = tid & 63, l32 = lane & 31, rr = 32 * wave + l32, h = g * G + (rr & (G - 1));
-        const bool live = (rr >> gs) < p.nt;
-        uint32_t again = tile_again<HD>(r, live);
-        const uint64_t slot = (uint64_t)(2 * b + (f == 0)) * 128;
-        const uint32_t rows = (uint32_t)__ballot(live) & ~again;
-        auto row_at = [&](int i) { return (uint64_t)(p.t0 + ((32 * wave + i) >> gs)) * a.nh + g * G + (i & (G - 1)); };
-        tile_store<HD>(r, tid, (whole ? out_factor(a, h, r.m, r.l * (1.0f / TILE_SCALE)) : 1.0f) * (1.0f / TILE_SCALE), lds, rows,
-                       [&](int i) { return whole ? a.out + row_at(i) * HD : w.tacc + (slot + 32 * wave + i) * HD; },
-                       [&](int i) { return whole && a.qg ? a.qg + row_at(i) * 2 * HD + HD : (const float*)nullptr; });
-        if (!whole && lane < 32 && ((rows >> l32) & 1)) w.tml[slot + rr] = make_float2(r.m, r.l * (1.0f / TILE_SCALE));
-        for (; again; again &= again - 1) {
-            const int rb = 32 * wave + __builtin_ctz(again), tb = p.t0 + (rb >> gs), hb = g * G + (rb & (G - 1));
-            const uint64_t rowb = (uint64_t)tb * a.nh + hb;
-            int lo, hi;
-            row_range<TREE>(a, keys, a.pos[tb], node_at(tb), lo, hi);
-            float ac[HD / 64], mm, ll;
-            paged_row_again<TREE, HD>(a, keys, node_at(tb), a.q + rowb * HD, g, max(lo, 64 * kb), min(hi, 64 * ke - 1), ac, mm, ll);
-            const float fo = whole ? out_factor(a, hb, mm, ll) : 1.0f;
-            float* dst = whole ? a.out + rowb * HD : w.tacc + (slot + rb) * HD;
-#pragma unroll
-            for (int d = 0; d < HD / 64; d++) {
-                const int col = lane + 64 * d;
-                dst[col] = whole && a.qg ? ac[d] * fo * sigmoid_f(a.qg[rowb * 2 * HD + HD + col]) : ac[d] * fo;
-            }
-            if (!whole && lane == 0) w.tml[slot + rb] = make_float2(mm, ll);
-        }
+        tile_piece<TREE, HD>(a, w, p, P, g, f, k, b, lds);
         f += k;
         if (f == p.nkt) {
             f = 0;
@@ -1296,6 +1319,84 @@ __device__ __forceinline__ void join_block(const PagedAttn& a, const PagedWs& w,
     }
 }
 
+// The same for trees, where a tile may be in many pieces (few sequences over long contexts): a block takes 4 RPW rows (HD / 8
+// blocks a tile), its waves every fourth piece, which meet in LDS; the loads of PF pieces of a wave are in flight together. (One tree of
+// 16 over 16000 keys, 128 pieces a tile: 100 us a call by join_block's walk over the pieces, 54 by this; 4 of 16 over 8000 97 and 53.)
+template <int HD>
+__device__ __forceinline__ void join_block_wide(const PagedAttn& a, const PagedWs& w, int b, int y) {
+    constexpr int NC = HD / 4, RPW = 64 / NC, U = 4, PF = 4, R = U * RPW;  // lanes a row (16 bytes each), rows a load, loads, rows
+    __shared__ float2 sml[4][R];
+    __shared__ float4 sacc[4][R][NC];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, last = sload(&w.cut[b].z);
+    if (last < 0) return;
+    const int g = sload(&w.cut[b].x), t0 = sload(&w.cut[b].y), nt = sload(&w.cut[b].w);  // (a TREE cut: KV head, first row, last block, rows)
+    const int G = a.nh / a.nkv, gs = 31 - __builtin_clz(G), nr = nt * G, ch = lane % NC, r0 = y * R + lane / NC;
+    if (y * R >= nr) return;
+    float M[U], L[U];
+    float4 acc[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        M[u] = -INFINITY;
+        L[u] = 0.0f;
+        acc[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
+    // one more partial of row u (one without a maximum has a sum of 0, or not a number)
+    auto add = [&](int u, const float2& ml, const float4& v) __attribute__((always_inline)) {
+        const float mnew = fmaxf(M[u], ml.x), f = M[u] == -INFINITY ? 0.0f : exp2_hw(M[u] - mnew);
+        const bool none = ml.x == -INFINITY;
+        const float e = none ? 0.0f : exp2_hw(ml.x - mnew);
+        L[u] = L[u] * (M[u] == -INFINITY ? 1.0f : f) + (none ? ml.y : ml.y * e);
+        acc[u].x = acc[u].x * f + (none ? 0.0f : v.x * e);
+        acc[u].y = acc[u].y * f + (none ? 0.0f : v.y * e);
+        acc[u].z = acc[u].z * f + (none ? 0.0f : v.z * e);
+        acc[u].w = acc[u].w * f + (none ? 0.0f : v.w * e);
+        M[u] = mnew;
+    };
+    for (int c0 = b + wave; c0 <= last; c0 += 4 * PF) {
+        float2 ml[PF][U];
+        float4 v[PF][U];
+#pragma unroll
+        for (int k = 0; k < PF; k++)
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int c = min(c0 + 4 * k, last);
+                const uint64_t at = (uint64_t)(2 * c + (c == b)) * 128 + min(r0 + u * RPW, nr - 1);
+                ml[k][u] = w.tml[at];
+                v[k][u] = *(const float4*)(w.tacc + at * HD + 4 * ch);
+            }
+#pragma unroll
+        for (int k = 0; k < PF; k++)
+            if (c0 + 4 * k <= last) {
+#pragma unroll
+                for (int u = 0; u < U; u++) add(u, ml[k][u], v[k][u]);
+            }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int r = u * RPW + lane / NC;
+        sacc[wave][r][ch] = acc[u];
+        if (ch == 0) sml[wave][r] = make_float2(M[u], L[u]);
+    }
+    __syncthreads();
+    // wave u finishes the rows of load u
+    const int r = wave * RPW + lane / NC, rr = y * R + r;
+    if (rr >= nr) return;
+    M[0] = -INFINITY;
+    L[0] = 0.0f;
+    acc[0] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int v = 0; v < 4; v++) add(0, sml[v][r], sacc[v][r][ch]);
+    const int h = g * G + (rr & (G - 1));
+    const uint64_t row = (uint64_t)(t0 + (rr >> gs)) * a.nh + h;
+    const float f = out_factor(a, h, M[0], L[0]);
+    float4 x = make_float4(acc[0].x * f, acc[0].y * f, acc[0].z * f, acc[0].w * f);
+    if (a.qg) {
+        const float4 gt = *(const float4*)(a.qg + row * 2 * HD + HD + 4 * ch);
+        x.x *= sigmoid_f(gt.x); x.y *= sigmoid_f(gt.y); x.z *= sigmoid_f(gt.z); x.w *= sigmoid_f(gt.w);
+    }
+    *(float4*)(a.out + row * HD + 4 * ch) = x;
+}
+
 // ---------------- the join of a decode sequence's rows ----------------
 // An item is a row and query head, of all rows or (DIRECT) of the pairs that blocks cut, from its partial sums: out = sum_i acc_i
 // 2^(m_i - M) / (sum_i l_i 2^(m_i - M) + 2^(sink - M)), the prefix's splits, then the own keys' pieces. Wave v of an item's MW takes
@@ -1303,22 +1404,22 @@ __device__ __forceinline__ void join_block(const PagedAttn& a, const PagedWs& w,
 // sequence, then these). Two waves an item: 2048 items of 64 sequences of 200 .. 6000 keys 5.7 us (four waves 7.1, one 5.4); 768 of
 // 4 .. 16 partials 6.6 us (8.4, 8.2). Four waves up to 512 items (a call with one sequence of 32768 keys and one KV head, 128
 // pieces, 17 us, with two 21.5; of 131072 keys and four 52 and 57).
-template <int HD, bool DIRECT, int MW>
+template <bool TREE, int HD, bool DIRECT, int MW>
 __device__ __forceinline__ void merge_block(const PagedAttn& a, const PagedWs& w, int x, int per) {
     constexpr int DL = HD / 64, ITEMS = 4 / MW, U = 4;
     __shared__ float sm[ITEMS][MW], sl[ITEMS][MW], so[ITEMS][MW][HD];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), v = wave % MW, it = wave / MW, lane = threadIdx.x & 63;
     const int G = a.nh / a.nkv, P = prefix_len(a);
-    const int y = ITEMS * x + it;
-    int s = min(y / a.nh / per, a.nseq - 1), h = y % a.nh, i = y / a.nh % per, first, pieces;
+    const int y = ITEMS * x + it, nseq = TREE ? a.nseq * w.rt : a.nseq;
+    int s = min(y / a.nh / per, nseq - 1), h = y % a.nh, i = y / a.nh % per, first, pieces;
     SeqInfo q;
     if constexpr (!DIRECT) {
         const int2* mp = w.map + s * a.nkv + h / G;
         first = sload(&mp->x), pieces = sload(&mp->y);  // (not set, and not used, without own keys)
-        q = seq_info<true>(a, s, G, w.dr, P);
+        q = seq_info<TREE, true>(a, w, s, G, P);
     } else {
-        if (x < a.nseq) {  // sequence x without own keys: its rows are 0
-            q = seq_info<true>(a, x, G, w.dr, P);
+        if (x < nseq) {  // sequence x without own keys: its rows are 0
+            q = seq_info<TREE, true>(a, w, x, G, P);
             if (q.nc == 0 && q.qn * G <= w.dr)
                 for (int j = threadIdx.x; j < q.qn * a.nh * (HD / 4); j += 256)
                     *(float4*)(a.out + (uint64_t)q.q0 * a.nh * HD + 4 * j) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1327,10 +1428,10 @@ __device__ __forceinline__ void merge_block(const PagedAttn& a, const PagedWs& w
         const int pair = sload(&w.map[first].x), c = y % w.dr;
         pieces = sload(&w.map[first].y);
         s = pair / a.nkv, h = pair % a.nkv * G + c % G, i = c / G;
-        q = seq_info<true>(a, s, G, w.dr, P);
+        q = seq_info<TREE, true>(a, w, s, G, P);
     }
     const int g = h / G, r = q.q0 + i;
-    const bool live = (DIRECT ? pieces > 0 && y < w.dblocks * w.dr : y < a.nseq * per * a.nh) && i < q.qn && q.qn * G <= w.dr;
+    const bool live = (DIRECT ? pieces > 0 && y < w.dblocks * w.dr : y < nseq * per * a.nh) && i < q.qn && q.qn * G <= w.dr;
     const uint64_t row = (uint64_t)r * a.nh + h;
     const int np = P > 0 ? w.nsp : 0, n = live ? np + (q.nc > 0 ? pieces : 0) : 0;
     const uint64_t own = (uint64_t)(first + s * a.nkv + g) * w.dr + (r - q.q0) * G + h % G;  // piece i of the own keys: own + i dr
@@ -1429,10 +1530,15 @@ __global__ __launch_bounds__(256, NT == 1 || HD == 64 ? 2 : 1) void attn_paged_k
 template <bool TREE, int HD, bool DIRECT, int MW>
 __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedAttn a, PagedWs w, int jblocks, int per) {
     const int b = blockIdx.x;
-    if (b < jblocks) return join_block<HD>(a, w, b / (HD / 32), b % (HD / 32));
-    merge_block<HD, DIRECT, MW>(a, w, b - jblocks, per);
+    if constexpr (TREE) {
+        if (b < jblocks) return join_block_wide<HD>(a, w, b / (HD / 8), b % (HD / 8));
+    } else {
+        if (b < jblocks) return join_block<HD>(a, w, b / (HD / 32), b % (HD / 32));
+    }
+    merge_block<TREE, HD, DIRECT, MW>(a, w, b - jblocks, per);
 }
 
+constexpr long long ROW_TILE_STEPS = 8192;
 static int div_up(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 // Tiles of the long sequences at most: each of them has more than dr / G rows.
@@ -1448,22 +1554,34 @@ static PagedWs plan(const PagedAttn& a, uint8_t* at, size_t* end) {
     // a sequence decodes up to 16 rows (one column tile), up to 32 where the longest has no more (64 sequences of 4 tokens, 8 heads a
     // KV head, over 2048 keys: 70 us, as tiles of 128 rows 97)
     const long long most_rows = (long long)a.max_q * G;
-    w.nct = most_rows > 16 && most_rows <= 32 ? 2 : 1;
+    // Trees of more rows go in row tiles of 16, all of which decode, where there is little to do: a plan, tiles of 128 rows and their
+    // joins take 30 us before anything else, but row tiles read their keys once each. The steps of 16 rows and 64 keys that the call's
+    // bounds allow decide (us as row tiles / as tiles, 32 heads over 4 of 128): one tree of 16 over 1000 keys 13 / 31, 16 of 16 over 500
+    // (4096 steps) 29 / 40, 16 of 8 over 2000 and 8 of 64 over 500 (8192) 39 / 49 and 42 / 45, 16 of 16 over 2000 (16384) 58 / 53, 8 of 8 over 8000
+    // 87 / 61
+    w.rt = 1;
+    if (a.mask && a.max_q <= 32 * a.words && most_rows > 32) {
+        const int rt = div_up(most_rows, 16);
+        if ((long long)a.nseq * a.nkv * rt * div_up((long long)a.max_pages << a.page_shift, 64) <= ROW_TILE_STEPS) w.rt = rt;
+    }
+    const long long nseq = (long long)a.nseq * w.rt;
+    w.nct = w.rt == 1 && most_rows > 16 && most_rows <= 32 ? 2 : 1;
     w.dr = (int)std::min<long long>(16 * w.nct, most_rows);
-    const long long most = (long long)a.nseq * a.nkv * (((long long)a.max_pages << a.page_shift) / DEC_CHUNK + 1);
+    const long long most = nseq * a.nkv * (((long long)a.max_pages << a.page_shift) / DEC_CHUNK + 1);
     // the blocks that run at once: two a CU (64 ragged sequences 117 us against 122, 300 of 700 keys 104 against 116; a few long ones
     // gain 3 to 5% from one), one where two column tiles of 128 values fill a CU's registers (of 64 values two: 100 sequences of 4
     // tokens 169 us against 211) or the prefix's blocks take the other's place (24 of 4 tokens over a prefix 24.2 us against 26.4, 64
     // over one of 4096 33 against 41)
-    w.dblocks = (int)std::min<long long>(most, (w.nct == 1 || a.hd == 64) && (!a.max_prefix || most_rows > w.dr) ? 512 : 256);
+    w.dblocks = (int)std::min<long long>(most, (w.nct == 1 || a.hd == 64) && (!a.max_prefix || (w.rt == 1 && most_rows > w.dr)) ? 512 : 256);
     // where no more (sequence, KV head) than blocks are there, most are cut and each of their rows is joined (64 sequences of 2000
     // keys over 4 KV heads 49 us, direct 53); else most are not (256: 196 and 187; 1000 of 300 keys 177 and 139)
-    w.direct = !a.max_prefix && (long long)a.nseq * a.nkv >= w.dblocks;
+    w.direct = !a.max_prefix && nseq * a.nkv >= w.dblocks;
     // splits of the prefix, of at least 128 keys: a block a CU (64 sequences over a prefix of 4096 31 us, for two a CU 46; of 16000 56
     // and 59): more of them cost more sums than they hide. The rows that count are those of sequences that may decode (all t rows
     // left the decode rows beside chunks with a few long splits: 512 tokens and 63 decoding sequences over 16000 511 us for 336,
     // 1500 tokens and 4 over 2000 212 for 169)
-    w.prows = (int)(most_rows > w.dr ? std::min<long long>(a.t, (long long)a.nseq * (w.dr / G)) : a.t);
+    const bool tiles = w.rt == 1 && most_rows > w.dr;  // there may be long sequences
+    w.prows = (int)(tiles ? std::min<long long>(a.t, (long long)a.nseq * (w.dr / G)) : a.t);
     const long long blocks = std::max<long long>((long long)div_up((long long)w.prows * G, 128) * a.nkv, 1);
     w.nsp = (int)std::max<long long>(1, std::min<long long>({div_up(256, blocks), div_up(a.max_prefix, 128), 64}));
     w.tblocks = 512;
@@ -1473,15 +1591,15 @@ static PagedWs plan(const PagedAttn& a, uint8_t* at, size_t* end) {
         o += (bytes + 255) & ~(size_t)255;
         return (void*)p;
     };
-    const size_t slots = (size_t)w.dblocks + (size_t)a.nseq * a.nkv, out_rows = (size_t)w.prows * a.nh;
-    w.map = (int2*)take(std::max((size_t)a.nseq * a.nkv, (size_t)w.dblocks) * sizeof(int2));
+    const size_t slots = (size_t)w.dblocks + (size_t)nseq * a.nkv, out_rows = (size_t)w.prows * a.nh;
+    w.map = (int2*)take(std::max((size_t)nseq * a.nkv, (size_t)w.dblocks) * sizeof(int2));
     w.dml = (float2*)take(slots * w.dr * sizeof(float2));
     w.dacc = (float*)take(slots * w.dr * a.hd * sizeof(float));
     if (a.max_prefix) {
         w.pml = (float2*)take(out_rows * w.nsp * sizeof(float2));
         w.pacc = (float*)take(out_rows * w.nsp * a.hd * sizeof(float));
     }
-    if (most_rows > w.dr) {
+    if (tiles) {
         w.plan = (int*)take((PLAN_HEAD + (size_t)max_tiles(a, w) * (sizeof(PlanTile) / 4)) * 4);
         if (a.max_prefix) {
             w.drows = (int*)take((size_t)a.t * 4);
@@ -1525,10 +1643,10 @@ static void launch_t(const PagedAttn& a, const PagedWs& w, hipStream_t s) {
         else if (w.direct) launch(one, no, no, yes);
         else launch(one, no, no, no);
     }
-    const int jblocks = w.plan ? w.tblocks * (HD / 32) : 0;
-    const long long items = w.direct ? (long long)w.dblocks * w.dr : (long long)a.nseq * per * a.nh;
+    const int jblocks = w.plan ? w.tblocks * (TREE ? HD / 8 : HD / 32) : 0;
+    const long long items = w.direct ? (long long)w.dblocks * w.dr : (long long)a.nseq * w.rt * per * a.nh;
     if (w.direct) {
-        const dim3 jgrid((unsigned)(jblocks + std::max(div_up(items, 2), a.nseq)));
+        const dim3 jgrid((unsigned)(jblocks + std::max(div_up(items, 2), a.nseq * w.rt)));
         attn_paged_join_kernel<TREE, HD, true, 2><<<jgrid, block, 0, s>>>(a, w, jblocks, per);
     } else if (items > 512) {
         attn_paged_join_kernel<TREE, HD, false, 2><<<dim3((unsigned)(jblocks + div_up(items, 2))), block, 0, s>>>(a, w, jblocks, per);

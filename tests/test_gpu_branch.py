@@ -412,11 +412,15 @@ def test_logprobs_of_the_longest_row(hip):
 
 # ---------------- attention ----------------
 class Trees(Batch):
-    """Batch whose sequences' rows are trees; shape: one for all, or a list."""
+    """Batch whose sequences' rows are trees; room: pages that a table has room for at least (many: the call's bounds allow much
+    work, which takes another form)."""
 
-    def __init__(self, hip, q, n, nh, nkv, hd, page, words, P=0, seed=0, shape="any", **kw):
+    def __init__(self, hip, q, n, nh, nkv, hd, page, words, P=0, seed=0, shape="any", room=0, **kw):
         super().__init__(hip, q, n, nh, nkv, hd, page, P=P, seed=seed, **kw)
         rng = np.random.default_rng(seed + 1000)
+        if room > self.max_pages:
+            self.tables = np.concatenate([self.tables, rng.integers(-5, self.n_pages + 5, (self.nseq, room - self.max_pages))], 1)
+            self.max_pages = room
         self.words = words
         self.parent = np.concatenate([random_tree(rng, k, shape) for k in q if k] + [np.full(kw.get("extra", 0), -1)]).astype(np.int64)
         self.pos, self.mask, _ = B.tree_step(self.q_start, self.parent, self.n, P, self.t, words)
@@ -442,14 +446,14 @@ SHAPES = [(8, 1, 128), (8, 2, 64), (4, 2, 128), (4, 4, 64), (3, 3, 128)]
 
 @pytest.mark.parametrize("nh,nkv,hd", SHAPES)
 @pytest.mark.parametrize("P,win", [(0, 0), (0, 40), (70, 0), (333, 100)])
-@pytest.mark.parametrize("most", [2, 4, 9, 32])
-def test_attn_tree(hip, nh, nkv, hd, P, win, most):
+@pytest.mark.parametrize("most,room", [(2, 0), (4, 0), (9, 0), (32, 0), (9, 6000), (32, 6000)])
+def test_attn_tree(hip, nh, nkv, hd, P, win, most, room):
     """Trees of 1 to `most` nodes over 0 to 700 keys around the borders of pages and tiles, sequences without rows, rows behind the
     last sequence."""
     rng = np.random.default_rng(most + P)
     before = [0, 0, 1, 15, 16, 31, 33, 63, 64, 65, 127, 129, 300, 700]
     q = [1, most] + rng.integers(1, most + 1, len(before) - 3).tolist() + [0]
-    b = Trees(hip, q, [k + m for k, m in zip(before, q)], nh, nkv, hd, 16, 1, P=P, seed=most, sink=P == 70, gate=P == 70, extra=3, big=True).upload()
+    b = Trees(hip, q, [k + m for k, m in zip(before, q)], nh, nkv, hd, 16, 1, P=P, seed=most, sink=P == 70, gate=P == 70, extra=3, big=True, room=room).upload()
     b.launch(win)
     b.check(b.get(), win)
 
@@ -486,24 +490,28 @@ def test_attn_tree_many_sequences(hip, nseq, P):
     b.check(b.get(), rows=sorted(rng.integers(0, b.t, 300).tolist()))
 
 
-def test_attn_tree_lines_give_the_line_s_bits(hip):
-    """Trees without branches: the masks say what the positions do."""
+def test_attn_tree_of_lines(hip):
+    """Trees without branches: the masks say what the positions do, as attn_paged has it (few rows: its bits)."""
     for q, P in (([1] * 9, 0), ([3, 1, 4], 70), ([20, 1, 17, 2, 32], 0), ([20, 1, 17, 2, 32], 130)):
         b = Trees(hip, q, [k + 40 * i for i, k in enumerate(q)], 8, 2, 128, 16, 1, P=P, seed=P, shape="line").upload()
         b.launch()
         got = b.get()
+        b.check(got)
         mask = b.b.pop("mask")
         Batch.launch(b)
-        np.testing.assert_array_equal(got, b.get())
+        if max(q) <= 8:
+            np.testing.assert_array_equal(got, b.get())
+        assert rel_l2(got, b.get()) <= 2.0 ** -20
         del mask
 
 
+@pytest.mark.parametrize("room", [0, 9000])
 @pytest.mark.parametrize("q", [[4, 1, 2], [40, 7, 60]])
-def test_attn_tree_masks_of_any_bits(hip, q):
+def test_attn_tree_masks_of_any_bits(hip, q, room):
     """The masks are taken as they are: rows that see nothing of the step, not even themselves; bits of rows behind them do not
     count. Without keys before the rows such a row is 0."""
     for P, before in ((0, 0), (0, 50), (20, 0)):
-        b = Trees(hip, q, [k + before for k in q], 8, 2, 64, 16, 2, P=P, seed=7)
+        b = Trees(hip, q, [k + before for k in q], 8, 2, 64, 16, 2, P=P, seed=7, room=room)
         rng = np.random.default_rng(before)
         b.mask = rng.integers(0, 2**32, b.mask.shape, dtype=np.uint64).astype(np.uint32)
         b.mask[::3] = 0
@@ -515,11 +523,11 @@ def test_attn_tree_masks_of_any_bits(hip, q):
 
 
 @pytest.mark.parametrize("bad", [np.nan, np.inf])
-@pytest.mark.parametrize("q", [[4, 3], [30, 40]])
-def test_attn_tree_non_finite(hip, bad, q):
+@pytest.mark.parametrize("q,room", [([4, 3], 0), ([30, 40], 0), ([30, 40], 9000)])
+def test_attn_tree_non_finite(hip, bad, q, room):
     """Keys and values that are not finite stay out of the rows whose masks do not name them."""
     for P in (0, 70):
-        b = Trees(hip, q, [k + 50 for k in q], 8, 2, 64, 16, 2, P=P, seed=3)
+        b = Trees(hip, q, [k + 50 for k in q], 8, 2, 64, 16, 2, P=P, seed=3, room=room)
         for s in range(len(q)):  # the last node's key and value: a leaf that no other row sees
             j = b.n[s] - 1
             row = b.tables[s][j // 16] * 16 + j % 16
@@ -534,11 +542,11 @@ def test_attn_tree_non_finite(hip, bad, q):
                 assert rel_l2(got[r, h], want[r, h]) <= 2.0 ** -23 * (14 + top[r, h]), (r, h)
 
 
-@pytest.mark.parametrize("q", [[3, 2], [60, 17]])
-def test_attn_tree_holes(hip, q):
+@pytest.mark.parametrize("q,room", [([3, 2], 0), ([60, 17], 0), ([60, 17], 9000)])
+def test_attn_tree_holes(hip, q, room):
     """Pages outside the pool hold no keys, in the context and under the tree."""
     for P in (0, 90):
-        b = Trees(hip, q, [k + 60 for k in q], 8, 1, 128, 16, 2, P=P, seed=5)
+        b = Trees(hip, q, [k + 60 for k in q], 8, 1, 128, 16, 2, P=P, seed=5, room=room)
         b.tables[0, 1], b.tables[1, 3], b.tables[0, 3] = -1, b.n_pages, 2**31 - 1
         if P:
             b.prefix[2] = -7
@@ -565,8 +573,8 @@ def test_attn_tree_offsets_past_32_bits(hip):
 
 def test_attn_tree_device_lengths_past_their_bounds(hip):
     """Lengths and row starts that say more than there is, and a sequence whose length does not hold its rows."""
-    for q in ([4, 3, 2], [40, 20, 30]):
-        b = Trees(hip, q, [k + 30 for k in q], 8, 2, 64, 16, 2, seed=4).upload()
+    for q, room in (([4, 3, 2], 0), ([40, 20, 30], 0), ([40, 20, 30], 9000)):
+        b = Trees(hip, q, [k + 30 for k in q], 8, 2, 64, 16, 2, seed=4, room=room).upload()
         b.launch()
         want = b.get()
         hip.htod(np.array([2**31 - 1, *b.n[1:]], np.int32), b.b["length"])
@@ -583,8 +591,8 @@ def test_attn_tree_two_graphs_and_contexts(hip):
     """Graphs of two shapes share the context's workspace; a second context runs the same at once."""
     other = S.HipBackend(0)
     try:
-        shapes = (([4] * 6, 0), ([60, 20], 100))
-        bs = [Trees(h, q, [k + 300 for k in q], 8, 2, 128, 16, 2, P=P, seed=1).upload() for h in (hip, other) for q, P in shapes]
+        shapes = (([4] * 6, 0, 0), ([60, 20], 100, 0), ([60, 20], 0, 9000))
+        bs = [Trees(h, q, [k + 300 for k in q], 8, 2, 128, 16, 2, P=P, seed=1, room=room).upload() for h in (hip, other) for q, P, room in shapes]
         for b in bs:
             b.launch()
         want = [b.get() for b in bs]
