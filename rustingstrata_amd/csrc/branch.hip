@@ -1,6 +1,8 @@
 // Sequences that go on from others (strata_kv_pages_fork) and rows of the caches moved from slot to slot (strata_kv_rows_move).
 #include "branch.h"
 
+#include <algorithm>
+
 namespace strata {
 
 // ---------------- forking, cutting and ending ----------------
@@ -13,11 +15,14 @@ namespace strata {
 // Pages that a changed sequence held go down by one each; those that nobody holds any more go on the stack, behind the pages
 // taken, in the order (sequence, place in its table) in which they are first met. That order comes from `claim`: the smallest
 // s * max_pages + j over a page's releases, so the stack does not depend on the order of atomics.
-// Four phases, each after all of the one before: the plan (a block; 4 sequences a thread) beside copies of the tables that others
-// go on from and cleared claims; the holders' counts; the pages that go; the stack and tables. Up to FORK_ONE sequences run them
-// in one block with a wave a sequence, more in four launches. Bound by latency: every phase is a chain of two or three trips to memory.
-constexpr int FORK_ONE = 16;
-enum { F_CHANGED = 1, F_OTHER = 2, F_TAKE = 4, F_COPY = 8, F_EMPTY = 16, F_LOST = 32 };
+// Phases, each after all of the one before: the plan (a block; 4 sequences a thread); copies of the tables that others go on from and
+// cleared claims; the holders' counts; the pages that go; the stack and tables. Where the tables have few entries one block of 1024
+// threads does them all over lists of the entries that are kept and let go, whatever sequence they belong to; else four launches, a wave
+// a sequence. Bound by latency: every phase is a chain of trips to memory. Beams, tables of 272 entries 12.3 us in one block, 15.9 in
+// four launches, 1344 15.7 and 17.2, 5376 34 and 20; cuts alone let few pages go (256 sequences after a step, 2560 entries: the end
+// of that step 19.8 and 23.6 us).
+constexpr long long FORK_ONE = 1 << 15, FORK_ONE_SRC = 1 << 11;
+enum { F_CHANGED = 1, F_OTHER = 2, F_TAKE = 4, F_COPY = 8 };
 
 struct ForkPlan {
     int flags, full, pg, fresh;  // pg: the page with the rem rows; fresh: its copy's
@@ -28,7 +33,7 @@ struct ForkScratch {
     ForkPlan* plan;               // [nseq]
     int* gone;                    // [nseq] pages that go back
     unsigned long long* claim;    // [n_pages]
-    int* snap;                    // [nseq][max_pages] the pages of src[s]
+    int* snap;                    // [nseq][max_pages] the pages of src[s]; of one block its lists
 };
 __host__ __device__ static inline ForkScratch fork_scratch(const PagesFork& a) {
     ForkScratch f;
@@ -41,7 +46,7 @@ __host__ __device__ static inline ForkScratch fork_scratch(const PagesFork& a) {
     return f;
 }
 size_t pages_fork_scratch_bytes(const PagesFork& a) {
-    return 64 + (sizeof(ForkPlan) + 4) * SERVE_MAX_SEQ + (size_t)a.n_pages * 8 + (a.src ? (size_t)a.nseq * a.max_pages * 4 : 0);
+    return 64 + (sizeof(ForkPlan) + 4) * SERVE_MAX_SEQ + (size_t)a.n_pages * 8 + std::max(a.src ? (size_t)a.nseq * a.max_pages * 4 : 0, (size_t)FORK_ONE * 12);
 }
 
 struct ForkSeq {
@@ -65,15 +70,36 @@ __device__ __forceinline__ bool in_pool(const PagesFork& a, int p) { return p >=
 __device__ __forceinline__ int shared_load(const int* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ unsigned long long shared_load(const unsigned long long* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
-// Phase 0a, a block of 1024 threads.
-__device__ void fork_plan(const PagesFork& a, const ForkScratch& f) {
-    __shared__ int heir[SERVE_MAX_SEQ], most[SERVE_MAX_SEQ], ws[16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// Exclusive sums of a value a thread over a block of 1024, and the total. ws: 16 words.
+__device__ __forceinline__ int fork_scan(int v, int& total, int* ws) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int inc = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(inc, o, 64);
+        if (lane >= o) inc += u;
+    }
+    __syncthreads();  // (ws is free)
+    if (lane == 63) ws[wave] = inc;
+    __syncthreads();
+    int at = inc - v;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < 16; w++) {
+        if (w < wave) at += ws[w];
+        total += ws[w];
+    }
+    return at;
+}
+
+// Phase 0a, a block of 1024 threads: thread i's sequences 4 i .. 4 i + 3 in p. heir, most: nseq words of LDS each; ws: 16.
+__device__ __forceinline__ void fork_plan(const PagesFork& a, ForkPlan (&p)[4], int& stack, int& used, int* heir, int* most, int* ws) {
+    const int tid = threadIdx.x;
     for (int s = tid; s < a.nseq; s += 1024) {
         heir[s] = INT32_MAX;
         most[s] = -1;
     }
-    const int stack = min(max(*a.n_free, 0), a.n_pages);
+    stack = min(max(*a.n_free, 0), a.n_pages);
     __syncthreads();
     ForkSeq q[4];
 #pragma unroll
@@ -85,7 +111,6 @@ __device__ void fork_plan(const PagesFork& a, const ForkScratch& f) {
         atomicMax(&most[q[i].src], q[i].k >> a.page_shift);
     }
     __syncthreads();
-    ForkPlan p[4];
     int need = 0, err = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -108,21 +133,7 @@ __device__ void fork_plan(const PagesFork& a, const ForkScratch& f) {
             need += !takes;
         }
     }
-    // the pages wanted before this thread's
-    int inc = need;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(inc, o, 64);
-        if (lane >= o) inc += u;
-    }
-    if (lane == 63) ws[wave] = inc;
-    __syncthreads();
-    int at = inc - need, total = 0;
-#pragma unroll
-    for (int w = 0; w < 16; w++) {
-        if (w < wave) at += ws[w];
-        total += ws[w];
-    }
+    int total, at = fork_scan(need, total, ws);  // the pages wanted before this thread's
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int s = 4 * tid + i;
@@ -143,14 +154,10 @@ __device__ void fork_plan(const PagesFork& a, const ForkScratch& f) {
                 p[i].flags = p[i].flags & F_OTHER ? F_CHANGED | F_OTHER : 0;
             }
         }
-        f.plan[s] = p[i];
     }
     err = __syncthreads_count(err & 1) + 2 * __syncthreads_count(err & 2) + 4 * __syncthreads_count(err & 4);  // (at most 4)
-    if (tid == 0) {
-        f.head[0] = stack;
-        f.head[1] = min(total, stack);
-        if (a.err && err) atomicAdd(a.err, err);
-    }
+    used = min(total, stack);
+    if (tid == 0 && a.err && err) atomicAdd(a.err, err);
 }
 // Phase 0b, a wave: the pages of the sequence that s goes on from, and the claims of those that it may let go.
 __device__ __forceinline__ void fork_copy(const PagesFork& a, const ForkScratch& f, int s) {
@@ -202,6 +209,15 @@ __device__ __forceinline__ void fork_gone(const PagesFork& a, const ForkScratch&
     }
     if (lane == 0) f.gone[s] = n;
 }
+// What the caller reads of sequence s, and its copied page's place.
+__device__ __forceinline__ void fork_report(const PagesFork& a, int s, const ForkPlan& p) {
+    if (p.flags & F_COPY) a.tables[(uint64_t)s * a.max_pages + p.full] = p.fresh;  // (a page from the stack has no other holder: refs 0)
+    const bool copy = (p.flags & F_COPY) && in_pool(a, p.fresh);
+    a.runs[3 * s] = copy ? p.pg << a.page_shift : 0;
+    a.runs[3 * s + 1] = copy ? p.fresh << a.page_shift : 0;
+    a.runs[3 * s + 2] = copy ? p.rem : 0;
+    a.len_out[s] = p.len;
+}
 // Phase 3, a wave: the stack, the table and what the caller reads. (It reads no input that an output may lie over.)
 __device__ __forceinline__ void fork_apply(const PagesFork& a, const ForkScratch& f, int s) {
     const int lane = threadIdx.x & 63;
@@ -236,14 +252,9 @@ __device__ __forceinline__ void fork_apply(const PagesFork& a, const ForkScratch
         // (the same lane wrote what it read above, or a place that nothing above reads)
         if (p.flags & F_OTHER)
             for (int j = lane; j < fork_kept(p); j += 64) a.tables[row + j] = f.snap[row + j];
-        if (lane == 0 && (p.flags & F_COPY)) a.tables[row + p.full] = p.fresh;  // (a page from the stack has no other holder: refs 0)
     }
     if (lane == 0) {
-        const bool copy = (p.flags & F_COPY) && in_pool(a, p.fresh);
-        a.runs[3 * s] = copy ? p.pg << a.page_shift : 0;
-        a.runs[3 * s + 1] = copy ? p.fresh << a.page_shift : 0;
-        a.runs[3 * s + 2] = copy ? p.rem : 0;
-        a.len_out[s] = p.len;
+        fork_report(a, s, p);
         if (s == 0) {
             *a.n_free_out = min(stack - used + all, a.n_pages);
             if (a.err && stack - used + all > a.n_pages) atomicAdd(a.err, 1);
@@ -251,22 +262,111 @@ __device__ __forceinline__ void fork_apply(const PagesFork& a, const ForkScratch
     }
 }
 
+// The last sequence with v[s] <= x.
+__device__ __forceinline__ int fork_find(const int* v, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (v[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
 __global__ __launch_bounds__(1024) void pages_fork_one_kernel(PagesFork a) {
+    __shared__ int heir[SERVE_MAX_SEQ], most[SERVE_MAX_SEQ], first[SERVE_MAX_SEQ], srcs[SERVE_MAX_SEQ], ws[16];
     const ForkScratch f = fork_scratch(a);
-    const int s = threadIdx.x >> 6;
-    fork_plan(a, f);
-    if (s < a.nseq) fork_copy(a, f, s);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    ForkPlan p[4];
+    int stack, used;
+    fork_plan(a, p, stack, used, heir, most, ws);
+    // the lists: entry i of those kept is the first ones of another's table, entry i of those let go at place `first` on
+    int *kept0 = heir, *gone0 = most, nkept = 0, ngone = 0, n_kept, n_gone;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int s = 4 * tid + i;
+        if (s >= a.nseq || !(p[i].flags & F_CHANGED)) continue;
+        if (p[i].flags & F_OTHER) nkept += fork_kept(p[i]);
+        ngone += max(pages_of(a, p[i].held) - fork_from(p[i]), 0);
+    }
+    int kat = fork_scan(nkept, n_kept, ws), gat = fork_scan(ngone, n_gone, ws);  // (its barriers: heir and most have been read)
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int s = 4 * tid + i;
+        if (s >= a.nseq) continue;
+        kept0[s] = kat;
+        gone0[s] = gat;
+        first[s] = fork_from(p[i]);
+        const int u = a.src ? a.src[s] : s;
+        srcs[s] = u;
+        if (!(p[i].flags & F_CHANGED)) continue;
+        if (p[i].flags & F_OTHER) kat += fork_kept(p[i]);
+        gat += max(pages_of(a, p[i].held) - fork_from(p[i]), 0);
+    }
     __syncthreads();
-    if (s < a.nseq) fork_count(a, f, s);
+    int *keep_page = f.snap, *keep_cell = keep_page + FORK_ONE, *gone_page = keep_cell + FORK_ONE;
+    for (int i = tid; i < n_kept; i += 1024) {
+        const int s = fork_find(kept0, a.nseq, i), j = i - kept0[s], pg = a.tables[(uint64_t)srcs[s] * a.max_pages + j];
+        keep_page[i] = pg;
+        keep_cell[i] = s * a.max_pages + j;
+        if (in_pool(a, pg)) atomicAdd(a.refs + pg, 1);
+    }
+    for (int i = tid; i < n_gone; i += 1024) {
+        const int s = fork_find(gone0, a.nseq, i), j = first[s] + i - gone0[s], pg = a.tables[(uint64_t)s * a.max_pages + j];
+        gone_page[i] = pg;
+        if (in_pool(a, pg)) __hip_atomic_store(f.claim + pg, ~0ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
     __syncthreads();
-    if (s < a.nseq) fork_gone(a, f, s);
+    for (int i = tid; i < n_gone; i += 1024) {
+        const int pg = gone_page[i];
+        if (in_pool(a, pg)) {
+            atomicSub(a.refs + pg, 1);
+            atomicMin(f.claim + pg, (unsigned long long)i);
+        }
+    }
     __syncthreads();
-    if (s < a.nseq) fork_apply(a, f, s);
+    int at = stack - used;  // the next place on the stack
+    for (int i0 = 0; i0 < n_gone; i0 += 1024) {
+        const int i = i0 + tid, pg = i < n_gone ? gone_page[i] : -1;
+        const bool goes = fork_goes(a, f, i, pg);
+        const uint64_t b = __ballot(goes);
+        __syncthreads();  // (ws is free)
+        if (lane == 0) ws[wave] = __popcll(b);
+        __syncthreads();
+        int to = at + __popcll(b & ((1ull << lane) - 1));
+#pragma unroll
+        for (int w = 0; w < 16; w++) {
+            if (w < wave) to += ws[w];
+            at += ws[w];
+        }
+        if (goes) {
+            if (to < a.n_pages) a.free_pages[to] = pg;
+            __hip_atomic_store(a.refs + pg, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    }
+    // (all table entries that others go on from, and all that go, have been read)
+    for (int i = tid; i < n_kept; i += 1024) a.tables[keep_cell[i]] = keep_page[i];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (4 * tid + i < a.nseq) fork_report(a, 4 * tid + i, p[i]);
+    if (tid == 0) {
+        *a.n_free_out = min(at, a.n_pages);
+        if (a.err && at > a.n_pages) atomicAdd(a.err, 1);
+    }
 }
 __global__ __launch_bounds__(1024) void pages_fork_plan_kernel(PagesFork a) {
     const ForkScratch f = fork_scratch(a);
     if (blockIdx.x == 0) {
-        fork_plan(a, f);
+        __shared__ int heir[SERVE_MAX_SEQ], most[SERVE_MAX_SEQ], ws[16];
+        ForkPlan p[4];
+        int stack, used;
+        fork_plan(a, p, stack, used, heir, most, ws);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (4 * (int)threadIdx.x + i < a.nseq) f.plan[4 * threadIdx.x + i] = p[i];
+        if (threadIdx.x == 0) {
+            f.head[0] = stack;
+            f.head[1] = used;
+        }
     } else {
         const int s = (blockIdx.x - 1) * 16 + (threadIdx.x >> 6);
         if (s < a.nseq) fork_copy(a, f, s);
@@ -284,7 +384,7 @@ __global__ __launch_bounds__(256) void pages_fork_kernel(PagesFork a) {
 
 hipError_t launch_pages_fork(const PagesFork& a, hipStream_t s) {
     if (!a.nseq) return hipSuccess;
-    if (a.nseq <= FORK_ONE) {
+    if ((long long)a.nseq * a.max_pages <= (a.src ? FORK_ONE_SRC : FORK_ONE)) {
         pages_fork_one_kernel<<<dim3(1), dim3(1024), 0, s>>>(a);
     } else {
         const dim3 grid((unsigned)(a.nseq + 3) / 4);
@@ -297,19 +397,20 @@ hipError_t launch_pages_fork(const PagesFork& a, hipStream_t s) {
 }
 
 // ---------------- rows of the caches ----------------
-// A block per group and cache takes the group's runs (from, to, n: n consecutive rows) in batches of rows: all of a batch are read
-// before any of it is written, and batches follow each other, so rows that move towards the front over rows already read come out
-// right (a confirmed path closing up). A row's 16-byte chunks go to `tpr` threads, a power of two from 8 to 256; MOVE_U rows a
-// thread are in flight.
+// A block takes a group's runs (from, to, n: n consecutive rows) in `cpb` caches, their rows one cache behind the other, in batches:
+// all of a batch are read before any of it is written, and batches follow each other, so rows that move towards the front over rows
+// already read come out right (a confirmed path closing up). A row's 16-byte chunks go to `tpr` threads, a power of two from 8 to
+// 256; MOVE_U rows a thread are in flight. Copies of pages are bound by their bytes (beams of 32 requests, 104 MB read and written
+// 23 us, 4.5 TB/s), a few rows a group by the chain of a block (the runs, their sums, the rows), hence several caches a block there.
 constexpr int MOVE_MAX_RUNS = 256, MOVE_U = 8;
 
-__global__ __launch_bounds__(256) void rows_move_kernel(RowsMove a, int tpr_shift) {
+__global__ __launch_bounds__(256) void rows_move_kernel(RowsMove a, int tpr_shift, int cpb) {
     typedef unsigned v4u __attribute__((ext_vector_type(4)));
-    __shared__ int from[MOVE_MAX_RUNS], to[MOVE_MAX_RUNS], rf[256], rt[256];
+    __shared__ int from[MOVE_MAX_RUNS], to[MOVE_MAX_RUNS];
+    __shared__ uint64_t rs[256], rd[256];
     __shared__ long long start[MOVE_MAX_RUNS], ws[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int g = blockIdx.x / a.n_caches, c = blockIdx.x % a.n_caches;
-    const uint64_t base = sload(a.caches + c);
+    const int parts = (a.n_caches + cpb - 1) / cpb, g = blockIdx.x / parts, c0 = blockIdx.x % parts * cpb, nc = min(cpb, a.n_caches - c0);
     long long n = 0;
     if (tid < a.per) {
         const int* r = a.runs + ((uint64_t)g * a.per + tid) * 3;
@@ -320,47 +421,49 @@ __global__ __launch_bounds__(256) void rows_move_kernel(RowsMove a, int tpr_shif
         if (n < 0 || r[0] < 0 || r[1] < 0 || (uint64_t)(r[0] + n) > a.n_slots || (uint64_t)(r[1] + n) > a.n_slots) n = 0;
     }
     long long inc = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
+    for (int o = 1; o < 64 && o < a.per; o <<= 1) {
         const long long u = __shfl_up(inc, o, 64);
         if (lane >= o) inc += u;
     }
-    if (lane == 63) ws[wave] = inc;
+    if (lane == min(63, a.per - 1 - 64 * wave)) ws[wave] = inc;
+    if (lane == 0 && 64 * wave >= a.per) ws[wave] = 0;
     __syncthreads();
     for (int w = 0; w < wave; w++) inc += ws[w];
-    const long long total = ws[0] + ws[1] + ws[2] + ws[3];
+    const long long rows = ws[0] + ws[1] + ws[2] + ws[3], total = rows * nc;
     if (!total) return;
     start[tid] = inc - n;
     __syncthreads();
-    const int tpr = 1 << tpr_shift, rows = 256 >> tpr_shift, batch = rows * MOVE_U, row = tid >> tpr_shift;
+    const int tpr = 1 << tpr_shift, step = 256 >> tpr_shift, batch = step * MOVE_U, row = tid >> tpr_shift;
     const uint64_t chunks = a.row_bytes / 16;
     for (long long b = 0; b < total; b += batch) {
         const int m = (int)min(total - b, (long long)batch);
-        if (tid < m) {  // row b + tid: the last run that begins there or before
+        if (tid < m) {  // row x of cache c: of the last run that begins there or before
+            const long long c = (b + tid) / rows, x = b + tid - c * rows;
             int lo = 0, hi = a.per;
             while (hi - lo > 1) {
                 const int mid = (lo + hi) >> 1;
-                if (start[mid] <= b + tid) lo = mid;
+                if (start[mid] <= x) lo = mid;
                 else hi = mid;
             }
-            const int i = (int)(b + tid - start[lo]);
-            rf[tid] = from[lo] + i;
-            rt[tid] = to[lo] + i;
+            const uint64_t base = a.caches[c0 + c];
+            const int i = (int)(x - start[lo]);
+            rs[tid] = base + (uint64_t)(from[lo] + i) * a.row_bytes;
+            rd[tid] = base + (uint64_t)(to[lo] + i) * a.row_bytes;
         }
         __syncthreads();
         for (uint64_t col = tid & (tpr - 1); col - (tid & (tpr - 1)) < chunks; col += tpr) {
             v4u v[MOVE_U];
 #pragma unroll
             for (int u = 0; u < MOVE_U; u++) {
-                const int i = u * rows + row;
-                if (i < m && col < chunks) v[u] = *gptr<v4u>(base + (uint64_t)rf[i] * a.row_bytes + 16 * col);
+                const int i = u * step + row;
+                if (i < m && col < chunks) v[u] = *gptr<v4u>(rs[i] + 16 * col);
             }
             wait_loads();
             __syncthreads();
 #pragma unroll
             for (int u = 0; u < MOVE_U; u++) {
-                const int i = u * rows + row;
-                if (i < m && col < chunks) *(v4u*)(base + (uint64_t)rt[i] * a.row_bytes + 16 * col) = v[u];
+                const int i = u * step + row;
+                if (i < m && col < chunks) *(v4u*)(rd[i] + 16 * col) = v[u];
             }
         }
         __syncthreads();
@@ -371,7 +474,9 @@ hipError_t launch_rows_move(const RowsMove& a, hipStream_t s) {
     if (!a.groups || !a.n_caches || !a.per) return hipSuccess;
     int shift = 3;
     while (shift < 8 && (16ull << shift) < a.row_bytes) shift++;
-    rows_move_kernel<<<dim3((unsigned)((uint64_t)a.groups * a.n_caches)), dim3(256), 0, s>>>(a, shift);
+    // one cache a block where a group is one run (pages' rows); else caches as leave four blocks a CU
+    const int cpb = a.per == 1 ? 1 : (int)std::max<long long>(1, std::min<long long>(8, (long long)a.groups * a.n_caches / 1024));
+    rows_move_kernel<<<dim3((unsigned)((uint64_t)a.groups * ((a.n_caches + cpb - 1) / cpb))), dim3(256), 0, s>>>(a, shift, cpb);
     return hipGetLastError();
 }
 
