@@ -1538,7 +1538,7 @@ __global__ __launch_bounds__(256) void attn_paged_join_kernel(PagedAttn a, Paged
     merge_block<TREE, HD, DIRECT, MW>(a, w, b - jblocks, per);
 }
 
-constexpr long long ROW_TILE_STEPS = 8192;
+constexpr long long row_tile_steps(int hd) { return hd == 128 ? 8192 : 5120; }
 static int div_up(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 // Tiles of the long sequences at most: each of them has more than dr / G rows.
@@ -1558,11 +1558,12 @@ static PagedWs plan(const PagedAttn& a, uint8_t* at, size_t* end) {
     // joins take 30 us before anything else, but row tiles read their keys once each. The steps of 16 rows and 64 keys that the call's
     // bounds allow decide (us as row tiles / as tiles, 32 heads over 4 of 128): one tree of 16 over 1000 keys 13 / 31, 16 of 16 over 500
     // (4096 steps) 29 / 40, 16 of 8 over 2000 and 8 of 64 over 500 (8192) 39 / 49 and 42 / 45, 16 of 16 over 2000 (16384) 58 / 53, 8 of 8 over 8000
-    // 87 / 61
+    // 87 / 61; 16 over 8 of 64: 4 of 40 over 2000 (5120) 27 / 36, 8 of 40 over 2000 (10240) 43 / 40. Up to 32 rows the other form is two column
+    // tiles a wave: 8 of 4 over 500 13.3 / 16.5, 32 of 4 over 1000 (4096) 30 / 33; heads of 64: 24 of 13 over 300 (1920) 22 / 26, over 700 (4224) 31 / 26
     w.rt = 1;
-    if (a.mask && a.max_q <= 32 * a.words && most_rows > 32) {
+    if (a.mask && a.max_q <= 32 * a.words && most_rows > 16) {
         const int rt = div_up(most_rows, 16);
-        if ((long long)a.nseq * a.nkv * rt * div_up((long long)a.max_pages << a.page_shift, 64) <= ROW_TILE_STEPS) w.rt = rt;
+        if ((long long)a.nseq * a.nkv * rt * div_up((long long)a.max_pages << a.page_shift, 64) <= row_tile_steps(a.hd) / (most_rows > 32 ? 1 : 2)) w.rt = rt;
     }
     const long long nseq = (long long)a.nseq * w.rt;
     w.nct = w.rt == 1 && most_rows > 16 && most_rows <= 32 ? 2 : 1;
