@@ -15,12 +15,12 @@ namespace strata {
 // Pages that a changed sequence held go down by one each; those that nobody holds any more go on the stack, behind the pages
 // taken, in the order (sequence, place in its table) in which they are first met. That order comes from `claim`: the smallest
 // s * max_pages + j over a page's releases, so the stack does not depend on the order of atomics.
-// Phases, each after all of the one before: the plan (a block; 4 sequences a thread); copies of the tables that others go on from and
+// Phases, each after all of the one before: the plan (a block); copies of the tables that others go on from and
 // cleared claims; the holders' counts; the pages that go; the stack and tables. Where the tables have few entries one block of 1024
 // threads does them all over lists of the entries that are kept and let go, whatever sequence they belong to; else four launches, a wave
-// a sequence. Bound by latency: every phase is a chain of trips to memory. Beams, tables of 272 entries 12.3 us in one block, 15.9 in
-// four launches, 1344 15.7 and 17.2, 5376 34 and 20; cuts alone let few pages go (256 sequences after a step, 2560 entries: the end
-// of that step 19.8 and 23.6 us).
+// a sequence. Bound by latency: every phase is a chain of trips to memory. Beams, tables of 272 entries 8.8 us in one block and 13.0 in
+// four launches, 1344 11.0 and 13.8, 5376 30 and 16.6; cuts alone let few pages go (the end of a step of 256 trees, 3072 entries, 16.1 us
+// and 20.9).
 constexpr long long FORK_ONE = 1 << 15, FORK_ONE_SRC = 1 << 11;
 enum { F_CHANGED = 1, F_OTHER = 2, F_TAKE = 4, F_COPY = 8 };
 
@@ -92,7 +92,8 @@ __device__ __forceinline__ int fork_scan(int v, int& total, int* ws) {
     return at;
 }
 
-// Phase 0a, a block of 1024 threads: thread i's sequences 4 i .. 4 i + 3 in p. heir, most: nseq words of LDS each; ws: 16.
+// Phase 0a, a block of 1024 threads: sequences tid + 1024 i of the thread in p[i] (up to 1024 sequences one a thread: four in a row wait
+// for each other's loads, 256 cut sequences 12.3 us for 8.5). heir, most: nseq words of LDS each; ws: 16.
 __device__ __forceinline__ void fork_plan(const PagesFork& a, ForkPlan (&p)[4], int& stack, int& used, int* heir, int* most, int* ws) {
     const int tid = threadIdx.x;
     for (int s = tid; s < a.nseq; s += 1024) {
@@ -104,17 +105,17 @@ __device__ __forceinline__ void fork_plan(const PagesFork& a, ForkPlan (&p)[4], 
     ForkSeq q[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const int s = 4 * tid + i;
+        const int s = tid + 1024 * i;
         if (s >= a.nseq) continue;
         q[i] = fork_seq(a, s);
         atomicMin(&heir[q[i].src], q[i].src == s ? -1 : s);
         atomicMax(&most[q[i].src], q[i].k >> a.page_shift);
     }
     __syncthreads();
-    int need = 0, err = 0;
+    int need[4] = {0, 0, 0, 0}, err = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const int s = 4 * tid + i;
+        const int s = tid + 1024 * i;
         p[i] = ForkPlan{0, 0, -1, -1, 0, 0, 0, 0};
         if (s >= a.nseq) continue;
         const int full = q[i].k >> a.page_shift, rem = q[i].k & ((1 << a.page_shift) - 1), u = q[i].src;
@@ -130,33 +131,30 @@ __device__ __forceinline__ void fork_plan(const PagesFork& a, ForkPlan (&p)[4], 
             const bool known = in_pool(a, p[i].pg);
             const bool takes = !known || (heir[u] == (u == s ? -1 : s) && most[u] <= full && a.refs[p[i].pg] == 0);
             p[i].flags |= takes ? F_TAKE : F_COPY;
-            need += !takes;
+            need[i] = !takes;
         }
     }
-    int total, at = fork_scan(need, total, ws);  // the pages wanted before this thread's
+    int wanted = 0;  // pages, by the sequences before
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const int s = 4 * tid + i;
-        if (s >= a.nseq) continue;
-        if (p[i].flags & F_CHANGED) {
-            bool refused = false;
-            if (p[i].flags & F_COPY) {
-                refused = at >= stack;
-                if (!refused) p[i].fresh = a.free_pages[stack - 1 - at];
-                at++;
-            }
-            if (!refused) {
-                p[i].len = q[i].k;
-            } else {  // no page: a cut is not made, a sequence that was to become another is empty
-                err++;
-                p[i].full = p[i].rem = 0;
-                if (p[i].flags & F_OTHER) p[i].len = 0;
-                p[i].flags = p[i].flags & F_OTHER ? F_CHANGED | F_OTHER : 0;
-            }
+        const int s = tid + 1024 * i;
+        if (1024 * i >= a.nseq) break;
+        int total, at = wanted + fork_scan(need[i], total, ws);
+        wanted += total;
+        if (s >= a.nseq || !(p[i].flags & F_CHANGED)) continue;
+        const bool refused = (p[i].flags & F_COPY) && at >= stack;
+        if (!refused) {
+            if (p[i].flags & F_COPY) p[i].fresh = a.free_pages[stack - 1 - at];
+            p[i].len = q[i].k;
+        } else {  // no page: a cut is not made, a sequence that was to become another is empty
+            err++;
+            p[i].full = p[i].rem = 0;
+            if (p[i].flags & F_OTHER) p[i].len = 0;
+            p[i].flags = p[i].flags & F_OTHER ? F_CHANGED | F_OTHER : 0;
         }
     }
     err = __syncthreads_count(err & 1) + 2 * __syncthreads_count(err & 2) + 4 * __syncthreads_count(err & 4);  // (at most 4)
-    used = min(total, stack);
+    used = min(wanted, stack);
     if (tid == 0 && a.err && err) atomicAdd(a.err, err);
 }
 // Phase 0b, a wave: the pages of the sequence that s goes on from, and the claims of those that it may let go.
@@ -280,28 +278,28 @@ __global__ __launch_bounds__(1024) void pages_fork_one_kernel(PagesFork a) {
     int stack, used;
     fork_plan(a, p, stack, used, heir, most, ws);
     // the lists: entry i of those kept is the first ones of another's table, entry i of those let go at place `first` on
-    int *kept0 = heir, *gone0 = most, nkept = 0, ngone = 0, n_kept, n_gone;
+    int *kept0 = heir, *gone0 = most;
+    unsigned sums = 0;  // of the sequences before: those kept in the upper half, those let go in the lower one (up to FORK_ONE each)
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const int s = 4 * tid + i;
-        if (s >= a.nseq || !(p[i].flags & F_CHANGED)) continue;
-        if (p[i].flags & F_OTHER) nkept += fork_kept(p[i]);
-        ngone += max(pages_of(a, p[i].held) - fork_from(p[i]), 0);
+        const int s = tid + 1024 * i;
+        if (1024 * i >= a.nseq) break;
+        unsigned n = 0;
+        if (s < a.nseq && (p[i].flags & F_CHANGED)) {
+            n = max(pages_of(a, p[i].held) - fork_from(p[i]), 0);
+            if (p[i].flags & F_OTHER) n += (unsigned)fork_kept(p[i]) << 16;
+        }
+        int total;
+        const unsigned at = sums + (unsigned)fork_scan((int)n, total, ws);  // (its barriers: heir and most have been read)
+        sums += (unsigned)total;
+        if (s < a.nseq) {
+            kept0[s] = at >> 16;
+            gone0[s] = at & 0xFFFF;
+            first[s] = fork_from(p[i]);
+            srcs[s] = a.src ? a.src[s] : s;
+        }
     }
-    int kat = fork_scan(nkept, n_kept, ws), gat = fork_scan(ngone, n_gone, ws);  // (its barriers: heir and most have been read)
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int s = 4 * tid + i;
-        if (s >= a.nseq) continue;
-        kept0[s] = kat;
-        gone0[s] = gat;
-        first[s] = fork_from(p[i]);
-        const int u = a.src ? a.src[s] : s;
-        srcs[s] = u;
-        if (!(p[i].flags & F_CHANGED)) continue;
-        if (p[i].flags & F_OTHER) kat += fork_kept(p[i]);
-        gat += max(pages_of(a, p[i].held) - fork_from(p[i]), 0);
-    }
+    const int n_kept = sums >> 16, n_gone = sums & 0xFFFF;
     __syncthreads();
     int *keep_page = f.snap, *keep_cell = keep_page + FORK_ONE, *gone_page = keep_cell + FORK_ONE;
     for (int i = tid; i < n_kept; i += 1024) {
@@ -347,7 +345,7 @@ __global__ __launch_bounds__(1024) void pages_fork_one_kernel(PagesFork a) {
     for (int i = tid; i < n_kept; i += 1024) a.tables[keep_cell[i]] = keep_page[i];
 #pragma unroll
     for (int i = 0; i < 4; i++)
-        if (4 * tid + i < a.nseq) fork_report(a, 4 * tid + i, p[i]);
+        if (tid + 1024 * i < a.nseq) fork_report(a, tid + 1024 * i, p[i]);
     if (tid == 0) {
         *a.n_free_out = min(at, a.n_pages);
         if (a.err && at > a.n_pages) atomicAdd(a.err, 1);
@@ -362,7 +360,7 @@ __global__ __launch_bounds__(1024) void pages_fork_plan_kernel(PagesFork a) {
         fork_plan(a, p, stack, used, heir, most, ws);
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            if (4 * (int)threadIdx.x + i < a.nseq) f.plan[4 * threadIdx.x + i] = p[i];
+            if ((int)threadIdx.x + 1024 * i < a.nseq) f.plan[threadIdx.x + 1024 * i] = p[i];
         if (threadIdx.x == 0) {
             f.head[0] = stack;
             f.head[1] = used;
@@ -400,8 +398,9 @@ hipError_t launch_pages_fork(const PagesFork& a, hipStream_t s) {
 // A block takes a group's runs (from, to, n: n consecutive rows) in `cpb` caches, their rows one cache behind the other, in batches:
 // all of a batch are read before any of it is written, and batches follow each other, so rows that move towards the front over rows
 // already read come out right (a confirmed path closing up). A row's 16-byte chunks go to `tpr` threads, a power of two from 8 to
-// 256; MOVE_U rows a thread are in flight. Copies of pages are bound by their bytes (beams of 32 requests, 104 MB read and written
-// 23 us, 4.5 TB/s), a few rows a group by the chain of a block (the runs, their sums, the rows), hence several caches a block there.
+// 256; MOVE_U rows a thread are in flight. Copies of pages are bound by their bytes (256 groups of 32 rows of 1 KB in 96 caches 311 us,
+// 5.2 TB/s), a few rows a group by the chain of a block (the runs, their sums, the rows), hence several caches a block there (256
+// confirmed paths in 24 caches 12.8 us with one, 5.6 with six).
 constexpr int MOVE_MAX_RUNS = 256, MOVE_U = 8;
 
 __global__ __launch_bounds__(256) void rows_move_kernel(RowsMove a, int tpr_shift, int cpb) {
