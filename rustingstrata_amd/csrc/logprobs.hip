@@ -3,16 +3,15 @@
 //   logp(v) = (x_v - M) - ln S,   entropy = ln S - W / S,   rank(v) = 1 + the tokens ordered before v,
 // tokens ordered as argmax_key.h orders them (by value, the first of equals).
 //
-// One pass over the logits, bound by their bytes: 1001 rows of 151936, a given token and 20 alternatives 135 us, 4.5 TB/s (the sums alone
-// 117), 2000 rows 239 (5.1). A thread keeps its own running maximum and the two sums, in f32, rescaled when a tile of 16 of its
-// values brings a larger maximum; a tile's terms are added as a tree. The K likeliest: a wave keeps a list in LDS of keys (value and
-// index in 64 bits) above `thr`, below which no key is among the block's K best. The first tile starts from a bound that K of its values
-// reach: of each wave's lanes' maxima the largest K / 4 (found bit by bit with ballots), of those the least. After 1, 2, 4, ..
+// One pass over the logits, bound by their bytes: 1001 rows of 151936, a given token and 20 alternatives 122 us, 5.0 TB/s. A thread keeps
+// its own running maximum and the two sums, in f32, rescaled when a tile of 16 of its values brings a larger maximum; a tile's
+// terms are added as a tree. The K likeliest: a wave keeps a list in LDS of keys (value and index in 64 bits) above `thr`, below
+// which no key is among the block's K best. The first tile starts from a bound that K of its values reach: of each wave's lanes'
+// maxima the largest K / 4 (found bit by bit with ballots; its upper 18 bits are bound enough), of those the least. After 1, 2, 4, ..
 // tiles the waves agree on the K best of all their lists, so that of a row's 37 tiles about a third bring a wave a candidate; a
-// wave's list of its own K best alone let 30 of them through (1001 rows 200 us, with the agreement 123). A tile without
-// one costs a comparison of the lane's maximum.
-// A block takes a row where there are many, else a part of one, and a second launch joins the parts: one row 16 us, the chain of a
-// tile's loads, its bound and its list (9), then the join's (6).
+// wave's list of its own K best alone let 30 of them through. A tile without one costs a comparison of the lane's maximum.
+// A block takes a row where there are many, else a part of one, and a second launch joins the parts: one row 15 us replayed, the
+// chain of a tile's loads, its bound and its list (9), then the join's (5).
 #include "argmax_key.h"
 #include "attn_dev.h"
 #include "branch.h"
@@ -350,9 +349,9 @@ __global__ __launch_bounds__(LG_T, 4) void logprobs_kernel(Logprobs a, LgScratch
         if constexpr (TOP) {
             if (t == t0) {  // of each wave's lanes' maxima the largest K / 4: the least of those is a bound that K values reach
                 const uint32_t o = order(mx);
-                auto reached = [&](int k) {  // the largest key that k of the wave's lanes reach
+                auto reached = [&](int k) {  // the largest key that k of the wave's lanes reach (its upper bits)
                     uint32_t bound = 0;
-                    for (int b = 31; b >= 0; b--) {
+                    for (int b = 31; b >= 14; b--) {
                         const uint32_t c = bound | (1u << b);
                         if (__popcll(__ballot(o >= c)) >= k) bound = c;
                     }
@@ -461,7 +460,7 @@ __global__ __launch_bounds__(LG_T) void logprobs_join_kernel(Logprobs a, LgScrat
 }
 
 // Tiles of a row (one more where the rows do not begin at a 16-byte border), and the parts of one: blocks for four a CU, as many as run
-// at once (1001 rows in one part each 135 us, in two 165).
+// at once (1001 rows in one part each 122 us, in two 165).
 static int lg_tiles(const Logprobs& a) { return (int)(((long long)a.n + 3 + LG_TILE - 1) / LG_TILE); }
 static int lg_parts(const Logprobs& a) { return (int)std::max(1, std::min<int>(lg_tiles(a), 1024 / a.rows)); }
 size_t logprobs_scratch_bytes(const Logprobs& a) {
