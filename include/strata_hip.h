@@ -462,7 +462,7 @@ int strata_tree_accept(strata_ctx* ctx, uint64_t nseq, uint64_t q_start, uint64_
 int strata_kv_pages_fork(strata_ctx* ctx, uint64_t nseq, uint64_t src, uint64_t keep, uint64_t len, uint64_t tables,
                          uint64_t max_pages, uint64_t page, uint64_t free_pages, uint64_t n_pages, uint64_t n_free, uint64_t refs,
                          uint64_t len_out, uint64_t n_free_out, uint64_t runs, uint64_t err);
-/* Rows of n_caches caches (device uint64 addresses, 16-byte aligned; the K and V caches of all layers) of row_bytes bytes (a
+/* Rows of n_caches caches (device uint64 addresses, 16-byte aligned, each once; the K and V caches of all layers) of row_bytes bytes (a
  * multiple of 16) from slot to slot: `groups` groups of `per` (1 to 256) runs (from, to, rows) of consecutive rows, device int32. A
  * group's runs are made in order; no run reads a row that the same or an earlier run of its group has written, and no group one that
  * another group writes. A run with a row outside 0 .. n_slots - 1, or of no rows, is left out. */

@@ -1,4 +1,4 @@
-// Device pieces that the attention kernels share (attn.hip: one sequence's contiguous cache; attn_paged.hip: a batch over
+// Device pieces that the attention kernels share (attn.hip: one sequence's contiguous cache; attn_paged.h: a batch over
 // pages): fragment types, wave reductions, the softmax's exp2, the f16 splits of queries and weights.
 #pragma once
 #include "xlane.h"

@@ -42,7 +42,8 @@ struct PagedWs {
     int* plan;     // long sequences (null: none): PlanHead, then a Tile each
     int* drows;    // with a plan and a prefix: the rows of decode sequences, one sequence's behind the other's
     int* dstart;   // and where sequence s's begin in that list
-    int4* cut;     // [tblocks] KV head and tile that block b's run cuts, and the last block of its pieces (below 0: none)
+    int4* cut;     // [tblocks] KV head and tile that block b's run cuts, and the last block of its pieces (below 0: none); TREE: KV
+                   // head, the tile's first row, that last block, the tile's rows
     float2* tml;   // [2 tblocks][128]: the pieces of tiles that more than one block computes
     float* tacc;   // [2 tblocks][128][hd]
     int direct;    // a (sequence, KV head) that one block holds is finished there, and the join takes those that a block cuts
@@ -1403,7 +1404,8 @@ __device__ __forceinline__ void join_block_wide(const PagedAttn& a, const PagedW
 // partials v, v + MW, .., their maxima a lane each and 4 rows requested together (a launch is a chain of trips to memory: the
 // sequence, then these). Two waves an item: 2048 items of 64 sequences of 200 .. 6000 keys 5.7 us (four waves 7.1, one 5.4); 768 of
 // 4 .. 16 partials 6.6 us (8.4, 8.2). Four waves up to 512 items (a call with one sequence of 32768 keys and one KV head, 128
-// pieces, 17 us, with two 21.5; of 131072 keys and four 52 and 57).
+// pieces, 17 us, with two 21.5; of 131072 keys and four 52 and 57). TREE, above 2048 items, one: a step's trees have many rows, and the
+// blocks no longer run all at once (24 trees over a prefix of 6001, 4992 items, 7.6 us for 10.1; lines keep the order of their sums).
 template <bool TREE, int HD, bool DIRECT, int MW>
 __device__ __forceinline__ void merge_block(const PagedAttn& a, const PagedWs& w, int x, int per) {
     constexpr int DL = HD / 64, ITEMS = 4 / MW, U = 4;
@@ -1649,6 +1651,8 @@ static void launch_t(const PagedAttn& a, const PagedWs& w, hipStream_t s) {
     if (w.direct) {
         const dim3 jgrid((unsigned)(jblocks + std::max(div_up(items, 2), a.nseq * w.rt)));
         attn_paged_join_kernel<TREE, HD, true, 2><<<jgrid, block, 0, s>>>(a, w, jblocks, per);
+    } else if (TREE && items > 2048) {
+        attn_paged_join_kernel<TREE, HD, false, TREE ? 1 : 2><<<dim3((unsigned)(jblocks + div_up(items, 4))), block, 0, s>>>(a, w, jblocks, per);
     } else if (items > 512) {
         attn_paged_join_kernel<TREE, HD, false, 2><<<dim3((unsigned)(jblocks + div_up(items, 2))), block, 0, s>>>(a, w, jblocks, per);
     } else {

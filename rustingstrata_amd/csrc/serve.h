@@ -1,5 +1,5 @@
 // Launchers of the operators that serve a batch of sequences over a paged f16 KV cache (serve.hip: page tables and slot
-// maps, penalties, biases and masks on logits; attn_paged.hip: attention). Arguments are checked in api.hip.
+// maps, penalties, biases and masks on logits; attn_paged.h: attention). Arguments are checked in api.hip.
 #pragma once
 #include "common.h"
 

@@ -480,12 +480,12 @@ def test_attn_tree_long(hip):
 
 
 @pytest.mark.parametrize("nseq", [300, 1030])
-@pytest.mark.parametrize("P", [0, 33])
-def test_attn_tree_many_sequences(hip, nseq, P):
+@pytest.mark.parametrize("P,hd", [(0, 64), (33, 64), (33, 128)])
+def test_attn_tree_many_sequences(hip, nseq, P, hd):
     rng = np.random.default_rng(nseq)
     q = rng.integers(0, 6, nseq).tolist()
     n = [k + int(m) for k, m in zip(q, rng.integers(0, 60, nseq))]
-    b = Trees(hip, q, n, 8, 2, 64, 16, 1, P=P, seed=P).upload()
+    b = Trees(hip, q, n, 8, 2, hd, 16, 1, P=P, seed=P).upload()
     b.launch()
     b.check(b.get(), rows=sorted(rng.integers(0, b.t, 300).tolist()))
 
