@@ -808,18 +808,19 @@ __device__ __forceinline__ void tile_run(const PagedAttn& a, const Keys& keys, u
             for (int i = 0; i < 16; i++) v = fmaxf(v, x[mt][i]);
         return max_half(v);
     };
+    // while tile kt is used (pg: tile kt + 1's pages): the next one's V, and the K of the one after
+    auto request = [&](int kt, int buf) __attribute__((always_inline)) {
+        load(kt + 1, pg, vg, vbuf + (buf ^ 1) * L::KB);
+        if (kt + 2 < ke) {
+            pages(kt + 2, pg);
+            load(kt + 2, pg, kg, kbuf + buf * L::KB);
+        }
+    };
     // one tile: its softmax beside the next one's scores, then its V products; NEXT: there is a next one
     auto tile = [&](int kt, auto NEXT) __attribute__((always_inline)) {
         constexpr bool next = decltype(NEXT)::value;
         const int buf = (kt - kb) & 1;
-        if constexpr (next) {
-            // (pg: tile kt + 1's pages; its V, and the K of the one after)
-            load(kt + 1, pg, vg, vbuf + (buf ^ 1) * L::KB);
-            if (kt + 2 < ke) {
-                pages(kt + 2, pg);
-                load(kt + 2, pg, kg, kbuf + buf * L::KB);
-            }
-        }
+        if constexpr (next) request(kt, buf);
         const float mxs = mx * usc;
         if (__ballot(mxs > m + 1.0f)) {  // (m follows the maximum when a weight would pass 2, column by column)
             const float mnew = mxs > m + 1.0f ? mxs : m, alpha = m == -INFINITY ? 0.0f : exp2_hw(m - mnew);
@@ -893,7 +894,19 @@ __device__ __forceinline__ void tile_run(const PagedAttn& a, const Keys& keys, u
             mx = largest(s);
         }
     };
-    if (kb < ke) {
+    if (TREE && kb < ke && !__ballot(live)) {
+        // a wave without rows (trees have few) loads its part of the tiles and leaves the SIMD to the CU's other block (32 trees over
+        // 4000 keys, 32 heads over 4: 5 rows each 93 us for 105, 12 98 for 103, 20 148 for 157)
+        wait_loads();
+        lds_barrier();
+        lds_barrier();
+        for (int kt = kb; kt + 1 < ke; kt++) {
+            request(kt, (kt - kb) & 1);
+            wait_loads();
+            lds_barrier();
+        }
+        lds_barrier();
+    } else if (kb < ke) {
         wait_loads();
         lds_barrier();
         scores(0, s);
