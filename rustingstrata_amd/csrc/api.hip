@@ -1102,21 +1102,21 @@ static int paged_attn_args(strata_ctx* c, const char* what, PagedAttn& a, uint64
                            uint64_t max_q, uint64_t pos, uint64_t q_start, uint64_t len, uint64_t nseq, uint64_t tables,
                            uint64_t max_pages, uint64_t page, uint64_t n_pages, uint64_t prefix, uint64_t prefix_len,
                            uint64_t max_prefix, uint64_t nh, uint64_t nkv, uint64_t hd, float scale, uint64_t sink, uint64_t win) {
-    const std::string w = what;
+    auto w = [&] { return std::string(what); };
     if (check_ctx(c) || check_attn(nh, nkv, hd, what) || check_pages(nseq, max_pages, page, n_pages, what)) return -1;
     if (!t || !nseq) return 0;
-    if (!q || !kc || !vc || !out || !pos || !q_start || !len || !tables) return set_error(w + ": null argument");
-    if (max_prefix && (!prefix || !prefix_len)) return set_error(w + ": null prefix or its length");
-    if (t > (1ull << 20) || !max_q || max_q > t) return set_error(w + ": " + std::to_string(t) + " rows (at most 2^20), at most " + std::to_string(max_q) + " a sequence");
-    if (max_prefix > (1ull << 30) || win >= (1ull << 31) || nkv > 65535 || nh > 65535) return set_error(w + ": too large");
+    if (!q || !kc || !vc || !out || !pos || !q_start || !len || !tables) return set_error(w() + ": null argument");
+    if (max_prefix && (!prefix || !prefix_len)) return set_error(w() + ": null prefix or its length");
+    if (t > (1ull << 20) || !max_q || max_q > t) return set_error(w() + ": " + std::to_string(t) + " rows (at most 2^20), at most " + std::to_string(max_q) + " a sequence");
+    if (max_prefix > (1ull << 30) || win >= (1ull << 31) || nkv > 65535 || nh > 65535) return set_error(w() + ": too large");
     if (max_prefix + max_pages * page > PAGED_ATTN_KEYS)
-        return set_error(w + ": " + std::to_string(max_prefix + max_pages * page) + " positions of a prefix and a sequence (at most 2^31 - 1024)");
-    if (nseq * nkv * (max_pages * page / 64 + 32) >= (1ull << 31)) return set_error(w + ": more than 2^31 chunks of keys (sequences x KV heads x positions / 64)");
+        return set_error(w() + ": " + std::to_string(max_prefix + max_pages * page) + " positions of a prefix and a sequence (at most 2^31 - 1024)");
+    if (nseq * nkv * (max_pages * page / 64 + 32) >= (1ull << 31)) return set_error(w() + ": more than 2^31 chunks of keys (sequences x KV heads x positions / 64)");
     if ((t / (128 / (nh / nkv)) + nseq + 1) * ((max_prefix + max_pages * page) / 64 + 5) >= (1ull << 31))
-        return set_error(w + ": more than 2^31 tiles of rows and keys (rows x group / 128 + sequences, times positions / 64)");
-    if (q % 16 || out % 16 || kc % 16 || vc % 16 || qg % 16) return set_error(w + ": q, qg, out and the caches must be 16-byte aligned");
-    if (out == q || out == qg) return set_error(w + ": out over an input");
-    if (!(scale > 0.0f) || std::isinf(scale)) return set_error(w + ": a scale of " + std::to_string(scale) + " (above 0)");
+        return set_error(w() + ": more than 2^31 tiles of rows and keys (rows x group / 128 + sequences, times positions / 64)");
+    if (q % 16 || out % 16 || kc % 16 || vc % 16 || qg % 16) return set_error(w() + ": q, qg, out and the caches must be 16-byte aligned");
+    if (out == q || out == qg) return set_error(w() + ": out over an input");
+    if (!(scale > 0.0f) || std::isinf(scale)) return set_error(w() + ": a scale of " + std::to_string(scale) + " (above 0)");
     a.q = (const float*)q; a.kc = (const uint16_t*)kc; a.vc = (const uint16_t*)vc; a.qg = (const float*)qg; a.out = (float*)out;
     a.t = (int)t; a.max_q = (int)max_q; a.pos = (const int*)pos; a.q_start = (const int*)q_start; a.len = (const int*)len;
     a.nseq = (int)nseq; a.tables = (const int*)tables; a.max_pages = (int)max_pages; a.page_shift = log2_of(page);

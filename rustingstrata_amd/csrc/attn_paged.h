@@ -47,8 +47,8 @@ struct PagedWs {
     float2* tml;   // [2 tblocks][128]: the pieces of tiles that more than one block computes
     float* tacc;   // [2 tblocks][128][hd]
     int direct;    // a (sequence, KV head) that one block holds is finished there, and the join takes those that a block cuts
-    int rt;        // TREE: row tiles of a sequence (above 1: of dr rows each, and all of them decode)
     int dblocks, nct, dr, nsp, prows, tblocks;  // decode blocks, their column tiles; rows (tokens x G) up to which a sequence decodes
+    int rt;        // TREE: row tiles of a sequence (above 1: of dr rows each, and all of them decode)
 };
 
 // ---------------- sequences ----------------
@@ -340,7 +340,7 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
         int last[2], ok;
     };
     auto pages = [&](const Piece& p, int c, int (&pg)[2]) __attribute__((always_inline)) {
-        const int* table = a.tables + (uint64_t)p.q.seq * a.max_pages;
+        const int* table = a.tables + (uint64_t)(TREE ? p.q.seq : p.s) * a.max_pages;
 #pragma unroll
         for (int t = 0; t < 2; t++) pg[t] = sload(table + (min(DEC_CHUNK * c + 32 * wave + 16 * t, p.q.len - 1) >> a.page_shift));
     };
@@ -602,7 +602,7 @@ __device__ __forceinline__ void dec_block(const PagedAttn& a, const PagedWs& w, 
                 const Node node = node_of<TREE>(a, pc.q.q0 + tok, pc.q.s0, pc.q.sn, pc.q.len);
                 own_range<TREE>(a, a.pos[pc.q.q0 + tok], pc.q.len, P, node, klo, khi);
                 float ac[HD / 64], mm, ll;
-                paged_row_again<TREE, HD>(a, Keys{nullptr, a.tables + (uint64_t)pc.q.seq * a.max_pages, 0, 0, pc.q.len}, node,
+                paged_row_again<TREE, HD>(a, Keys{nullptr, a.tables + (uint64_t)(TREE ? pc.q.seq : pc.s) * a.max_pages, 0, 0, pc.q.len}, node,
                                     a.q + ((uint64_t)(pc.q.q0 + tok) * a.nh + pc.g * G + cb % G) * HD, pc.g, max(klo, DEC_CHUNK * c0),
                                     min(khi, DEC_CHUNK * c1 - 1), ac, mm, ll);
                 const uint64_t r = (uint64_t)(b + pair) * w.dr + cb, row = (uint64_t)(pc.q.q0 + tok) * a.nh + pc.g * G + cb % G;
