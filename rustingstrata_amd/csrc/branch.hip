@@ -381,7 +381,6 @@ __global__ __launch_bounds__(256) void pages_fork_kernel(PagesFork a) {
 }
 
 hipError_t launch_pages_fork(const PagesFork& a, hipStream_t s) {
-    if (!a.nseq) return hipSuccess;
     if ((long long)a.nseq * a.max_pages <= (a.src ? FORK_ONE_SRC : FORK_ONE)) {
         pages_fork_one_kernel<<<dim3(1), dim3(1024), 0, s>>>(a);
     } else {

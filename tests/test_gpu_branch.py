@@ -191,6 +191,10 @@ def test_pages_fork_of_anything(hip, nseq):
 def test_pages_fork_of_nothing(hip):
     Fork(hip, np.zeros(0, int), np.zeros(0, int), 16, 3, np.arange(4), 2, 4, np.zeros(4, int)).run()
     b = i32(hip, [0] * 64)
+    for n, want in ((3, 3), (9, 4), (-2, 0)):  # (the stack's height is written all the same)
+        out = guarded(hip, 1)
+        hip.kv_pages_fork(0, 0, 0, 0, 0, 3, 16, b, 4, i32(hip, [n]), b, 0, out, 0)
+        check_i32(hip, out, [want])
     hip.kv_rows_move(b, 0, 16, 4, b, 3, 1)
     hip.kv_rows_move(b, 2, 16, 4, b, 0, 1)
 
