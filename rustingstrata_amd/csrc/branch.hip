@@ -20,7 +20,7 @@ namespace strata {
 // threads does them all over lists of the entries that are kept and let go, whatever sequence they belong to; else four launches, a wave
 // a sequence. Bound by latency: every phase is a chain of trips to memory. Beams, tables of 272 entries 8.8 us in one block and 13.0 in
 // four launches, 1344 11.0 and 13.8, 5376 30 and 16.6; cuts alone let few pages go (the end of a step of 256 trees over tables of
-// 12 16.1 us and 20.9).
+// 12: 16.1 us and 20.9).
 constexpr long long FORK_ONE = 1 << 15, FORK_ONE_SRC = 1 << 11;
 enum { F_CHANGED = 1, F_OTHER = 2, F_TAKE = 4, F_COPY = 8 };
 
