@@ -319,13 +319,19 @@ __global__ __launch_bounds__(LG_T, 4) void logprobs_kernel(Logprobs a, LgScratch
 #pragma unroll
                     for (int u = 0; u < LG_U; u++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) n += __popcll(__ballot(order(cur[u][e]) >= l + (4 * LG_T * u + e >= at)));
+                        for (int e = 0; e < 4; e++) {
+                            const uint32_t o = order(cur[u][e]);
+                            n += __popcll(__ballot(o > l || (o == l && 4 * LG_T * u + e < at)));
+                        }
                 } else if (odd || y == 0.0f || !(y > -INFINITY)) {
+                    // (keys >= from; the largest key, a NaN's, has none above it to count from)
                     const uint32_t from = l + (id < first);
+                    if (from >= l) {
 #pragma unroll
-                    for (int u = 0; u < LG_U; u++)
+                        for (int u = 0; u < LG_U; u++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) n += __popcll(__ballot(order(cur[u][e]) >= from));
+                            for (int e = 0; e < 4; e++) n += __popcll(__ballot(order(cur[u][e]) >= from));
+                    }
                 } else if (!__ballot(mx >= y)) {  // (a likely token: nothing of most tiles comes before it)
                 } else if (id < first) {  // (other numbers compare as their keys do)
 #pragma unroll
@@ -403,7 +409,7 @@ __global__ __launch_bounds__(LG_T, 4) void logprobs_kernel(Logprobs a, LgScratch
     if (RANK && tid < a.m) {
         // values outside the row are not before anything
         if (t0 == 0 && none >= lim[tid] + (ids[tid] < 0)) before[tid] -= off;
-        if (t1 == tiles && none >= lim[tid] + 1) before[tid] -= (int)((long long)tiles * LG_TILE - off - a.n);
+        if (t1 == tiles && none > lim[tid]) before[tid] -= (int)((long long)tiles * LG_TILE - off - a.n);
     }
     if (parts == 1) {
         lg_finish<TOP>(a, r, v, before, lists, cnt);

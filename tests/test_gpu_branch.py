@@ -364,6 +364,30 @@ def test_logprobs(hip, rows, n, m, k, kind):
         Logp(hip, x, ids, k, stride=n + 5, shift=1).run().check()
 
 
+@pytest.mark.parametrize("rows,n", [(1, 5), (2, 9001), (600, 9001), (1, 50001)])
+def test_logprobs_ranks_at_the_ends_of_the_order(hip, rows, n):
+    """Given tokens that are the greatest and the least of all values (the NaN whose bits are 0x7FFFFFFF, and 0xFFFFFFFF), alone and
+    twice, at the first, a middle and the last index, beside tokens around them."""
+    rng = np.random.default_rng(n)
+    x = logits(rows, n, n)
+    for r in range(rows):
+        at = [0, n // 2, n - 1]
+        top, low = int(rng.integers(0, 3)), int(rng.integers(0, 3))
+        bits = x[r].view(np.uint32)
+        bits[at[top]] = 0x7FFFFFFF
+        if r % 3 == 1:
+            bits[at[(top + 1) % 3]] = 0x7FFFFFFF
+        if low != top:
+            bits[at[low]] = 0xFFFFFFFF
+        if r % 3 == 2:
+            bits[min(n - 1, n // 2 + 3)] = 0xFFFFFFFF
+    ids = np.stack([np.full(rows, v) for v in (0, n // 2, n - 1, 1, min(n - 1, n // 2 + 3), max(0, n - 2), -1, n)], 1)
+    Logp(hip, x, ids, 4).run().check()
+    Logp(hip, x, ids, 0, stride=n + 2, shift=1).run().check()
+    for i in range(ids.shape[1]):
+        Logp(hip, x, ids[:, i:i + 1], 0).run().check()
+
+
 def test_logprobs_parts_alone(hip):
     """Each output alone gives what all together do."""
     x, ids = logits(7, 30001, 5), np.random.default_rng(1).integers(0, 30001, (7, 2))
