@@ -132,7 +132,8 @@ __device__ __forceinline__ int lg_place(const uint64_t* lists, const int* cnt, i
     }
     return place;
 }
-// The waves' lists cut to the K best of all of them together, and the bound that follows.
+// The waves' lists cut to the K best of all of them together, and the bound that follows. shared: a word that the call before did not
+// use (a wave may still read that one when this call clears its own; of the call before it, the barriers between have all waves past).
 __device__ __forceinline__ void lg_agree(TopList& top, const uint64_t* lists, int* cnt, uint64_t* shared) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     top.cut();
@@ -226,7 +227,7 @@ __device__ __forceinline__ void lg_finish(const Logprobs& a, int r, const LgSums
 // that rule 168; any four 175 and 174).
 template <bool RANK, bool TOP>
 __global__ __launch_bounds__(LG_T, 4) void logprobs_kernel(Logprobs a, LgScratch f, int parts, int tiles) {
-    __shared__ uint64_t lists[TOP ? LG_W * LG_LIST : 1], shared;
+    __shared__ uint64_t lists[TOP ? LG_W * LG_LIST : 1], shared[2];
     __shared__ LgSums ws[LG_W];
     __shared__ uint32_t wb[LG_W], lim[LOGP_MAX_IDS];
     __shared__ int cnt[LG_W], before[LOGP_MAX_IDS], ids[LOGP_MAX_IDS];
@@ -389,7 +390,8 @@ __global__ __launch_bounds__(LG_T, 4) void logprobs_kernel(Logprobs a, LgScratch
                     hit &= hit - 1;
                 }
             }
-            if (((t - t0 + 1) & (t - t0)) == 0 && t + 1 < t1) lg_agree(top, lists, cnt, &shared);  // after 1, 2, 4, .. tiles
+            if (((t - t0 + 1) & (t - t0)) == 0 && t + 1 < t1)  // after 1, 2, 4, .. tiles, the words in turn
+                lg_agree(top, lists, cnt, shared + (__builtin_ctz(t - t0 + 1) & 1));
         }
 #pragma unroll
         for (int u = 0; u < LG_U; u++)
