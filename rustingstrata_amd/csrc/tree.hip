@@ -29,7 +29,7 @@ __global__ __launch_bounds__(W <= 2 ? 64 : 32 * W) void tree_step_kernel(TreeSte
     const int s = blockIdx.x, i = threadIdx.x;
     const int P = a.prefix_len ? max(sload(a.prefix_len), 0) : 0;
     if (s == a.nseq) {  // rows behind the last sequence
-        for (int r = max(sload(a.q_start + a.nseq), 0) + i; r < a.t; r += T) {
+        for (int r = min(max(sload(a.q_start + a.nseq), 0), a.t) + i; r < a.t; r += T) {
             a.pos[r] = -1;
             for (int w = 0; w < a.words; w++) a.mask[(uint64_t)r * a.words + w] = 0;
         }

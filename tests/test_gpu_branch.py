@@ -69,6 +69,24 @@ def test_tree_step_of_bad_parents(hip):
     assert get_i32(hip, err, 1)[0] == 5 + bad
 
 
+def test_tree_step_of_row_starts_past_the_rows(hip):
+    """Row starts that say more than there is, up to 2^31 - 1: nothing is written past the t rows or before them."""
+    t = 40
+    parent = [-1 if i < 1 else i - 1 for i in range(t)]
+    for q_start in ([0, 5, 2**31 - 1], [2**31 - 1] * 3, [-5, 9, 2**31 - 200], [-2**31, -1, 17]):
+        pos, mask = i32(hip, [GUARD] * (2 * t + 1)), i32(hip, [GUARD] * (2 * t + 1))
+        hip.tree_step(2, i32(hip, q_start), i32(hip, parent), i32(hip, [70, 60]), t, 1, int(pos) + 4 * t, int(mask) + 4 * t)
+        want, bits, _ = B.tree_step(q_start, parent, [70, 60], 0, t, 1)
+        written = np.zeros(t, bool)  # (rows of no sequence, before the end that the starts give, are left as they are)
+        written[min(max(q_start[2], 0), t):] = True
+        for s in range(2):
+            written[min(max(q_start[s], 0), t):min(max(q_start[s + 1], 0), t)] = True
+        for b, w in ((pos, want), (mask, bits[:, 0].astype(np.int64).astype(np.uint32).astype(np.int32))):
+            got = get_i32(hip, b, 2 * t + 1)
+            assert (got[:t] == GUARD).all() and got[-1] == GUARD
+            np.testing.assert_array_equal(got[t:-1], np.where(written, w, GUARD))
+
+
 # ---------------- the confirmed path ----------------
 def accept_case(rng, sizes, words, agree, vocab=50):
     q_start = np.concatenate([[0], np.cumsum(sizes)])
