@@ -402,13 +402,15 @@ hipError_t launch_pages_fork(const PagesFork& a, hipStream_t s) {
 // confirmed paths in 24 caches 12.8 us with one, 5.6 with six).
 constexpr int MOVE_MAX_RUNS = 256, MOVE_U = 8;
 
-__global__ __launch_bounds__(256) void rows_move_kernel(RowsMove a, int tpr_shift, int cpb) {
+__global__ __launch_bounds__(256) void rows_move_kernel(RowsMove a, int tpr_shift, int cpb, unsigned first) {
     typedef unsigned v4u __attribute__((ext_vector_type(4)));
     __shared__ int from[MOVE_MAX_RUNS], to[MOVE_MAX_RUNS];
     __shared__ uint64_t rs[256], rd[256];
     __shared__ long long start[MOVE_MAX_RUNS], ws[4];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int parts = (a.n_caches + cpb - 1) / cpb, g = blockIdx.x / parts, c0 = blockIdx.x % parts * cpb, nc = min(cpb, a.n_caches - c0);
+    const int parts = (a.n_caches + cpb - 1) / cpb;
+    const unsigned at = first + blockIdx.x;
+    const int g = at / parts, c0 = at % parts * cpb, nc = min(cpb, a.n_caches - c0);
     long long n = 0;
     if (tid < a.per) {
         const int* r = a.runs + ((uint64_t)g * a.per + tid) * 3;
@@ -474,7 +476,11 @@ hipError_t launch_rows_move(const RowsMove& a, hipStream_t s) {
     while (shift < 8 && (16ull << shift) < a.row_bytes) shift++;
     // one cache a block where a group is one run (pages' rows); else caches as leave four blocks a CU
     const int cpb = a.per == 1 ? 1 : (int)std::max<long long>(1, std::min<long long>(8, (long long)a.groups * a.n_caches / 1024));
-    rows_move_kernel<<<dim3((unsigned)((uint64_t)a.groups * ((a.n_caches + cpb - 1) / cpb))), dim3(256), 0, s>>>(a, shift, cpb);
+    // HIP's launches have fewer than 2^32 threads: more blocks go on in further ones (a captured launch of more is refused)
+    constexpr uint64_t most = 1 << 23;
+    const uint64_t blocks = (uint64_t)a.groups * ((a.n_caches + cpb - 1) / cpb);
+    for (uint64_t first = 0; first < blocks; first += most)
+        rows_move_kernel<<<dim3((unsigned)std::min(blocks - first, most)), dim3(256), 0, s>>>(a, shift, cpb, (unsigned)first);
     return hipGetLastError();
 }
 

@@ -271,6 +271,29 @@ def test_rows_move(hip, row_bytes, caches):
         check_i32(hip, b, w)
 
 
+def test_rows_move_of_more_blocks_than_one_launch(hip):
+    """2^20 groups of 17 caches, more than 2^24 pieces of work: runs of the first and the last groups and of those on both sides of
+    every 2^23rd piece, eager and recorded."""
+    groups, caches, n_slots, row_bytes = 1 << 20, 17, 64, 16
+    rng = np.random.default_rng(1)
+    data = rng.integers(-2**31, 2**31, (caches, n_slots, row_bytes // 4)).astype(np.int32)
+    runs = np.zeros((groups, 1, 3), np.int32)
+    busy = sorted({0, 1, groups - 2, groups - 1} | {(k << 23) // caches + d for k in (1, 2) for d in (-1, 0, 1)})
+    for i, g in enumerate(busy):  # (no run reads a row that another writes)
+        runs[g, 0] = i, 32 + 2 * i, 1 + i % 2
+    bufs = [up(hip, np.concatenate([c.reshape(-1), [GUARD]]).astype(np.int32)) for c in data]
+    table, moves = up(hip, np.array([int(b) for b in bufs], np.uint64)), up(hip, runs)
+    call = lambda: hip.kv_rows_move(table, caches, row_bytes, n_slots, moves, groups, 1)  # noqa: E731
+    g = hip.record_graph(call, keep=[table, moves, *bufs])
+    for run in (call, g.launch):
+        for b, c in zip(bufs, data):
+            hip.htod(c, b)
+        run()
+        for b, c in zip(bufs, data):
+            check_i32(hip, b, B.rows_move(c.copy(), runs[busy].astype(np.int64), n_slots))
+    g.close()
+
+
 def test_rows_move_of_a_whole_page(hip):
     """One run a group, longer than a batch, to another page."""
     rng = np.random.default_rng(1)
