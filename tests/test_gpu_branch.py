@@ -188,6 +188,20 @@ def test_pages_fork(hip, nseq, page, max_pages, spare, what):
         Fork(hip, length, tables, page, max_pages, free, n_free, n_pages, refs, src, keep, place).run().check(want)
 
 
+def full_pool(rng, length, page, max_pages):
+    """Sequences of these lengths, each next to the one before sharing a random part of its full pages, over a pool of just their pages."""
+    nseq, rows, at = len(length), np.full((len(length), max_pages), -1), 0
+    for s, n in enumerate(length):
+        have = -(-n // page)
+        k = min(int(rng.integers(0, max_pages)), n // page, length[s - 1] // page) if s and rng.random() < 0.3 else 0
+        rows[s, :k] = rows[s - 1, :k]
+        rows[s, k:have] = np.arange(at, at + have - k)
+        at += have - k
+    order = rng.permutation(at)
+    tables = np.where(rows >= 0, order[np.maximum(rows, 0)], rng.integers(-3, at + 3, rows.shape))
+    return length, tables, rng.integers(0, at, at), 0, at, np.maximum(np.bincount(order[rows[rows >= 0]], minlength=at) - 1, 0)
+
+
 @pytest.mark.parametrize("nseq", [9, 300])
 def test_pages_fork_of_anything(hip, nseq):
     """Lengths, sources, page ids, counts and stacks outside their limits."""
@@ -204,6 +218,26 @@ def test_pages_fork_of_anything(hip, nseq):
         want = B.pages_fork(src, keep, length, tables, 4, 16, free, n_pages, n, refs)
         assert want["refused"] > 0
         Fork(hip, length, tables, 16, 4, free, n, n_pages, refs, src, keep).run().check(want)
+
+
+@pytest.mark.parametrize("nseq,max_pages", [(256, 128), (32, 1024), (4096, 8), (257, 128), (300, 128), (33, 1024), (4096, 9)])
+@pytest.mark.parametrize("what", ["cut", "few", "end", "all", "none"])
+def test_pages_fork_of_wide_tables(hip, nseq, max_pages, what):
+    """Cuts and ends of a server's sequences without sources, on both sides of the tables that one block takes (2^15 entries): a few
+    pages let go and all of them, pages that others hold, cuts refused for want of a page; in place as well as not."""
+    page, rng = 16, np.random.default_rng(nseq + len(what))
+    length, tables, free, n_free, n_pages, refs = pool_case(rng, nseq, page, max_pages, 40)
+    if what == "all":
+        length[:] = max_pages * page
+        length, tables, free, n_free, n_pages, refs = full_pool(rng, length, page, max_pages)
+    keep = dict(cut=rng.integers(0, max_pages * page + 1, nseq), few=length - rng.integers(0, 40, nseq), end=np.where(rng.random(nseq) < 0.3, 0, length), all=np.zeros(nseq, np.int64)).get(what)
+    n_free = min(n_free, 5) if what in ("cut", "few") else n_free
+    want = B.pages_fork(None, keep, length, tables, max_pages, page, free, n_pages, n_free, refs)
+    assert what in ("cut", "few") or want["refused"] == 0
+    if what == "all":
+        assert want["n_free_out"] == [n_pages] and not want["refs"].any()
+    for place in (False, True):
+        Fork(hip, length, tables, page, max_pages, free, n_free, n_pages, refs, None, keep, place).run().check(want)
 
 
 def test_pages_fork_of_nothing(hip):
