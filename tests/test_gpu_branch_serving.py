@@ -189,3 +189,69 @@ def test_serving_trees(hip, graph):
     assert get_i32(hip, sv.n_free, 1)[0] == sv.n_free0 and not get_i32(hip, sv.refs, sv.N_PAGES).any()
     if g:
         g.close()
+
+
+class PartsServer(TreeServer):
+    """TreeServer whose step leaves the cut to a call of its own, so that the host may say what stays in between."""
+
+    def fork(self, src, keep):
+        pass
+
+    def cut(self):
+        super().fork(0, self.keep)
+
+    def step_then_cut(self, whole):
+        """The calls of a step up to the confirmed path's rows, then those of the cut; sequences `whole` keep all their positions."""
+        hip = self.hip
+        self.parts[0]()
+        keep, length = get_i32(hip, self.keep, self.NSEQ), get_i32(hip, self.len, self.NSEQ)
+        hip.htod(np.where(whole, length, keep).astype(np.int32), self.keep)
+        self.parts[1]()
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_serving_chunks_beside_trees(hip, graph):
+    """Chunks of a prompt of no more rows than a tree has, as trees without branches beside drafted ones: all of their positions stay, the
+    choice after the last chunk is the one after its last row, and the sequence goes on with trees. Eager and as two recorded parts."""
+    rng = np.random.default_rng(21)
+    sv = PartsServer(hip, 10)
+    prompts = [rng.integers(0, sv.vocab, k) for k in (5, 17, 15, 4)]
+    truth = plain_tokens(hip, 10, prompts, 50)
+    n, first = sv.NSEQ, [5, 17, 1, 4]  # (14 of the third prompt's tokens come in chunks)
+    sv.inputs(np.concatenate([p[:k] for p, k in zip(prompts, first)]))
+    hip.htod(np.array(first, np.int32), sv.add)
+    sv.layer(sum(first), max(first))
+    toks, got = [p[:k].tolist() for p, k in zip(prompts, first)], [[truth[s][0]] if first[s] == len(prompts[s]) else [] for s in range(n)]
+    sv.parts = (sv.step, sv.cut)
+    graphs, cut_short = [], 0
+    for k in range(7):
+        chunk = min(NODES - (k == 0), len(prompts[2]) - len(toks[2])) if not got[2] else 0
+        sizes = [chunk if s == 2 and chunk else int(rng.integers(2, NODES + 1)) for s in range(n)]
+        trees = [draft(rng, truth[s], len(got[s]), q, sv.vocab) if got[s] else (list(range(-1, q - 1)), prompts[s][len(toks[s]):len(toks[s]) + q].tolist()) for s, q in enumerate(sizes)]
+        parent, tokens = (np.concatenate([np.array(tr[i], np.int64) for tr in trees] + [np.zeros(sv.t, np.int64)])[:sv.t] for i in (0, 1))
+        sv.inputs(tokens)
+        for v, b in ((sizes, sv.add), (parent, sv.parent), (tokens, sv.tokens)):
+            hip.htod(np.asarray(v, np.int32), b)
+        if graph and k == 1:  # (the step before has sized the workspace)
+            graphs = [hip.record_graph(f, keep=[sv]) for f in sv.parts]
+            sv.parts = [g.launch for g in graphs]
+        sv.step_then_cut(np.array([s == 2 and chunk > 0 for s in range(n)]))
+        n_path, chosen = get_i32(hip, sv.n_path, n), get_i32(hip, sv.chosen, n * PATH).reshape(n, PATH)
+        ids, q_start = get_i32(hip, sv.row_ids, sv.t), np.concatenate([[0], np.cumsum(sizes)])
+        for s in range(n):
+            if s == 2 and chunk:
+                cut_short += n_path[s] < chunk
+                toks[s] = toks[s] + prompts[s][len(toks[s]):len(toks[s]) + chunk].tolist()
+                if len(toks[s]) == len(prompts[s]):
+                    assert ids[q_start[s + 1] - 1] == truth[s][0]
+                    got[s] = [truth[s][0]]
+                continue
+            c = int(n_path[s])
+            assert chosen[s, :c].tolist() == truth[s][len(got[s]):len(got[s]) + c], (k, s)
+            toks[s] = toks[s] + [got[s][-1]] + chosen[s, :c - 1].tolist()
+            got[s] = got[s] + chosen[s, :c].tolist()
+        sv.check_pool()
+        sv.check_cache(toks)
+    assert cut_short and len(got[2]) > 2 and get_i32(hip, sv.err, 1)[0] == 0
+    for g in graphs:
+        g.close()
