@@ -328,6 +328,26 @@ def test_rows_move_of_more_blocks_than_one_launch(hip):
     g.close()
 
 
+@pytest.mark.parametrize("groups,caches,per", [(300, 13, 7), (2100, 1, 2), (700, 3, 64), (260, 9, 65), (150, 16, 256), (90, 30, 129)])
+def test_rows_move_of_many_caches(hip, groups, caches, per):
+    """Groups and caches enough for a block to take several caches, the last one fewer, and runs of 2 to 256 a group: paths that close
+    up, each in slots of its own."""
+    rng = np.random.default_rng(per)
+    row_bytes, room = 32, per + 3
+    n_slots = groups * room
+    data = rng.integers(-2**31, 2**31, (caches, n_slots, row_bytes // 4)).astype(np.int32)
+    runs = np.zeros((groups, per, 3), np.int64)
+    for g in range(groups):
+        k = int(rng.integers(0, per + 1))
+        path = np.sort(rng.choice(room, k, replace=False))
+        runs[g, :k] = np.stack([g * room + path, g * room + np.arange(k), path != np.arange(k)], 1)
+    want = np.stack([B.rows_move(c.copy(), runs, n_slots) for c in data])
+    bufs = [up(hip, np.concatenate([c.reshape(-1), [GUARD]]).astype(np.int32)) for c in data]
+    hip.kv_rows_move(up(hip, np.array([int(b) for b in bufs], np.uint64)), caches, row_bytes, n_slots, i32(hip, runs), groups, per)
+    for b, w in zip(bufs, want):
+        check_i32(hip, b, w)
+
+
 def test_rows_move_of_a_whole_page(hip):
     """One run a group, longer than a batch, to another page."""
     rng = np.random.default_rng(1)
@@ -684,6 +704,27 @@ def test_attn_tree_offsets_past_32_bits(hip):
     b.launch()
     b.n_pages -= far
     b.check(b.get())
+
+
+@pytest.mark.parametrize("q,room", [([4, 1, 2], 0), ([12, 9, 30], 0), ([40, 70, 3], 0), ([40, 30, 3], 9000)])
+def test_attn_tree_prefix_lengths_on_the_device(hip, q, room):
+    """A prefix that the call makes room for and the device says is shorter or not there."""
+    for P in (1, 50):
+        b = Trees(hip, q, [k + 70 for k in q], 8, 2, 64, 16, 2, P=P, seed=8, room=room, sink=True).upload()
+        b.launch(max_prefix=4096)
+        b.check(b.get())
+    b.launch(max_prefix=49)
+    less = b.get()
+    hip.htod(np.array([49], np.int32), b.pb["prefix_len"])
+    b.launch(max_prefix=50)
+    np.testing.assert_array_equal(less, b.get())
+    a = Trees(hip, q, [k + 70 for k in q], 8, 2, 64, 16, 2, seed=8, room=room, sink=True).upload()
+    prefix, none = i32(hip, [0] * 300), i32(hip, [0])
+    a.pb |= dict(prefix=prefix, prefix_len=none)
+    for n in (0, -5):
+        hip.htod(np.array([n], np.int32), none)
+        a.launch(max_prefix=4096)
+        a.check(a.get())
 
 
 def test_attn_tree_device_lengths_past_their_bounds(hip):
