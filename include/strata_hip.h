@@ -363,7 +363,8 @@ int strata_attn_decode_gq(strata_ctx* ctx, uint64_t q, uint64_t kc, uint64_t vc,
 
 /* One step of the page tables, all on the device: sequence s (nseq of them, len[s] positions cached) brings add[s] new tokens.
  * add[s] < 0: it ends; its pages go back on the stack of free pages (free_pages: n_pages entries, *n_free of them in use, the
- * top last) in order of sequence and page, before any page is taken. Then, in order of sequence, new pages come from the
+ * top last) in order of sequence and page, before any page is taken, whoever else holds them (a sequence that shares pages ends by
+ * strata_kv_pages_fork). Then, in order of sequence, new pages come from the
  * top of the stack into the tables. Writes q_start[nseq + 1], for each row t < q_start[nseq] its position pos[t] (*prefix_len
  * more than its own one, nothing where that is below 0; prefix_len may be 0) and its slot slots[t], -1 in both for the rows up to t_max behind them, and len_out
  * and *n_free_out (which may be len and n_free). A sequence is refused where its positions exceed max_pages pages, its rows
@@ -429,7 +430,8 @@ int strata_tree_step(strata_ctx* ctx, uint64_t nseq, uint64_t q_start, uint64_t 
 /* strata_attn_paged over trees: the arguments and limits of that call, and each row's mask (device uint32 words, rows of `words`
  * words). A row of a tree sees the prefix, its sequence's own keys before its rows, and row j's key where bit j of its mask is
  * set, j up to its own row; a row of a line sees what strata_attn_paged shows it. pos is used for lines and windows only; win
- * is 0 or at least 32 words, so that a window hides no ancestor. A row that sees no key is 0. */
+ * is 0 or at least 32 words, so that a window hides no ancestor. A row that sees no key is 0. The call's bounds (nseq, max_q, max_pages)
+ * choose its form before the lengths are known: tables much wider than the sequences cost a small step time, not its result. */
 int strata_attn_paged_tree(strata_ctx* ctx, uint64_t q, uint64_t kc, uint64_t vc, uint64_t qg, uint64_t out, uint64_t t,
                            uint64_t max_q, uint64_t pos, uint64_t q_start, uint64_t len, uint64_t nseq, uint64_t tables,
                            uint64_t max_pages, uint64_t page, uint64_t n_pages, uint64_t prefix, uint64_t prefix_len,
@@ -463,7 +465,8 @@ int strata_kv_pages_fork(strata_ctx* ctx, uint64_t nseq, uint64_t src, uint64_t 
                          uint64_t max_pages, uint64_t page, uint64_t free_pages, uint64_t n_pages, uint64_t n_free, uint64_t refs,
                          uint64_t len_out, uint64_t n_free_out, uint64_t runs, uint64_t err);
 /* Rows of n_caches caches (device uint64 addresses, 16-byte aligned, each once; the K and V caches of all layers) of row_bytes bytes (a
- * multiple of 16) from slot to slot: `groups` groups of `per` (1 to 256) runs (from, to, rows) of consecutive rows, device int32. A
+ * multiple of 16) from slot to slot: `groups` groups of `per` (1 to 256) runs (from, to, rows) of consecutive rows, device int32; groups and
+ * n_caches up to 2^20, their product below 2^31. A
  * group's runs are made in order; no run reads a row that the same or an earlier run of its group has written, and no group one that
  * another group writes. A run with a row outside 0 .. n_slots - 1, or of no rows, is left out. */
 int strata_kv_rows_move(strata_ctx* ctx, uint64_t caches, uint64_t n_caches, uint64_t row_bytes, uint64_t n_slots, uint64_t runs,

@@ -18,9 +18,12 @@ namespace strata {
 // Phases, each after all of the one before: the plan (a block); copies of the tables that others go on from and
 // cleared claims; the holders' counts; the pages that go; the stack and tables. Where the tables have few entries one block of 1024
 // threads does them all over lists of the entries that are kept and let go, whatever sequence they belong to; else four launches, a wave
-// a sequence. Bound by latency: every phase is a chain of trips to memory. Beams, tables of 272 entries 8.8 us in one block and 13.0 in
-// four launches, 1344 11.0 and 13.8, 5376 30 and 16.6; cuts alone let few pages go (the end of a step of 256 trees over tables of
-// 12: 16.1 us and 20.9).
+// a sequence. Bound by latency: every phase is a chain of trips to memory. Entries are those that the tables have room for (the host knows no
+// lengths). Beams, tables of 272 entries 8.8 us in one block and 13.0 in four launches, 1344 11.0 and 13.8, 5376 30 and 16.6. Without src the
+// pages let go decide (us in one block / in four launches, pages of 16, 4096, 16384 and 32768 entries of 256 sequences): all cut
+// inside their last page 5.8 / 11.4 at each, every 16th ended 8.8 / 12.1, 14.9 / 12.2, 24 / 14, all ended at once 34 / 14, 141 / 16,
+// 279 / 21; 32 sequences of 1024 pages 5.5 / 10.2, 24 / 47, 278 / 94. The cuts of every step are what the limit serves; the end of
+// everything at once pays for it. (The end of a step of 256 trees over tables of 12: 16.1 us and 20.9.)
 constexpr long long FORK_ONE = 1 << 15, FORK_ONE_SRC = 1 << 11;
 enum { F_CHANGED = 1, F_OTHER = 2, F_TAKE = 4, F_COPY = 8 };
 
